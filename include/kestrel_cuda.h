@@ -81,8 +81,9 @@ enum {
   KC_ERR_OOM = 8      /* device allocation failed                           */
 };
 
-/* ggml type ids (crates/kestrel-gguf/src/types.rs:48-86) with CUDA kernels. */
-enum { KC_F32 = 0, KC_Q8_0 = 8, KC_Q4_K = 12, KC_Q6_K = 14 };
+/* ggml type ids (crates/kestrel-gguf/src/types.rs:48-86) with CUDA kernels
+   (F16 and BF16: the paged cache's types, kc_kv_cache). */
+enum { KC_F32 = 0, KC_F16 = 1, KC_Q8_0 = 8, KC_Q4_K = 12, KC_Q6_K = 14, KC_BF16 = 30 };
 
 /* ---- context ------------------------------------------------------------ */
 
@@ -425,6 +426,83 @@ KC_API int kc_load_gguf(kc_ctx* ctx, const char* path, int n_ctx, char* info_jso
    (version, alignment, derived hyper-parameters, tensors with file offsets,
    sizes and strides) into out (cap bytes). Errors: kc_last_error(NULL). */
 KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
+
+/* ---- paged key-value cache and its attention ------------------------------
+   No counterpart in Kestrel, whose Transformer holds one contiguous cache per
+   sequence (transformer.rs:147-272). A cache is a pool of pages of `page`
+   positions that sequences hold through a table, so that memory follows what
+   sequences use, and sequences with a common beginning share its pages. All
+   buffers are device memory of the caller, who keeps them until kc_kv_drop
+   (or another registration of the id, or kc_free):
+
+     k, v   [n_layer][n_pages][n_head_kv][page][head_dim] of type t (16-byte
+            aligned)
+     table  [n_seq][max_pages] page ids; -1 past a sequence's last page
+     len    [n_seq] positions held
+     refs   [n_pages] sequences that hold the page (0: free)
+
+   An empty cache has table -1, len 0 and refs 0; the caller fills them in
+   before the first call (or hands in a state saved earlier). The calls below
+   change them in stream order, with no host synchronisation and no device
+   allocation, so decode steps with them can be captured into CUDA graphs.
+   Lists of sequences, counts and pages are device arrays too; what only the
+   device can see wrong in them (an index out of range or given twice, too few
+   free pages, a bad table entry) is left out and reported by kc_sync. `seqs`
+   NULL means sequences 0 .. n-1; n is at most n_seq. A context's calls share
+   one workspace: after kc_set_stream the caller orders the new stream behind
+   the old one.
+
+   kc_kv_cache registers a cache under an id >= 0 (t KC_F16 or KC_BF16; page 16,
+   32, 64, 128 or 256; head_dim a multiple of 8 up to 256).
+
+   kc_kv_fork_dev: sequence dst[i], which must be empty, becomes a copy of
+   src[i] by sharing its pages. An entry with an error is left out.
+   kc_kv_extend_dev: n_new[i] more positions for each sequence. New pages are
+   the lowest free ones, in the order of the call. A partly full last page that
+   others hold too is first copied (its rows, all layers), for its holders in
+   their order until one is left. All or nothing: KC_ERR_OOM (too few free
+   pages) or any other error leaves every sequence as it was.
+   kc_kv_write_dev: rows row_start[i] .. row_start[i+1]-1 of k and v (row
+   strides in elements, heads contiguous; type KC_F32 or the cache's) become
+   the last positions of sequence i in one layer; row_start NULL: one row each.
+   kc_kv_free_dev: forget positions from keep[i] on (NULL: all) and release the
+   pages that hold none of the kept ones.
+   kc_kv_compact_dev: live pages move to ids 0 .. live-1 (the i-th live page at
+   or past `live` to the i-th free one below it), tables and refs follow;
+   *n_live (optional, device) = live.
+   kc_kv_copy_pages_dev: the contents of page src[i] to page dst[i], all layers
+   (for hosts that keep their own tables). No page may be a destination twice,
+   or a destination and a source; then nothing is copied. */
+KC_API int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int page, int n_head_kv, int head_dim,
+                       int n_seq, int max_pages, void* k, void* v, int32_t* table, int32_t* len, int32_t* refs);
+KC_API int kc_kv_drop(kc_ctx* ctx, int cache);
+KC_API int kc_kv_fork_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n);
+KC_API int kc_kv_extend_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* n_new, int n);
+KC_API int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
+                           int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride);
+KC_API int kc_kv_free_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* keep, int n);
+KC_API int kc_kv_compact_dev(kc_ctx* ctx, int cache, int32_t* n_live);
+KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n);
+
+/* Attention over the cache. A query row at position i sees position j when
+   j <= i and (j > i - window or j < sinks); window 0: every j <= i. out =
+   sum p_j v_j / sum p_j with p_j = exp(scale q.k_j - max); zeros where nothing
+   is visible. What is not visible does not reach the result, whatever it holds
+   (stale rows of a page, NaN). q and out: rows of n_head * head_dim, the row
+   strides in elements; type t is the cache's, or KC_F32 over a KC_F16 cache;
+   n_head a multiple of n_head_kv (at most 128 query heads to one). Softmax and
+   sums are f32 for every type.
+   kc_attn_decode_dev: row i is the last position of sequence i.
+   kc_attn_prompt_dev: rows row_start[i] .. row_start[i+1]-1 are the last
+   positions of sequence i, in order (already extended and written); row_start
+   [n + 1] ascends within 0 .. n_rows. Rows in no sequence's range are not
+   written. */
+KC_API int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, int n_head, int t,
+                              const void* q, int64_t q_stride, float scale, int window, int sinks, void* out,
+                              int64_t out_stride);
+KC_API int kc_attn_prompt_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
+                              int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale, int window,
+                              int sinks, void* out, int64_t out_stride);
 
 /* ---- expert parallelism (one process per GPU, NCCL over NVLink) -------- */
 

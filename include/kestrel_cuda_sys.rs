@@ -35,9 +35,11 @@ pub const KC_ERR_OOM: c_int = 8;
 
 // ggml tensor types
 pub const KC_F32: c_int = 0;
+pub const KC_F16: c_int = 1;
 pub const KC_Q8_0: c_int = 8;
 pub const KC_Q4_K: c_int = 12;
 pub const KC_Q6_K: c_int = 14;
+pub const KC_BF16: c_int = 30;
 
 // expert cache policies
 pub const KC_EXPERT_POLICY_LFRU: c_int = 0;
@@ -195,6 +197,27 @@ unsafe extern "C" {
     pub fn kc_load_gguf(ctx: *mut kc_ctx, path: *const c_char, n_ctx: c_int, info_json: *mut c_char,
         cap: i64) -> c_int;
     pub fn kc_gguf_inspect(path: *const c_char, out: *mut c_char, cap: i64) -> c_int;
+    // paged key-value cache and its attention (device buffers)
+    pub fn kc_kv_cache(ctx: *mut kc_ctx, cache: c_int, t: c_int, n_layer: c_int, n_pages: c_int, page: c_int,
+        n_head_kv: c_int, head_dim: c_int, n_seq: c_int, max_pages: c_int, k: *mut c_void, v: *mut c_void,
+        table: *mut i32, len: *mut i32, refs: *mut i32) -> c_int;
+    pub fn kc_kv_drop(ctx: *mut kc_ctx, cache: c_int) -> c_int;
+    pub fn kc_kv_fork_dev(ctx: *mut kc_ctx, cache: c_int, src: *const i32, dst: *const i32, n: c_int) -> c_int;
+    pub fn kc_kv_extend_dev(ctx: *mut kc_ctx, cache: c_int, seqs: *const i32, n_new: *const i32,
+        n: c_int) -> c_int;
+    pub fn kc_kv_write_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32, row_start: *const i32,
+        n: c_int, n_rows: c_int, t: c_int, k: *const c_void, v: *const c_void, k_stride: i64,
+        v_stride: i64) -> c_int;
+    pub fn kc_kv_free_dev(ctx: *mut kc_ctx, cache: c_int, seqs: *const i32, keep: *const i32, n: c_int) -> c_int;
+    pub fn kc_kv_compact_dev(ctx: *mut kc_ctx, cache: c_int, n_live: *mut i32) -> c_int;
+    pub fn kc_kv_copy_pages_dev(ctx: *mut kc_ctx, cache: c_int, src: *const i32, dst: *const i32,
+        n: c_int) -> c_int;
+    pub fn kc_attn_decode_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32, n: c_int,
+        n_head: c_int, t: c_int, q: *const c_void, q_stride: i64, scale: f32, window: c_int, sinks: c_int,
+        out: *mut c_void, out_stride: i64) -> c_int;
+    pub fn kc_attn_prompt_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32,
+        row_start: *const i32, n: c_int, n_rows: c_int, n_head: c_int, t: c_int, q: *const c_void, q_stride: i64,
+        scale: f32, window: c_int, sinks: c_int, out: *mut c_void, out_stride: i64) -> c_int;
     // expert parallelism (one process per GPU)
     pub fn kc_ep_unique_id(out: *mut c_char) -> c_int; // out: 128 bytes
     pub fn kc_ep_init(ctx: *mut kc_ctx, rank: c_int, world: c_int, uid: *const c_char) -> c_int; // uid: 128 bytes

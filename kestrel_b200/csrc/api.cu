@@ -17,6 +17,7 @@
 #include "expert_cache.h"
 #include "ep.h"
 #include "kernels.h"
+#include "kv.h"
 #include "mma.h"
 #include "loader.h"
 #include "model.h"
@@ -217,6 +218,7 @@ struct kc_ctx {
   EpState ep;
   EpBufs epb;
   Prof prof;
+  KvState kv;  // registered paged caches (kc_kv_*)
 };
 
 namespace {
@@ -402,8 +404,20 @@ int check_status(kc_ctx* ctx) {
                                   "expert-parallel exchange (the ranks chose different paths, peer memory "
                                   "and NCCL, in one call: every rank must be on the same side of the "
                                   "kc_ep_reserve capacity)",
-                                  "tcgen05 producer (a slot tile larger than the launch's bound)"};
+                                  "tcgen05 producer (a slot tile larger than the launch's bound)",
+                                  "paged cache: a sequence index out of range or given twice",
+                                  "paged cache: fork into a sequence that holds positions, is given twice or is a "
+                                  "source of the call",
+                                  "paged cache: not enough free pages (nothing was extended)",
+                                  "paged cache: more positions than a table row holds (nothing was extended)",
+                                  "paged cache: a table entry outside the pool",
+                                  "paged cache: a negative count, rows that do not ascend, or more rows than "
+                                  "positions",
+                                  "paged cache: a page to copy out of range, a destination given twice or also a "
+                                  "source (nothing was copied)"};
     const int site = st >> 8;
+    if (site >= W_KV_SEQ && site < (int)(sizeof(sites) / sizeof(sites[0])))
+      return fail(ctx, st & 0xFF, "%s", sites[site]);
     return fail(ctx, st & 0xFF, "a kernel's bounded wait expired (status %d) at: %s", st & 0xFF,
                 site >= 0 && site < (int)(sizeof(sites) / sizeof(sites[0])) ? sites[site] : "unknown");
   }
@@ -1885,6 +1899,7 @@ void kc_free(kc_ctx* ctx) {
     cudaEventDestroy(r.b);
   }
   for (auto e : ctx->prof.pool) cudaEventDestroy(e);
+  for (auto& [id, C] : ctx->kv.caches) cudaFree(C.work);
   cudaFree(ctx->ws.arena);
   cudaFree(ctx->ws_ep.arena);
   cudaFree(ctx->status);
@@ -1937,7 +1952,9 @@ int kc_sync(kc_ctx* ctx) {
 int64_t kc_device_bytes(const kc_ctx* ctx) {
   if (!ctx) return 0;
   const int64_t slots = ctx->xs.arena ? (int64_t)ctx->xs.cache.slots() * ctx->xs.slot_bytes : 0;
-  return ctx->weight_bytes + (int64_t)ctx->ws.bytes + (int64_t)ctx->ws_ep.bytes + slots;
+  int64_t kv = 0;
+  for (const auto& [id, C] : ctx->kv.caches) kv += C.work_bytes;
+  return ctx->weight_bytes + (int64_t)ctx->ws.bytes + (int64_t)ctx->ws_ep.bytes + slots + kv;
 }
 
 int kc_upload_experts_range(kc_ctx* ctx, int layer, int n_expert, int first_expert, int n_local, int d, int ff,
@@ -2981,6 +2998,233 @@ int kc_load_gguf(kc_ctx* ctx, const char* path, int n_ctx, char* info_json, int6
     return rc;
   }
   return KC_OK;
+}
+
+// ---- paged key-value cache and its attention ---------------------------------
+}  // extern "C"
+
+namespace {
+
+// Calls fn with the context's device current; what C++ throws (the registry's
+// allocations) becomes a status.
+template <class Fn>
+int kv_guard(kc_ctx* ctx, const char* what, Fn&& fn) {
+  if (!ctx) return KC_ERR_ARG;
+  try {
+    ctx->err.clear();
+    cudaSetDevice(ctx->device);
+    return fn();
+  } catch (...) {
+    return fail(ctx, KC_ERR_OOM, "%s: out of host memory", what);
+  }
+}
+
+// fn(view) on a registered cache, then the launch check.
+template <class Fn>
+int kv_call(kc_ctx* ctx, int cache, const char* what, Fn&& fn) {
+  return kv_guard(ctx, what, [&]() -> int {
+    const auto it = ctx->kv.caches.find(cache);
+    if (it == ctx->kv.caches.end()) return fail(ctx, KC_ERR_STATE, "%s: cache %d not registered", what, cache);
+    RC(fn(it->second.view));
+    CKL();
+    return KC_OK;
+  });
+}
+
+int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t* seqs, const int32_t* row_start,
+              bool prompt, int n, int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale,
+              int window, int sinks, void* out, int64_t out_stride) {
+  return kv_call(ctx, cache, what, [&](const KvView& c) -> int {
+    if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "%s: layer %d of %d", what, layer, c.n_layer);
+    if (n < 0 || n > c.n_seq || n_rows < 0 || window < 0 || sinks < 0)
+      return fail(ctx, KC_ERR_ARG, "%s: n=%d (of %d sequences), n_rows=%d, window=%d, sinks=%d", what, n, c.n_seq,
+                  n_rows, window, sinks);
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(ctx, KC_ERR_ARG, "%s: scale is not finite", what);
+    if (n == 0 || n_rows == 0) return KC_OK;
+    if (!q || !out || (prompt && !row_start)) return fail(ctx, KC_ERR_ARG, "%s: null buffer", what);
+    if (n_head <= 0 || n_head % c.nkv || n_head / c.nkv > 128)
+      return fail(ctx, KC_ERR_SHAPE, "%s: %d query heads over %d key-value heads (1 to 128 each)", what, n_head,
+                  c.nkv);
+    if ((int64_t)n_rows * (n_head / c.nkv) > INT32_MAX / 2)
+      return fail(ctx, KC_ERR_SHAPE, "%s: %d rows of %d heads", what, n_rows, n_head);
+    if (t != c.type && !(t == T_F32 && c.type == T_F16))
+      return fail(ctx, KC_ERR_TYPE, "%s: queries of type %d over a cache of type %d (the cache's type, or F32 over F16)",
+                  what, t, c.type);
+    const int64_t row = (int64_t)n_head * c.hd;
+    if (q_stride < row || out_stride < row)
+      return fail(ctx, KC_ERR_SHAPE, "%s: row strides %lld / %lld below n_head * head_dim", what,
+                  (long long)q_stride, (long long)out_stride);
+    const size_t el = t == T_F32 ? 4 : 2;
+    if ((uintptr_t)q % el || (uintptr_t)out % el) return fail(ctx, KC_ERR_ARG, "%s: misaligned buffer", what);
+    AttnArgs a{};
+    a.c = c;
+    a.layer = layer;
+    a.seqs = seqs;
+    a.row_start = row_start;
+    a.n = n;
+    a.n_rows = n_rows;
+    a.nh = n_head;
+    a.t_q = t;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.scale = scale;
+    a.window = window;
+    a.sinks = window > 0 ? sinks : 0;
+    const int rc = launch_attention_paged(a, ctx->stream);
+    return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);
+  });
+}
+
+}  // namespace
+
+extern "C" {
+
+int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int page, int n_head_kv, int head_dim,
+                int n_seq, int max_pages, void* k, void* v, int32_t* table, int32_t* len, int32_t* refs) {
+  return kv_guard(ctx, "kc_kv_cache", [&]() -> int {
+    if (cache < 0) return fail(ctx, KC_ERR_ARG, "kc_kv_cache: cache id %d", cache);
+    if (!k || !v || !table || !len || !refs) return fail(ctx, KC_ERR_ARG, "kc_kv_cache: null buffer");
+    if (t != T_F16 && t != T_BF16) return fail(ctx, KC_ERR_TYPE, "kc_kv_cache: type %d (F16 or BF16)", t);
+    if (n_layer < 1 || n_pages < 1 || n_head_kv < 1 || n_seq < 1 || max_pages < 1)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: %d layers, %d pages, %d heads, %d sequences of %d pages", n_layer,
+                  n_pages, n_head_kv, n_seq, max_pages);
+    if (page < 16 || page > 256 || (page & (page - 1)))
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: page of %d positions (16, 32, 64, 128 or 256)", page);
+    if (head_dim < 8 || head_dim > 256 || head_dim % 8)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: head_dim %d (a multiple of 8 up to 256)", head_dim);
+    if ((int64_t)max_pages * page > INT32_MAX || (int64_t)n_seq * max_pages > INT32_MAX ||
+        (int64_t)n_layer * n_pages > INT32_MAX || n_head_kv > 4096)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: sizes past 32 bits (max_pages * page, n_seq * max_pages or "
+                                     "n_layer * n_pages)");
+    if (((uintptr_t)k | (uintptr_t)v) & 15) return fail(ctx, KC_ERR_ARG, "kc_kv_cache: k and v must be 16-byte aligned");
+    if (((uintptr_t)table | (uintptr_t)len | (uintptr_t)refs) & 3)
+      return fail(ctx, KC_ERR_ARG, "kc_kv_cache: misaligned table, len or refs");
+    KvCache C{};
+    KvView& w = C.view;
+    w.k = static_cast<uint8_t*>(k);
+    w.v = static_cast<uint8_t*>(v);
+    w.table = table;
+    w.len = len;
+    w.refs = refs;
+    w.type = t;
+    w.n_layer = n_layer;
+    w.n_pages = n_pages;
+    w.page = page;
+    while ((1 << w.page_log2) < page) ++w.page_log2;
+    w.nkv = n_head_kv;
+    w.hd = head_dim;
+    w.n_seq = n_seq;
+    w.max_pages = max_pages;
+    w.status = ctx->status;
+    C.work_bytes = kv_workspace_ints(w) * (int64_t)sizeof(int);
+    KvCache& slot = ctx->kv.caches[cache];  // an id registered before is replaced
+    if (slot.work) {
+      CK(cudaStreamSynchronize(ctx->stream));
+      cudaFree(slot.work);
+    }
+    slot = KvCache{};
+    cudaError_t e = cudaMalloc(&C.work, C.work_bytes);
+    if (e == cudaSuccess) e = kv_workspace_init(w, C.work, ctx->stream);
+    if (e != cudaSuccess) {
+      cudaFree(C.work);
+      ctx->kv.caches.erase(cache);
+      cudaGetLastError();
+      return fail(ctx, e == cudaErrorMemoryAllocation ? KC_ERR_OOM : KC_ERR_CUDA, "kc_kv_cache: workspace: %s",
+                  cudaGetErrorString(e));
+    }
+    slot = C;
+    return KC_OK;
+  });
+}
+
+int kc_kv_drop(kc_ctx* ctx, int cache) {
+  return kv_guard(ctx, "kc_kv_drop", [&]() -> int {
+    const auto it = ctx->kv.caches.find(cache);
+    if (it == ctx->kv.caches.end()) return fail(ctx, KC_ERR_STATE, "kc_kv_drop: cache %d not registered", cache);
+    CK(cudaStreamSynchronize(ctx->stream));
+    cudaFree(it->second.work);
+    ctx->kv.caches.erase(it);
+    return KC_OK;
+  });
+}
+
+int kc_kv_fork_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n) {
+  return kv_call(ctx, cache, "kc_kv_fork", [&](const KvView& c) -> int {
+    if (n < 0 || n > c.n_seq || (n > 0 && (!src || !dst)))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_fork: n=%d (of %d sequences) or null buffer", n, c.n_seq);
+    if (n) launch_kv_fork(c, src, dst, n, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_kv_extend_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* n_new, int n) {
+  return kv_call(ctx, cache, "kc_kv_extend", [&](const KvView& c) -> int {
+    if (n < 0 || n > c.n_seq || (n > 0 && !n_new))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_extend: n=%d (of %d sequences) or null buffer", n, c.n_seq);
+    if (n) launch_kv_extend(c, seqs, n_new, n, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
+                    int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride) {
+  return kv_call(ctx, cache, "kc_kv_write", [&](const KvView& c) -> int {
+    if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "kc_kv_write: layer %d of %d", layer, c.n_layer);
+    if (n < 0 || n > c.n_seq || n_rows < 0 || (!row_start && n_rows != n))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_write: n=%d (of %d sequences), n_rows=%d", n, c.n_seq, n_rows);
+    if (t != T_F32 && t != c.type)
+      return fail(ctx, KC_ERR_TYPE, "kc_kv_write: rows of type %d into a cache of type %d (its type or F32)", t, c.type);
+    if (n == 0 || n_rows == 0) return KC_OK;
+    if (!k || !v) return fail(ctx, KC_ERR_ARG, "kc_kv_write: null buffer");
+    const int64_t row = (int64_t)c.nkv * c.hd;
+    if (k_stride < row || v_stride < row)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_write: row strides %lld / %lld below n_head_kv * head_dim",
+                  (long long)k_stride, (long long)v_stride);
+    const size_t el = t == T_F32 ? 4 : 2;
+    if ((uintptr_t)k % el || (uintptr_t)v % el) return fail(ctx, KC_ERR_ARG, "kc_kv_write: misaligned buffer");
+    launch_kv_write(c, layer, seqs, row_start, n, n_rows, t, k, v, k_stride, v_stride, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_kv_free_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* keep, int n) {
+  return kv_call(ctx, cache, "kc_kv_free", [&](const KvView& c) -> int {
+    if (n < 0 || n > c.n_seq) return fail(ctx, KC_ERR_ARG, "kc_kv_free: n=%d (of %d sequences)", n, c.n_seq);
+    if (n) launch_kv_free(c, seqs, keep, n, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_kv_compact_dev(kc_ctx* ctx, int cache, int32_t* n_live) {
+  return kv_call(ctx, cache, "kc_kv_compact", [&](const KvView& c) -> int {
+    launch_kv_compact(c, n_live, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n) {
+  return kv_call(ctx, cache, "kc_kv_copy_pages", [&](const KvView& c) -> int {
+    if (n < 0 || n > c.n_pages || (n > 0 && (!src || !dst)))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_copy_pages: n=%d (of %d pages) or null buffer", n, c.n_pages);
+    if (n) launch_kv_copy_pages(c, src, dst, n, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, int n_head, int t,
+                       const void* q, int64_t q_stride, float scale, int window, int sinks, void* out,
+                       int64_t out_stride) {
+  return attn_call(ctx, cache, "kc_attn_decode", layer, seqs, nullptr, false, n, n, n_head, t, q, q_stride, scale,
+                   window, sinks, out, out_stride);
+}
+
+int kc_attn_prompt_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
+                       int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale, int window,
+                       int sinks, void* out, int64_t out_stride) {
+  return attn_call(ctx, cache, "kc_attn_prompt", layer, seqs, row_start, true, n, n_rows, n_head, t, q, q_stride,
+                   scale, window, sinks, out, out_stride);
 }
 
 }  // extern "C"

@@ -74,6 +74,16 @@ SIGNATURES = {
     "kc_expert_prefetch": (I, [P, I, P, I]),
     "kc_expert_cache_stats": (I, [P, P, I]),
     "kc_expert_cache_decay": (I, [P]),
+    "kc_kv_cache": (I, [P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]),
+    "kc_kv_drop": (I, [P, I]),
+    "kc_kv_fork_dev": (I, [P, I, P, P, I]),
+    "kc_kv_extend_dev": (I, [P, I, P, P, I]),
+    "kc_kv_write_dev": (I, [P, I, I, P, P, I, I, I, P, P, I64, I64]),
+    "kc_kv_free_dev": (I, [P, I, P, P, I]),
+    "kc_kv_compact_dev": (I, [P, I, P]),
+    "kc_kv_copy_pages_dev": (I, [P, I, P, P, I]),
+    "kc_attn_decode_dev": (I, [P, I, I, P, I, I, I, P, I64, F, I, I, P, I64]),
+    "kc_attn_prompt_dev": (I, [P, I, I, P, P, I, I, I, I, P, I64, F, I, I, P, I64]),
 }
 
 # Options (kc_set_option) and whole-model tensor kinds (kc_model_tensor).
@@ -142,6 +152,39 @@ def _host_u8(a):
     return np.ascontiguousarray(a, dtype=np.uint8).reshape(-1) if isinstance(a, np.ndarray) else a
 
 
+# ggml ids of the element types the paged cache takes, by torch's name.
+_FLOAT_TYPES = {"torch.float32": G.F32, "torch.float16": G.F16, "torch.bfloat16": G.BF16}
+
+
+def _float_type(name: str, a) -> int:
+    t = _FLOAT_TYPES.get(str(a.dtype))
+    if t is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, not {a.dtype}")
+    return t
+
+
+def _dev_ints(name: str, a, size: int | None = None):
+    """A contiguous int32 CUDA tensor of `size` values (None: any)."""
+    if a is None:
+        return None
+    if not _is_dev(a) or str(a.dtype) != "torch.int32" or not a.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
+    if size is not None and a.numel() != size:
+        raise ValueError(f"{name} holds {a.numel()} values, {size} needed")
+    return a.data_ptr()
+
+
+def _dev_rows(name: str, a, heads: int | None = None, head_dim: int | None = None):
+    """Row stride (elements) of a CUDA tensor [rows, heads, head_dim] whose
+    heads are contiguous within a row."""
+    if not _is_dev(a) or a.dim() != 3 or (heads is not None and a.shape[1] != heads) or \
+            (head_dim is not None and a.shape[2] != head_dim):
+        raise ValueError(f"{name} must be a CUDA tensor [rows, heads, head_dim]")
+    if (a.shape[2] > 1 and a.stride(2) != 1) or (a.shape[1] > 1 and a.stride(1) != a.shape[2]):
+        raise ValueError(f"the heads of a row of {name} must be contiguous")
+    return a.stride(0) if a.shape[0] > 1 else a.shape[1] * a.shape[2]
+
+
 class Context:
     """One GPU's backend context (kc_ctx)."""
 
@@ -154,6 +197,7 @@ class Context:
         self.device = device
         self._k = {}           # layer -> top-k of its uploaded router
         self._dense_rows = {}  # tensor id -> rows
+        self._kv = {}          # cache id -> its tensors (kept alive while registered)
 
     def close(self):
         if getattr(self, "h", None):
@@ -410,6 +454,102 @@ class Context:
         self._check(rc)
         self._n_vocab = int(info.get("n_vocab", getattr(self, "_n_vocab", 0)))
         return info
+
+    # ---- paged key-value cache (torch CUDA tensors) ------------------------------
+    def kv_cache(self, cache: int, k, v, table, length, refs):
+        """Register the caller's tensors as paged cache `cache`: k and v
+        [n_layer, n_pages, n_kv, page, head_dim], table [n_seq, max_pages],
+        length [n_seq] and refs [n_pages] int32 (an empty cache: -1, 0, 0).
+        They stay the caller's; the calls below change them in stream order."""
+        if not _is_dev(k) or not _is_dev(v) or k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype \
+                or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("k and v must be contiguous CUDA tensors [n_layer, n_pages, n_kv, page, head_dim] of "
+                             "one type")
+        n_layer, n_pages, n_kv, page, hd = k.shape
+        if table.dim() != 2:
+            raise ValueError("table must be [n_seq, max_pages]")
+        n_seq, max_pages = table.shape
+        t = _dev_ints("table", table), _dev_ints("length", length, n_seq), _dev_ints("refs", refs, n_pages)
+        self._check(lib().kc_kv_cache(self.h, cache, _float_type("k", k), n_layer, n_pages, page, n_kv, hd, n_seq,
+                                      max_pages, k.data_ptr(), v.data_ptr(), *t))
+        self._kv[cache] = (k, v, table, length, refs)
+
+    def kv_drop(self, cache: int):
+        self._check(lib().kc_kv_drop(self.h, cache))
+        self._kv.pop(cache, None)
+
+    def _kv_shape(self, cache: int):
+        """(n_seq, n_kv, head_dim) of a registered cache."""
+        if cache not in self._kv:
+            raise ValueError(f"paged cache {cache} is not registered through this Context")
+        k, _, table, _, _ = self._kv[cache]
+        return table.shape[0], k.shape[2], k.shape[4]
+
+    def kv_fork_dev(self, cache: int, src, dst):
+        """Sequences dst (int32 CUDA tensor, empty ones) share the pages of src."""
+        n = src.numel()
+        self._check(lib().kc_kv_fork_dev(self.h, cache, _dev_ints("src", src), _dev_ints("dst", dst, n), n))
+
+    def kv_extend_dev(self, cache: int, seqs, n_new):
+        """n_new more positions for each of `seqs` (None: sequences 0, 1, ...)."""
+        n = n_new.numel()
+        self._check(lib().kc_kv_extend_dev(self.h, cache, _dev_ints("seqs", seqs, n), _dev_ints("n_new", n_new), n))
+
+    def kv_write_dev(self, cache: int, layer: int, k, v, seqs=None, row_start=None):
+        """Rows k, v [rows, n_kv, head_dim] become the last positions of their
+        sequences: one row each, or rows row_start[i] .. row_start[i+1]-1."""
+        _, n_kv, hd = self._kv_shape(cache)
+        ks, vs = _dev_rows("k", k, n_kv, hd), _dev_rows("v", v, n_kv, hd)
+        rows = k.shape[0]
+        if v.shape[0] != rows or v.dtype != k.dtype:
+            raise ValueError("k and v differ in rows or type")
+        n = rows if row_start is None else row_start.numel() - 1
+        self._check(lib().kc_kv_write_dev(self.h, cache, layer, _dev_ints("seqs", seqs, n),
+                                          _dev_ints("row_start", row_start), n, rows, _float_type("k", k),
+                                          k.data_ptr(), v.data_ptr(), ks, vs))
+
+    def kv_free_dev(self, cache: int, seqs=None, keep=None):
+        """Forget positions keep[i] and on (None: all) of each of `seqs` (None:
+        every sequence, or the first len(keep))."""
+        n = seqs.numel() if seqs is not None else keep.numel() if keep is not None else self._kv_shape(cache)[0]
+        self._check(lib().kc_kv_free_dev(self.h, cache, _dev_ints("seqs", seqs), _dev_ints("keep", keep, n), n))
+
+    def kv_compact_dev(self, cache: int, n_live=None):
+        """Move the live pages to the front of the pool; n_live (int32 [1],
+        optional) gets their number."""
+        self._check(lib().kc_kv_compact_dev(self.h, cache, _dev_ints("n_live", n_live, 1)))
+
+    def kv_copy_pages_dev(self, cache: int, src, dst):
+        n = src.numel()
+        self._check(lib().kc_kv_copy_pages_dev(self.h, cache, _dev_ints("src", src), _dev_ints("dst", dst, n), n))
+
+    def _attn(self, cache, q, out):
+        _, n_kv, hd = self._kv_shape(cache)
+        qs, os_ = _dev_rows("q", q, None, hd), _dev_rows("out", out, q.shape[1], hd)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and type")
+        return q.shape[0], q.shape[1], hd, qs, os_
+
+    def attn_decode_dev(self, cache: int, layer: int, q, out, seqs=None, scale: float | None = None,
+                        window: int = 0, sinks: int = 0):
+        """Row i of q [n, n_head, head_dim] attends from the last position of
+        sequence seqs[i]; scale None: head_dim ** -0.5."""
+        n, nh, hd, qs, os_ = self._attn(cache, q, out)
+        self._check(lib().kc_attn_decode_dev(self.h, cache, layer, _dev_ints("seqs", seqs, n), n, nh,
+                                             _float_type("q", q), q.data_ptr(), qs,
+                                             hd ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                             os_))
+
+    def attn_prompt_dev(self, cache: int, layer: int, q, row_start, out, seqs=None, scale: float | None = None,
+                        window: int = 0, sinks: int = 0):
+        """Rows row_start[i] .. row_start[i+1]-1 of q attend from the last
+        positions of sequence seqs[i], causally."""
+        rows, nh, hd, qs, os_ = self._attn(cache, q, out)
+        n = row_start.numel() - 1
+        self._check(lib().kc_attn_prompt_dev(self.h, cache, layer, _dev_ints("seqs", seqs, n),
+                                             _dev_ints("row_start", row_start), n, rows, nh, _float_type("q", q),
+                                             q.data_ptr(), qs, hd ** -0.5 if scale is None else scale, window, sinks,
+                                             out.data_ptr(), os_))
 
     def ep_reserve(self, max_tokens: int):
         """Collective: map the peer exchange arenas for up to max_tokens tokens
