@@ -414,9 +414,10 @@ int check_status(kc_ctx* ctx) {
                                   "paged cache: a negative count, rows that do not ascend, or more rows than "
                                   "positions",
                                   "paged cache: a page to copy out of range, a destination given twice or also a "
-                                  "source (nothing was copied)"};
+                                  "source (nothing was copied)",
+                                  "paged attention (a chunk of the cache)"};
     const int site = st >> 8;
-    if (site >= W_KV_SEQ && site < (int)(sizeof(sites) / sizeof(sites[0])))
+    if (site >= W_KV_SEQ && site <= W_KV_COPY)
       return fail(ctx, st & 0xFF, "%s", sites[site]);
     return fail(ctx, st & 0xFF, "a kernel's bounded wait expired (status %d) at: %s", st & 0xFF,
                 site >= 0 && site < (int)(sizeof(sites) / sizeof(sites[0])) ? sites[site] : "unknown");
@@ -1900,6 +1901,7 @@ void kc_free(kc_ctx* ctx) {
   }
   for (auto e : ctx->prof.pool) cudaEventDestroy(e);
   for (auto& [id, C] : ctx->kv.caches) cudaFree(C.work);
+  cudaFree(ctx->kv.part);
   cudaFree(ctx->ws.arena);
   cudaFree(ctx->ws_ep.arena);
   cudaFree(ctx->status);
@@ -1952,7 +1954,7 @@ int kc_sync(kc_ctx* ctx) {
 int64_t kc_device_bytes(const kc_ctx* ctx) {
   if (!ctx) return 0;
   const int64_t slots = ctx->xs.arena ? (int64_t)ctx->xs.cache.slots() * ctx->xs.slot_bytes : 0;
-  int64_t kv = 0;
+  int64_t kv = ctx->kv.bytes;
   for (const auto& [id, C] : ctx->kv.caches) kv += C.work_bytes;
   return ctx->weight_bytes + (int64_t)ctx->ws.bytes + (int64_t)ctx->ws_ep.bytes + slots + kv;
 }
@@ -3025,7 +3027,7 @@ int kv_call(kc_ctx* ctx, int cache, const char* what, Fn&& fn) {
   return kv_guard(ctx, what, [&]() -> int {
     const auto it = ctx->kv.caches.find(cache);
     if (it == ctx->kv.caches.end()) return fail(ctx, KC_ERR_STATE, "%s: cache %d not registered", what, cache);
-    RC(fn(it->second.view));
+    RC(fn(it->second));
     CKL();
     return KC_OK;
   });
@@ -3034,7 +3036,8 @@ int kv_call(kc_ctx* ctx, int cache, const char* what, Fn&& fn) {
 int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t* seqs, const int32_t* row_start,
               bool prompt, int n, int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale,
               int window, int sinks, void* out, int64_t out_stride) {
-  return kv_call(ctx, cache, what, [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, what, [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "%s: layer %d of %d", what, layer, c.n_layer);
     if (n < 0 || n > c.n_seq || n_rows < 0 || window < 0 || sinks < 0)
       return fail(ctx, KC_ERR_ARG, "%s: n=%d (of %d sequences), n_rows=%d, window=%d, sinks=%d", what, n, c.n_seq,
@@ -3072,7 +3075,8 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     a.scale = scale;
     a.window = window;
     a.sinks = window > 0 ? sinks : 0;
-    const int rc = launch_attention_paged(a, ctx->stream);
+    const int rc = prompt ? launch_attn_prompt(a, ctx->stream)
+                          : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
     return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);
   });
 }
@@ -3119,6 +3123,17 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
     w.max_pages = max_pages;
     w.status = ctx->status;
     C.work_bytes = kv_workspace_ints(w) * (int64_t)sizeof(int);
+    if (make_kv_maps(w, 16, C.rows16) != KC_OK)
+      return fail(ctx, KC_ERR_CUDA, "kc_kv_cache: cuTensorMapEncodeTiled refused the pools");
+    if (!ctx->kv.part) {
+      const size_t cnt = (size_t)num_sms() * sizeof(int), all = attn_decode_part_bytes() + cnt;
+      void* p = nullptr;
+      CK(cudaMalloc(&p, all));
+      ctx->kv.part = static_cast<float*>(p);
+      ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + attn_decode_part_bytes());
+      ctx->kv.bytes = (int64_t)all;
+      CK(cudaMemsetAsync(ctx->kv.count, 0, cnt, ctx->stream));
+    }
     KvCache& slot = ctx->kv.caches[cache];  // an id registered before is replaced
     if (slot.work) {
       CK(cudaStreamSynchronize(ctx->stream));
@@ -3151,7 +3166,8 @@ int kc_kv_drop(kc_ctx* ctx, int cache) {
 }
 
 int kc_kv_fork_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n) {
-  return kv_call(ctx, cache, "kc_kv_fork", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_fork", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (n < 0 || n > c.n_seq || (n > 0 && (!src || !dst)))
       return fail(ctx, KC_ERR_ARG, "kc_kv_fork: n=%d (of %d sequences) or null buffer", n, c.n_seq);
     if (n) launch_kv_fork(c, src, dst, n, ctx->stream);
@@ -3160,7 +3176,8 @@ int kc_kv_fork_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* ds
 }
 
 int kc_kv_extend_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* n_new, int n) {
-  return kv_call(ctx, cache, "kc_kv_extend", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_extend", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (n < 0 || n > c.n_seq || (n > 0 && !n_new))
       return fail(ctx, KC_ERR_ARG, "kc_kv_extend: n=%d (of %d sequences) or null buffer", n, c.n_seq);
     if (n) launch_kv_extend(c, seqs, n_new, n, ctx->stream);
@@ -3170,7 +3187,8 @@ int kc_kv_extend_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t*
 
 int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
                     int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride) {
-  return kv_call(ctx, cache, "kc_kv_write", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_write", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "kc_kv_write: layer %d of %d", layer, c.n_layer);
     if (n < 0 || n > c.n_seq || n_rows < 0 || (!row_start && n_rows != n))
       return fail(ctx, KC_ERR_ARG, "kc_kv_write: n=%d (of %d sequences), n_rows=%d", n, c.n_seq, n_rows);
@@ -3190,7 +3208,8 @@ int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, cons
 }
 
 int kc_kv_free_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* keep, int n) {
-  return kv_call(ctx, cache, "kc_kv_free", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_free", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (n < 0 || n > c.n_seq) return fail(ctx, KC_ERR_ARG, "kc_kv_free: n=%d (of %d sequences)", n, c.n_seq);
     if (n) launch_kv_free(c, seqs, keep, n, ctx->stream);
     return KC_OK;
@@ -3198,14 +3217,16 @@ int kc_kv_free_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* k
 }
 
 int kc_kv_compact_dev(kc_ctx* ctx, int cache, int32_t* n_live) {
-  return kv_call(ctx, cache, "kc_kv_compact", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_compact", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     launch_kv_compact(c, n_live, ctx->stream);
     return KC_OK;
   });
 }
 
 int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n) {
-  return kv_call(ctx, cache, "kc_kv_copy_pages", [&](const KvView& c) -> int {
+  return kv_call(ctx, cache, "kc_kv_copy_pages", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
     if (n < 0 || n > c.n_pages || (n > 0 && (!src || !dst)))
       return fail(ctx, KC_ERR_ARG, "kc_kv_copy_pages: n=%d (of %d pages) or null buffer", n, c.n_pages);
     if (n) launch_kv_copy_pages(c, src, dst, n, ctx->stream);

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(AT_THREADS) attn_tile_kernel(AttnArgs a) {
   __shared__ int page_of[AT_KEYS];
   // The block's sequence and its first row within it.
   int i = -1, row0 = 0, start = 0, count = 0;
-  if (a.row_start) {
+  {
     int t = blockIdx.x;
     for (int e = 0; e < a.n; ++e) {
       const int lo = a.row_start[e], hi = a.row_start[e + 1];
@@ -51,11 +51,6 @@ __global__ void __launch_bounds__(AT_THREADS) attn_tile_kernel(AttnArgs a) {
       t -= tiles;
     }
     if (i < 0) return;
-  } else {
-    const int tiles = (group + AT_ROWS - 1) / AT_ROWS;
-    i = start = blockIdx.x / tiles;
-    row0 = (blockIdx.x % tiles) * AT_ROWS;
-    count = 1;
   }
   const int s = a.seqs ? a.seqs[i] : i;
   if (s < 0 || s >= c.n_seq) {
@@ -143,8 +138,7 @@ __global__ void __launch_bounds__(AT_THREADS) attn_tile_kernel(AttnArgs a) {
 template <typename TQ, typename TKV>
 static int launch_tile(const AttnArgs& a, cudaStream_t st) {
   const int group = a.nh / a.c.nkv;
-  const int64_t blocks = a.row_start ? ((int64_t)a.n_rows * group + AT_ROWS - 1) / AT_ROWS + a.n
-                                     : (int64_t)a.n * ((group + AT_ROWS - 1) / AT_ROWS);
+  const int64_t blocks = ((int64_t)a.n_rows * group + AT_ROWS - 1) / AT_ROWS + a.n;
   static PerDeviceOnce attr;
   const size_t smem = (size_t)(AT_ROWS + 2 * AT_KEYS) * (a.c.hd + 1) * 4;
   if (smem_attr_once(attr, attn_tile_kernel<TQ, TKV>, (AT_ROWS + 2 * AT_KEYS) * (AT_HD + 1) * 4) != cudaSuccess)
@@ -153,7 +147,7 @@ static int launch_tile(const AttnArgs& a, cudaStream_t st) {
   return KC_OK;
 }
 
-int launch_attention_paged(const AttnArgs& a, cudaStream_t st) {
+int launch_attn_prompt(const AttnArgs& a, cudaStream_t st) {
   if (a.c.type == T_BF16) return launch_tile<__nv_bfloat16, __nv_bfloat16>(a, st);
   if (a.t_q == T_F32) return launch_tile<float, __half>(a, st);
   return launch_tile<__half, __half>(a, st);

@@ -1,0 +1,593 @@
+// Attention of one new token per sequence over the paged key-value cache,
+// split over the cache's length and joined (formulas: attn.cu).
+//
+// A decode step reads every visible key and value once and computes 4 flops a
+// byte and query head: it is bound by the memory rate, and what matters is that
+// all SMs read all the time, however unequal the sequences are. So the work is
+// one line of 16-position chunks, sequence after sequence and head after head,
+// cut into equal ranges for one block per SM; a range may begin and end inside
+// a sequence. Each warp runs its own ring of chunks (TMA boxes of one page's
+// rows, 128-byte swizzle, 192 KB in flight per SM) and its own softmax state, so
+// warps meet only where a sequence ends. The parts of a sequence that several
+// blocks hold go to a workspace; the block that finishes last joins them in
+// block order, so the sums do not depend on timing.
+//
+// The eight heads of a group share each chunk as the rows of one m16n8k16
+// product. f32 queries and the f32 weights are each carried by two 16-bit rows
+// (value and rest, 22 bits for f16), which fill the product's other eight rows
+// at no cost: results are f32-grade although the cache is 16-bit. Groups of
+// more than eight heads with 16-bit queries use all sixteen rows for heads.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_dev.cuh"
+#include "common.cuh"
+#include "kernels.h"
+#include "kv.h"
+#include "kv_dev.cuh"
+
+namespace kc {
+
+constexpr int DC = 16;  // positions per chunk: the smallest page
+
+template <int NB, int HT>
+struct DecShape {
+  static constexpr int HD = 64 * NB;                           // padded head size
+  static constexpr int W = NB <= 2 ? 8 : 4;                    // warps
+  static constexpr int CHUNK = 2 * NB * DC * 128;              // K and V of one chunk
+  static constexpr int ST = 196608 / (W * CHUNK);              // ring stages per warp
+  static constexpr int LD = HD + 2;                            // a head's partial: values, maximum, sum
+  static constexpr int MERGE = W / 2 * HT * LD * 4;            // partials of half the warps
+  static constexpr int SMEM = W * ST * CHUNK + MERGE + 1024;
+};
+
+struct DecArgs {
+  AttnArgs a;
+  float* part;  // [grid][2][HT][LD]
+  int* count;   // [grid], zero between launches
+};
+
+// Chunks of the visible positions of a sequence of `len` positions as seen from
+// its last one: `head` chunks of the first tokens, then chunks w0 .. w1-1.
+struct Span {
+  int head, w0, n, lo;
+};
+__device__ __forceinline__ Span dec_span(int len, int window, int sinks) {
+  Span s;
+  s.lo = window > 0 ? max(0, len - window) : 0;
+  s.head = (min(sinks, s.lo) + DC - 1) / DC;
+  s.w0 = max(s.lo / DC, s.head);
+  s.n = len > 0 ? s.head + (len + DC - 1) / DC - s.w0 : 0;
+  return s;
+}
+
+// A block's range of the line, segment by segment (one segment: consecutive
+// chunks of one unit, a unit being a sequence's key-value head and head tile).
+struct SegIter {
+  long long pos, end, base;  // base: line position of sequence i's first unit
+  int i, pad;                // pad: chunks each unit takes of the line (0: as many as it has)
+  int s, len;
+  Span span;
+  // the segment
+  int unit, c0, c1, n_unit;
+  long long unit_at;  // line position of the unit's first chunk
+};
+
+__device__ __forceinline__ void seg_sequence(SegIter& t, const AttnArgs& a) {
+  t.s = a.seqs ? a.seqs[t.i] : t.i;
+  t.len = t.s >= 0 && t.s < a.c.n_seq ? kv_len(a.c, t.s) : 0;
+  t.span = dec_span(t.len, a.window, a.sinks);
+}
+__device__ __forceinline__ bool seg_next(SegIter& t, const AttnArgs& a, int units) {
+  while (t.pos < t.end) {
+    const int np = t.pad ? t.pad : t.span.n;
+    const long long off = t.pos - t.base;
+    if (off >= (long long)np * units) {
+      t.base += (long long)np * units;
+      if (++t.i >= a.n) return false;
+      seg_sequence(t, a);
+      continue;
+    }
+    t.unit = (int)(off / np);
+    t.c0 = (int)(off - (long long)t.unit * np);
+    const int take = (int)min(t.end - t.pos, (long long)(np - t.c0));
+    t.unit_at = t.pos - t.c0;
+    t.c1 = min(t.c0 + take, t.span.n);
+    t.n_unit = t.span.n;
+    t.pos += take;
+    if (t.c0 < t.c1) return true;
+  }
+  return false;
+}
+
+template <typename TQ, typename TKV, int NB, int HT>
+__global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
+    attn_decode_kernel(const DecArgs d, const __grid_constant__ KvMaps maps) {
+  using S = DecShape<NB, HT>;
+  constexpr int W = S::W, ST = S::ST, RH = HT / 8, LD = S::LD;
+  constexpr bool kSplit = HT == 8;               // rows 8 .. 15 carry the rests
+  constexpr bool kHalf = std::is_same_v<TKV, __half>;
+  constexpr float kLift = kHalf ? 15.f : 0.f;    // f16 weights up to 2^15: small ones keep their bits
+  pdl_enter();
+  extern __shared__ uint8_t dec_raw[];
+  __shared__ __align__(8) uint64_t full[W][ST];
+  __shared__ long long red[3][W];
+  __shared__ int last_sh;
+  const AttnArgs& a = d.a;
+  const KvView& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = dec_raw + ((1024 - (smem_u32(dec_raw) & 1023)) & 1023);
+  float* merge = reinterpret_cast<float*>(ring + W * ST * S::CHUNK);
+  const int group = a.nh / c.nkv, tiles = (group + HT - 1) / HT, units = c.nkv * tiles;
+  if (lane == 0) {
+    for (int s = 0; s < ST; ++s) mbar_init(&full[warp][s], 1);
+    fence_mbar_init();
+  }
+
+  // ---- the line, and this block's range of it --------------------------------
+  // Chunks of all sequences, and the longest one. On the way the rows of
+  // sequences that hold nothing become zeros.
+  long long sum = 0;
+  int most = 0;
+  for (int i0 = 32 * warp; i0 < a.n; i0 += 32 * W) {
+    const int i = i0 + lane;
+    int n = 0;
+    bool none = false;
+    if (i < a.n) {
+      const int s = a.seqs ? a.seqs[i] : i;
+      if (s >= 0 && s < c.n_seq) n = dec_span(kv_len(c, s), a.window, a.sinks).n;
+      else if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
+      none = n == 0 && i % gridDim.x == blockIdx.x;
+    }
+    for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
+      TQ* out = static_cast<TQ*>(a.out) + (int64_t)(i0 + __ffs(rows) - 1) * a.out_stride;
+      for (int x = lane; x < a.nh * c.hd; x += 32) out[x] = (TQ)0.f;
+    }
+    sum += n;
+    most = max(most, n);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if (lane == 0) {
+    red[0][warp] = sum;
+    red[1][warp] = most;
+  }
+  __syncthreads();
+  long long line = 0;
+  for (int w = 0; w < W; ++w) {
+    line += red[0][w];
+    most = max(most, (int)red[1][w]);
+  }
+  line *= units;
+  if (line == 0) return;
+  // Equal ranges of at least one chunk per warp. When the units are few and
+  // nearly of one length, each is cut into the same whole number of parts
+  // instead (its stretch of the line padded to `pad` chunks): ranges that
+  // begin with their unit save a join. That is taken when it is not slower by
+  // more than a round of chunks.
+  long long per = max((line + gridDim.x - 1) / gridDim.x, (long long)W);
+  per = (per + W - 1) / W * W;
+  int pad = 0;
+  const long long all = (long long)a.n * units;
+  if (all <= gridDim.x) {
+    const int parts = (int)(gridDim.x / all);
+    const int q = ((most + parts - 1) / parts + W - 1) / W * W;
+    if (q <= per + W) {
+      per = q;
+      pad = q * ((most + q - 1) / q);
+      line = all * pad;
+    }
+  }
+  SegIter at;
+  at.pos = blockIdx.x * per;
+  at.end = min(line, at.pos + per);
+  at.pad = pad;
+  if (at.pos >= at.end) return;
+  // The sequence in which the range begins: the last whose first chunk is at
+  // or before it.
+  if (pad) {
+    at.i = (int)(at.pos / ((long long)pad * units));
+    at.base = (long long)at.i * pad * units;
+  } else {
+    long long before = 0;  // chunks of the sequences before the block of 32 * W at hand
+    at.i = 0;
+    at.base = 0;
+    for (int b = 0; b < a.n; b += 32 * W) {
+      const int i = b + tid;
+      long long n = 0;
+      if (i < a.n) {
+        const int s = a.seqs ? a.seqs[i] : i;
+        if (s >= 0 && s < c.n_seq) n = (long long)dec_span(kv_len(c, s), a.window, a.sinks).n * units;
+      }
+      long long x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) red[2][warp] = x;
+      __syncthreads();
+      long long mine = before + x - n, total = 0;
+      for (int w = 0; w < W; ++w) {
+        if (w < warp) mine += red[2][w];
+        total += red[2][w];
+      }
+      // Exactly one sequence holds the position.
+      if (n > 0 && mine <= at.pos && at.pos < mine + n) {
+        red[0][0] = i;
+        red[1][0] = mine;
+      }
+      before += total;
+      if (before > at.pos) break;
+    }
+    __syncthreads();
+    at.i = (int)red[0][0];
+    at.base = red[1][0];
+  }
+  seg_sequence(at, a);
+
+  // ---- this warp's ring ---------------------------------------------------------
+  SegIter ahead = at;  // what is loaded next
+  bool more = seg_next(ahead, a, units);
+  int next = ahead.c0 + warp, issued = 0, used = 0;
+  bool ok = true;
+  uint8_t* slots = ring + warp * ST * S::CHUNK;
+  auto issue = [&]() {
+    while (more && next >= ahead.c1) {
+      more = seg_next(ahead, a, units);
+      next = ahead.c0 + warp;
+    }
+    if (!more) return;
+    if (lane == 0) {
+      const int x = next < ahead.span.head ? next : next - ahead.span.head + ahead.span.w0, p = x * DC;
+      int id = c.table[(int64_t)ahead.s * c.max_pages + (p >> c.page_log2)];
+      int lp = a.layer * c.n_pages + id;
+      if (id < 0 || id >= c.n_pages) {
+        report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
+        lp = c.n_layer * c.n_pages;  // past the pool: zeros
+      }
+      const int st = issued % ST;
+      uint8_t* to = slots + st * S::CHUNK;
+      mbar_expect_tx(&full[warp][st], S::CHUNK);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        kv_load(to + b * DC * 128, &maps.k, 64 * b, p & (c.page - 1), ahead.unit / tiles, lp, &full[warp][st]);
+        kv_load(to + (NB + b) * DC * 128, &maps.v, 64 * b, p & (c.page - 1), ahead.unit / tiles, lp,
+                &full[warp][st]);
+      }
+    }
+    ++issued;
+    next += W;
+  };
+  __syncwarp();
+  for (int s = 0; s < ST; ++s) issue();
+
+  const int r0 = lane >> 2, cc = 2 * (lane & 3);  // fragment row and first column
+  const float log2e = 1.4426950408889634f;
+  while (seg_next(at, a, units)) {
+    const int kvh = at.unit / tiles, h0 = (at.unit - kvh * tiles) * HT;
+    // ---- queries as A fragments: rows r0 (and r0 + 8: rests, or more heads) -----
+    uint32_t qa[4 * NB][4];
+    float cq[RH];  // score units of base-2 exponents per product unit
+    {
+      const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)at.i * a.q_stride + (int64_t)(kvh * group + h0) * c.hd;
+#pragma unroll
+      for (int rr = 0; rr < RH; ++rr) {
+        const int h = r0 + 8 * rr;
+        const bool real = h0 + h < group;
+        float v[4 * NB][4], amax = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = 16 * ks + cc + (e & 1) + 8 * (e >> 1);
+            v[ks][e] = real && x < c.hd ? (float)q[(int64_t)h * c.hd + x] : 0.f;
+            amax = fmaxf(amax, fabsf(v[ks][e]));
+          }
+        float f = 1.f;
+        if constexpr (sizeof(TQ) == 4) {
+          // A power of two puts the row's largest value in [2^14, 2^15).
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int ex = (int)(__float_as_uint(amax) >> 23);
+          if (ex > 0 && ex < 255) f = __uint_as_float((uint32_t)min(254, max(1, 127 + 14 + 127 - ex)) << 23);
+        }
+        cq[rr] = __fdiv_rn(a.scale * log2e, f);
+#pragma unroll
+        for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = v[ks][2 * e] * f, y = v[ks][2 * e + 1] * f;
+            const uint32_t hi = pack2<TKV>(x, y);
+            if constexpr (kSplit) {
+              qa[ks][2 * e] = hi;
+              qa[ks][2 * e + 1] = sizeof(TQ) == 4 ? rest2<TKV>(x, y, hi) : 0u;
+            } else {
+              qa[ks][2 * e + rr] = hi;
+            }
+          }
+      }
+    }
+    float m[RH], l[RH], o[8 * NB][4];
+#pragma unroll
+    for (int rr = 0; rr < RH; ++rr) {
+      m[rr] = -INFINITY;
+      l[rr] = 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < 8 * NB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+
+    for (int x = at.c0 + warp; x < at.c1; x += W) {
+      const int st = used % ST;
+      if (ok && !mbar_wait(&full[warp][st], (used / ST) & 1, c.status, W_ATT_DEC)) ok = false;
+      if (!ok) break;
+      ++used;
+      const uint32_t kb = smem_u32(slots + st * S::CHUNK), vb = kb + NB * DC * 128;
+      const int ch = x < at.span.head ? x : x - at.span.head + at.span.w0, p0 = ch * DC;
+      // Scores: 16 rows x 16 positions (two column tiles).
+      float sc[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[t][e] = 0.f;
+      {
+        // ldmatrix: lanes 8 g .. 8 g + 7 address the rows of matrix g: positions
+        // 8 (g / 2) .., dims 8 (g % 2) ..
+        const int pr = (lane & 7) + 8 * (lane >> 4), g = (lane >> 3) & 1;
+#pragma unroll
+        for (int ks = 0; ks < 4 * NB; ++ks) {
+          const int u = 2 * (ks & 3) + g;
+          uint32_t b[4];
+          ldsm4(b, kb + (ks >> 2) * DC * 128 + pr * 128 + ((u ^ (pr & 7)) << 4));
+          mma16816<TKV>(sc[0], qa[ks], b[0], b[1]);
+          mma16816<TKV>(sc[1], qa[ks], b[2], b[3]);
+        }
+      }
+      // Rows of this thread: rr; its positions: p0 + 8 t + cc + e.
+      float tt[RH][4];
+#pragma unroll
+      for (int rr = 0; rr < RH; ++rr)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            tt[rr][2 * t + e] = (kSplit ? sc[t][e] + sc[t][e + 2] : sc[t][e + 2 * rr]) * cq[rr];
+      const bool edge = p0 + DC > at.len || (p0 < at.span.lo && p0 + DC > a.sinks);
+      if (edge) {
+        // Positions that the row does not see: no weight, and zeros in place of
+        // their values (what a page holds there may be NaN).
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = p0 + 8 * t + cc + e;
+            if (j >= at.len || (j < at.span.lo && j >= a.sinks))
+#pragma unroll
+              for (int rr = 0; rr < RH; ++rr) tt[rr][2 * t + e] = -INFINITY;
+          }
+        for (int y = lane; y < DC * 8 * NB; y += 32) {
+          const int r = (y >> 3) & (DC - 1), j = p0 + r;
+          if (j >= at.len || (j < at.span.lo && j >= a.sinks))
+            *reinterpret_cast<uint4*>(slots + st * S::CHUNK + NB * DC * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_shared();  // before the slot's next load
+        __syncwarp();
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int rr = 0; rr < RH; ++rr) {
+        float top = fmaxf(fmaxf(tt[rr][0], tt[rr][1]), fmaxf(tt[rr][2], tt[rr][3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (__any_sync(0xffffffffu, top > m[rr])) {
+          const float mn = fmaxf(m[rr], top), shrink = mn == -INFINITY ? 1.f : exp2_fast(m[rr] - mn);
+          m[rr] = mn;
+          l[rr] *= shrink;
+#pragma unroll
+          for (int t = 0; t < 8 * NB; ++t) {
+            o[t][2 * rr] *= shrink;
+            o[t][2 * rr + 1] *= shrink;
+            if constexpr (kSplit) {
+              o[t][2] *= shrink;
+              o[t][3] *= shrink;
+            }
+          }
+        }
+        const float base = (m[rr] == -INFINITY ? 0.f : m[rr]) - kLift;
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = exp2_fast(tt[rr][e] - base);
+          l[rr] += p[e];
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t hi = pack2<TKV>(p[2 * t], p[2 * t + 1]);
+          if constexpr (kSplit) {
+            pa[2 * t] = hi;
+            pa[2 * t + 1] = rest2<TKV>(p[2 * t], p[2 * t + 1], hi);
+          } else {
+            pa[2 * t + rr] = hi;
+          }
+        }
+      }
+      {
+        const int pr = (lane & 7) + 8 * ((lane >> 3) & 1), g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < 4 * NB; ++t) {
+          const int u = 2 * (t & 3) + g;
+          uint32_t b[4];
+          ldsm4t(b, vb + (t >> 2) * DC * 128 + pr * 128 + ((u ^ (pr & 7)) << 4));
+          mma16816<TKV>(o[2 * t], pa, b[0], b[1]);
+          mma16816<TKV>(o[2 * t + 1], pa, b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      issue();
+    }
+
+    // ---- the warps' states into warp 0's ---------------------------------------
+#pragma unroll
+    for (int rr = 0; rr < RH; ++rr) {
+      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
+      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
+    }
+    if constexpr (kSplit)
+#pragma unroll
+      for (int t = 0; t < 8 * NB; ++t) {
+        o[t][0] += o[t][2];
+        o[t][1] += o[t][3];
+      }
+    const int holders = min(W, at.c1 - at.c0);  // warps that had a chunk
+#pragma unroll
+    for (int half = W / 2; half >= 1; half >>= 1) {
+      if (holders <= half) continue;
+      __syncthreads();
+      if (warp >= half && warp < 2 * half && warp < holders) {
+#pragma unroll
+        for (int rr = 0; rr < RH; ++rr) {
+          float* to = merge + ((warp - half) * HT + r0 + 8 * rr) * LD;
+#pragma unroll
+          for (int t = 0; t < 8 * NB; ++t)
+            *reinterpret_cast<float2*>(to + 8 * t + cc) = make_float2(o[t][2 * rr], o[t][2 * rr + 1]);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(to + S::HD) = make_float2(m[rr], l[rr]);
+        }
+      }
+      __syncthreads();
+      if (warp < half && warp + half < holders) {
+#pragma unroll
+        for (int rr = 0; rr < RH; ++rr) {
+          const float* from = merge + (warp * HT + r0 + 8 * rr) * LD;
+          const float2 ml = *reinterpret_cast<const float2*>(from + S::HD);
+          const float mn = fmaxf(m[rr], ml.x);
+          const float mine = mn == -INFINITY ? 1.f : exp2_fast(m[rr] - mn);
+          const float theirs = mn == -INFINITY ? 1.f : exp2_fast(ml.x - mn);
+          m[rr] = mn;
+          l[rr] = __fmaf_rn(l[rr], mine, ml.y * theirs);
+#pragma unroll
+          for (int t = 0; t < 8 * NB; ++t) {
+            const float2 v = *reinterpret_cast<const float2*>(from + 8 * t + cc);
+            o[t][2 * rr] = __fmaf_rn(o[t][2 * rr], mine, v.x * theirs);
+            o[t][2 * rr + 1] = __fmaf_rn(o[t][2 * rr + 1], mine, v.y * theirs);
+          }
+        }
+      }
+    }
+
+    // ---- the result, or this block's part of it ------------------------------------
+    const int b0 = (int)(at.unit_at / per), b1 = (int)((at.unit_at + at.n_unit - 1) / per);
+    TQ* out = static_cast<TQ*>(a.out) + (int64_t)at.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
+    if (b0 == b1) {
+      if (warp == 0) {
+#pragma unroll
+        for (int rr = 0; rr < RH; ++rr) {
+          const int h = r0 + 8 * rr;
+          if (h0 + h >= group) continue;
+          const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
+#pragma unroll
+          for (int t = 0; t < 8 * NB; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (8 * t + cc + e < c.hd) out[(int64_t)h * c.hd + 8 * t + cc + e] = (TQ)(o[t][2 * rr + e] * inv);
+        }
+      }
+      continue;
+    }
+    // The part's place: 0 if the unit is the block's first, else 1.
+    const int slot = 2 * blockIdx.x + (at.unit_at + at.c0 == blockIdx.x * per ? 0 : 1);
+    if (warp == 0) {
+      float* to = d.part + (int64_t)slot * HT * LD;
+#pragma unroll
+      for (int rr = 0; rr < RH; ++rr) {
+#pragma unroll
+        for (int t = 0; t < 8 * NB; ++t)
+          *reinterpret_cast<float2*>(to + (r0 + 8 * rr) * LD + 8 * t + cc) =
+              make_float2(o[t][2 * rr], o[t][2 * rr + 1]);
+        if ((lane & 3) == 0)
+          *reinterpret_cast<float2*>(to + (r0 + 8 * rr) * LD + S::HD) = make_float2(m[rr], l[rr]);
+      }
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) last_sh = atomicAdd(d.count + b0, 1) == b1 - b0 ? 1 : 0;
+    }
+    __syncthreads();
+    if (last_sh) {
+      __threadfence();
+      if (tid == 0) d.count[b0] = 0;
+      // Parts in block order; the unit is the first of every block but b0,
+      // where it is unless it begins inside the block's range.
+      const int first = 2 * b0 + (at.unit_at == b0 * per ? 0 : 1);
+      constexpr int PAIRS = HT * S::HD / 2;
+      for (int x = tid; x < PAIRS; x += 32 * W) {
+        const int h = x / (S::HD / 2), y = 2 * (x - h * (S::HD / 2));
+        if (h0 + h >= group || y >= c.hd) continue;
+        float top = -INFINITY;
+        for (int b = b0; b <= b1; ++b)
+          top = fmaxf(top, __ldcg(d.part + ((int64_t)(b == b0 ? first : 2 * b) * HT + h) * LD + S::HD));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sl = 0.f, s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+        for (int b = b0; b <= b1; ++b) {
+          const float* from = d.part + ((int64_t)(b == b0 ? first : 2 * b) * HT + h) * LD;
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + S::HD));
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(from + y));
+          const float w = exp2_fast(ml.x - base);
+          sl = __fmaf_rn(w, ml.y, sl);
+          s0 = __fmaf_rn(w, v.x, s0);
+          s1 = __fmaf_rn(w, v.y, s1);
+        }
+        const float inv = sl == 0.f ? 0.f : __fdiv_rn(1.f, sl);
+        out[(int64_t)h * c.hd + y] = (TQ)(s0 * inv);
+        out[(int64_t)h * c.hd + y + 1] = (TQ)(s1 * inv);
+      }
+    }
+    __syncthreads();  // last_sh is read before the next segment writes it
+  }
+  // A failed wait leaves loads in flight: they land before the block ends.
+  if (!ok)
+    for (; used < issued; ++used) mbar_wait(&full[warp][used % ST], (used / ST) & 1, c.status, W_ATT_DEC);
+}
+
+size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 2) * sizeof(float); }
+
+template <typename TQ, typename TKV, int NB, int HT>
+static int launch_decode(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
+  using S = DecShape<NB, HT>;
+  static_assert(S::ST >= 2 && S::SMEM <= 226 * 1024, "two stages fit");
+  static PerDeviceOnce attr;
+  if (smem_attr_once(attr, attn_decode_kernel<TQ, TKV, NB, HT>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
+  // One block per SM, fewer when the tables hold less than a chunk per warp of each.
+  const int64_t units = (int64_t)d.a.n * d.a.c.nkv * ((d.a.nh / d.a.c.nkv + HT - 1) / HT);
+  const int64_t most = (int64_t)d.a.c.max_pages * d.a.c.page / DC;
+  const int grid = (int)std::min<int64_t>(num_sms(), units * ((most + S::W - 1) / S::W));
+  launch_k(attn_decode_kernel<TQ, TKV, NB, HT>, grid, 32 * S::W, S::SMEM, st, d, maps);
+  return KC_OK;
+}
+
+template <typename TQ, typename TKV, int HT>
+static int launch_decode_hd(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
+  switch ((d.a.c.hd + 63) / 64) {
+    case 1: return launch_decode<TQ, TKV, 1, HT>(d, maps, st);
+    case 2: return launch_decode<TQ, TKV, 2, HT>(d, maps, st);
+    case 3: return launch_decode<TQ, TKV, 3, HT>(d, maps, st);
+    default: return launch_decode<TQ, TKV, 4, HT>(d, maps, st);
+  }
+}
+
+int launch_attn_decode(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
+  const DecArgs d{a, part, count};
+  const bool many = a.nh / a.c.nkv > 8;
+  if (a.c.type == T_BF16)
+    return many ? launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 16>(d, maps, st)
+                : launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 8>(d, maps, st);
+  if (a.t_q == T_F32) return launch_decode_hd<float, __half, 8>(d, maps, st);
+  return many ? launch_decode_hd<__half, __half, 16>(d, maps, st) : launch_decode_hd<__half, __half, 8>(d, maps, st);
+}
+
+}  // namespace kc

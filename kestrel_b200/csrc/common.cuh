@@ -205,7 +205,8 @@ enum : int {
   W_MMA_OP_FULL = 7, W_MMA_ACC_EMPTY = 8, W_MMA_RAW_FULL = 9, W_MMA_OP_EMPTY_D = 10, W_MMA_ACC_FULL = 11,
   W_ROUTER = 12, W_MMA_TC_DRAIN = 13, W_DEC_PREV = 14, W_EP_PEER = 15, W_EP_PATH = 16, W_MMA_BOUND = 17,
   // Paged cache: what the device found wrong (no waits).
-  W_KV_SEQ = 18, W_KV_FORK = 19, W_KV_ROOM = 20, W_KV_CAP = 21, W_KV_PAGE = 22, W_KV_ROWS = 23, W_KV_COPY = 24
+  W_KV_SEQ = 18, W_KV_FORK = 19, W_KV_ROOM = 20, W_KV_CAP = 21, W_KV_PAGE = 22, W_KV_ROWS = 23, W_KV_COPY = 24,
+  W_ATT_DEC = 25
 };
 
 // ---- bulk async copy (TMA, non-tensor): global -> shared ------------------

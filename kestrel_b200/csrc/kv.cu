@@ -6,6 +6,9 @@
 // deterministic: the lowest free pages, in the order of the call. There is no
 // free list to keep in step: a page is free when refs says 0, and the few
 // kernels that look for free or live pages scan refs (4 bytes a page).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 
 #include "common.cuh"
@@ -470,6 +473,28 @@ void launch_kv_write(const KvView& c, int layer, const int32_t* seqs, const int3
     if (t == T_F32) write_rows<float, __nv_bfloat16>(c, layer, seqs, row_start, n, n_rows, k, v, ks, vs, st);
     else write_rows<__nv_bfloat16, __nv_bfloat16>(c, layer, seqs, row_start, n, n_rows, k, v, ks, vs, st);
   }
+}
+
+// ---- tensor maps -------------------------------------------------------------
+int make_kv_maps(const KvView& c, int box_rows, KvMaps& maps) {
+  cudaDriverEntryPointQueryResult q;
+  void* fn = nullptr;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+      q != cudaDriverEntryPointSuccess || !fn)
+    return KC_ERR_CUDA;
+  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  const cuuint64_t row = (cuuint64_t)c.hd * 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)c.hd, (cuuint64_t)c.page, (cuuint64_t)c.nkv,
+                              (cuuint64_t)c.n_layer * c.n_pages};
+  const cuuint64_t strides[3] = {row, row * c.page, row * c.page * c.nkv};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = c.type == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int i = 0; i < 2; ++i)
+    if (encode(reinterpret_cast<CUtensorMap*>(i ? maps.v.b : maps.k.b), t, 4, i ? c.v : c.k, dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return KC_ERR_CUDA;
+  return KC_OK;
 }
 
 // ---- workspace ---------------------------------------------------------------

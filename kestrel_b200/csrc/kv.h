@@ -30,15 +30,30 @@ struct KvView {
   int *status;
 };
 
+// CUtensorMaps (128 bytes each) of the k and v pools as [layer and page][head]
+// [row][column], boxes of 64 columns x some rows of one page, 128B swizzle.
+struct alignas(64) KvMap {
+  unsigned char b[128];
+};
+struct KvMaps {
+  KvMap k, v;
+};
+int make_kv_maps(const KvView& c, int box_rows, KvMaps& maps);
+
 struct KvCache {
   KvView view;
   int* work;
   int64_t work_bytes;
+  KvMaps rows16;  // boxes of 16 rows
 };
 
-// What a context holds of caches.
+// What a context holds of caches, and the attention kernels' workspace (made
+// with the first cache).
 struct KvState {
   std::map<int, KvCache> caches;
+  float* part = nullptr;  // attn_decode_part_bytes()
+  int* count = nullptr;   // one per SM, zero between launches
+  int64_t bytes = 0;
 };
 
 int64_t kv_workspace_ints(const KvView& c);
@@ -68,6 +83,10 @@ struct AttnArgs {
   float scale;
   int window, sinks;         // window 0: none
 };
-int launch_attention_paged(const AttnArgs& a, cudaStream_t st);
+size_t attn_decode_part_bytes();
+// One row per sequence (row_start null).
+int launch_attn_decode(const AttnArgs& a, const KvMaps& rows16, float* part, int* count, cudaStream_t st);
+// row_start non-null.
+int launch_attn_prompt(const AttnArgs& a, cudaStream_t st);
 
 }  // namespace kc
