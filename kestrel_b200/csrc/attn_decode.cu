@@ -29,6 +29,7 @@
 namespace kc {
 
 constexpr int DC = 16;  // positions per chunk: the smallest page
+constexpr int DEC_MAX_PARTS = 160;  // most blocks of a launch
 
 template <int NB, int HT>
 struct DecShape {
@@ -36,7 +37,7 @@ struct DecShape {
   static constexpr int W = NB <= 2 ? 8 : 4;                    // warps
   static constexpr int CHUNK = 2 * NB * DC * 128;              // K and V of one chunk
   static constexpr int ST = 196608 / (W * CHUNK);              // ring stages per warp
-  static constexpr int LD = HD + 2;                            // a head's partial: values, maximum, sum
+  static constexpr int LD = HD + 4;                            // a head's partial: values, maximum, sum, (16-byte rows)
   static constexpr int MERGE = W / 2 * HT * LD * 4;            // partials of half the warps
   static constexpr int SMEM = W * ST * CHUNK + MERGE + 1024;
 };
@@ -66,6 +67,7 @@ __device__ __forceinline__ Span dec_span(int len, int window, int sinks) {
 struct SegIter {
   long long pos, end, base;  // base: line position of sequence i's first unit
   int i, pad;                // pad: chunks each unit takes of the line (0: as many as it has)
+  bool whole;                // the units that begin in the range, none of them cut
   int s, len;
   Span span;
   // the segment
@@ -90,7 +92,11 @@ __device__ __forceinline__ bool seg_next(SegIter& t, const AttnArgs& a, int unit
     }
     t.unit = (int)(off / np);
     t.c0 = (int)(off - (long long)t.unit * np);
-    const int take = (int)min(t.end - t.pos, (long long)(np - t.c0));
+    if (t.whole && t.c0) {
+      t.pos += np - t.c0;
+      continue;
+    }
+    const int take = t.whole ? np : (int)min(t.end - t.pos, (long long)(np - t.c0));
     t.unit_at = t.pos - t.c0;
     t.c1 = min(t.c0 + take, t.span.n);
     t.n_unit = t.span.n;
@@ -167,35 +173,44 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // nearly of one length, each is cut into the same whole number of parts
   // instead (its stretch of the line padded to `pad` chunks): ranges that
   // begin with their unit save a join. That is taken when it is not slower by
-  // more than a round of chunks.
+  // more than a round of chunks. When the units are many and none is longer
+  // than a warp's share of the line, each warp takes whole units of its own and
+  // nothing is merged or joined.
   long long per = max((line + gridDim.x - 1) / gridDim.x, (long long)W);
-  per = (per + W - 1) / W * W;
-  int pad = 0;
   const long long all = (long long)a.n * units;
-  if (all <= gridDim.x) {
-    const int parts = (int)(gridDim.x / all);
-    const int q = ((most + parts - 1) / parts + W - 1) / W * W;
-    if (q <= per + W) {
-      per = q;
-      pad = q * ((most + q - 1) / q);
-      line = all * pad;
+  const bool whole = most <= max((per + W - 1) / W, 4ll) && all >= (long long)gridDim.x * W;
+  int pad = 0;
+  if (whole) {
+    per = (per + W - 1) / W;
+  } else {
+    per = (per + W - 1) / W * W;
+    if (all <= gridDim.x) {
+      const int parts = (int)(gridDim.x / all);
+      const int q = ((most + parts - 1) / parts + W - 1) / W * W;
+      if (q <= per + W) {
+        per = q;
+        pad = q * ((most + q - 1) / q);
+        line = all * pad;
+      }
     }
   }
   SegIter at;
-  at.pos = blockIdx.x * per;
+  at.pos = (whole ? blockIdx.x * W + warp : blockIdx.x) * per;
   at.end = min(line, at.pos + per);
   at.pad = pad;
-  if (at.pos >= at.end) return;
+  at.whole = whole;
+  if (!whole && at.pos >= at.end) return;
   // The sequence in which the range begins: the last whose first chunk is at
-  // or before it.
+  // or before it (of every warp's range, where warps have their own).
   if (pad) {
     at.i = (int)(at.pos / ((long long)pad * units));
     at.base = (long long)at.i * pad * units;
   } else {
-    long long before = 0;  // chunks of the sequences before the block of 32 * W at hand
-    at.i = 0;
-    at.base = 0;
-    for (int b = 0; b < a.n; b += 32 * W) {
+    const long long block_end = whole ? (blockIdx.x + 1) * W * per : at.end;
+    long long before = 0;  // chunks of the sequences before the 32 * W at hand
+    __syncthreads();
+    if (lane == 0) red[0][warp] = a.n;  // a range past the line has no sequence
+    for (int b = 0; b < a.n && before < block_end; b += 32 * W) {
       const int i = b + tid;
       long long n = 0;
       if (i < a.n) {
@@ -211,35 +226,40 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       __syncthreads();
       if (lane == 31) red[2][warp] = x;
       __syncthreads();
-      long long mine = before + x - n, total = 0;
+      long long mine = before + x - n;
       for (int w = 0; w < W; ++w) {
         if (w < warp) mine += red[2][w];
-        total += red[2][w];
+        before += red[2][w];
       }
-      // Exactly one sequence holds the position.
-      if (n > 0 && mine <= at.pos && at.pos < mine + n) {
-        red[0][0] = i;
-        red[1][0] = mine;
-      }
-      before += total;
-      if (before > at.pos) break;
+      // Exactly one sequence holds each position.
+      if (n > 0)
+        for (int w = 0; w < (whole ? W : 1); ++w) {
+          const long long pos = (whole ? blockIdx.x * W + w : blockIdx.x) * per;
+          if (mine <= pos && pos < mine + n) {
+            red[0][w] = i;
+            red[1][w] = mine;
+          }
+        }
     }
     __syncthreads();
-    at.i = (int)red[0][0];
-    at.base = red[1][0];
+    at.i = (int)red[0][whole ? warp : 0];
+    at.base = red[1][whole ? warp : 0];
+    if (at.i >= a.n) at.pos = at.end;
   }
-  seg_sequence(at, a);
+  if (at.pos < at.end) seg_sequence(at, a);
 
   // ---- this warp's ring ---------------------------------------------------------
+  // Its chunks are every `stride`-th of each segment, from the `mine`-th on.
+  const int stride = whole ? 1 : W, mine = whole ? 0 : warp;
   SegIter ahead = at;  // what is loaded next
   bool more = seg_next(ahead, a, units);
-  int next = ahead.c0 + warp, issued = 0, used = 0;
+  int next = ahead.c0 + mine, issued = 0, used = 0;
   bool ok = true;
   uint8_t* slots = ring + warp * ST * S::CHUNK;
   auto issue = [&]() {
     while (more && next >= ahead.c1) {
       more = seg_next(ahead, a, units);
-      next = ahead.c0 + warp;
+      next = ahead.c0 + mine;
     }
     if (!more) return;
     if (lane == 0) {
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
     }
     ++issued;
-    next += W;
+    next += stride;
   };
   __syncwarp();
   for (int s = 0; s < ST; ++s) issue();
@@ -323,7 +343,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
 
-    for (int x = at.c0 + warp; x < at.c1; x += W) {
+    for (int x = at.c0 + mine; x < at.c1; x += stride) {
       const int st = used % ST;
       if (ok && !mbar_wait(&full[warp][st], (used / ST) & 1, c.status, W_ATT_DEC)) ok = false;
       if (!ok) break;
@@ -444,7 +464,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         o[t][0] += o[t][2];
         o[t][1] += o[t][3];
       }
-    const int holders = min(W, at.c1 - at.c0);  // warps that had a chunk
+    const int holders = whole ? 1 : min(W, at.c1 - at.c0);  // warps that had a chunk
 #pragma unroll
     for (int half = W / 2; half >= 1; half >>= 1) {
       if (holders <= half) continue;
@@ -481,10 +501,11 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     }
 
     // ---- the result, or this block's part of it ------------------------------------
-    const int b0 = (int)(at.unit_at / per), b1 = (int)((at.unit_at + at.n_unit - 1) / per);
+    const int b0 = whole ? 0 : (int)(at.unit_at / per);
+    const int b1 = whole ? 0 : (int)((at.unit_at + at.n_unit - 1) / per);
     TQ* out = static_cast<TQ*>(a.out) + (int64_t)at.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
     if (b0 == b1) {
-      if (warp == 0) {
+      if (whole || warp == 0) {
 #pragma unroll
         for (int rr = 0; rr < RH; ++rr) {
           const int h = r0 + 8 * rr;
@@ -523,28 +544,56 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       // Parts in block order; the unit is the first of every block but b0,
       // where it is unless it begins inside the block's range.
       const int first = 2 * b0 + (at.unit_at == b0 * per ? 0 : 1);
-      constexpr int PAIRS = HT * S::HD / 2;
-      for (int x = tid; x < PAIRS; x += 32 * W) {
-        const int h = x / (S::HD / 2), y = 2 * (x - h * (S::HD / 2));
-        if (h0 + h >= group || y >= c.hd) continue;
-        float top = -INFINITY;
-        for (int b = b0; b <= b1; ++b)
-          top = fmaxf(top, __ldcg(d.part + ((int64_t)(b == b0 ? first : 2 * b) * HT + h) * LD + S::HD));
-        const float base = top == -INFINITY ? 0.f : top;
-        float sl = 0.f, s0 = 0.f, s1 = 0.f;
-#pragma unroll 4
-        for (int b = b0; b <= b1; ++b) {
-          const float* from = d.part + ((int64_t)(b == b0 ? first : 2 * b) * HT + h) * LD;
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + S::HD));
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(from + y));
-          const float w = exp2_fast(ml.x - base);
-          sl = __fmaf_rn(w, ml.y, sl);
-          s0 = __fmaf_rn(w, v.x, s0);
-          s1 = __fmaf_rn(w, v.y, s1);
+      // First every part's share of each head's result (a warp per head, the
+      // parts over its lanes), then the sums over the parts.
+      const int parts = b1 - b0 + 1;
+      float* share = merge;  // [HT][parts]
+      auto part_of = [&](int p) { return d.part + (int64_t)(p == 0 ? first : 2 * (b0 + p)) * HT * LD; };
+      for (int h = warp; h < HT; h += W) {
+        float2 ml[DEC_MAX_PARTS / 32];
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
+          const int p = lane + 32 * u;
+          ml[u] = p < parts ? __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + S::HD))
+                            : make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, ml[u].x);
         }
-        const float inv = sl == 0.f ? 0.f : __fdiv_rn(1.f, sl);
-        out[(int64_t)h * c.hd + y] = (TQ)(s0 * inv);
-        out[(int64_t)h * c.hd + y + 1] = (TQ)(s1 * inv);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
+          ml[u].x = exp2_fast(ml[u].x - base);
+          total = __fmaf_rn(ml[u].x, ml[u].y, total);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+#pragma unroll
+        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
+          if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
+      }
+      __syncthreads();
+      constexpr int QUADS = HT * S::HD / 4;
+      for (int x = tid; x < QUADS; x += 32 * W) {
+        const int h = x / (S::HD / 4), y = 4 * (x - h * (S::HD / 4));
+        if (h0 + h >= group || y >= c.hd) continue;
+        float4 sum4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p) + h * LD + y));
+          const float w = share[h * parts + p];
+          sum4.x = __fmaf_rn(w, v.x, sum4.x);
+          sum4.y = __fmaf_rn(w, v.y, sum4.y);
+          sum4.z = __fmaf_rn(w, v.z, sum4.z);
+          sum4.w = __fmaf_rn(w, v.w, sum4.w);
+        }
+        TQ* to = out + (int64_t)h * c.hd + y;
+        to[0] = (TQ)sum4.x;
+        to[1] = (TQ)sum4.y;
+        to[2] = (TQ)sum4.z;
+        to[3] = (TQ)sum4.w;
       }
     }
     __syncthreads();  // last_sh is read before the next segment writes it
@@ -554,7 +603,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     for (; used < issued; ++used) mbar_wait(&full[warp][used % ST], (used / ST) & 1, c.status, W_ATT_DEC);
 }
 
-size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 2) * sizeof(float); }
+size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 4) * sizeof(float); }
 
 template <typename TQ, typename TKV, int NB, int HT>
 static int launch_decode(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
@@ -565,7 +614,7 @@ static int launch_decode(const DecArgs& d, const KvMaps& maps, cudaStream_t st) 
   // One block per SM, fewer when the tables hold less than a chunk per warp of each.
   const int64_t units = (int64_t)d.a.n * d.a.c.nkv * ((d.a.nh / d.a.c.nkv + HT - 1) / HT);
   const int64_t most = (int64_t)d.a.c.max_pages * d.a.c.page / DC;
-  const int grid = (int)std::min<int64_t>(num_sms(), units * ((most + S::W - 1) / S::W));
+  const int grid = (int)std::min<int64_t>(std::min(num_sms(), DEC_MAX_PARTS), units * ((most + S::W - 1) / S::W));
   launch_k(attn_decode_kernel<TQ, TKV, NB, HT>, grid, 32 * S::W, S::SMEM, st, d, maps);
   return KC_OK;
 }
