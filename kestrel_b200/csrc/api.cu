@@ -415,7 +415,8 @@ int check_status(kc_ctx* ctx) {
                                   "positions",
                                   "paged cache: a page to copy out of range, a destination given twice or also a "
                                   "source (nothing was copied)",
-                                  "paged attention (a chunk of the cache)"};
+                                  "paged decode attention (a chunk of the cache)",
+                                  "paged prompt attention"};
     const int site = st >> 8;
     if (site >= W_KV_SEQ && site <= W_KV_COPY)
       return fail(ctx, st & 0xFF, "%s", sites[site]);
@@ -3075,7 +3076,7 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     a.scale = scale;
     a.window = window;
     a.sinks = window > 0 ? sinks : 0;
-    const int rc = prompt ? launch_attn_prompt(a, ctx->stream)
+    const int rc = prompt ? launch_attn_prompt(a, kv.tiles, ctx->stream)
                           : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
     return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);
   });
@@ -3123,7 +3124,8 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
     w.max_pages = max_pages;
     w.status = ctx->status;
     C.work_bytes = kv_workspace_ints(w) * (int64_t)sizeof(int);
-    if (make_kv_maps(w, 16, C.rows16) != KC_OK)
+    if (make_kv_maps(w, 16, C.rows16) != KC_OK ||
+        make_kv_maps(w, attn_prompt_box_rows(page, head_dim), C.tiles) != KC_OK)
       return fail(ctx, KC_ERR_CUDA, "kc_kv_cache: cuTensorMapEncodeTiled refused the pools");
     if (!ctx->kv.part) {
       const size_t cnt = (size_t)num_sms() * sizeof(int), all = attn_decode_part_bytes() + cnt;

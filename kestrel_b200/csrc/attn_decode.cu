@@ -1,5 +1,5 @@
 // Attention of one new token per sequence over the paged key-value cache,
-// split over the cache's length and joined (formulas: attn.cu).
+// split over the cache's length and joined (formulas: attn_prompt.cu).
 //
 // A decode step reads every visible key and value once and computes 4 flops a
 // byte and query head: it is bound by the memory rate, and what matters is that
@@ -313,8 +313,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
           // A power of two puts the row's largest value in [2^14, 2^15).
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          const int ex = (int)(__float_as_uint(amax) >> 23);
-          if (ex > 0 && ex < 255) f = __uint_as_float((uint32_t)min(254, max(1, 127 + 14 + 127 - ex)) << 23);
+          f = pow2_factor(amax);
         }
         cq[rr] = __fdiv_rn(a.scale * log2e, f);
 #pragma unroll

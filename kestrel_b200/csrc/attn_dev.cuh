@@ -52,6 +52,54 @@ __device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t pair) {
   return pack2<T>(lo - a, hi - b);
 }
 
+// The power of two that puts a row's largest magnitude in [2^14, 2^15), within
+// f16's range (1 for a row of zeros or one that is not finite).
+__device__ __forceinline__ float pow2_factor(float amax) {
+  const int ex = (int)(__float_as_uint(amax) >> 23);
+  return ex > 0 && ex < 255 ? __uint_as_float((uint32_t)min(254, 127 + 14 + 127 - ex) << 23) : 1.f;
+}
+
+// Two f32 lanes at once: v * m + a, v + w.
+__device__ __forceinline__ float2 fma2(float2 v, float m, float a) {
+  uint64_t r, x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(v.x), "f"(v.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(m));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(z) : "f"(a));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 v, float2 w) {
+  uint64_t r, x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(v.x), "f"(v.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(w.x), "f"(w.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+
+// Four consecutive values, aligned to four; eight, aligned to 16 bytes.
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(p);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+  alignas(8) T x[4];
+  *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+}
+__device__ __forceinline__ void store8(float* p, const float* v) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

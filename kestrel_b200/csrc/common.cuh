@@ -206,7 +206,7 @@ enum : int {
   W_ROUTER = 12, W_MMA_TC_DRAIN = 13, W_DEC_PREV = 14, W_EP_PEER = 15, W_EP_PATH = 16, W_MMA_BOUND = 17,
   // Paged cache: what the device found wrong (no waits).
   W_KV_SEQ = 18, W_KV_FORK = 19, W_KV_ROOM = 20, W_KV_CAP = 21, W_KV_PAGE = 22, W_KV_ROWS = 23, W_KV_COPY = 24,
-  W_ATT_DEC = 25
+  W_ATT_DEC = 25, W_ATT_PROMPT = 26
 };
 
 // ---- bulk async copy (TMA, non-tensor): global -> shared ------------------

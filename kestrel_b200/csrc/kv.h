@@ -1,4 +1,5 @@
-// Paged key-value cache (kv.cu) and the attention over it (attn.cu): the
+// Paged key-value cache (kv.cu) and the attention over it (attn_decode.cu,
+// attn_prompt.cu): the
 // caller's buffers as the kernels see them, and the host-side launchers.
 #pragma once
 
@@ -45,6 +46,7 @@ struct KvCache {
   int* work;
   int64_t work_bytes;
   KvMaps rows16;  // boxes of 16 rows
+  KvMaps tiles;   // boxes of attn_prompt_box_rows rows
 };
 
 // What a context holds of caches, and the attention kernels' workspace (made
@@ -87,6 +89,7 @@ size_t attn_decode_part_bytes();
 // One row per sequence (row_start null).
 int launch_attn_decode(const AttnArgs& a, const KvMaps& rows16, float* part, int* count, cudaStream_t st);
 // row_start non-null.
-int launch_attn_prompt(const AttnArgs& a, cudaStream_t st);
+int attn_prompt_box_rows(int page, int hd);
+int launch_attn_prompt(const AttnArgs& a, const KvMaps& tiles, cudaStream_t st);
 
 }  // namespace kc

@@ -1,4 +1,4 @@
-// Device helpers of the paged cache shared by its kernels (kv.cu, attn.cu).
+// Device helpers of the paged cache shared by its kernels (kv.cu, attn_*.cu).
 #pragma once
 
 #include <cuda_bf16.h>
