@@ -59,26 +59,70 @@ __device__ __forceinline__ float pow2_factor(float amax) {
   return ex > 0 && ex < 255 ? __uint_as_float((uint32_t)min(254, 127 + 14 + 127 - ex) << 23) : 1.f;
 }
 
-// Two f32 lanes at once: v * m + a, v + w.
-__device__ __forceinline__ float2 fma2(float2 v, float m, float a) {
-  uint64_t r, x, y, z;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(v.x), "f"(v.y));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(m));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(z) : "f"(a));
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
+// Two f32 lanes at once (sm_100's packed instructions).
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
 }
-__device__ __forceinline__ float2 add2(float2 v, float2 w) {
-  uint64_t r, x, y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(v.x), "f"(v.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(w.x), "f"(w.y));
+__device__ __forceinline__ float2 f2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
 }
 
-// Four consecutive values, aligned to four; eight, aligned to 16 bytes.
+// 2^x of two lanes on the FMA pipes, beside the special-function unit, for
+// weights that are rounded to 16 bits: x = n + f with f in [-1/2, 1/2] (the
+// rounding that adding 1.5 * 2^23 does), 2^f by the cubic whose largest
+// relative error there is least (7.5e-5, a sixth of f16's half unit; computed
+// by Lawson's reweighted least squares), n into the exponent. x <= 120; below
+// -126 the result is 0 but for 2^-126; a NaN comes out as a value past the
+// 16-bit types' range.
+__device__ __forceinline__ float2 exp2_cubic(float2 v) {
+  const uint64_t x = f2(max_nan(v.x, -126.f), max_nan(v.y, -126.f));
+  const uint64_t t = add2(x, f2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
+  uint64_t p = fma2(f, f2(0.05517137654f, 0.05517137654f), f2(0.24261121067f, 0.24261121067f));
+  p = fma2(p, f, f2(0.69326103069f, 0.69326103069f));
+  p = fma2(p, f, f2(0.99992806957f, 0.99992806957f));
+  const float2 a = f2(p), n = f2(t);
+  return make_float2(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(n.y) << 23)));
+}
+
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+// Four consecutive values, aligned to four.
 __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
   const float4 x = *reinterpret_cast<const float4*>(p);
   v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
@@ -90,12 +134,12 @@ __device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
 }
-__device__ __forceinline__ void store8(float* p, const float* v) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+// 16 bytes of values of T.
+__device__ __forceinline__ void store_piece(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
+__device__ __forceinline__ void store_piece(T* p, const float* v) {
   *reinterpret_cast<uint4*>(p) =
       make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }

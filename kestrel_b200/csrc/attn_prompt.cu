@@ -38,6 +38,10 @@ namespace kc {
 
 constexpr int PM = 128;  // rows of a tile
 constexpr int P_STAGES_MAX = 8;
+// One pair of weights in this many takes its exponentials from exp2_cubic.
+constexpr int kCubicEvery = 4;
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * 168, "within the registers of the launch");
 
 template <typename TQ, int NB, bool TWO>
 struct PromptShape {
@@ -53,12 +57,16 @@ struct PromptShape {
   static constexpr int FIT = (CAP - 1024 - Q_ALL) / KV;
   static constexpr int ST = FIT < P_STAGES_MAX ? FIT : P_STAGES_MAX;
   static constexpr int SMEM = Q_ALL + ST * KV + 1024;
-  static constexpr int THREADS = 128 * NS + 64;
+  // Two streams: three warpgroups of 168 registers a thread at launch, of which
+  // the third (loads, MMAs, two idle warps) gives the softmax warps 32 each.
+  static constexpr int THREADS = NS == 2 ? 384 : 192;
   static constexpr int T_O = 256;                  // TMEM columns: S of stream w at 128 w, its O at T_O + HD w
   static constexpr int JOIN_LD = HD + 4;           // floats of a row handed over between the streams
   static_assert(!TWO || NS == 2, "two row tiles need two streams");
   static_assert(ST >= 2 && T_O + NS * HD <= 512, "fits");
-  static_assert(NS == 1 || TWO || PM * JOIN_LD * 4 <= Q_ALL + ST * KV, "the join fits");
+  // Shared memory after the last product: the join, then the rows going out.
+  static constexpr int OUT_AT = TWO || NS == 1 ? 0 : (PM * JOIN_LD * 4 + 1023) / 1024 * 1024;
+  static_assert(TWO || OUT_AT + PM * HD * (int)sizeof(TQ) <= Q_ALL + ST * KV, "join and output fit");
 };
 
 // The position tiles that a row tile reads: `head` tiles of the first tokens,
@@ -67,6 +75,11 @@ struct TileSpan {
   int head, w0, n;
   __device__ int start(int t, int bn) const { return (t < head ? t : t - head + w0) * bn; }
 };
+
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+}
 
 struct RowTile {
   int i, s, len, count, start;  // entry, sequence, its positions, its rows, its first row
@@ -131,7 +144,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   constexpr float kGrow = 8.f;
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
-  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_full[NS], o_full[NS], q_full, drained;
+  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_half[NS], p_full[NS], o_full[NS];
+  __shared__ __align__(8) uint64_t q_full, drained;
   __shared__ uint32_t tmem_sh;
   __shared__ RowTile rt_sh;
   __shared__ float factor_sh[S::QT][PM];  // what a row's queries were multiplied with (f32 queries)
@@ -191,6 +205,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       }
       for (int w = 0; w < NS; ++w) {
         mbar_init(&s_full[w], 1);
+        mbar_init(&p_half[w], 128);
         mbar_init(&p_full[w], 128);
         mbar_init(&o_full[w], 1);
       }
@@ -226,6 +241,9 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   constexpr int AHEAD = TWO ? 1 : NS;  // K tiles loaded before the first V
   bool ok = true;
 
+  if (warp >= W_TMA) {
+    if constexpr (NS == 2) regs_down<kOtherRegs>();  // with the idle warps: a warpgroup at a time
+  }
   if (warp == W_TMA) {
     // ---- K and V tiles: K 0 .. AHEAD-1, then V t, K t + AHEAD ----------------
     const int piece = min(c.page, BN), pieces = BN / piece;
@@ -271,7 +289,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // Every load lands before the block may end.
     for (int i = max(0, it - ST); i < it; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, c.status, W_ATT_PROMPT);
   } else if (warp == W_MMA) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0 && elect_one()) {
       const uint32_t id_s = tc_idesc<TKV>(BN, false), id_o = tc_idesc<TKV>(hd16, true);
       const int ksteps = hd16 / 16;
       const uint32_t qa = smem_u32(q_sm), ra = smem_u32(ring);
@@ -281,27 +299,38 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         tc_fence_after();
         return ra + (it % ST) * S::KV;
       };
+      // One instruction covers 16 of K; descriptors step in units of 16 bytes.
+      // (Unrolled with constant steps: computing each descriptor in a loop
+      // takes longer than the product it is for.)
       auto scores = [&](int w, uint32_t k) {
+        const uint64_t kd = sw128_desc(k);
 #pragma unroll
-        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-          for (int ks = 0; ks < ksteps; ++ks)
-            tc_mma(tmem + 128 * w,
-                   sw128_desc(qa + ((TWO ? w : 0) * (kSplit ? 2 : 1) + part) * S::QB + (ks >> 2) * PM * 128 +
-                              32 * (ks & 3)),
-                   sw128_desc(k + (ks >> 2) * BN * 128 + 32 * (ks & 3)), id_s, part > 0 || ks > 0);
+        for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
+          const uint64_t qd = sw128_desc(qa + ((TWO ? w : 0) * (kSplit ? 2 : 1) + part) * S::QB);
+#pragma unroll
+          for (int ks = 0; ks < 4 * NB; ++ks)
+            if (ks < ksteps)
+              tc_mma(tmem + 128 * w, qd + ((ks >> 2) * PM * 128 + 32 * (ks & 3)) / 16,
+                     kd + ((ks >> 2) * BN * 128 + 32 * (ks & 3)) / 16, id_s, part > 0 || ks > 0);
+        }
         tc_commit(&s_full[w]);
       };
-      auto values = [&](int w, uint32_t v, bool add) {
+      // The weights come in two halves, so that the first half's products run
+      // beside the exponentials of the second.
+      auto values = [&](int w, int k, uint32_t v, bool add) {
+        const uint64_t vd = sw128_desc_mn(v, BN * 128);
 #pragma unroll
-        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+        for (int half = 0; half < 2; ++half) {
+          if (ok && !mbar_wait(half ? &p_full[w] : &p_half[w], k & 1, c.status, W_ATT_PROMPT)) ok = false;
+          if (!ok) return;
+          tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + 128 * w + part * (BN / 2) + 8 * ks,
-                      sw128_desc_mn(v + ks * 2048, BN * 128), id_o, add || part > 0 || ks > 0);
-      };
-      auto weights_wait = [&](int w, int k) {
-        if (ok && !mbar_wait(&p_full[w], k & 1, c.status, W_ATT_PROMPT)) ok = false;
-        tc_fence_after();
+          for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+            for (int ks = half * (BN / 32); ks < (half + 1) * (BN / 32); ++ks)
+              tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + 128 * w + part * (BN / 2) + 8 * ks, vd + ks * 2048 / 16,
+                        id_o, add || half > 0 || part > 0 || ks > 0);
+        }
       };
       if (!mbar_wait(&q_full, 0, c.status, W_ATT_PROMPT)) ok = false;
       if constexpr (TWO) {
@@ -320,9 +349,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           k = 0;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            weights_wait(w, t);
+            values(w, t, v, t > 0);
             if (!ok) break;
-            values(w, v, t > 0);
             if (w == 1) tc_commit(&kv_empty[v_it % ST]);
             if (!more) {
               tc_commit(&o_full[w]);
@@ -346,9 +374,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         for (int t = 0; t < nt && ok; ++t) {
           const int w = t % NS;
           const uint32_t v = stage_wait();
-          weights_wait(w, t / NS);
+          values(w, t / NS, v, t >= NS);
           if (!ok) break;
-          values(w, v, t >= NS);
           tc_commit(&kv_empty[it % ST]);
           ++it;
           if (t + NS < nt) {
@@ -366,27 +393,54 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       tc_commit(&drained);
       mbar_wait(&drained, 0, c.status, W_ATT_PROMPT);
     }
-  } else {
+  } else if (warp < W_TMA) {
+    if constexpr (NS == 2) regs_up<kSoftmaxRegs>();
     // ---- softmax: stream w, a thread per row ---------------------------------
     const int w = warp >> 2, r = tid & 127, my_tile = TWO ? w : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_t = tmem + lanes + 128 * w, o_t = tmem + lanes + S::T_O + w * S::HD;
     const TQ* q = static_cast<const TQ*>(a.q);
     const float flip = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;  // score factors are positive: see below
-    // Queries into shared memory, a warp per row, four values a lane.
-    {
+    // Row f of the block: its token among the sequence's rows, its head of the
+    // group ((x * magic) >> 16 = x / group for x < 512, group <= 128).
+    const int tok0 = rt.row0 / group, rem = rt.row0 - tok0 * group;
+    const uint32_t magic = 65536u / group + 1;
+    auto token = [&](int f) { return tok0 + (int)(((uint32_t)(rem + f) * magic) >> 16); };
+    auto row_of = [&](int f, int64_t stride) {
+      const int t = token(f);
+      return (int64_t)(rt.start + t) * stride + (int64_t)(kvh * group + rem + f - (t - tok0) * group) * c.hd;
+    };
+    // ---- queries into shared memory ------------------------------------------
+    constexpr int LOADERS = TWO ? 128 : 128 * NS;
+    const int loader = TWO ? r : tid;
+    bool copied = false;
+    if constexpr (!kSplit) {
+      copied = flip == 1.f && !((uintptr_t)a.q % 16) && a.q_stride % 8 == 0;
+      if (copied) {
+#pragma unroll 8
+        for (int y = loader; y < PM * 8 * NB; y += LOADERS) {
+          const int rr = y / (8 * NB), p = y - rr * 8 * NB, f = my_tile * PM + rr;
+          const bool real = f < rows && 8 * p < c.hd;
+          copy16_async(smem_u32(q_sm + my_tile * S::QB) + (p >> 3) * PM * 128 + (rr >> 3) * 1024 + (rr & 7) * 128 +
+                           (((p & 7) ^ (rr & 7)) << 4),
+                       real ? q + row_of(f, a.q_stride) + 8 * p : q, real);
+        }
+        copies_wait();
+      }
+    }
+    if (!copied) {
+      // A warp per row, four values a lane.
       const bool wide = !((uintptr_t)a.q % (4 * sizeof(TQ))) && a.q_stride % 4 == 0;
-      constexpr int ROWS = TWO ? PM / 4 : PM / (4 * NS);  // rows of a warp
-      const int first = (TWO ? (warp & 3) : warp) * ROWS;
-      for (int x0 = 0; x0 < ROWS; x0 += 4) {
-        float v[4][NB <= 2 ? 1 : 2][4];
+      constexpr int H = NB <= 2 ? 1 : 2, BATCH = 8, ROWS = 32 * PM / LOADERS;  // rows of a warp
+      const int first = loader / 32 * ROWS;
+      for (int x0 = 0; x0 < ROWS; x0 += BATCH) {
+        float v[BATCH][H][4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int f = my_tile * PM + first + x0 + y;  // row among the block's
-          const int g = rt.row0 + f;
-          const TQ* from = q + (int64_t)(rt.start + g / group) * a.q_stride + (int64_t)(kvh * group + g % group) * c.hd;
+        for (int y = 0; y < BATCH; ++y) {
+          const int f = my_tile * PM + first + x0 + y;
+          const TQ* from = q + row_of(f < rows ? f : 0, a.q_stride);
 #pragma unroll
-          for (int h = 0; h < (NB <= 2 ? 1 : 2); ++h) {
+          for (int h = 0; h < H; ++h) {
             const int d = 4 * lane + 128 * h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[y][h][e] = 0.f;
@@ -401,14 +455,14 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           }
         }
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
+        for (int y = 0; y < BATCH; ++y) {
           const int rr = first + x0 + y;
           float f = 1.f;
           if constexpr (kSplit) {
             // A power of two puts the row's largest value in [2^14, 2^15).
             float amax = 0.f;
 #pragma unroll
-            for (int h = 0; h < (NB <= 2 ? 1 : 2); ++h)
+            for (int h = 0; h < H; ++h)
 #pragma unroll
               for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(v[y][h][e]));
 #pragma unroll
@@ -418,7 +472,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           }
           f *= flip;
 #pragma unroll
-          for (int h = 0; h < (NB <= 2 ? 1 : 2); ++h) {
+          for (int h = 0; h < H; ++h) {
             const int d = 4 * lane + 128 * h;
             if (d >= S::HD) continue;
             uint8_t* to = q_sm + my_tile * (kSplit ? 2 : 1) * S::QB + (d >> 6) * PM * 128 + (rr >> 3) * 1024 +
@@ -433,18 +487,17 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           }
         }
       }
-      fence_async_shared();
-      mbar_arrive(&q_full);
     }
-    const int f = my_tile * PM + r, g = rt.row0 + f;
+    fence_async_shared();
+    mbar_arrive(&q_full);
+    const int f = my_tile * PM + r;
     const bool real = f < rows;
-    const int at = real ? rt.len - rt.count + g / group : -1;
+    const int at = real ? rt.len - rt.count + token(f) : -1;
     const int lo = a.window > 0 ? at - a.window + 1 : 0;
     // Tiles whose positions every row of this tile sees need no mask.
-    const int t_at0 = rt.len - rt.count + (rt.row0 + my_tile * PM) / group;
-    const int t_lo1 = a.window > 0 ? rt.len - rt.count + (rt.row0 + min(rows, (my_tile + 1) * PM) - 1) / group -
-                                         a.window + 1
-                                   : 0;
+    const int t_at0 = rt.len - rt.count + token(my_tile * PM);
+    const int t_lo1 =
+        a.window > 0 ? rt.len - rt.count + token(min(rows, (my_tile + 1) * PM) - 1) - a.window + 1 : 0;
     float cq = 0.f, m = -INFINITY, l = 0.f;
     const int mine = tiles_of(w);
     if (mine > 0 && !mbar_wait(&q_full, 0, c.status, W_ATT_PROMPT)) ok = false;
@@ -465,14 +518,22 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       for (int x = 0; x < BN; x += 32) tmem_ld32(s_t + x, s + x);
       tmem_wait_ld();
       if (j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks)) {
+        // A bit per position: up to the row's own, and not before its window
+        // unless among the first tokens.
         const int hi = at - j0, from = lo - j0, first = a.sinks - j0;
 #pragma unroll
-        for (int x = 0; x < BN; ++x)
-          if (x > hi || (x < from && x >= first)) s[x] = -INFINITY;
-      }
-      float top = s[0];
+        for (int x = 0; x < BN; x += 32) {
+          const uint32_t see = low_bits(hi + 1 - x) & (~low_bits(from - x) | low_bits(first - x));
 #pragma unroll
-      for (int x = 1; x < BN; ++x) top = fmaxf(top, s[x]);
+          for (int e = 0; e < 32; ++e) s[x + e] = see >> e & 1 ? s[x + e] : -INFINITY;
+        }
+      }
+      float tops[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) tops[x] = s[x];
+#pragma unroll
+      for (int x = 8; x < BN; x += 2) tops[x / 2 & 7] = max3(tops[x / 2 & 7], s[x], s[x + 1]);
+      float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
       top = top == -INFINITY ? top : top * cq;
       if (k == 0) {
         m = top;
@@ -492,27 +553,9 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             for (int e = 0; e < 16; ++e) o[e] *= shrink;
             tmem_st16(o_t + x, o);
           }
+          tmem_wait_st();
         }
       }
-      const float base = kLift - (m == -INFINITY ? 0.f : m);
-      float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int x = 0; x < BN; x += 32) {
-        uint32_t p[16], rest[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 y = fma2(make_float2(s[x + 2 * e], s[x + 2 * e + 1]), cq, base);
-          y.x = exp2_fast(y.x);
-          y.y = exp2_fast(y.y);
-          sum = add2(sum, y);
-          p[e] = pack2<TKV>(y.x, y.y);
-          if constexpr (kSplit) rest[e] = rest2<TKV>(y.x, y.y, p[e]);
-        }
-        tmem_st16(s_t + x / 2, p);
-        if constexpr (kSplit) tmem_st16(s_t + BN / 2 + x / 2, rest);
-      }
-      l += sum.x + sum.y;
-      tmem_wait_st();
       if (t == nt - 1 && j0 + BN > rt.len) {
         // Rows past the sequence's end hold whatever the page held before:
         // zeros in their place (the last V is the last load of the ring).
@@ -523,8 +566,34 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           if (j0 + ((y >> 3) & (BN - 1)) >= rt.len) *reinterpret_cast<uint4*>(v + y * 16) = make_uint4(0, 0, 0, 0);
         fence_async_shared();
       }
-      tc_fence_before();
-      mbar_arrive(&p_full[w]);
+      const float base = kLift - (m == -INFINITY ? 0.f : m);
+      const uint64_t cq2 = f2(cq, cq), base2 = f2(base, base);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int x = 0; x < BN; x += 32) {
+        uint32_t p[16], rest[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float2 y = f2(fma2(f2(s[x + 2 * e], s[x + 2 * e + 1]), cq2, base2));
+          if (!kSplit && e % kCubicEvery == kCubicEvery - 1) {
+            y = exp2_cubic(y);
+          } else {
+            y.x = exp2_fast(y.x);
+            y.y = exp2_fast(y.y);
+          }
+          sum = add2(sum, f2(y.x, y.y));
+          p[e] = pack2<TKV>(y.x, y.y);
+          if constexpr (kSplit) rest[e] = rest2<TKV>(y.x, y.y, p[e]);
+        }
+        tmem_st16(s_t + x / 2, p);
+        if constexpr (kSplit) tmem_st16(s_t + BN / 2 + x / 2, rest);
+        if (x == BN / 2 - 32 || x == BN - 32) {
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(x == BN - 32 ? &p_full[w] : &p_half[w]);
+        }
+      }
+      l += f2(sum).x + f2(sum).y;
     }
     if (ok && mine > 0 && !mbar_wait(&o_full[w], 0, c.status, W_ATT_PROMPT)) ok = false;
     ok = __all_sync(0xffffffffu, ok);
@@ -561,10 +630,12 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       }
     }
     if (TWO || w == 0) {
+      // Rows go out through shared memory (this warp's 32, 16-byte pieces
+      // swizzled), so that a warp's stores cover whole lines.
       const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-      TQ* out = static_cast<TQ*>(a.out) + (int64_t)(rt.start + g / group) * a.out_stride +
-                (int64_t)(kvh * group + g % group) * c.hd;
-      const bool wide = !((uintptr_t)a.out % 16) && a.out_stride * sizeof(TQ) % 16 == 0;
+      constexpr int PIECES = S::HD * sizeof(TQ) / 16, PER = 16 / sizeof(TQ);
+      uint8_t* stage = q_sm + (TWO ? my_tile * S::QB : S::OUT_AT) +
+                       (warp & 3) * 32 * PIECES * 16;
       bool bad = l != l || l == INFINITY;
       for (int x = 0; x < hd16; x += 16) {
         float o[16];
@@ -583,25 +654,33 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           bad |= !(fabsf(o[e]) <= 3.4028234e38f);
           o[e] = l == 0.f ? 0.f : o[e] * inv;
         }
-        if (!real) continue;
+#pragma unroll
+        for (int p = 0; p < 16 / PER; ++p)
+          store_piece(reinterpret_cast<TQ*>(stage + (lane * PIECES + ((x / PER + p) ^ (lane & 7))) * 16), o + p * PER);
+      }
+      __syncwarp();
+      const bool wide = !((uintptr_t)a.out % 16) && a.out_stride * sizeof(TQ) % 16 == 0;
+      const int first = my_tile * PM + 32 * (warp & 3);  // the warp's first row
+#pragma unroll 4
+      for (int y = lane; y < 32 * PIECES; y += 32) {
+        const int row = y / PIECES, p = y - row * PIECES;
+        if (first + row >= rows || p * PER >= c.hd) continue;
+        TQ* to = static_cast<TQ*>(a.out) + row_of(first + row, a.out_stride) + p * PER;
+        const uint8_t* from = stage + (row * PIECES + (p ^ (row & 7))) * 16;
         if (wide) {
-          store8(out + x, o);
-          if (x + 8 < c.hd) store8(out + x + 8, o + 8);
+          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (x + e < c.hd) out[x + e] = (TQ)o[e];
+          for (int e = 0; e < PER; ++e) to[e] = reinterpret_cast<const TQ*>(from)[e];
         }
       }
+      __syncwarp();
       // A row that a value beyond its mask has spoilt (or that sees one that is
       // not finite) is computed again by itself.
       for (unsigned again = __ballot_sync(0xffffffffu, ok && real && bad); again; again &= again - 1) {
-        const int src = __ffs(again) - 1, g1 = __shfl_sync(0xffffffffu, g, src);
-        __syncwarp();
-        prompt_row<TQ, TKV>(a, rt.s, kvh, rt.len - rt.count + g1 / group,
-                            q + (int64_t)(rt.start + g1 / group) * a.q_stride + (int64_t)(kvh * group + g1 % group) * c.hd,
-                            static_cast<TQ*>(a.out) + (int64_t)(rt.start + g1 / group) * a.out_stride +
-                                (int64_t)(kvh * group + g1 % group) * c.hd);
+        const int f1 = first + __ffs(again) - 1;
+        prompt_row<TQ, TKV>(a, rt.s, kvh, rt.len - rt.count + token(f1), q + row_of(f1, a.q_stride),
+                            static_cast<TQ*>(a.out) + row_of(f1, a.out_stride));
       }
     }
   }
