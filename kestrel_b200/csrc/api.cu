@@ -3076,7 +3076,7 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     a.scale = scale;
     a.window = window;
     a.sinks = window > 0 ? sinks : 0;
-    const int rc = prompt ? launch_attn_prompt(a, kv.tiles, ctx->stream)
+    const int rc = prompt ? launch_attn_prompt(a, kv.tiles, ctx->kv.part, ctx->kv.count, ctx->stream)
                           : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
     return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);
   });
@@ -3128,11 +3128,12 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
         make_kv_maps(w, attn_prompt_box_rows(page, head_dim), C.tiles) != KC_OK)
       return fail(ctx, KC_ERR_CUDA, "kc_kv_cache: cuTensorMapEncodeTiled refused the pools");
     if (!ctx->kv.part) {
-      const size_t cnt = (size_t)num_sms() * sizeof(int), all = attn_decode_part_bytes() + cnt;
+      const size_t part = std::max(attn_decode_part_bytes(), attn_prompt_part_bytes());
+      const size_t cnt = (size_t)std::max(num_sms(), attn_prompt_counts()) * sizeof(int), all = part + cnt;
       void* p = nullptr;
       CK(cudaMalloc(&p, all));
       ctx->kv.part = static_cast<float*>(p);
-      ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + attn_decode_part_bytes());
+      ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + part);
       ctx->kv.bytes = (int64_t)all;
       CK(cudaMemsetAsync(ctx->kv.count, 0, cnt, ctx->stream));
     }

@@ -23,6 +23,13 @@ __device__ __forceinline__ void kv_load(void* dst, const KvMap* map, int x, int 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void* dst, const KvMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -90,58 +97,53 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
-__device__ __forceinline__ float max_nan(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
-
-// 2^x of two lanes on the FMA pipes, beside the special-function unit, for
-// weights that are rounded to 16 bits: x = n + f with f in [-1/2, 1/2] (the
-// rounding that adding 1.5 * 2^23 does), 2^f by the cubic whose largest
-// relative error there is least (7.5e-5, a sixth of f16's half unit; computed
-// by Lawson's reweighted least squares), n into the exponent. x <= 120; below
-// -126 the result is 0 but for 2^-126; a NaN comes out as a value past the
-// 16-bit types' range.
-__device__ __forceinline__ float2 exp2_cubic(float2 v) {
-  const uint64_t x = f2(max_nan(v.x, -126.f), max_nan(v.y, -126.f));
-  const uint64_t t = add2(x, f2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
-  uint64_t p = fma2(f, f2(0.05517137654f, 0.05517137654f), f2(0.24261121067f, 0.24261121067f));
-  p = fma2(p, f, f2(0.69326103069f, 0.69326103069f));
-  p = fma2(p, f, f2(0.99992806957f, 0.99992806957f));
-  const float2 a = f2(p), n = f2(t);
-  return make_float2(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(n.y) << 23)));
-}
-
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-}
-
-// Four consecutive values, aligned to four.
-__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(p);
+// Eight consecutive values, aligned to 16 bytes.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
   v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
-  alignas(8) T x[4];
-  *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  alignas(16) T x[8];
+  *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(p);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+  for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
 }
-// 16 bytes of values of T.
-__device__ __forceinline__ void store_piece(float* p, const float* v) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+
+// The first n of 16 values (n a multiple of 8) to p, whose row starts and
+// lengths are multiples of the lowest set bit of `grain` bytes. 32 bytes a
+// store where they are aligned: a whole sector.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+               "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
 }
 template <typename T>
-__device__ __forceinline__ void store_piece(T* p, const float* v) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+__device__ __forceinline__ void store16(T* p, const float* v, int n, uint32_t grain) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t u[2][8];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i / 8][i % 8] = __float_as_uint(v[i]);
+    if (!(grain & 31)) {
+      store32(p, u[0]);
+      if (n > 8) store32(p + 8, u[1]);
+      return;
+    }
+  } else {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    if (!(grain & 31) && n > 8) return store32(p, u);
+    if (!(grain & 15)) {
+      reinterpret_cast<uint4*>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+      if (n > 8) reinterpret_cast<uint4*>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < n) p[i] = (T)v[i];
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {

@@ -8,17 +8,22 @@
 //
 // The rows of a key-value head (tokens outermost, then the heads of its group)
 // are cut into tiles of 128, the M of an MMA, so that the group shares every
-// key and value. Positions pass in tiles of BN. Roles:
+// key and value. Positions pass in tiles of BN. One block per SM takes items
+// (row tiles of a head) as it comes to them, those that see most first. Roles:
 //   softmax warps  four per stream, a thread per row: scores from TMEM, the
 //                  mask where the tile needs it, weights back to TMEM as the
 //                  16-bit A operand of the second product. The accumulator is
 //                  rescaled only when a row's maximum has grown by 2^8.
 //   a TMA warp     K and V tiles, a box per page, through one ring.
 //   an MMA warp    S = Q K^T (both in shared memory), O += P V (P in TMEM).
+//   two more       find the next item and bring its queries, while the others
+//                  are at the last one.
 // Two streams take turns on the tensor cores, so that one's exponentials run
 // beside the other's products (an MMA tile of 128 x 128 x 128 takes as long as
 // its 16384 exponentials): either two row tiles over the same positions, or
-// one row tile whose position tiles alternate, joined at the end.
+// one row tile whose position tiles alternate, joined at the end. With fewer
+// items than SMs their positions are split further, over several blocks; the
+// block that finishes last joins the parts in their order.
 //
 // f32 queries are carried by two f16 operands (value and rest), and so are
 // their weights: twice the products, f32-grade results over a 16-bit cache.
@@ -38,9 +43,7 @@ namespace kc {
 
 constexpr int PM = 128;  // rows of a tile
 constexpr int P_STAGES_MAX = 8;
-// One pair of weights in this many takes its exponentials from exp2_cubic.
-constexpr int kCubicEvery = 4;
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * 168, "within the registers of the launch");
 
 template <typename TQ, int NB, bool TWO>
@@ -53,43 +56,67 @@ struct PromptShape {
   static constexpr int QB = PM * 128 * NB;         // bytes of a query operand
   static constexpr int Q_ALL = QT * (kSplit ? 2 : 1) * QB;
   static constexpr int KV = BN * 128 * NB;         // bytes of a K or V tile
-  static constexpr int CAP = 226 * 1024;
+  static constexpr int CAP = (NB <= 2 ? 221 : 225) * 1024;  // beside up to 6 (1.5) KB of static arrays
   static constexpr int FIT = (CAP - 1024 - Q_ALL) / KV;
   static constexpr int ST = FIT < P_STAGES_MAX ? FIT : P_STAGES_MAX;
   static constexpr int SMEM = Q_ALL + ST * KV + 1024;
   // Two streams: three warpgroups of 168 registers a thread at launch, of which
-  // the third (loads, MMAs, two idle warps) gives the softmax warps 32 each.
-  static constexpr int THREADS = NS == 2 ? 384 : 192;
+  // the third (loads, MMAs) gives the softmax warps 32 a thread.
+  static constexpr int THREADS = 128 * NS + 128;
   static constexpr int T_O = 256;                  // TMEM columns: S of stream w at 128 w, its O at T_O + HD w
-  static constexpr int JOIN_LD = HD + 4;           // floats of a row handed over between the streams
+  static constexpr int LD = HD + 4;                // floats of a row's part of a split item: values, maximum, sum
   static_assert(!TWO || NS == 2, "two row tiles need two streams");
   static_assert(ST >= 2 && T_O + NS * HD <= 512, "fits");
-  // Shared memory after the last product: the join, then the rows going out.
-  static constexpr int OUT_AT = TWO || NS == 1 ? 0 : (PM * JOIN_LD * 4 + 1023) / 1024 * 1024;
-  static_assert(TWO || OUT_AT + PM * HD * (int)sizeof(TQ) <= Q_ALL + ST * KV, "join and output fit");
 };
 
-// The position tiles that a row tile reads: `head` tiles of the first tokens,
-// then tiles w0 .. (n tiles in all).
-struct TileSpan {
-  int head, w0, n;
-  __device__ int start(int t, int bn) const { return (t < head ? t : t - head + w0) * bn; }
-};
+// 16 values times f; whether any of them was infinite or NaN (times 0 it is NaN).
+__device__ __forceinline__ bool normalise16(float (&v)[16], float f) {
+  uint64_t odd = 0;
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    const uint64_t x = f2(v[e], v[e + 1]);
+    odd = fma2(x, f2(0.f, 0.f), odd);
+    const float2 y = f2(mul2(x, f2(f, f)));
+    v[e] = y.x;
+    v[e + 1] = y.y;
+  }
+  return f2(odd).x + f2(odd).y != 0.f;
+}
 
 // The lowest n bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
 
-struct RowTile {
-  int i, s, len, count, start;  // entry, sequence, its positions, its rows, its first row
-  int row0;                     // first (token, head) row of the block's tiles
+// Row f of an item: its token among the entry's rows, its head of the group.
+// (x * magic) >> 16 = x / group for x < 512, group <= 128.
+struct RowMap {
+  int tok0, rem, group;
+  uint32_t magic;
+  __device__ RowMap(int row0, int g) : tok0(row0 / g), rem(row0 - row0 / g * g), group(g), magic(65536u / g + 1) {}
+  __device__ int token(int f) const { return tok0 + (int)(((uint32_t)(rem + f) * magic) >> 16); }
+  __device__ int64_t offset(int f, int64_t stride, int hd) const {
+    const int t = token(f);
+    return t * stride + (int64_t)(rem + f - (t - tok0) * group) * hd;
+  }
+};
+
+// An item: the rows row0 .. row0 + rows - 1 ((token, head) pairs) of head kvh
+// of entry i, over position tiles t0 .. t1-1 of those they see. Tile t begins
+// at position BN * (t < head ? t : t - head + w0): `head` tiles of the first
+// tokens, then those of the window.
+struct Item {
+  int valid, s, len, count, start, row0, rows, kvh;
+  int head, w0, nt, t0, t1;
+  int unit, split, splits;
+  __device__ int pos(int t, int bn) const { return (t < head ? t : t - head + w0) * bn; }
 };
 
 // One row computed position by position by a warp: what the products cannot
-// give when a value that the row does not see is not finite (0 * NaN).
+// give when a value that the row does not see is not finite (0 * NaN). Columns
+// col0 .. col1-1 are written.
 template <typename TQ, typename TKV>
-__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int at, const TQ* q, TQ* out) {
+__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int at, const TQ* q, TQ* out, int col0, int col1) {
   const KvView& c = a.c;
   const int lane = threadIdx.x & 31, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
   float x[8], o[8], m = -INFINITY, l = 0.f;
@@ -130,172 +157,155 @@ __device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int a
   }
 #pragma unroll
   for (int u = 0; u < 8; ++u)
-    if (lane + 32 * u < c.hd) out[lane + 32 * u] = (TQ)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(o[u], l));
+    if (lane + 32 * u >= col0 && lane + 32 * u < col1) out[lane + 32 * u] = (TQ)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(o[u], l));
 }
+
+struct PromptArgs {
+  AttnArgs a;
+  int splits;   // blocks an item's positions may be split over
+  float* part;  // [unit][split][PM][LD]
+  int* count;   // per unit, zero between launches
+  int* next;    // [2] items dealt beyond one per block, blocks done: zero between launches
+  bool q_map;   // queries come by TMA
+};
 
 template <typename TQ, typename TKV, int NB, bool TWO>
 __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
-    attn_prompt_kernel(const AttnArgs a, const __grid_constant__ KvMaps maps) {
+    attn_prompt_kernel(const PromptArgs d, const __grid_constant__ KvMaps maps, const __grid_constant__ KvMap q_map) {
   using S = PromptShape<TQ, NB, TWO>;
   constexpr int BN = S::BN, NS = S::NS, ST = S::ST;
   constexpr bool kSplit = S::kSplit;
   // Weights reach 2^(lift + 8): small ones of f16 keep their bits.
   constexpr float kLift = std::is_same_v<TKV, __half> ? 7.f : 0.f;
   constexpr float kGrow = 8.f;
+  constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1, W_AUX = W_TMA + 2;  // W_AUX: and the next
+  constexpr int AHEAD = TWO ? 1 : NS;  // K tiles loaded before the first V
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
-  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_half[NS], p_full[NS], o_full[NS];
-  __shared__ __align__(8) uint64_t q_full, drained;
+  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_half[NS], p_full[NS], o_full[NS],
+      o_empty[NS];
+  __shared__ __align__(8) uint64_t q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint32_t tmem_sh;
-  __shared__ RowTile rt_sh;
-  __shared__ float factor_sh[S::QT][PM];  // what a row's queries were multiplied with (f32 queries)
+  __shared__ Item items[2];
+  __shared__ __align__(8) uint64_t drained, join_full, part_full, last_full;
+  __shared__ float factor_sh[2][S::QT][PM];  // what a row's queries were multiplied with (f32 queries)
+  __shared__ float2 join_sh[2][NS][PM];      // maximum and sum of a stream's rows
+  __shared__ int last_sh;
+  const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1;
   const int group = a.nh / c.nkv;
-  const int block = gridDim.x - 1 - blockIdx.x;  // later rows see more: they begin first
-  const int kvh = block % c.nkv;
-
-  // ---- the block's rows ------------------------------------------------------
-  if (warp == 0) {
-    RowTile r{};
-    r.i = -1;
-    int t = block / c.nkv;
-    for (int b = 0; b < a.n && r.i < 0; b += 32) {
-      int lo = 0, hi = 0;
-      if (b + lane < a.n) {
-        lo = a.row_start[b + lane];
-        hi = a.row_start[b + lane + 1];
-        if (lo < 0 || hi < lo || hi > a.n_rows) {
-          if (block == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
-          lo = hi = 0;
-        }
-      }
-      const int n = (int)(((int64_t)(hi - lo) * group + S::QT * PM - 1) / (S::QT * PM));
-      int x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const unsigned mine = __ballot_sync(0xffffffffu, t >= x - n && t < x);
-      if (mine) {
-        const int l = __ffs(mine) - 1;
-        r.i = b + l;
-        r.start = __shfl_sync(0xffffffffu, lo, l);
-        r.count = __shfl_sync(0xffffffffu, hi - lo, l);
-        r.row0 = (t - __shfl_sync(0xffffffffu, x - n, l)) * S::QT * PM;
-      }
-      t -= __shfl_sync(0xffffffffu, x, 31);
+  const int hd16 = (c.hd + 15) / 16 * 16;  // columns of the products that are computed
+  const float flip = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;  // into the queries: score factors are positive
+  uint8_t* q_sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
+  uint8_t* ring = q_sm + S::Q_ALL;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
     }
-    if (lane == 0) {
-      if (r.i >= 0) {
-        r.s = a.seqs ? a.seqs[r.i] : r.i;
-        if (r.s < 0 || r.s >= c.n_seq) {
-          report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
-          r.i = -1;
-        } else {
-          r.len = kv_len(c, r.s);
-        }
-      }
-      rt_sh = r;
-      for (int i = 0; i < ST; ++i) {
-        mbar_init(&kv_full[i], 1);
-        mbar_init(&kv_empty[i], 1);
-      }
-      for (int w = 0; w < NS; ++w) {
-        mbar_init(&s_full[w], 1);
-        mbar_init(&p_half[w], 128);
-        mbar_init(&p_full[w], 128);
-        mbar_init(&o_full[w], 1);
-      }
-      mbar_init(&q_full, 128 * NS);
-      mbar_init(&drained, 1);
-      fence_mbar_init();
+    for (int w = 0; w < NS; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_half[w], 128);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_full[w], 1);
+      mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
+    mbar_init(&q_full, 2);
+    mbar_init(&q_empty, 1);
+    mbar_init(&drained, 1);
+    mbar_init(&join_full, 128 * NS);
+    mbar_init(&part_full, 128 * NS);
+    mbar_init(&last_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 4 * NS + 3);
+    }
+    fence_mbar_init();
   }
-  __syncthreads();
-  const RowTile rt = rt_sh;
-  if (rt.i < 0) return;
   if (warp == W_MMA) tmem_alloc(&tmem_sh, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_sh;
-  uint8_t* q_sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
-  uint8_t* ring = q_sm + S::Q_ALL;
-  const int rows = min(S::QT * PM, rt.count * group - rt.row0);
-  // Positions of the first and last row, and the tiles they read.
-  const int at0 = rt.len - rt.count + rt.row0 / group, at1 = rt.len - rt.count + (rt.row0 + rows - 1) / group;
-  TileSpan span{0, 0, 0};
-  if (at1 >= 0) {
-    const int lo = a.window > 0 ? max(0, at0 - a.window + 1) : 0;
-    span.head = (min(a.sinks, lo) + BN - 1) / BN;
-    span.w0 = max(lo / BN, span.head);
-    span.n = span.head + at1 / BN + 1 - span.w0;
-  }
-  const int nt = span.n;
-  const int hd16 = (c.hd + 15) / 16 * 16;  // columns of the products that are computed
-  // Stream w's k-th tile is k (two row tiles) or NS k + w.
-  auto tiles_of = [&](int w) { return TWO ? nt : (nt - w + NS - 1) / NS; };
-  constexpr int AHEAD = TWO ? 1 : NS;  // K tiles loaded before the first V
   bool ok = true;
+  // Item n of this block, for every role but the one that finds it. A role
+  // gives it back once it has read what it needs of it.
+  auto item_wait = [&](int n) -> bool {
+    if (ok && !mbar_wait(&item_full[n & 1], (n >> 1) & 1, c.status, W_ATT_PROMPT)) ok = false;
+    return ok;
+  };
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (ok && !mbar_wait(bar, phase & 1, c.status, W_ATT_PROMPT)) ok = false;
+  };
 
   if (warp >= W_TMA) {
-    if constexpr (NS == 2) regs_down<kOtherRegs>();  // with the idle warps: a warpgroup at a time
+    if constexpr (NS == 2) regs_down<kOtherRegs>();  // a warpgroup at a time
   }
   if (warp == W_TMA) {
     // ---- K and V tiles: K 0 .. AHEAD-1, then V t, K t + AHEAD ----------------
     const int piece = min(c.page, BN), pieces = BN / piece;
     int it = 0;
-    auto page_at = [&](int t) {
-      if (lane >= pieces || t >= nt) return -1;
-      const int p = span.start(t, BN) + lane * piece;
-      if (p >= rt.len) return -1;
-      const int id = c.table[(int64_t)rt.s * c.max_pages + (p >> c.page_log2)];
-      if (id < 0 || id >= c.n_pages) {
-        report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
-        return -1;
-      }
-      return id;
-    };
-    auto load = [&](const KvMap* map, int t, int id) {
-      const int st = it % ST;
-      if (it >= ST && !mbar_wait(&kv_empty[st], (it / ST - 1) & 1, c.status, W_ATT_PROMPT)) ok = false;
+    for (int n = 0; ok; ++n) {
+      item_wait(n);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      uint8_t* to = ring + st * S::KV;
-      if (lane == 0) mbar_expect_tx(&kv_full[st], S::KV);
+      if (!ok) break;
+      const Item x = items[n & 1];
       __syncwarp();
-      if (lane < pieces) {
-        const int p = span.start(t, BN) + lane * piece;
-        const int lp = id >= 0 ? a.layer * c.n_pages + id : c.n_layer * c.n_pages;  // past the pool: zeros
+      if (lane == 0) mbar_arrive(&item_empty[n & 1]);
+      if (!x.valid) break;
+      auto page_at = [&](int t) {
+        if (lane >= pieces || t >= x.t1) return -1;
+        const int p = x.pos(t, BN) + lane * piece;
+        if (p >= x.len) return -1;
+        const int id = c.table[(int64_t)x.s * c.max_pages + (p >> c.page_log2)];
+        if (id < 0 || id >= c.n_pages) {
+          report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
+          return -1;
+        }
+        return id;
+      };
+      auto load = [&](const KvMap* map, int t, int id) {
+        const int st = it % ST;
+        if (it >= ST) wait(&kv_empty[st], it / ST - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        uint8_t* to = ring + st * S::KV;
+        if (lane == 0) mbar_expect_tx(&kv_full[st], S::KV);
+        __syncwarp();
+        if (lane < pieces) {
+          const int p = x.pos(t, BN) + lane * piece;
+          const int lp = id >= 0 ? a.layer * c.n_pages + id : c.n_layer * c.n_pages;  // past the pool: zeros
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          kv_load(to + b * BN * 128 + lane * piece * 128, map, 64 * b, p & (c.page - 1), kvh, lp, &kv_full[st]);
+          for (int b = 0; b < NB; ++b)
+            kv_load(to + b * BN * 128 + lane * piece * 128, map, 64 * b, p & (c.page - 1), x.kvh, lp, &kv_full[st]);
+        }
+        ++it;
+      };
+      int kid[AHEAD + 1];  // pages of tiles t .. t + AHEAD
+      for (int u = 0; u < AHEAD; ++u) kid[u] = page_at(x.t0 + u);
+      for (int u = 0; u < AHEAD && x.t0 + u < x.t1 && ok; ++u) load(&maps.k, x.t0 + u, kid[u]);
+      for (int t = x.t0; t < x.t1 && ok; ++t) {
+        kid[AHEAD] = page_at(t + AHEAD);
+        load(&maps.v, t, kid[0]);
+        if (ok && t + AHEAD < x.t1) load(&maps.k, t + AHEAD, kid[AHEAD]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) kid[u] = kid[u + 1];
       }
-      ++it;
-    };
-    int kid[AHEAD + 1];  // pages of tiles t .. t + AHEAD
-    for (int t = 0; t < AHEAD; ++t) kid[t] = page_at(t);
-    for (int t = 0; t < AHEAD && t < nt && ok; ++t) load(&maps.k, t, kid[t]);
-    for (int t = 0; t < nt && ok; ++t) {
-      kid[AHEAD] = page_at(t + AHEAD);
-      load(&maps.v, t, kid[0]);
-      if (ok && t + AHEAD < nt) load(&maps.k, t + AHEAD, kid[AHEAD]);
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) kid[u] = kid[u + 1];
     }
     // Every load lands before the block may end.
     for (int i = max(0, it - ST); i < it; ++i) mbar_wait(&kv_full[i % ST], (i / ST) & 1, c.status, W_ATT_PROMPT);
   } else if (warp == W_MMA) {
-    if (nt > 0 && elect_one()) {
+    if (elect_one()) {
       const uint32_t id_s = tc_idesc<TKV>(BN, false), id_o = tc_idesc<TKV>(hd16, true);
       const int ksteps = hd16 / 16;
       const uint32_t qa = smem_u32(q_sm), ra = smem_u32(ring);
-      int it = 0;  // next stage of the ring, in the order of its loads
+      int it = 0;         // next stage of the ring, in the order of its loads
+      int kp[NS];         // weight tiles of each stream so far
+      int used = 0;       // items with products so far
+      for (int w = 0; w < NS; ++w) kp[w] = 0;
       auto stage_wait = [&]() {
-        if (ok && !mbar_wait(&kv_full[it % ST], (it / ST) & 1, c.status, W_ATT_PROMPT)) ok = false;
+        wait(&kv_full[it % ST], it / ST);
         tc_fence_after();
         return ra + (it % ST) * S::KV;
       };
@@ -317,11 +327,11 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       };
       // The weights come in two halves, so that the first half's products run
       // beside the exponentials of the second.
-      auto values = [&](int w, int k, uint32_t v, bool add) {
+      auto values = [&](int w, uint32_t v, bool add) {
         const uint64_t vd = sw128_desc_mn(v, BN * 128);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (ok && !mbar_wait(half ? &p_full[w] : &p_half[w], k & 1, c.status, W_ATT_PROMPT)) ok = false;
+          wait(half ? &p_full[w] : &p_half[w], kp[w]);
           if (!ok) return;
           tc_fence_after();
 #pragma unroll
@@ -331,213 +341,414 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
               tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + 128 * w + part * (BN / 2) + 8 * ks, vd + ks * 2048 / 16,
                         id_o, add || half > 0 || part > 0 || ks > 0);
         }
+        ++kp[w];
       };
-      if (!mbar_wait(&q_full, 0, c.status, W_ATT_PROMPT)) ok = false;
-      if constexpr (TWO) {
-        uint32_t k = stage_wait();
-        if (ok) {
+      // Before an item's first products into the accumulators: the last item's
+      // results have been read from them.
+      auto results_read = [&](int w) {
+        if (used > 0) wait(&o_empty[w], used - 1);
+        tc_fence_after();
+      };
+      for (int n = 0; ok; ++n) {
+        if (!item_wait(n)) break;
+        const int valid = items[n & 1].valid, nt = items[n & 1].t1 - items[n & 1].t0;
+        mbar_arrive(&item_empty[n & 1]);
+        if (!valid) break;
+        if (nt <= 0) continue;
+        wait(&q_full, used);
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (TWO) {
+          uint32_t k = stage_wait();
+          if (!ok) break;
           scores(0, k);
           scores(1, k);
           tc_commit(&kv_empty[it % ST]);
-        }
-        ++it;
-        for (int t = 0; t < nt && ok; ++t) {
-          const int v_it = it;
-          const uint32_t v = stage_wait();
           ++it;
-          const bool more = t + 1 < nt;
-          k = 0;
+          if (nt == 1) tc_commit(&q_empty);
+          for (int t = 0; t < nt && ok; ++t) {
+            const int v_it = it;
+            const uint32_t v = stage_wait();
+            ++it;
+            const bool more = t + 1 < nt;
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            values(w, t, v, t > 0);
-            if (!ok) break;
-            if (w == 1) tc_commit(&kv_empty[v_it % ST]);
-            if (!more) {
-              tc_commit(&o_full[w]);
-              continue;
+            for (int w = 0; w < 2; ++w) {
+              if (t == 0) results_read(w);
+              values(w, v, t > 0);
+              if (!ok) break;
+              if (w == 1) tc_commit(&kv_empty[v_it % ST]);
+              if (!more) {
+                tc_commit(&o_full[w]);
+                continue;
+              }
+              if (w == 0) k = stage_wait();
+              if (!ok) break;
+              scores(w, k);
             }
-            if (w == 0) k = stage_wait();
-            if (!ok) break;
-            scores(w, k);
+            if (ok && more) {
+              tc_commit(&kv_empty[it % ST]);
+              ++it;
+              if (t + 2 == nt) tc_commit(&q_empty);
+            }
           }
-          if (ok && more) tc_commit(&kv_empty[it % ST]);
-          if (more) ++it;
-        }
-      } else {
-        for (int w = 0; w < NS && w < nt && ok; ++w) {
-          const uint32_t k = stage_wait();
-          if (!ok) break;
-          scores(w, k);
-          tc_commit(&kv_empty[it % ST]);
-          ++it;
-        }
-        for (int t = 0; t < nt && ok; ++t) {
-          const int w = t % NS;
-          const uint32_t v = stage_wait();
-          values(w, t / NS, v, t >= NS);
-          if (!ok) break;
-          tc_commit(&kv_empty[it % ST]);
-          ++it;
-          if (t + NS < nt) {
+        } else {
+          for (int w = 0; w < NS && w < nt && ok; ++w) {
             const uint32_t k = stage_wait();
             if (!ok) break;
             scores(w, k);
             tc_commit(&kv_empty[it % ST]);
             ++it;
-          } else {
-            tc_commit(&o_full[w]);
+          }
+          if (ok && nt <= NS) tc_commit(&q_empty);
+#pragma unroll
+          for (int w = 0; w < NS; ++w) results_read(w);
+          for (int t = 0; t < nt && ok; ++t) {
+            const int w = t % NS;
+            const uint32_t v = stage_wait();
+            values(w, v, t >= NS);
+            if (!ok) break;
+            tc_commit(&kv_empty[it % ST]);
+            ++it;
+            if (t + NS < nt) {
+              const uint32_t k = stage_wait();
+              if (!ok) break;
+              scores(w, k);
+              tc_commit(&kv_empty[it % ST]);
+              ++it;
+              if (t + NS + 1 == nt) tc_commit(&q_empty);
+            } else {
+              tc_commit(&o_full[w]);
+            }
           }
         }
+        ++used;
       }
       // The tensor cores are done with TMEM and shared memory.
       tc_commit(&drained);
       mbar_wait(&drained, 0, c.status, W_ATT_PROMPT);
     }
-  } else if (warp < W_TMA) {
+  } else if (warp >= W_AUX) {
+    // ---- the next item, and its queries -----------------------------------------
+    const bool finder = warp == W_AUX;
+    // Row tiles of an entry (0 where its rows are out of order).
+    auto tiles_of = [&](int i, int& lo, int& hi) {
+      lo = hi = 0;
+      if (i < a.n) {
+        lo = a.row_start[i];
+        hi = a.row_start[i + 1];
+        if (lo < 0 || hi < lo || hi > a.n_rows) {
+          if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
+          lo = hi = 0;
+        }
+      }
+      return (int)(((int64_t)(hi - lo) * group + S::QT * PM - 1) / (S::QT * PM));
+    };
+    auto scan = [&](int v) {  // inclusive, over the warp
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+      }
+      return v;
+    };
+    // Up to 32 entries are taken in the order of their positions, most last
+    // (items are dealt from the end); this lane holds the lane-th of them.
+    int e_i = lane, e_lo = 0, e_hi = 0, e_len = 0, e_sum = 0, tiles = 0;
+    const bool sorted = a.n <= 32;
+    if (finder) {
+      if (sorted) {
+        const int s = lane < a.n ? (a.seqs ? a.seqs[lane] : lane) : -1;
+        const int len = s >= 0 && s < c.n_seq ? kv_len(c, s) : 0;
+        int rank = 0;
+        for (int j = 0; j < 32; ++j) {
+          const int other = __shfl_sync(0xffffffffu, len, j);
+          rank += other < len || (other == len && j < lane);
+        }
+        for (int j = 0; j < 32; ++j)
+          if (__shfl_sync(0xffffffffu, rank, j) == lane) e_i = j;
+        const int m = tiles_of(e_i, e_lo, e_hi);
+        e_len = __shfl_sync(0xffffffffu, len, e_i);
+        e_sum = scan(m);
+        tiles = __shfl_sync(0xffffffffu, e_sum, 31);
+      } else {
+        int m = 0, lo, hi;
+        for (int b = 0; b < a.n; b += 32) m += tiles_of(b + lane, lo, hi);
+        tiles = __shfl_sync(0xffffffffu, scan(m), 31);
+      }
+    }
+    const int64_t total = (int64_t)tiles * c.nkv * d.splits;
+    int used = 0;
+    int64_t idx = blockIdx.x;  // the block's first item; the rest as it comes to them
+    for (int n = 0; ok; ++n) {
+      Item x{};
+      if (finder) {
+        while (true) {
+          x.valid = idx < total;
+          if (!x.valid) break;
+          x.split = (int)(idx % d.splits);
+          x.unit = (int)(total / d.splits - 1 - idx / d.splits);
+          int more = 0;
+          if (lane == 0) more = atomicAdd(d.next, 1);
+          idx = (int64_t)gridDim.x + __shfl_sync(0xffffffffu, more, 0);
+          x.kvh = x.unit % c.nkv;
+          int t = x.unit / c.nkv, l = 0, i = 0;
+          if (sorted) {
+            l = __ffs(__ballot_sync(0xffffffffu, t < e_sum)) - 1;
+            i = __shfl_sync(0xffffffffu, e_i, l);
+            x.start = __shfl_sync(0xffffffffu, e_lo, l);
+            x.count = __shfl_sync(0xffffffffu, e_hi, l) - x.start;
+            x.len = __shfl_sync(0xffffffffu, e_len, l);
+            if (l > 0) t -= __shfl_sync(0xffffffffu, e_sum, l - 1);
+          } else {
+            for (int b = 0; b < a.n; b += 32) {
+              int lo, hi;
+              const int m = tiles_of(b + lane, lo, hi), y = scan(m);
+              const unsigned at = __ballot_sync(0xffffffffu, t < y);
+              if (at) {
+                l = __ffs(at) - 1;
+                i = b + l;
+                x.start = __shfl_sync(0xffffffffu, lo, l);
+                x.count = __shfl_sync(0xffffffffu, hi, l) - x.start;
+                t -= __shfl_sync(0xffffffffu, y - m, l);
+                break;
+              }
+              t -= __shfl_sync(0xffffffffu, y, 31);
+            }
+          }
+          x.row0 = t * S::QT * PM;
+          x.s = a.seqs ? a.seqs[i] : i;
+          if (x.s < 0 || x.s >= c.n_seq) {
+            if (lane == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
+            continue;
+          }
+          if (!sorted) x.len = kv_len(c, x.s);
+          x.rows = min(S::QT * PM, x.count * group - x.row0);
+          // Positions of the first and last row, and the tiles they see.
+          const int at0 = x.len - x.count + x.row0 / group, at1 = x.len - x.count + (x.row0 + x.rows - 1) / group;
+          x.head = x.w0 = x.nt = 0;
+          if (at1 >= 0) {
+            const int lo = a.window > 0 ? max(0, at0 - a.window + 1) : 0;
+            x.head = (min(a.sinks, lo) + BN - 1) / BN;
+            x.w0 = max(lo / BN, x.head);
+            x.nt = x.head + at1 / BN + 1 - x.w0;
+          }
+          // At least four tiles to a part: a join takes about as long.
+          x.splits = max(1, min(d.splits, x.nt / 4));
+          if (x.split >= x.splits) continue;
+          x.t0 = (int)((int64_t)x.nt * x.split / x.splits);
+          x.t1 = (int)((int64_t)x.nt * (x.split + 1) / x.splits);
+          break;
+        }
+        if (n >= 2) wait(&item_empty[n & 1], (n >> 1) - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          items[n & 1] = x;
+          mbar_arrive(&item_full[n & 1]);
+        }
+      } else {
+        item_wait(n);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        x = items[n & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[n & 1]);
+      }
+      if (!x.valid) break;
+      if (x.nt <= 0) continue;
+      if (used > 0) wait(&q_empty, used - 1);
+      ++used;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const RowMap rm(x.row0, group);
+      const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride + (int64_t)x.kvh * group * c.hd;
+      const int loader = tid - 32 * W_AUX;
+      constexpr int TILE_Q = (kSplit ? 2 : 1) * S::QB;
+      if (!kSplit && d.q_map) {
+        // As they are: a box per tile and 64 columns. (Rows past the entry's
+        // are another's or zeros; nothing comes of them.)
+        if (finder && lane == 0) {
+          mbar_expect_tx(&q_full, S::Q_ALL);
+          for (int y = 0; y < S::QT; ++y)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              tma_load_3d(q_sm + y * TILE_Q + b * PM * 128, &q_map, 64 * b, x.kvh * group,
+                          x.start + rm.tok0 + y * (PM / group), &q_full);
+        } else if (lane == 0) {
+          mbar_arrive(&q_full);
+        }
+        continue;
+      }
+      {
+        // Eight lanes per row, eight values of each 64 a lane.
+        const bool wide = !((uintptr_t)a.q % 16) && a.q_stride * sizeof(TQ) % 16 == 0;
+        const int part = loader & 7;
+        constexpr int BATCH = NB <= 2 ? 4 : 1;  // rows of a lane under way
+        for (int f0 = loader >> 3; f0 < S::QT * PM; f0 += 8 * BATCH) {
+          float v[BATCH][NB][8];
+#pragma unroll
+          for (int y = 0; y < BATCH; ++y) {
+            const int f = f0 + 8 * y;
+            const TQ* from = q + rm.offset(f < x.rows ? f : 0, a.q_stride, c.hd) + 8 * part;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+              const bool real = f < x.rows && 64 * j + 8 * part < c.hd;
+              if (real && wide) {
+                load8(from + 64 * j, v[y][j]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[y][j][e] = real ? (float)from[64 * j + e] : 0.f;
+              }
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < BATCH; ++y) {
+            const int rr = (f0 + 8 * y) & (PM - 1), tile = (f0 + 8 * y) >> 7;
+            float f = 1.f;
+            if constexpr (kSplit) {
+              // A power of two puts the row's largest value in [2^14, 2^15).
+              float amax = 0.f;
+#pragma unroll
+              for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[y][j][e]));
+#pragma unroll
+              for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+              f = pow2_factor(amax);
+              if (part == 0) factor_sh[(used - 1) & 1][tile][rr] = f;
+            }
+            f *= flip;
+            uint8_t* to = q_sm + tile * TILE_Q + rr * 128 + ((part ^ (rr & 7)) << 4);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+              uint32_t hi[4], rest[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float z0 = v[y][j][2 * e] * f, z1 = v[y][j][2 * e + 1] * f;
+                hi[e] = pack2<TKV>(z0, z1);
+                if constexpr (kSplit) rest[e] = rest2<TKV>(z0, z1, hi[e]);
+              }
+              *reinterpret_cast<uint4*>(to + j * PM * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if constexpr (kSplit)
+                *reinterpret_cast<uint4*>(to + S::QB + j * PM * 128) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            }
+          }
+        }
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
+    // The last block to find nothing left puts the counters back.
+    if (finder && lane == 0 && atomicAdd(d.next + 1, 1) == (int)gridDim.x - 1) d.next[0] = d.next[1] = 0;
+  } else {
     if constexpr (NS == 2) regs_up<kSoftmaxRegs>();
     // ---- softmax: stream w, a thread per row ---------------------------------
     const int w = warp >> 2, r = tid & 127, my_tile = TWO ? w : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_t = tmem + lanes + 128 * w, o_t = tmem + lanes + S::T_O + w * S::HD;
-    const TQ* q = static_cast<const TQ*>(a.q);
-    const float flip = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;  // score factors are positive: see below
-    // Row f of the block: its token among the sequence's rows, its head of the
-    // group ((x * magic) >> 16 = x / group for x < 512, group <= 128).
-    const int tok0 = rt.row0 / group, rem = rt.row0 - tok0 * group;
-    const uint32_t magic = 65536u / group + 1;
-    auto token = [&](int f) { return tok0 + (int)(((uint32_t)(rem + f) * magic) >> 16); };
-    auto row_of = [&](int f, int64_t stride) {
-      const int t = token(f);
-      return (int64_t)(rt.start + t) * stride + (int64_t)(kvh * group + rem + f - (t - tok0) * group) * c.hd;
-    };
-    // ---- queries into shared memory ------------------------------------------
-    constexpr int LOADERS = TWO ? 128 : 128 * NS;
-    const int loader = TWO ? r : tid;
-    bool copied = false;
-    if constexpr (!kSplit) {
-      copied = flip == 1.f && !((uintptr_t)a.q % 16) && a.q_stride % 8 == 0;
-      if (copied) {
-#pragma unroll 8
-        for (int y = loader; y < PM * 8 * NB; y += LOADERS) {
-          const int rr = y / (8 * NB), p = y - rr * 8 * NB, f = my_tile * PM + rr;
-          const bool real = f < rows && 8 * p < c.hd;
-          copy16_async(smem_u32(q_sm + my_tile * S::QB) + (p >> 3) * PM * 128 + (rr >> 3) * 1024 + (rr & 7) * 128 +
-                           (((p & 7) ^ (rr & 7)) << 4),
-                       real ? q + row_of(f, a.q_stride) + 8 * p : q, real);
+    const uint32_t s_t = tmem + lanes + 128 * w;
+    const float unit = flip == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    int ks = 0, used = 0, ring_at = 0;  // score tiles, items with products, loads before this item's
+    int full[NS] = {}, parts = 0;       // results of each stream, split items before this one
+    for (int n = 0;; ++n) {
+      item_wait(n);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const Item& x = items[n & 1];  // (given back at the end: read from there as needed, it takes no registers)
+      if (!x.valid) break;
+      const RowMap rm(x.row0, group);
+      const int f = my_tile * PM + r, nt = x.t1 - x.t0, at_base = x.len - x.count;
+      const bool real = f < x.rows;
+      const int at = real ? at_base + rm.token(f) : -1;
+      const int lo = a.window > 0 ? at - a.window + 1 : 0;
+      // Tiles whose positions every row of this tile sees need no mask.
+      const int t_at0 = at_base + rm.token(my_tile * PM);
+      const int t_lo1 = a.window > 0 ? at_base + rm.token(min(x.rows, (my_tile + 1) * PM) - 1) - a.window + 1 : 0;
+      float m = -INFINITY, l = 0.f;
+      // Stream w's k-th tile is k (two row tiles) or NS k + w.
+      const int mine = TWO ? nt : (nt - w + NS - 1) / NS;
+      // Base-2 exponents per score unit (a zero scale has zero queries instead,
+      // so that a masked score's -inf survives the product).
+      float cq = unit;
+      const uint32_t o_t = tmem + lanes + S::T_O + w * S::HD;
+      for (int k = 0; k < mine; ++k, ++ks) {
+        const int t = TWO ? k : NS * k + w, j0 = x.pos(x.t0 + t, BN);
+        wait(&s_full[w], ks);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
         }
-        copies_wait();
-      }
-    }
-    if (!copied) {
-      // A warp per row, four values a lane.
-      const bool wide = !((uintptr_t)a.q % (4 * sizeof(TQ))) && a.q_stride % 4 == 0;
-      constexpr int H = NB <= 2 ? 1 : 2, BATCH = 8, ROWS = 32 * PM / LOADERS;  // rows of a warp
-      const int first = loader / 32 * ROWS;
-      for (int x0 = 0; x0 < ROWS; x0 += BATCH) {
-        float v[BATCH][H][4];
+        tc_fence_after();
+        if constexpr (kSplit)
+          if (k == 0) cq = __fdiv_rn(unit, factor_sh[used & 1][my_tile][r]);
+        float s[BN];
 #pragma unroll
-        for (int y = 0; y < BATCH; ++y) {
-          const int f = my_tile * PM + first + x0 + y;
-          const TQ* from = q + row_of(f < rows ? f : 0, a.q_stride);
+        for (int e = 0; e < BN; e += 32) tmem_ld32(s_t + e, s + e);
+        tmem_wait_ld();
+        if (j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks)) {
+          // A bit per position: up to the row's own, and not before its window
+          // unless among the first tokens.
+          const int hi = at - j0, from = lo - j0, first = a.sinks - j0;
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int d = 4 * lane + 128 * h;
+          for (int y = 0; y < BN; y += 32) {
+            const uint32_t see = low_bits(hi + 1 - y) & (~low_bits(from - y) | low_bits(first - y));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[y][h][e] = 0.f;
-            if (f < rows && d < c.hd) {
-              if (wide) {
-                load4(from + d, v[y][h]);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[y][h][e] = (float)from[d + e];
-              }
-            }
+            for (int e = 0; e < 32; ++e) s[y + e] = see >> e & 1 ? s[y + e] : -INFINITY;
           }
         }
-#pragma unroll
-        for (int y = 0; y < BATCH; ++y) {
-          const int rr = first + x0 + y;
-          float f = 1.f;
-          if constexpr (kSplit) {
-            // A power of two puts the row's largest value in [2^14, 2^15).
-            float amax = 0.f;
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(v[y][h][e]));
-#pragma unroll
-            for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            f = pow2_factor(amax);
-            if (lane == 0) factor_sh[my_tile][rr] = f;
-          }
-          f *= flip;
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int d = 4 * lane + 128 * h;
-            if (d >= S::HD) continue;
-            uint8_t* to = q_sm + my_tile * (kSplit ? 2 : 1) * S::QB + (d >> 6) * PM * 128 + (rr >> 3) * 1024 +
-                          (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 7) * 2;
-            float z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = v[y][h][e] * f;
-            const uint32_t h0 = pack2<TKV>(z[0], z[1]), h1 = pack2<TKV>(z[2], z[3]);
-            *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
-            if constexpr (kSplit)
-              *reinterpret_cast<uint2*>(to + S::QB) = make_uint2(rest2<TKV>(z[0], z[1], h0), rest2<TKV>(z[2], z[3], h1));
-          }
+        if (j0 + BN > x.len) {
+          // Rows past the sequence's end hold whatever the page held before:
+          // zeros in their place (only the last tile has such rows; its V is
+          // the item's last load).
+          const int v_it = ring_at + 2 * nt - 1, st = v_it % ST;
+          wait(&kv_full[st], v_it / ST);
+          uint8_t* v = ring + st * S::KV;
+          for (int y = r; y < BN * 8 * NB; y += 128)
+            if (j0 + ((y >> 3) & (BN - 1)) >= x.len) *reinterpret_cast<uint4*>(v + y * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_shared();
         }
-      }
-    }
-    fence_async_shared();
-    mbar_arrive(&q_full);
-    const int f = my_tile * PM + r;
-    const bool real = f < rows;
-    const int at = real ? rt.len - rt.count + token(f) : -1;
-    const int lo = a.window > 0 ? at - a.window + 1 : 0;
-    // Tiles whose positions every row of this tile sees need no mask.
-    const int t_at0 = rt.len - rt.count + token(my_tile * PM);
-    const int t_lo1 =
-        a.window > 0 ? rt.len - rt.count + token(min(rows, (my_tile + 1) * PM) - 1) - a.window + 1 : 0;
-    float cq = 0.f, m = -INFINITY, l = 0.f;
-    const int mine = tiles_of(w);
-    if (mine > 0 && !mbar_wait(&q_full, 0, c.status, W_ATT_PROMPT)) ok = false;
-    // Base-2 exponents per score unit (a zero scale has zero queries instead,
-    // so that a masked score's -inf survives the product).
-    cq = flip == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
-    if constexpr (kSplit) cq = __fdiv_rn(cq, factor_sh[my_tile][r]);
-    for (int k = 0; k < mine; ++k) {
-      const int t = TWO ? k : NS * k + w, j0 = span.start(t, BN);
-      if (ok && !mbar_wait(&s_full[w], k & 1, c.status, W_ATT_PROMPT)) ok = false;
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float s[BN];
+        // Weights of half the tile's positions against maximum mx.
+        auto weigh = [&](int half, float mx, uint32_t* p, uint32_t* rest) {
+          const float base = kLift - (mx == -INFINITY ? 0.f : mx);
+          const uint64_t cq2 = f2(cq, cq), base2 = f2(base, base);
+          uint64_t sum = 0;
 #pragma unroll
-      for (int x = 0; x < BN; x += 32) tmem_ld32(s_t + x, s + x);
-      tmem_wait_ld();
-      if (j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks)) {
-        // A bit per position: up to the row's own, and not before its window
-        // unless among the first tokens.
-        const int hi = at - j0, from = lo - j0, first = a.sinks - j0;
+          for (int e = 0; e < BN / 4; ++e) {
+            const int i = half * (BN / 2) + 2 * e;
+            float2 y = f2(fma2(f2(s[i], s[i + 1]), cq2, base2));
+            y.x = exp2_fast(y.x);
+            y.y = exp2_fast(y.y);
+            sum = add2(sum, f2(y.x, y.y));
+            p[e] = pack2<TKV>(y.x, y.y);
+            if constexpr (kSplit) rest[e] = rest2<TKV>(y.x, y.y, p[e]);
+          }
+          return f2(sum).x + f2(sum).y;
+        };
+        auto hand_over = [&](int half, const uint32_t* p, const uint32_t* rest) {
 #pragma unroll
-        for (int x = 0; x < BN; x += 32) {
-          const uint32_t see = low_bits(hi + 1 - x) & (~low_bits(from - x) | low_bits(first - x));
+          for (int e = 0; e < BN / 4; e += 16) {
+            tmem_st16(s_t + half * (BN / 4) + e, p + e);
+            if constexpr (kSplit) tmem_st16(s_t + BN / 2 + half * (BN / 4) + e, rest + e);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(half ? &p_full[w] : &p_half[w]);
+        };
+        float tops[8];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[x + e] = see >> e & 1 ? s[x + e] : -INFINITY;
-        }
-      }
-      float tops[8];
+        for (int e = 0; e < 8; ++e) tops[e] = s[e];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) tops[x] = s[x];
-#pragma unroll
-      for (int x = 8; x < BN; x += 2) tops[x / 2 & 7] = max3(tops[x / 2 & 7], s[x], s[x + 1]);
-      float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
-      top = top == -INFINITY ? top : top * cq;
-      if (k == 0) {
-        m = top;
-      } else {
+        for (int e = 8; e < BN; e += 2) tops[e / 2 & 7] = max3(tops[e / 2 & 7], s[e], s[e + 1]);
+        float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
+        top = top == -INFINITY ? top : top * cq;
+        if (k == 0) m = top;
+        // 16-bit weights of the first half are computed against the maximum so
+        // far while this tile's is found, and again in the rare case that it has
+        // grown too much. (With two operands that takes more registers than
+        // there are.)
+        uint32_t p[BN / 4], rest[kSplit ? BN / 4 : 1];
+        float sum = 0.f;
+        if constexpr (!kSplit) sum = weigh(0, m, p, rest);
         const bool grow = top > m + kGrow;
         if (__any_sync(0xffffffffu, grow)) {
           // The products before these scores are complete, and the next ones
@@ -545,143 +756,169 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           const float shrink = grow ? exp2_fast(m - top) : 1.f;
           if (grow) m = top;
           l *= shrink;
-          for (int x = 0; x < hd16; x += 16) {
+          for (int e0 = 0; e0 < hd16; e0 += 16) {
             float o[16];
-            tmem_ld16(o_t + x, o);
+            tmem_ld16(o_t + e0, o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] *= shrink;
-            tmem_st16(o_t + x, o);
+            tmem_st16(o_t + e0, o);
           }
-          tmem_wait_st();
+          if constexpr (!kSplit) sum = weigh(0, m, p, rest);
         }
+        if constexpr (kSplit) sum = weigh(0, m, p, rest);
+        hand_over(0, p, rest);
+        sum += weigh(1, m, p, rest);
+        hand_over(1, p, rest);
+        l += sum;
       }
-      if (t == nt - 1 && j0 + BN > rt.len) {
-        // Rows past the sequence's end hold whatever the page held before:
-        // zeros in their place (the last V is the last load of the ring).
-        const int v_it = 2 * nt - 1, st = v_it % ST;
-        if (!mbar_wait(&kv_full[st], (v_it / ST) & 1, c.status, W_ATT_PROMPT)) ok = false;
-        uint8_t* v = ring + st * S::KV;
-        for (int y = r; y < BN * 8 * NB; y += 128)
-          if (j0 + ((y >> 3) & (BN - 1)) >= rt.len) *reinterpret_cast<uint4*>(v + y * 16) = make_uint4(0, 0, 0, 0);
-        fence_async_shared();
-      }
-      const float base = kLift - (m == -INFINITY ? 0.f : m);
-      const uint64_t cq2 = f2(cq, cq), base2 = f2(base, base);
-      uint64_t sum = 0;
-#pragma unroll
-      for (int x = 0; x < BN; x += 32) {
-        uint32_t p[16], rest[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 y = f2(fma2(f2(s[x + 2 * e], s[x + 2 * e + 1]), cq2, base2));
-          if (!kSplit && e % kCubicEvery == kCubicEvery - 1) {
-            y = exp2_cubic(y);
-          } else {
-            y.x = exp2_fast(y.x);
-            y.y = exp2_fast(y.y);
-          }
-          sum = add2(sum, f2(y.x, y.y));
-          p[e] = pack2<TKV>(y.x, y.y);
-          if constexpr (kSplit) rest[e] = rest2<TKV>(y.x, y.y, p[e]);
-        }
-        tmem_st16(s_t + x / 2, p);
-        if constexpr (kSplit) tmem_st16(s_t + BN / 2 + x / 2, rest);
-        if (x == BN / 2 - 32 || x == BN - 32) {
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(x == BN - 32 ? &p_full[w] : &p_half[w]);
-        }
-      }
-      l += f2(sum).x + f2(sum).y;
-    }
-    if (ok && mine > 0 && !mbar_wait(&o_full[w], 0, c.status, W_ATT_PROMPT)) ok = false;
-    ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
 
-    // ---- the streams' join, and the result -------------------------------------
-    float* join = reinterpret_cast<float*>(q_sm);
-    float mine_f = 1.f, their_f = 0.f;
-    const bool two = NS == 2 && !TWO && nt > 1;
-    if (two) {
-      // Both streams' products are complete (each waited for its own) when
-      // both have come to the first barrier: shared memory is free.
-      named_sync(1, 256);
-      if (w == 1) {
-        join[r * S::JOIN_LD + S::HD] = m;
-        join[r * S::JOIN_LD + S::HD + 1] = l;
-        for (int x = 0; x < hd16; x += 16) {
-          float o[16];
-          tmem_ld16(o_t + x, o);
-          tmem_wait_ld();
+      // ---- the item's result -------------------------------------------------------
+      // Of one row tile both streams' warps write half the columns each, from
+      // both accumulators (a warp reads the lanes of its quarter, whoever's).
+      constexpr bool kJoin = NS == 2 && !TWO;
+      const int half = kJoin ? (hd16 / 16 + 1) / 2 * 16 : hd16;
+      const int col0 = kJoin && w == 1 ? half : 0, col1 = kJoin && w == 0 ? half : hd16;
+      float scale_of[NS];  // what each accumulator counts
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(join + r * S::JOIN_LD + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      for (int v = 0; v < NS; ++v) scale_of[v] = 1.f;
+      if (nt > 0) {
+#pragma unroll
+        for (int v = 0; v < NS; ++v)
+          if (TWO ? v == w : v < nt) wait(&o_full[v], full[v]++);
+        if constexpr (kJoin) {
+          join_sh[used & 1][w][r] = make_float2(m, l);
+          mbar_arrive(&join_full);
+          wait(&join_full, used);
+          const float2 o = join_sh[used & 1][w ^ 1][r];
+          const float mn = fmaxf(m, o.x);
+          const float mine_f = mn == -INFINITY ? 0.f : exp2_fast(m - mn);
+          const float their_f = mn == -INFINITY ? 0.f : exp2_fast(o.x - mn);
+          // The same order of operations on both sides.
+          l = w == 0 ? __fmaf_rn(l, mine_f, o.y * their_f) : __fmaf_rn(o.y, their_f, l * mine_f);
+          m = mn;
+          scale_of[w] = mine_f;
+          scale_of[w ^ 1] = their_f;
         }
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
       }
-      named_sync(1, 256);
-      if (w == 0) {
-        const float m1 = join[r * S::JOIN_LD + S::HD], l1 = join[r * S::JOIN_LD + S::HD + 1], mn = fmaxf(m, m1);
-        if (mn != -INFINITY) {
-          mine_f = exp2_fast(m - mn);
-          their_f = exp2_fast(m1 - mn);
-        }
-        l = __fmaf_rn(l, mine_f, l1 * their_f);
-      }
-    }
-    if (TWO || w == 0) {
-      // Rows go out through shared memory (this warp's 32, 16-byte pieces
-      // swizzled), so that a warp's stores cover whole lines.
-      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-      constexpr int PIECES = S::HD * sizeof(TQ) / 16, PER = 16 / sizeof(TQ);
-      uint8_t* stage = q_sm + (TWO ? my_tile * S::QB : S::OUT_AT) +
-                       (warp & 3) * 32 * PIECES * 16;
+      const bool split = x.splits > 1;
+      TQ* out = static_cast<TQ*>(a.out) + (int64_t)x.start * a.out_stride + (int64_t)x.kvh * group * c.hd;
+      const uint32_t grain = (uint32_t)((uintptr_t)a.out | (uint64_t)a.out_stride * sizeof(TQ) | c.hd * sizeof(TQ));
+      float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
       bool bad = l != l || l == INFINITY;
-      for (int x = 0; x < hd16; x += 16) {
-        float o[16];
-        if (ok && mine > 0) {
-          tmem_ld16(o_t + x, o);
+      TQ* to_row = out + rm.offset(real ? f : 0, a.out_stride, c.hd);
+      float* part_row = d.part + (((int64_t)x.unit * d.splits + x.split) * PM + r) * S::LD;
+      for (int e0 = col0; e0 < col1; e0 += 32) {
+        float o[2][16];
+        const uint32_t o_0 = tmem + lanes + S::T_O + (TWO ? w : 0) * S::HD + e0;
+        const bool both = e0 + 16 < col1;
+        if (nt > 0 && ok) {
+          tmem_ld16(o_0, o[0]);
+          if (both) tmem_ld16(o_0 + 16, o[1]);
+          if (kJoin && nt > 1) {
+            float o1[2][16];
+            tmem_ld16(o_0 + S::HD, o1[0]);
+            if (both) tmem_ld16(o_0 + S::HD + 16, o1[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e >> 4][e & 15] = __fmaf_rn(o[e >> 4][e & 15], scale_of[0], o1[e >> 4][e & 15] * scale_of[NS - 1]);
+          }
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+          for (int e = 0; e < 32; ++e) o[e >> 4][e & 15] = 0.f;
         }
-        if (two)
+        if (!real) continue;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __fmaf_rn(o[e], mine_f, join[r * S::JOIN_LD + x + e] * their_f);
+        for (int y = 0; y < 2; ++y) {
+          if (y && !both) break;
+          const int e1 = e0 + 16 * y;
+          if (split) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          bad |= !(fabsf(o[e]) <= 3.4028234e38f);
-          o[e] = l == 0.f ? 0.f : o[e] * inv;
-        }
-#pragma unroll
-        for (int p = 0; p < 16 / PER; ++p)
-          store_piece(reinterpret_cast<TQ*>(stage + (lane * PIECES + ((x / PER + p) ^ (lane & 7))) * 16), o + p * PER);
-      }
-      __syncwarp();
-      const bool wide = !((uintptr_t)a.out % 16) && a.out_stride * sizeof(TQ) % 16 == 0;
-      const int first = my_tile * PM + 32 * (warp & 3);  // the warp's first row
-#pragma unroll 4
-      for (int y = lane; y < 32 * PIECES; y += 32) {
-        const int row = y / PIECES, p = y - row * PIECES;
-        if (first + row >= rows || p * PER >= c.hd) continue;
-        TQ* to = static_cast<TQ*>(a.out) + row_of(first + row, a.out_stride) + p * PER;
-        const uint8_t* from = stage + (row * PIECES + (p ^ (row & 7))) * 16;
-        if (wide) {
-          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-        } else {
-#pragma unroll
-          for (int e = 0; e < PER; ++e) to[e] = reinterpret_cast<const TQ*>(from)[e];
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(part_row + e1 + e) =
+                  make_float4(o[y][e], o[y][e + 1], o[y][e + 2], o[y][e + 3]);
+            if (e1 == 0) *reinterpret_cast<float2*>(part_row + S::HD) = make_float2(m, l);
+            continue;
+          }
+          bad |= normalise16(o[y], inv);
+          store16(to_row + e1, o[y], c.hd - e1, grain);
         }
       }
-      __syncwarp();
+      if (nt > 0) {
+        tc_fence_before();
+#pragma unroll
+        for (int v = 0; v < NS; ++v)
+          if (!TWO || v == w) mbar_arrive(&o_empty[v]);
+        ++used;
+        ring_at += 2 * nt;
+      }
+      bool write = !split;
+      if (split) {
+        // The parts in their order, by the block that brings the last one.
+        __threadfence();
+        mbar_arrive(&part_full);
+        if (tid == 0) {
+          wait(&part_full, parts);
+          last_sh = ok && atomicAdd(d.count + x.unit, 1) == x.splits - 1;
+          if (last_sh) d.count[x.unit] = 0;
+          __threadfence();
+          mbar_arrive(&last_full);
+        }
+        wait(&last_full, parts);
+        ++parts;
+        ok = __all_sync(0xffffffffu, ok);
+        write = ok && last_sh;
+        if (write) {
+          __threadfence();
+          const float* from = d.part + ((int64_t)x.unit * d.splits * PM + r) * S::LD;
+          const int64_t next = (int64_t)PM * S::LD;
+          float top = -INFINITY;
+          l = 0.f;
+          if (real) {
+            for (int p = 0; p < x.splits; ++p) top = fmaxf(top, __ldcg(from + p * next + S::HD));
+            for (int p = 0; p < x.splits; ++p) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + p * next + S::HD));
+              l = __fmaf_rn(top == -INFINITY ? 0.f : exp2_fast(ml.x - top), ml.y, l);
+            }
+          }
+          inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+          bad = l != l || l == INFINITY;
+          for (int e0 = col0; e0 < col1 && real; e0 += 16) {
+            float o[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0.f;
+            for (int p = 0; p < x.splits; ++p) {
+              const float wt = top == -INFINITY ? 0.f : exp2_fast(__ldcg(from + p * next + S::HD) - top);
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(from + p * next + e0 + e));
+                o[e] = __fmaf_rn(wt, y.x, o[e]);
+                o[e + 1] = __fmaf_rn(wt, y.y, o[e + 1]);
+                o[e + 2] = __fmaf_rn(wt, y.z, o[e + 2]);
+                o[e + 3] = __fmaf_rn(wt, y.w, o[e + 3]);
+              }
+            }
+            bad |= normalise16(o, inv);
+            store16(to_row + e0, o, c.hd - e0, grain);
+          }
+        }
+      }
       // A row that a value beyond its mask has spoilt (or that sees one that is
       // not finite) is computed again by itself.
-      for (unsigned again = __ballot_sync(0xffffffffu, ok && real && bad); again; again &= again - 1) {
-        const int f1 = first + __ffs(again) - 1;
-        prompt_row<TQ, TKV>(a, rt.s, kvh, rt.len - rt.count + token(f1), q + row_of(f1, a.q_stride),
-                            static_cast<TQ*>(a.out) + row_of(f1, a.out_stride));
+      for (unsigned again = __ballot_sync(0xffffffffu, ok && write && real && bad); again; again &= again - 1) {
+        const int f1 = my_tile * PM + 32 * (warp & 3) + __ffs(again) - 1;
+        prompt_row<TQ, TKV>(a, x.s, x.kvh, at_base + rm.token(f1),
+                            static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride +
+                                (int64_t)x.kvh * group * c.hd + rm.offset(f1, a.q_stride, c.hd),
+                            out + rm.offset(f1, a.out_stride, c.hd), col0, min(col1, c.hd));
       }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[n & 1]);
     }
   }
   tc_fence_before();
@@ -689,44 +926,69 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   if (warp == W_MMA) tmem_free(tmem, 512);
 }
 
+// Parts of split items: what 192 items of 128 rows take at a head size of 128.
+constexpr size_t PROMPT_PART_BYTES = (size_t)192 * PM * (128 + 4) * sizeof(float);
+constexpr int PROMPT_MAX_UNITS = 192;
+size_t attn_prompt_part_bytes() { return PROMPT_PART_BYTES; }
+int attn_prompt_counts() { return PROMPT_MAX_UNITS + 2; }
+
 template <typename TQ, typename TKV, int NB, bool TWO>
-static int launch_prompt(const AttnArgs& a, const KvMaps& maps, cudaStream_t st) {
+static int launch_prompt(PromptArgs d, const KvMaps& maps, cudaStream_t st) {
   using S = PromptShape<TQ, NB, TWO>;
+  const AttnArgs& a = d.a;
   static PerDeviceOnce attr;
   if (smem_attr_once(attr, attn_prompt_kernel<TQ, TKV, NB, TWO>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
   // Every sequence may leave its last tile partly filled.
-  const int64_t tiles = (int64_t)a.n_rows * (a.nh / a.c.nkv) / (S::QT * PM) + std::min(a.n, a.n_rows);
-  if (tiles * a.c.nkv > INT32_MAX) return KC_ERR_SHAPE;
-  launch_k(attn_prompt_kernel<TQ, TKV, NB, TWO>, dim3((unsigned)(tiles * a.c.nkv)), S::THREADS, S::SMEM, st, a, maps);
+  const int64_t rows = (int64_t)a.n_rows * (a.nh / a.c.nkv), tile = S::QT * PM;
+  const int64_t most = (rows / tile + std::min(a.n, a.n_rows)) * a.c.nkv;
+  if (most > INT32_MAX / 16) return KC_ERR_SHAPE;
+  d.splits = 1;
+  if (!TWO) {
+    // Fewer items than SMs: their positions over as many blocks as there are,
+    // within the workspace.
+    const int64_t likely = std::max<int64_t>((rows + tile - 1) / tile, std::min(a.n, a.n_rows)) * a.c.nkv;
+    const int64_t slots = std::min<int64_t>(PROMPT_MAX_UNITS, PROMPT_PART_BYTES / ((size_t)PM * S::LD * sizeof(float)));
+    d.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, slots / most, 16}));
+  }
+  const int grid = (int)std::min<int64_t>(num_sms(), most * d.splits);
+  // 16-bit queries as they are, where a tile is whole tokens and TMA can
+  // address them; otherwise two warps bring them.
+  KvMap q_map{};
+  const int group = a.nh / a.c.nkv;
+  d.q_map = !S::kSplit && a.scale > 0.f && PM % group == 0 && !((uintptr_t)a.q % 16) && a.q_stride % 8 == 0 &&
+            make_q_map(a, q_map) == KC_OK;
+  launch_k(attn_prompt_kernel<TQ, TKV, NB, TWO>, grid, S::THREADS, S::SMEM, st, d, maps, q_map);
   return KC_OK;
 }
 
 template <typename TQ, typename TKV>
-static int launch_prompt_hd(const AttnArgs& a, const KvMaps& maps, cudaStream_t st) {
-  // Two row tiles per block read every key and value once for both; with few
-  // rows, or f32 queries (two operands each), a block takes one.
+static int launch_prompt_hd(const PromptArgs& d, const KvMaps& maps, cudaStream_t st) {
+  // Two row tiles per item read every key and value once for both; with few
+  // rows, or f32 queries (two operands each), an item is one.
+  const AttnArgs& a = d.a;
   const int64_t pairs = ((int64_t)a.n_rows * (a.nh / a.c.nkv) + 2 * PM - 1) / (2 * PM) * a.c.nkv;
   const bool two = sizeof(TQ) == 2 && pairs >= num_sms();
   switch ((a.c.hd + 63) / 64) {
     case 1:
       if constexpr (sizeof(TQ) == 2)
-        if (two) return launch_prompt<TQ, TKV, 1, true>(a, maps, st);
-      return launch_prompt<TQ, TKV, 1, false>(a, maps, st);
+        if (two) return launch_prompt<TQ, TKV, 1, true>(d, maps, st);
+      return launch_prompt<TQ, TKV, 1, false>(d, maps, st);
     case 2:
       if constexpr (sizeof(TQ) == 2)
-        if (two) return launch_prompt<TQ, TKV, 2, true>(a, maps, st);
-      return launch_prompt<TQ, TKV, 2, false>(a, maps, st);
-    case 3: return launch_prompt<TQ, TKV, 3, false>(a, maps, st);
-    default: return launch_prompt<TQ, TKV, 4, false>(a, maps, st);
+        if (two) return launch_prompt<TQ, TKV, 2, true>(d, maps, st);
+      return launch_prompt<TQ, TKV, 2, false>(d, maps, st);
+    case 3: return launch_prompt<TQ, TKV, 3, false>(d, maps, st);
+    default: return launch_prompt<TQ, TKV, 4, false>(d, maps, st);
   }
 }
 
 int attn_prompt_box_rows(int page, int hd) { return std::min(page, hd <= 128 ? 128 : 64); }
 
-int launch_attn_prompt(const AttnArgs& a, const KvMaps& maps, cudaStream_t st) {
-  if (a.c.type == T_BF16) return launch_prompt_hd<__nv_bfloat16, __nv_bfloat16>(a, maps, st);
-  if (a.t_q == T_F32) return launch_prompt_hd<float, __half>(a, maps, st);
-  return launch_prompt_hd<__half, __half>(a, maps, st);
+int launch_attn_prompt(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
+  const PromptArgs d{a, 1, part, count, count + PROMPT_MAX_UNITS, false};
+  if (a.c.type == T_BF16) return launch_prompt_hd<__nv_bfloat16, __nv_bfloat16>(d, maps, st);
+  if (a.t_q == T_F32) return launch_prompt_hd<float, __half>(d, maps, st);
+  return launch_prompt_hd<__half, __half>(d, maps, st);
 }
 
 }  // namespace kc

@@ -476,25 +476,47 @@ void launch_kv_write(const KvView& c, int layer, const int32_t* seqs, const int3
 }
 
 // ---- tensor maps -------------------------------------------------------------
-int make_kv_maps(const KvView& c, int box_rows, KvMaps& maps) {
-  cudaDriverEntryPointQueryResult q;
-  void* fn = nullptr;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-      q != cudaDriverEntryPointSuccess || !fn)
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* fn = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  return encode;
+}
+
+static int encode_16bit(KvMap& map, int t, int rank, const void* base, const cuuint64_t* dims,
+                        const cuuint64_t* strides, const cuuint32_t* box) {
+  const auto encode = tensor_map_encode();
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  if (!encode || encode(reinterpret_cast<CUtensorMap*>(map.b),
+                        t == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                        const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return KC_ERR_CUDA;
-  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  return KC_OK;
+}
+
+int make_kv_maps(const KvView& c, int box_rows, KvMaps& maps) {
   const cuuint64_t row = (cuuint64_t)c.hd * 2;
   const cuuint64_t dims[4] = {(cuuint64_t)c.hd, (cuuint64_t)c.page, (cuuint64_t)c.nkv,
                               (cuuint64_t)c.n_layer * c.n_pages};
   const cuuint64_t strides[3] = {row, row * c.page, row * c.page * c.nkv};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType t = c.type == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  for (int i = 0; i < 2; ++i)
-    if (encode(reinterpret_cast<CUtensorMap*>(i ? maps.v.b : maps.k.b), t, 4, i ? c.v : c.k, dims, strides, box, step,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return KC_ERR_CUDA;
-  return KC_OK;
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  const int rc = encode_16bit(maps.k, c.type, 4, c.k, dims, strides, box);
+  return rc == KC_OK ? encode_16bit(maps.v, c.type, 4, c.v, dims, strides, box) : rc;
+}
+
+int make_q_map(const AttnArgs& a, KvMap& map) {
+  const int group = a.nh / a.c.nkv;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.c.hd, (cuuint64_t)a.nh, (cuuint64_t)a.n_rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.c.hd * 2, (cuuint64_t)a.q_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(128 / group)};
+  return encode_16bit(map, a.c.type, 3, a.q, dims, strides, box);
 }
 
 // ---- workspace ---------------------------------------------------------------

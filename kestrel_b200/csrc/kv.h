@@ -53,8 +53,8 @@ struct KvCache {
 // with the first cache).
 struct KvState {
   std::map<int, KvCache> caches;
-  float* part = nullptr;  // attn_decode_part_bytes()
-  int* count = nullptr;   // one per SM, zero between launches
+  float* part = nullptr;  // parts to be joined: the larger of the two kernels' needs
+  int* count = nullptr;   // arrival counts, zero between launches
   int64_t bytes = 0;
 };
 
@@ -85,11 +85,17 @@ struct AttnArgs {
   float scale;
   int window, sinks;         // window 0: none
 };
+// The query rows of a call as [row][head][column], boxes of 128 (token, head)
+// rows of one key-value head's group (which divides 128) x 64 columns.
+int make_q_map(const AttnArgs& a, KvMap& map);
+
 size_t attn_decode_part_bytes();
 // One row per sequence (row_start null).
 int launch_attn_decode(const AttnArgs& a, const KvMaps& rows16, float* part, int* count, cudaStream_t st);
 // row_start non-null.
 int attn_prompt_box_rows(int page, int hd);
-int launch_attn_prompt(const AttnArgs& a, const KvMaps& tiles, cudaStream_t st);
+size_t attn_prompt_part_bytes();
+int attn_prompt_counts();
+int launch_attn_prompt(const AttnArgs& a, const KvMaps& tiles, float* part, int* count, cudaStream_t st);
 
 }  // namespace kc
