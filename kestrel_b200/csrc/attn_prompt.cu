@@ -43,6 +43,7 @@ namespace kc {
 
 constexpr int PM = 128;  // rows of a tile
 constexpr int P_STAGES_MAX = 8;
+constexpr int P_SPLITS_MAX = 8;  // blocks an item's positions are split over, at most
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * 168, "within the registers of the launch");
 
@@ -64,7 +65,9 @@ struct PromptShape {
   // the third (loads, MMAs) gives the softmax warps 32 a thread.
   static constexpr int THREADS = 128 * NS + 128;
   static constexpr int T_O = 256;                  // TMEM columns: S of stream w at 128 w, its O at T_O + HD w
-  static constexpr int LD = HD + 4;                // floats of a row's part of a split item: values, maximum, sum
+  // A split item's part: per four columns the rows' values ([HD / 4][PM][4]),
+  // then the rows' maxima and sums ([PM][2]).
+  static constexpr int PART = PM * (HD + 2);
   static_assert(!TWO || NS == 2, "two row tiles need two streams");
   static_assert(ST >= 2 && T_O + NS * HD <= 512, "fits");
 };
@@ -163,7 +166,7 @@ __device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int a
 struct PromptArgs {
   AttnArgs a;
   int splits;   // blocks an item's positions may be split over
-  float* part;  // [unit][split][PM][LD]
+  float* part;  // [unit][split][PART]
   int* count;   // per unit, zero between launches
   int* next;    // [2] items dealt beyond one per block, blocks done: zero between launches
   bool q_map;   // queries come by TMA
@@ -180,11 +183,12 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   constexpr float kGrow = 8.f;
   constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1, W_AUX = W_TMA + 2;  // W_AUX: and the next
   constexpr int AHEAD = TWO ? 1 : NS;  // K tiles loaded before the first V
+  if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : &q_map);
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
   __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_half[NS], p_full[NS], o_full[NS],
       o_empty[NS];
-  __shared__ __align__(8) uint64_t q_full, q_empty, item_full[2], item_empty[2];
+  __shared__ __align__(8) uint64_t q_raw, q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint32_t tmem_sh;
   __shared__ Item items[2];
   __shared__ __align__(8) uint64_t drained, join_full, part_full, last_full;
@@ -211,6 +215,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       mbar_init(&o_full[w], 1);
       mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
+    mbar_init(&q_raw, 1);
     mbar_init(&q_full, 2);
     mbar_init(&q_empty, 1);
     mbar_init(&drained, 1);
@@ -479,17 +484,21 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     const int64_t total = (int64_t)tiles * c.nkv * d.splits;
     int used = 0;
     int64_t idx = blockIdx.x;  // the block's first item; the rest as it comes to them
+    bool dealt = false;
     for (int n = 0; ok; ++n) {
       Item x{};
       if (finder) {
         while (true) {
+          if (dealt) {
+            int more = 0;
+            if (lane == 0) more = atomicAdd(d.next, 1);
+            idx = (int64_t)gridDim.x + __shfl_sync(0xffffffffu, more, 0);
+          }
+          dealt = true;
           x.valid = idx < total;
           if (!x.valid) break;
           x.split = (int)(idx % d.splits);
           x.unit = (int)(total / d.splits - 1 - idx / d.splits);
-          int more = 0;
-          if (lane == 0) more = atomicAdd(d.next, 1);
-          idx = (int64_t)gridDim.x + __shfl_sync(0xffffffffu, more, 0);
           x.kvh = x.unit % c.nkv;
           int t = x.unit / c.nkv, l = 0, i = 0;
           if (sorted) {
@@ -564,23 +573,31 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride + (int64_t)x.kvh * group * c.hd;
       const int loader = tid - 32 * W_AUX;
       constexpr int TILE_Q = (kSplit ? 2 : 1) * S::QB;
-      if (!kSplit && d.q_map) {
-        // As they are: a box per tile and 64 columns. (Rows past the entry's
-        // are another's or zeros; nothing comes of them.)
-        if (finder && lane == 0) {
-          mbar_expect_tx(&q_full, S::Q_ALL);
-          for (int y = 0; y < S::QT; ++y)
+      if (d.q_map && finder && lane == 0) {
+        // A box per tile and 128 bytes of columns. (Rows past the entry's are
+        // another's or zeros; nothing comes of them.)
+        uint64_t* bar = kSplit ? &q_raw : &q_full;
+        mbar_expect_tx(bar, S::Q_ALL);
+        for (int y = 0; y < S::QT; ++y)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              tma_load_3d(q_sm + y * TILE_Q + b * PM * 128, &q_map, 64 * b, x.kvh * group,
-                          x.start + rm.tok0 + y * (PM / group), &q_full);
-        } else if (lane == 0) {
-          mbar_arrive(&q_full);
-        }
+          for (int b = 0; b < TILE_Q / (PM * 128); ++b)
+            tma_load_3d(q_sm + y * TILE_Q + b * PM * 128, &q_map, 128 / (int)sizeof(TQ) * b, x.kvh * group,
+                        x.start + rm.tok0 + y * (PM / group), bar);
+      }
+      if (!kSplit && d.q_map) {
+        if (!finder && lane == 0) mbar_arrive(&q_full);
         continue;
       }
+      const bool staged = kSplit && d.q_map;
+      if (staged) {
+        wait(&q_raw, used - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
       {
-        // Eight lanes per row, eight values of each 64 a lane.
+        // Eight lanes per row, eight values of each 64 a lane. f32 rows that TMA
+        // brought lie where their two operands go, row for row: a warp reads its
+        // rows whole before it writes them.
         const bool wide = !((uintptr_t)a.q % 16) && a.q_stride * sizeof(TQ) % 16 == 0;
         const int part = loader & 7;
         constexpr int BATCH = NB <= 2 ? 4 : 1;  // rows of a lane under way
@@ -593,7 +610,15 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
               const bool real = f < x.rows && 64 * j + 8 * part < c.hd;
-              if (real && wide) {
+              if (staged) {
+                const uint8_t* raw = q_sm + (f >> 7) * TILE_Q + (2 * j + (part >> 2)) * PM * 128 + (f & (PM - 1)) * 128;
+                const int c0 = 2 * (part & 3), sw = f & 7, flip_c = part >> 2;  // (bank order)
+                const float4 u = *reinterpret_cast<const float4*>(raw + (((c0 + flip_c) ^ sw) << 4));
+                const float4 w = *reinterpret_cast<const float4*>(raw + (((c0 + 1 - flip_c) ^ sw) << 4));
+                const float4 lo4 = flip_c ? w : u, hi4 = flip_c ? u : w;
+                v[y][j][0] = lo4.x; v[y][j][1] = lo4.y; v[y][j][2] = lo4.z; v[y][j][3] = lo4.w;
+                v[y][j][4] = hi4.x; v[y][j][5] = hi4.y; v[y][j][6] = hi4.z; v[y][j][7] = hi4.w;
+              } else if (real && wide) {
                 load8(from + 64 * j, v[y][j]);
               } else {
 #pragma unroll
@@ -618,6 +643,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
               if (part == 0) factor_sh[(used - 1) & 1][tile][rr] = f;
             }
             f *= flip;
+            if (y == 0) __syncwarp();
             uint8_t* to = q_sm + tile * TILE_Q + rr * 128 + ((part ^ (rr & 7)) << 4);
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
@@ -809,7 +835,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
       bool bad = l != l || l == INFINITY;
       TQ* to_row = out + rm.offset(real ? f : 0, a.out_stride, c.hd);
-      float* part_row = d.part + (((int64_t)x.unit * d.splits + x.split) * PM + r) * S::LD;
+      float* part_row = d.part + ((int64_t)x.unit * d.splits + x.split) * S::PART + 4 * r;
       for (int e0 = col0; e0 < col1; e0 += 32) {
         float o[2][16];
         const uint32_t o_0 = tmem + lanes + S::T_O + (TWO ? w : 0) * S::HD + e0;
@@ -839,9 +865,9 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           if (split) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(part_row + e1 + e) =
+              *reinterpret_cast<float4*>(part_row + (e1 + e) * PM) =
                   make_float4(o[y][e], o[y][e + 1], o[y][e + 2], o[y][e + 3]);
-            if (e1 == 0) *reinterpret_cast<float2*>(part_row + S::HD) = make_float2(m, l);
+            if (e1 == 0) *reinterpret_cast<float2*>(part_row + S::HD * PM - 2 * r) = make_float2(m, l);
             continue;
           }
           bad |= normalise16(o[y], inv);
@@ -874,15 +900,21 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         write = ok && last_sh;
         if (write) {
           __threadfence();
-          const float* from = d.part + ((int64_t)x.unit * d.splits * PM + r) * S::LD;
-          const int64_t next = (int64_t)PM * S::LD;
-          float top = -INFINITY;
+          const float* from = d.part + (int64_t)x.unit * d.splits * S::PART + 4 * r;
+          float share[P_SPLITS_MAX], top = -INFINITY;
           l = 0.f;
-          if (real) {
-            for (int p = 0; p < x.splits; ++p) top = fmaxf(top, __ldcg(from + p * next + S::HD));
-            for (int p = 0; p < x.splits; ++p) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + p * next + S::HD));
-              l = __fmaf_rn(top == -INFINITY ? 0.f : exp2_fast(ml.x - top), ml.y, l);
+          {
+            float2 ml[P_SPLITS_MAX];
+#pragma unroll
+            for (int p = 0; p < P_SPLITS_MAX; ++p) {
+              ml[p] = p < x.splits ? __ldcg(reinterpret_cast<const float2*>(from + p * S::PART + S::HD * PM - 2 * r))
+                                   : make_float2(-INFINITY, 0.f);
+              top = fmaxf(top, ml[p].x);
+            }
+#pragma unroll
+            for (int p = 0; p < P_SPLITS_MAX; ++p) {
+              share[p] = top == -INFINITY ? 0.f : exp2_fast(ml[p].x - top);
+              l = __fmaf_rn(share[p], ml[p].y, l);
             }
           }
           inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
@@ -891,15 +923,16 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0.f;
-            for (int p = 0; p < x.splits; ++p) {
-              const float wt = top == -INFINITY ? 0.f : exp2_fast(__ldcg(from + p * next + S::HD) - top);
+#pragma unroll
+            for (int p = 0; p < P_SPLITS_MAX; ++p) {
+              if (p >= x.splits) break;
 #pragma unroll
               for (int e = 0; e < 16; e += 4) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(from + p * next + e0 + e));
-                o[e] = __fmaf_rn(wt, y.x, o[e]);
-                o[e + 1] = __fmaf_rn(wt, y.y, o[e + 1]);
-                o[e + 2] = __fmaf_rn(wt, y.z, o[e + 2]);
-                o[e + 3] = __fmaf_rn(wt, y.w, o[e + 3]);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(from + p * S::PART + (e0 + e) * PM));
+                o[e] = __fmaf_rn(share[p], y.x, o[e]);
+                o[e + 1] = __fmaf_rn(share[p], y.y, o[e + 1]);
+                o[e + 2] = __fmaf_rn(share[p], y.z, o[e + 2]);
+                o[e + 3] = __fmaf_rn(share[p], y.w, o[e + 3]);
               }
             }
             bad |= normalise16(o, inv);
@@ -927,7 +960,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 }
 
 // Parts of split items: what 192 items of 128 rows take at a head size of 128.
-constexpr size_t PROMPT_PART_BYTES = (size_t)192 * PM * (128 + 4) * sizeof(float);
+constexpr size_t PROMPT_PART_BYTES = (size_t)192 * PM * (128 + 2) * sizeof(float);
 constexpr int PROMPT_MAX_UNITS = 192;
 size_t attn_prompt_part_bytes() { return PROMPT_PART_BYTES; }
 int attn_prompt_counts() { return PROMPT_MAX_UNITS + 2; }
@@ -947,16 +980,16 @@ static int launch_prompt(PromptArgs d, const KvMaps& maps, cudaStream_t st) {
     // Fewer items than SMs: their positions over as many blocks as there are,
     // within the workspace.
     const int64_t likely = std::max<int64_t>((rows + tile - 1) / tile, std::min(a.n, a.n_rows)) * a.c.nkv;
-    const int64_t slots = std::min<int64_t>(PROMPT_MAX_UNITS, PROMPT_PART_BYTES / ((size_t)PM * S::LD * sizeof(float)));
-    d.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, slots / most, 16}));
+    const int64_t slots = std::min<int64_t>(PROMPT_MAX_UNITS, PROMPT_PART_BYTES / (S::PART * sizeof(float)));
+    d.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, slots / most, P_SPLITS_MAX}));
   }
   const int grid = (int)std::min<int64_t>(num_sms(), most * d.splits);
-  // 16-bit queries as they are, where a tile is whole tokens and TMA can
-  // address them; otherwise two warps bring them.
+  // Queries by TMA where a tile is whole tokens and TMA can address them (16-bit
+  // ones go to the tensor cores as they are); otherwise two warps bring them.
   KvMap q_map{};
   const int group = a.nh / a.c.nkv;
-  d.q_map = !S::kSplit && a.scale > 0.f && PM % group == 0 && !((uintptr_t)a.q % 16) && a.q_stride % 8 == 0 &&
-            make_q_map(a, q_map) == KC_OK;
+  d.q_map = (S::kSplit || a.scale > 0.f) && PM % group == 0 && !((uintptr_t)a.q % 16) &&
+            a.q_stride * sizeof(TQ) % 16 == 0 && make_q_map(a, q_map) == KC_OK;
   launch_k(attn_prompt_kernel<TQ, TKV, NB, TWO>, grid, S::THREADS, S::SMEM, st, d, maps, q_map);
   return KC_OK;
 }

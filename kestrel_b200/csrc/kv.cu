@@ -488,13 +488,14 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode() {
   return encode;
 }
 
-static int encode_16bit(KvMap& map, int t, int rank, const void* base, const cuuint64_t* dims,
+static int encode_map(KvMap& map, int t, int rank, const void* base, const cuuint64_t* dims,
                         const cuuint64_t* strides, const cuuint32_t* box) {
   const auto encode = tensor_map_encode();
   const cuuint32_t step[4] = {1, 1, 1, 1};
-  if (!encode || encode(reinterpret_cast<CUtensorMap*>(map.b),
-                        t == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
-                        const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType el = t == T_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : t == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (!encode || encode(reinterpret_cast<CUtensorMap*>(map.b), el, rank, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return KC_ERR_CUDA;
@@ -507,16 +508,17 @@ int make_kv_maps(const KvView& c, int box_rows, KvMaps& maps) {
                               (cuuint64_t)c.n_layer * c.n_pages};
   const cuuint64_t strides[3] = {row, row * c.page, row * c.page * c.nkv};
   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  const int rc = encode_16bit(maps.k, c.type, 4, c.k, dims, strides, box);
-  return rc == KC_OK ? encode_16bit(maps.v, c.type, 4, c.v, dims, strides, box) : rc;
+  const int rc = encode_map(maps.k, c.type, 4, c.k, dims, strides, box);
+  return rc == KC_OK ? encode_map(maps.v, c.type, 4, c.v, dims, strides, box) : rc;
 }
 
 int make_q_map(const AttnArgs& a, KvMap& map) {
   const int group = a.nh / a.c.nkv;
   const cuuint64_t dims[3] = {(cuuint64_t)a.c.hd, (cuuint64_t)a.nh, (cuuint64_t)a.n_rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)a.c.hd * 2, (cuuint64_t)a.q_stride * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(128 / group)};
-  return encode_16bit(map, a.c.type, 3, a.q, dims, strides, box);
+  const int el = a.t_q == T_F32 ? 4 : 2;
+  const cuuint64_t strides[2] = {(cuuint64_t)a.c.hd * el, (cuuint64_t)a.q_stride * el};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / el), (cuuint32_t)group, (cuuint32_t)(128 / group)};
+  return encode_map(map, a.t_q, 3, a.q, dims, strides, box);
 }
 
 // ---- workspace ---------------------------------------------------------------

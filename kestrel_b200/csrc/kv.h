@@ -86,7 +86,7 @@ struct AttnArgs {
   int window, sinks;         // window 0: none
 };
 // The query rows of a call as [row][head][column], boxes of 128 (token, head)
-// rows of one key-value head's group (which divides 128) x 64 columns.
+// rows of one key-value head's group (which divides 128) x 128 bytes of columns.
 int make_q_map(const AttnArgs& a, KvMap& map);
 
 size_t attn_decode_part_bytes();

@@ -152,23 +152,32 @@ def _host_u8(a):
     return np.ascontiguousarray(a, dtype=np.uint8).reshape(-1) if isinstance(a, np.ndarray) else a
 
 
-# ggml ids of the element types the paged cache takes, by torch's name.
-_FLOAT_TYPES = {"torch.float32": G.F32, "torch.float16": G.F16, "torch.bfloat16": G.BF16}
+# ggml ids of the element types the paged cache takes: by torch's name, and by
+# the dtype objects seen so far (these helpers are on the per-call path).
+_FLOAT_NAMES = {"torch.float32": G.F32, "torch.float16": G.F16, "torch.bfloat16": G.BF16}
+_FLOAT_TYPES = {}
 
 
 def _float_type(name: str, a) -> int:
-    t = _FLOAT_TYPES.get(str(a.dtype))
+    t = _FLOAT_TYPES.get(a.dtype)
     if t is None:
-        raise ValueError(f"{name} must be float32, float16 or bfloat16, not {a.dtype}")
+        t = _FLOAT_NAMES.get(str(a.dtype))
+        if t is None:
+            raise ValueError(f"{name} must be float32, float16 or bfloat16, not {a.dtype}")
+        _FLOAT_TYPES[a.dtype] = t
     return t
+
+
+_INT32 = set()  # torch.int32, once seen
 
 
 def _dev_ints(name: str, a, size: int | None = None):
     """A contiguous int32 CUDA tensor of `size` values (None: any)."""
     if a is None:
         return None
-    if not _is_dev(a) or str(a.dtype) != "torch.int32" or not a.is_contiguous():
+    if not _is_dev(a) or not (a.dtype in _INT32 or str(a.dtype) == "torch.int32") or not a.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
+    _INT32.add(a.dtype)
     if size is not None and a.numel() != size:
         raise ValueError(f"{name} holds {a.numel()} values, {size} needed")
     return a.data_ptr()
@@ -177,12 +186,15 @@ def _dev_ints(name: str, a, size: int | None = None):
 def _dev_rows(name: str, a, heads: int | None = None, head_dim: int | None = None):
     """Row stride (elements) of a CUDA tensor [rows, heads, head_dim] whose
     heads are contiguous within a row."""
-    if not _is_dev(a) or a.dim() != 3 or (heads is not None and a.shape[1] != heads) or \
-            (head_dim is not None and a.shape[2] != head_dim):
+    shape = a.shape
+    if not _is_dev(a) or len(shape) != 3 or (heads is not None and shape[1] != heads) or \
+            (head_dim is not None and shape[2] != head_dim):
         raise ValueError(f"{name} must be a CUDA tensor [rows, heads, head_dim]")
-    if (a.shape[2] > 1 and a.stride(2) != 1) or (a.shape[1] > 1 and a.stride(1) != a.shape[2]):
+    rows, nh, hd = shape
+    stride = a.stride()
+    if (hd > 1 and stride[2] != 1) or (nh > 1 and stride[1] != hd):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
-    return a.stride(0) if a.shape[0] > 1 else a.shape[1] * a.shape[2]
+    return stride[0] if rows > 1 else nh * hd
 
 
 class Context:
@@ -197,7 +209,8 @@ class Context:
         self.device = device
         self._k = {}           # layer -> top-k of its uploaded router
         self._dense_rows = {}  # tensor id -> rows
-        self._kv = {}          # cache id -> its tensors (kept alive while registered)
+        self._kv = {}          # paged cache id -> its tensors (kept alive while registered)
+        self._kv_dims = {}     # and (sequences, key-value heads, head size)
 
     def close(self):
         if getattr(self, "h", None):
@@ -473,17 +486,19 @@ class Context:
         self._check(lib().kc_kv_cache(self.h, cache, _float_type("k", k), n_layer, n_pages, page, n_kv, hd, n_seq,
                                       max_pages, k.data_ptr(), v.data_ptr(), *t))
         self._kv[cache] = (k, v, table, length, refs)
+        self._kv_dims[cache] = (n_seq, n_kv, hd)
 
     def kv_drop(self, cache: int):
         self._check(lib().kc_kv_drop(self.h, cache))
         self._kv.pop(cache, None)
+        self._kv_dims.pop(cache, None)
 
     def _kv_shape(self, cache: int):
         """(n_seq, n_kv, head_dim) of a registered cache."""
-        if cache not in self._kv:
+        dims = self._kv_dims.get(cache)
+        if dims is None:
             raise ValueError(f"paged cache {cache} is not registered through this Context")
-        k, _, table, _, _ = self._kv[cache]
-        return table.shape[0], k.shape[2], k.shape[4]
+        return dims
 
     def kv_fork_dev(self, cache: int, src, dst):
         """Sequences dst (int32 CUDA tensor, empty ones) share the pages of src."""
@@ -524,11 +539,12 @@ class Context:
         self._check(lib().kc_kv_copy_pages_dev(self.h, cache, _dev_ints("src", src), _dev_ints("dst", dst, n), n))
 
     def _attn(self, cache, q, out):
-        _, n_kv, hd = self._kv_shape(cache)
-        qs, os_ = _dev_rows("q", q, None, hd), _dev_rows("out", out, q.shape[1], hd)
-        if out.shape != q.shape or out.dtype != q.dtype:
+        hd = self._kv_shape(cache)[2]
+        qs, os_ = _dev_rows("q", q, None, hd), _dev_rows("out", out, None, hd)
+        shape = q.shape
+        if out.shape != shape or out.dtype != q.dtype:
             raise ValueError("out must have q's shape and type")
-        return q.shape[0], q.shape[1], hd, qs, os_
+        return shape[0], shape[1], hd, qs, os_
 
     def attn_decode_dev(self, cache: int, layer: int, q, out, seqs=None, scale: float | None = None,
                         window: int = 0, sinks: int = 0):

@@ -56,7 +56,7 @@ def test_null_context_is_refused():
 def test_binding_refuses_tensors_it_cannot_pass():
     from kestrel_b200 import cuda
     ctx = cuda.Context.__new__(cuda.Context)  # no GPU here: the checks come before any call
-    ctx.h, ctx._kv = None, {}
+    ctx.h, ctx._kv, ctx._kv_dims = None, {}, {}
     x = torch.zeros((2, 3, 1, 16, 8))
     i = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
