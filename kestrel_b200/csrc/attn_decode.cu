@@ -30,6 +30,7 @@ namespace kc {
 
 constexpr int DC = 16;  // positions per chunk: the smallest page
 constexpr int DEC_MAX_PARTS = 160;  // most blocks of a launch
+constexpr int FEW_PARTS = 4;        // parts that one warp joins by itself
 
 template <int NB, int HT>
 struct DecShape {
@@ -117,7 +118,8 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   pdl_enter();
   extern __shared__ uint8_t dec_raw[];
   __shared__ __align__(8) uint64_t full[W][ST];
-  __shared__ long long red[3][W];
+  __shared__ long long red[3][W], found_at[W];
+  __shared__ int found[W];
   __shared__ int last_sh;
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
@@ -132,50 +134,62 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
 
   // ---- the line, and this block's range of it --------------------------------
   // Chunks of all sequences, and the longest one. On the way the rows of
-  // sequences that hold nothing become zeros.
-  long long sum = 0;
-  int most = 0;
+  // sequences that hold nothing become zeros. One round of the block's threads
+  // covers 32 W sequences; `here` and `before` are of the last round.
+  long long sum = 0, before = 0;
+  int most = 0, here = 0;
   for (int i0 = 32 * warp; i0 < a.n; i0 += 32 * W) {
     const int i = i0 + lane;
-    int n = 0;
+    here = 0;
     bool none = false;
     if (i < a.n) {
       const int s = a.seqs ? a.seqs[i] : i;
-      if (s >= 0 && s < c.n_seq) n = dec_span(kv_len(c, s), a.window, a.sinks).n;
+      if (s >= 0 && s < c.n_seq) here = dec_span(kv_len(c, s), a.window, a.sinks).n;
       else if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
-      none = n == 0 && i % gridDim.x == blockIdx.x;
+      none = here == 0 && i % gridDim.x == blockIdx.x;
     }
     for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)(i0 + __ffs(rows) - 1) * a.out_stride;
       for (int x = lane; x < a.nh * c.hd; x += 32) out[x] = (TQ)0.f;
     }
-    sum += n;
-    most = max(most, n);
+    sum += here;
+    most = max(most, here);
   }
+  {
+    // Sequences before this thread's among its warp's, and the warp's sum.
+    long long x = sum;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  }
-  if (lane == 0) {
-    red[0][warp] = sum;
-    red[1][warp] = most;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    before = x - here;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 31) red[0][warp] = x;
+    if (lane == 0) {
+      red[1][warp] = most;
+      found[warp] = a.n;  // (a range past the line has no sequence)
+    }
   }
   __syncthreads();
   long long line = 0;
   for (int w = 0; w < W; ++w) {
+    if (w < warp) before += red[0][w];
     line += red[0][w];
     most = max(most, (int)red[1][w]);
   }
   line *= units;
   if (line == 0) return;
-  // Equal ranges of at least one chunk per warp. When the units are few and
-  // nearly of one length, each is cut into the same whole number of parts
-  // instead (its stretch of the line padded to `pad` chunks): ranges that
-  // begin with their unit save a join. That is taken when it is not slower by
-  // more than a round of chunks. When the units are many and none is longer
-  // than a warp's share of the line, each warp takes whole units of its own and
-  // nothing is merged or joined.
+  // Equal ranges of at least one chunk per warp. When the units are few, each
+  // is cut into the same whole number of parts instead (its stretch of the line
+  // padded to `pad` chunks) where that is not slower: ranges that begin with
+  // their unit have one segment instead of two or three, and a unit in one part
+  // needs no join. (A segment's end and a join take about as long as two and
+  // four more rounds of chunks: 32 sequences of 2048 positions took 37 us in
+  // equal ranges and 29 in one part each.) When the units are many and none is
+  // longer than a warp's share of the line, each warp takes whole units of its
+  // own and nothing is merged or joined.
   long long per = max((line + gridDim.x - 1) / gridDim.x, (long long)W);
   const long long all = (long long)a.n * units;
   const bool whole = most <= max((per + W - 1) / W, 4ll) && all >= (long long)gridDim.x * W;
@@ -187,7 +201,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     if (all <= gridDim.x) {
       const int parts = (int)(gridDim.x / all);
       const int q = ((most + parts - 1) / parts + W - 1) / W * W;
-      if (q <= per + W) {
+      if (q <= per + (parts == 1 ? 6 : 2) * W) {
         per = q;
         pad = q * ((most + q - 1) / q);
         line = all * pad;
@@ -206,131 +220,172 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     at.i = (int)(at.pos / ((long long)pad * units));
     at.base = (long long)at.i * pad * units;
   } else {
-    const long long block_end = whole ? (blockIdx.x + 1) * W * per : at.end;
-    long long before = 0;  // chunks of the sequences before the 32 * W at hand
-    __syncthreads();
-    if (lane == 0) red[0][warp] = a.n;  // a range past the line has no sequence
-    for (int b = 0; b < a.n && before < block_end; b += 32 * W) {
-      const int i = b + tid;
-      long long n = 0;
-      if (i < a.n) {
-        const int s = a.seqs ? a.seqs[i] : i;
-        if (s >= 0 && s < c.n_seq) n = (long long)dec_span(kv_len(c, s), a.window, a.sinks).n * units;
-      }
-      long long x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      __syncthreads();
-      if (lane == 31) red[2][warp] = x;
-      __syncthreads();
-      long long mine = before + x - n;
-      for (int w = 0; w < W; ++w) {
-        if (w < warp) mine += red[2][w];
-        before += red[2][w];
-      }
-      // Exactly one sequence holds each position.
-      if (n > 0)
-        for (int w = 0; w < (whole ? W : 1); ++w) {
-          const long long pos = (whole ? blockIdx.x * W + w : blockIdx.x) * per;
-          if (mine <= pos && pos < mine + n) {
-            red[0][w] = i;
-            red[1][w] = mine;
-          }
+    // Exactly one sequence holds each position.
+    auto look = [&](int i, long long first, int n) {
+      for (int w = 0; w < (whole ? W : 1); ++w) {
+        const long long pos = (whole ? blockIdx.x * W + w : blockIdx.x) * per - first * units;
+        if (pos >= 0 && pos < (long long)n * units) {
+          found[w] = i;
+          found_at[w] = first * units;
         }
+      }
+    };
+    if (a.n <= 32 * W) {
+      look(tid, before, here);
+    } else {
+      const long long block_end = whole ? (blockIdx.x + 1) * W * per : at.end;
+      long long base = 0;  // chunks of the sequences before the 32 * W at hand
+      for (int b = 0; b < a.n && base * units < block_end; b += 32 * W) {
+        const int i = b + tid;
+        int n = 0;
+        if (i < a.n) {
+          const int s = a.seqs ? a.seqs[i] : i;
+          if (s >= 0 && s < c.n_seq) n = dec_span(kv_len(c, s), a.window, a.sinks).n;
+        }
+        long long x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) red[2][warp] = x;
+        __syncthreads();
+        long long mine = base + x - n;
+        for (int w = 0; w < W; ++w) {
+          if (w < warp) mine += red[2][w];
+          base += red[2][w];
+        }
+        look(i, mine, n);
+      }
     }
     __syncthreads();
-    at.i = (int)red[0][whole ? warp : 0];
-    at.base = red[1][whole ? warp : 0];
+    at.i = found[whole ? warp : 0];
+    at.base = found_at[whole ? warp : 0];
     if (at.i >= a.n) at.pos = at.end;
   }
   if (at.pos < at.end) seg_sequence(at, a);
 
+  // ---- queries ------------------------------------------------------------------
+  // A segment's, as this lane holds them in A fragments (row r0, and r0 + 8 in
+  // the form of 16 heads; columns cc, cc + 1 of each 8). They are asked for a
+  // segment ahead, where there are registers for it: behind the chunks under way
+  // a load takes as long as those.
+  const int r0 = lane >> 2, cc = 2 * (lane & 3);  // fragment row and first column
+  constexpr bool kAhead = NB <= 2;
+  TQ raw[RH][4 * NB][4];
+  auto ask = [&](const SegIter& g) {
+    const int kvh = g.unit / tiles, h0 = (g.unit - kvh * tiles) * HT;
+    const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)g.i * a.q_stride + (int64_t)(kvh * group + h0) * c.hd;
+#pragma unroll
+    for (int rr = 0; rr < RH; ++rr) {
+      const bool real = h0 + r0 + 8 * rr < group;
+#pragma unroll
+      for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 16 * ks + cc + (e & 1) + 8 * (e >> 1);
+          raw[rr][ks][e] = real && x < c.hd ? q[(int64_t)(r0 + 8 * rr) * c.hd + x] : (TQ)0.f;
+        }
+    }
+  };
+  SegIter ahead = at;  // what is loaded next
+  bool more = seg_next(ahead, a, units), have = more;
+  SegIter to_come = ahead;  // the segment after the one at hand
+  if (kAhead && have) ask(to_come);
+
   // ---- this warp's ring ---------------------------------------------------------
   // Its chunks are every `stride`-th of each segment, from the `mine`-th on.
   const int stride = whole ? 1 : W, mine = whole ? 0 : warp;
-  SegIter ahead = at;  // what is loaded next
-  bool more = seg_next(ahead, a, units);
   int next = ahead.c0 + mine, issued = 0, used = 0;
   bool ok = true;
   uint8_t* slots = ring + warp * ST * S::CHUNK;
-  auto issue = [&]() {
+  // The next chunk: first position, sequence and head. False when there is none.
+  auto plan = [&](int& p, int& s, int& head) {
     while (more && next >= ahead.c1) {
       more = seg_next(ahead, a, units);
       next = ahead.c0 + mine;
     }
-    if (!more) return;
-    if (lane == 0) {
-      const int x = next < ahead.span.head ? next : next - ahead.span.head + ahead.span.w0, p = x * DC;
-      int id = c.table[(int64_t)ahead.s * c.max_pages + (p >> c.page_log2)];
-      int lp = a.layer * c.n_pages + id;
-      if (id < 0 || id >= c.n_pages) {
-        report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
-        lp = c.n_layer * c.n_pages;  // past the pool: zeros
-      }
-      const int st = issued % ST;
-      uint8_t* to = slots + st * S::CHUNK;
-      mbar_expect_tx(&full[warp][st], S::CHUNK);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        kv_load(to + b * DC * 128, &maps.k, 64 * b, p & (c.page - 1), ahead.unit / tiles, lp, &full[warp][st]);
-        kv_load(to + (NB + b) * DC * 128, &maps.v, 64 * b, p & (c.page - 1), ahead.unit / tiles, lp,
-                &full[warp][st]);
-      }
-    }
-    ++issued;
+    if (!more) return false;
+    p = (next < ahead.span.head ? next : next - ahead.span.head + ahead.span.w0) * DC;
+    s = ahead.s;
+    head = ahead.unit / tiles;
     next += stride;
+    ++issued;
+    return true;
+  };
+  auto load = [&](int st, int p, int s, int head) {
+    const int id = c.table[(int64_t)s * c.max_pages + (p >> c.page_log2)];
+    int lp = a.layer * c.n_pages + id;
+    if (id < 0 || id >= c.n_pages) {
+      report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
+      lp = c.n_layer * c.n_pages;  // past the pool: zeros
+    }
+    uint8_t* to = slots + st * S::CHUNK;
+    mbar_expect_tx(&full[warp][st], S::CHUNK);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      kv_load(to + b * DC * 128, &maps.k, 64 * b, p & (c.page - 1), head, lp, &full[warp][st]);
+      kv_load(to + (NB + b) * DC * 128, &maps.v, 64 * b, p & (c.page - 1), head, lp, &full[warp][st]);
+    }
   };
   __syncwarp();
-  for (int s = 0; s < ST; ++s) issue();
-
-  const int r0 = lane >> 2, cc = 2 * (lane & 3);  // fragment row and first column
-  const float log2e = 1.4426950408889634f;
-  while (seg_next(at, a, units)) {
-    const int kvh = at.unit / tiles, h0 = (at.unit - kvh * tiles) * HT;
-    // ---- queries as A fragments: rows r0 (and r0 + 8: rests, or more heads) -----
-    uint32_t qa[4 * NB][4];
-    float cq[RH];  // score units of base-2 exponents per product unit
-    {
-      const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)at.i * a.q_stride + (int64_t)(kvh * group + h0) * c.hd;
+  {
+    // The first ones at once, a lane per stage.
+    int p = 0, s = 0, head = 0;
+    bool go = false;
 #pragma unroll
-      for (int rr = 0; rr < RH; ++rr) {
-        const int h = r0 + 8 * rr;
-        const bool real = h0 + h < group;
-        float v[4 * NB][4], amax = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 4 * NB; ++ks)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = 16 * ks + cc + (e & 1) + 8 * (e >> 1);
-            v[ks][e] = real && x < c.hd ? (float)q[(int64_t)h * c.hd + x] : 0.f;
-            amax = fmaxf(amax, fabsf(v[ks][e]));
-          }
-        float f = 1.f;
-        if constexpr (sizeof(TQ) == 4) {
-          // A power of two puts the row's largest value in [2^14, 2^15).
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          f = pow2_factor(amax);
-        }
-        cq[rr] = __fdiv_rn(a.scale * log2e, f);
-#pragma unroll
-        for (int ks = 0; ks < 4 * NB; ++ks)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = v[ks][2 * e] * f, y = v[ks][2 * e + 1] * f;
-            const uint32_t hi = pack2<TKV>(x, y);
-            if constexpr (kSplit) {
-              qa[ks][2 * e] = hi;
-              qa[ks][2 * e + 1] = sizeof(TQ) == 4 ? rest2<TKV>(x, y, hi) : 0u;
-            } else {
-              qa[ks][2 * e + rr] = hi;
-            }
-          }
+    for (int st = 0; st < ST; ++st) {
+      int p1, s1, head1;
+      if (plan(p1, s1, head1) && lane == st) {
+        p = p1;
+        s = s1;
+        head = head1;
+        go = true;
       }
     }
+    if (go) load(lane, p, s, head);
+  }
+  __syncwarp();
+
+  const float log2e = 1.4426950408889634f;
+  while (have) {
+    at = to_come;
+    if (!kAhead) ask(at);
+    const int kvh = at.unit / tiles, h0 = (at.unit - kvh * tiles) * HT;
+    uint32_t qa[4 * NB][4];
+    float cq[RH];  // base-2 exponents per score unit
+#pragma unroll
+    for (int rr = 0; rr < RH; ++rr) {
+      float f = 1.f;
+      if constexpr (sizeof(TQ) == 4) {
+        // A power of two puts the row's largest value in [2^14, 2^15).
+        float amax = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf((float)raw[rr][ks][e]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        f = pow2_factor(amax);
+      }
+      cq[rr] = __fdiv_rn(a.scale * log2e, f);
+#pragma unroll
+      for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = (float)raw[rr][ks][2 * e] * f, y = (float)raw[rr][ks][2 * e + 1] * f;
+          const uint32_t hi = pack2<TKV>(x, y);
+          if constexpr (kSplit) {
+            qa[ks][2 * e] = hi;
+            qa[ks][2 * e + 1] = sizeof(TQ) == 4 ? rest2<TKV>(x, y, hi) : 0u;
+          } else {
+            qa[ks][2 * e + rr] = hi;
+          }
+        }
+    }
+    have = seg_next(to_come, a, units);
+    if (kAhead && have) ask(to_come);
     float m[RH], l[RH], o[8 * NB][4];
 #pragma unroll
     for (int rr = 0; rr < RH; ++rr) {
@@ -448,7 +503,11 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         }
       }
       __syncwarp();
-      issue();
+      {
+        int p1, s1, head1;
+        const int slot = issued % ST;
+        if (plan(p1, s1, head1) && lane == 0) load(slot, p1, s1, head1);
+      }
     }
 
     // ---- the warps' states into warp 0's ---------------------------------------
@@ -521,6 +580,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     }
     // The part's place: 0 if the unit is the block's first, else 1.
     const int slot = 2 * blockIdx.x + (at.unit_at + at.c0 == blockIdx.x * per ? 0 : 1);
+    const int parts = b1 - b0 + 1;
+    // Parts in block order; the unit is the first of every block but b0,
+    // where it is unless it begins inside the block's range.
+    const int first = 2 * b0 + (at.unit_at == b0 * per ? 0 : 1);
+    auto part_of = [&](int p) { return d.part + (int64_t)(p == 0 ? first : 2 * (b0 + p)) * HT * LD; };
+    bool last = false;
     if (warp == 0) {
       float* to = d.part + (int64_t)slot * HT * LD;
 #pragma unroll
@@ -534,20 +599,62 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
       __threadfence();
       __syncwarp();
-      if (lane == 0) last_sh = atomicAdd(d.count + b0, 1) == b1 - b0 ? 1 : 0;
+      int seen = 0;
+      if (lane == 0) {
+        seen = atomicAdd(d.count + b0, 1);
+        if (seen == parts - 1) d.count[b0] = 0;
+      }
+      last = __shfl_sync(0xffffffffu, seen, 0) == parts - 1;
+      __threadfence();
+      if (parts > FEW_PARTS && lane == 0) last_sh = last;
+    }
+    if (parts <= FEW_PARTS) {
+      // Warp 0 joins them by itself; the others go on.
+      if (last) {
+#pragma unroll
+        for (int rr = 0; rr < RH; ++rr) {
+          const int h = r0 + 8 * rr;
+          float2 ml[FEW_PARTS];
+          float top = -INFINITY, total = 0.f;
+#pragma unroll
+          for (int p = 0; p < FEW_PARTS; ++p) {
+            ml[p] = p < parts ? __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + S::HD))
+                              : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, ml[p].x);
+          }
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int p = 0; p < FEW_PARTS; ++p) {
+            ml[p].x = exp2_fast(ml[p].x - base);
+            total = __fmaf_rn(ml[p].x, ml[p].y, total);
+          }
+          const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+          if (h0 + h >= group) continue;
+#pragma unroll
+          for (int t = 0; t < 8 * NB; ++t) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int p = 0; p < FEW_PARTS; ++p)
+              if (p < parts) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + 8 * t + cc));
+                s0 = __fmaf_rn(ml[p].x, v.x, s0);
+                s1 = __fmaf_rn(ml[p].x, v.y, s1);
+              }
+            if (8 * t + cc < c.hd) {
+              out[(int64_t)h * c.hd + 8 * t + cc] = (TQ)(s0 * inv);
+              out[(int64_t)h * c.hd + 8 * t + cc + 1] = (TQ)(s1 * inv);
+            }
+          }
+        }
+      }
+      continue;
     }
     __syncthreads();
     if (last_sh) {
       __threadfence();
-      if (tid == 0) d.count[b0] = 0;
-      // Parts in block order; the unit is the first of every block but b0,
-      // where it is unless it begins inside the block's range.
-      const int first = 2 * b0 + (at.unit_at == b0 * per ? 0 : 1);
       // First every part's share of each head's result (a warp per head, the
       // parts over its lanes), then the sums over the parts.
-      const int parts = b1 - b0 + 1;
       float* share = merge;  // [HT][parts]
-      auto part_of = [&](int p) { return d.part + (int64_t)(p == 0 ? first : 2 * (b0 + p)) * HT * LD; };
       for (int h = warp; h < HT; h += W) {
         float2 ml[DEC_MAX_PARTS / 32];
         float top = -INFINITY, total = 0.f;
