@@ -5,12 +5,13 @@
 // byte and query head: it is bound by the memory rate, and what matters is that
 // all SMs read all the time, however unequal the sequences are. So the work is
 // one line of 16-position chunks, sequence after sequence and head after head,
-// cut into equal ranges for one block per SM; a range may begin and end inside
-// a sequence. Each warp runs its own ring of chunks (TMA boxes of one page's
-// rows, 128-byte swizzle, 192 KB in flight per SM) and its own softmax state, so
-// warps meet only where a sequence ends. The parts of a sequence that several
-// blocks hold go to a workspace; the block that finishes last joins them in
-// block order, so the sums do not depend on timing.
+// cut into equal ranges for one block per SM and its warps; a range may begin
+// and end inside a sequence. Each warp runs its own ring of chunks (TMA boxes of
+// one page's rows, 128-byte swizzle, up to 192 KB in flight per SM) and its own
+// softmax state, writes what it has whole, and meets the others once, at the
+// end: the parts of a block are joined in shared memory, and those of a sequence
+// that several blocks hold in a workspace, by the block that finishes last. Both
+// go in the order of the line, so the sums do not depend on timing.
 //
 // The eight heads of a group share each chunk as the rows of one m16n8k16
 // product. f32 queries and the f32 weights are each carried by two 16-bit rows
@@ -30,17 +31,21 @@ namespace kc {
 
 constexpr int DC = 16;  // positions per chunk: the smallest page
 constexpr int DEC_MAX_PARTS = 160;  // most blocks of a launch
-constexpr int FEW_PARTS = 4;        // parts that one warp joins by itself
 
 template <int NB, int HT>
 struct DecShape {
   static constexpr int HD = 64 * NB;                           // padded head size
   static constexpr int W = NB <= 2 ? 8 : 4;                    // warps
   static constexpr int CHUNK = 2 * NB * DC * 128;              // K and V of one chunk
-  static constexpr int ST = 196608 / (W * CHUNK);              // ring stages per warp
-  static constexpr int LD = HD + 4;                            // a head's partial: values, maximum, sum, (16-byte rows)
-  static constexpr int MERGE = W / 2 * HT * LD * 4;            // partials of half the warps
-  static constexpr int SMEM = W * ST * CHUNK + MERGE + 1024;
+  static constexpr int LD = HD + 4;                            // a head's part: values, maximum, sum, (16-byte rows)
+  static constexpr int FIRST = W * HT * LD * 4;                // a part per warp, kept beside the ring
+  static constexpr int FIT = (225 * 1024 - FIRST) / (W * CHUNK);
+  static constexpr int ST = FIT < 6 ? FIT : 6;                 // ring stages per warp
+  static constexpr int SMEM = W * ST * CHUNK + FIRST + 1024;
+  // After the chunks: a warp's last part where its ring was, and behind warp
+  // 0's what each part counts for, and each unit's maxima and sums.
+  static_assert(HT * LD * 4 + 2 * W * HT * 12 <= ST * CHUNK, "fits");
+  static_assert(2 * HT <= 32, "a thread per part and head");
 };
 
 struct DecArgs {
@@ -63,12 +68,11 @@ __device__ __forceinline__ Span dec_span(int len, int window, int sinks) {
   return s;
 }
 
-// A block's range of the line, segment by segment (one segment: consecutive
+// A warp's range of the line, segment by segment (one segment: consecutive
 // chunks of one unit, a unit being a sequence's key-value head and head tile).
 struct SegIter {
   long long pos, end, base;  // base: line position of sequence i's first unit
   int i, pad;                // pad: chunks each unit takes of the line (0: as many as it has)
-  bool whole;                // the units that begin in the range, none of them cut
   int s, len;
   Span span;
   // the segment
@@ -84,20 +88,16 @@ __device__ __forceinline__ void seg_sequence(SegIter& t, const AttnArgs& a) {
 __device__ __forceinline__ bool seg_next(SegIter& t, const AttnArgs& a, int units) {
   while (t.pos < t.end) {
     const int np = t.pad ? t.pad : t.span.n;
-    const long long off = t.pos - t.base;
-    if (off >= (long long)np * units) {
-      t.base += (long long)np * units;
+    const long long off = t.pos - t.base;  // (a sequence's stretch fits 31 bits: the host sees to it)
+    if (off >= np * units) {
+      t.base += np * units;
       if (++t.i >= a.n) return false;
       seg_sequence(t, a);
       continue;
     }
-    t.unit = (int)(off / np);
-    t.c0 = (int)(off - (long long)t.unit * np);
-    if (t.whole && t.c0) {
-      t.pos += np - t.c0;
-      continue;
-    }
-    const int take = t.whole ? np : (int)min(t.end - t.pos, (long long)(np - t.c0));
+    t.unit = (int)((uint32_t)off / (uint32_t)np);
+    t.c0 = (int)off - t.unit * np;
+    const int take = (int)min(t.end - t.pos, (long long)(np - t.c0));
     t.unit_at = t.pos - t.c0;
     t.c1 = min(t.c0 + take, t.span.n);
     t.n_unit = t.span.n;
@@ -106,6 +106,12 @@ __device__ __forceinline__ bool seg_next(SegIter& t, const AttnArgs& a, int unit
   }
   return false;
 }
+
+// What a warp has of a unit that it does not hold whole.
+struct DecPart {
+  int have, i, unit, n_unit;
+  long long unit_at;
+};
 
 template <typename TQ, typename TKV, int NB, int HT>
 __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
@@ -120,12 +126,13 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   __shared__ __align__(8) uint64_t full[W][ST];
   __shared__ long long red[3][W], found_at[W];
   __shared__ int found[W];
-  __shared__ int last_sh;
+  __shared__ DecPart parts_sh[2 * W];  // per warp: of its range's first segment, and of its last
+  __shared__ int last_sh[2];
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = dec_raw + ((1024 - (smem_u32(dec_raw) & 1023)) & 1023);
-  float* merge = reinterpret_cast<float*>(ring + W * ST * S::CHUNK);
+  float* firsts = reinterpret_cast<float*>(ring + W * ST * S::CHUNK);
   const int group = a.nh / c.nkv, tiles = (group + HT - 1) / HT, units = c.nkv * tiles;
   if (lane == 0) {
     for (int s = 0; s < ST; ++s) mbar_init(&full[warp][s], 1);
@@ -187,43 +194,40 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // their unit have one segment instead of two or three, and a unit in one part
   // needs no join. (A segment's end and a join take about as long as two and
   // four more rounds of chunks: 32 sequences of 2048 positions took 37 us in
-  // equal ranges and 29 in one part each.) When the units are many and none is
-  // longer than a warp's share of the line, each warp takes whole units of its
-  // own and nothing is merged or joined.
+  // equal ranges and 29 in one part each.)
   long long per = max((line + gridDim.x - 1) / gridDim.x, (long long)W);
+  per = (per + W - 1) / W * W;
   const long long all = (long long)a.n * units;
-  const bool whole = most <= max((per + W - 1) / W, 4ll) && all >= (long long)gridDim.x * W;
   int pad = 0;
-  if (whole) {
-    per = (per + W - 1) / W;
-  } else {
-    per = (per + W - 1) / W * W;
-    if (all <= gridDim.x) {
-      const int parts = (int)(gridDim.x / all);
-      const int q = ((most + parts - 1) / parts + W - 1) / W * W;
-      if (q <= per + (parts == 1 ? 6 : 2) * W) {
-        per = q;
-        pad = q * ((most + q - 1) / q);
-        line = all * pad;
-      }
+  if (all <= gridDim.x) {
+    const int parts = (int)(gridDim.x / all);
+    const int q = ((most + parts - 1) / parts + W - 1) / W * W;
+    if (q <= per + (parts == 1 ? 6 : 2) * W) {
+      per = q;
+      pad = q * ((most + q - 1) / q);
+      line = all * pad;
     }
   }
+  const long long block_at = blockIdx.x * per, block_end = min(line, block_at + per), share_of = per / W;
+  if (block_at >= block_end) return;
   SegIter at;
-  at.pos = (whole ? blockIdx.x * W + warp : blockIdx.x) * per;
-  at.end = min(line, at.pos + per);
+  // A block of one unit's part deals its chunks to the warps in turn (so that
+  // they read side by side: 131071 positions took 54 us, in stretches 57);
+  // otherwise each warp has a stretch of the range.
+  const int stride = pad ? W : 1, mine = pad ? warp : 0;
+  at.pos = pad ? block_at : min(block_end, block_at + warp * share_of);
+  at.end = pad ? block_end : min(block_end, at.pos + share_of);
   at.pad = pad;
-  at.whole = whole;
-  if (!whole && at.pos >= at.end) return;
-  // The sequence in which the range begins: the last whose first chunk is at
-  // or before it (of every warp's range, where warps have their own).
+  // The sequence in which each warp's range begins: the last whose first chunk
+  // is at or before it.
   if (pad) {
     at.i = (int)(at.pos / ((long long)pad * units));
     at.base = (long long)at.i * pad * units;
   } else {
     // Exactly one sequence holds each position.
     auto look = [&](int i, long long first, int n) {
-      for (int w = 0; w < (whole ? W : 1); ++w) {
-        const long long pos = (whole ? blockIdx.x * W + w : blockIdx.x) * per - first * units;
+      for (int w = 0; w < W; ++w) {
+        const long long pos = block_at + w * share_of - first * units;
         if (pos >= 0 && pos < (long long)n * units) {
           found[w] = i;
           found_at[w] = first * units;
@@ -233,7 +237,6 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     if (a.n <= 32 * W) {
       look(tid, before, here);
     } else {
-      const long long block_end = whole ? (blockIdx.x + 1) * W * per : at.end;
       long long base = 0;  // chunks of the sequences before the 32 * W at hand
       for (int b = 0; b < a.n && base * units < block_end; b += 32 * W) {
         const int i = b + tid;
@@ -260,8 +263,8 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
     }
     __syncthreads();
-    at.i = found[whole ? warp : 0];
-    at.base = found_at[whole ? warp : 0];
+    at.i = found[warp];
+    at.base = found_at[warp];
     if (at.i >= a.n) at.pos = at.end;
   }
   if (at.pos < at.end) seg_sequence(at, a);
@@ -295,8 +298,6 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   if (kAhead && have) ask(to_come);
 
   // ---- this warp's ring ---------------------------------------------------------
-  // Its chunks are every `stride`-th of each segment, from the `mine`-th on.
-  const int stride = whole ? 1 : W, mine = whole ? 0 : warp;
   int next = ahead.c0 + mine, issued = 0, used = 0;
   bool ok = true;
   uint8_t* slots = ring + warp * ST * S::CHUNK;
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       kv_load(to + (NB + b) * DC * 128, &maps.v, 64 * b, p & (c.page - 1), head, lp, &full[warp][st]);
     }
   };
+  if (lane < 2) parts_sh[2 * warp + lane].have = 0;
   __syncwarp();
   {
     // The first ones at once, a lane per stage.
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
     }
 
-    // ---- the warps' states into warp 0's ---------------------------------------
+    // ---- the result, or this warp's part of it ------------------------------------
 #pragma unroll
     for (int rr = 0; rr < RH; ++rr) {
       l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
@@ -522,191 +524,204 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         o[t][0] += o[t][2];
         o[t][1] += o[t][3];
       }
-    const int holders = whole ? 1 : min(W, at.c1 - at.c0);  // warps that had a chunk
-#pragma unroll
-    for (int half = W / 2; half >= 1; half >>= 1) {
-      if (holders <= half) continue;
-      __syncthreads();
-      if (warp >= half && warp < 2 * half && warp < holders) {
-#pragma unroll
-        for (int rr = 0; rr < RH; ++rr) {
-          float* to = merge + ((warp - half) * HT + r0 + 8 * rr) * LD;
-#pragma unroll
-          for (int t = 0; t < 8 * NB; ++t)
-            *reinterpret_cast<float2*>(to + 8 * t + cc) = make_float2(o[t][2 * rr], o[t][2 * rr + 1]);
-          if ((lane & 3) == 0) *reinterpret_cast<float2*>(to + S::HD) = make_float2(m[rr], l[rr]);
-        }
-      }
-      __syncthreads();
-      if (warp < half && warp + half < holders) {
-#pragma unroll
-        for (int rr = 0; rr < RH; ++rr) {
-          const float* from = merge + (warp * HT + r0 + 8 * rr) * LD;
-          const float2 ml = *reinterpret_cast<const float2*>(from + S::HD);
-          const float mn = fmaxf(m[rr], ml.x);
-          const float mine = mn == -INFINITY ? 1.f : exp2_fast(m[rr] - mn);
-          const float theirs = mn == -INFINITY ? 1.f : exp2_fast(ml.x - mn);
-          m[rr] = mn;
-          l[rr] = __fmaf_rn(l[rr], mine, ml.y * theirs);
-#pragma unroll
-          for (int t = 0; t < 8 * NB; ++t) {
-            const float2 v = *reinterpret_cast<const float2*>(from + 8 * t + cc);
-            o[t][2 * rr] = __fmaf_rn(o[t][2 * rr], mine, v.x * theirs);
-            o[t][2 * rr + 1] = __fmaf_rn(o[t][2 * rr + 1], mine, v.y * theirs);
-          }
-        }
-      }
-    }
-
-    // ---- the result, or this block's part of it ------------------------------------
-    const int b0 = whole ? 0 : (int)(at.unit_at / per);
-    const int b1 = whole ? 0 : (int)((at.unit_at + at.n_unit - 1) / per);
-    TQ* out = static_cast<TQ*>(a.out) + (int64_t)at.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
-    if (b0 == b1) {
-      if (whole || warp == 0) {
-#pragma unroll
-        for (int rr = 0; rr < RH; ++rr) {
-          const int h = r0 + 8 * rr;
-          if (h0 + h >= group) continue;
-          const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
-#pragma unroll
-          for (int t = 0; t < 8 * NB; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (8 * t + cc + e < c.hd) out[(int64_t)h * c.hd + 8 * t + cc + e] = (TQ)(o[t][2 * rr + e] * inv);
-        }
-      }
-      continue;
-    }
-    // The part's place: 0 if the unit is the block's first, else 1.
-    const int slot = 2 * blockIdx.x + (at.unit_at + at.c0 == blockIdx.x * per ? 0 : 1);
-    const int parts = b1 - b0 + 1;
-    // Parts in block order; the unit is the first of every block but b0,
-    // where it is unless it begins inside the block's range.
-    const int first = 2 * b0 + (at.unit_at == b0 * per ? 0 : 1);
-    auto part_of = [&](int p) { return d.part + (int64_t)(p == 0 ? first : 2 * (b0 + p)) * HT * LD; };
-    bool last = false;
-    if (warp == 0) {
-      float* to = d.part + (int64_t)slot * HT * LD;
+    if (!pad && at.c0 == 0 && at.c1 == at.n_unit) {
+      TQ* out = static_cast<TQ*>(a.out) + (int64_t)at.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
 #pragma unroll
       for (int rr = 0; rr < RH; ++rr) {
+        const int h = r0 + 8 * rr;
+        if (h0 + h >= group) continue;
+        const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
 #pragma unroll
         for (int t = 0; t < 8 * NB; ++t)
-          *reinterpret_cast<float2*>(to + (r0 + 8 * rr) * LD + 8 * t + cc) =
-              make_float2(o[t][2 * rr], o[t][2 * rr + 1]);
-        if ((lane & 3) == 0)
-          *reinterpret_cast<float2*>(to + (r0 + 8 * rr) * LD + S::HD) = make_float2(m[rr], l[rr]);
-      }
-      __threadfence();
-      __syncwarp();
-      int seen = 0;
-      if (lane == 0) {
-        seen = atomicAdd(d.count + b0, 1);
-        if (seen == parts - 1) d.count[b0] = 0;
-      }
-      last = __shfl_sync(0xffffffffu, seen, 0) == parts - 1;
-      __threadfence();
-      if (parts > FEW_PARTS && lane == 0) last_sh = last;
-    }
-    if (parts <= FEW_PARTS) {
-      // Warp 0 joins them by itself; the others go on.
-      if (last) {
 #pragma unroll
-        for (int rr = 0; rr < RH; ++rr) {
-          const int h = r0 + 8 * rr;
-          float2 ml[FEW_PARTS];
-          float top = -INFINITY, total = 0.f;
-#pragma unroll
-          for (int p = 0; p < FEW_PARTS; ++p) {
-            ml[p] = p < parts ? __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + S::HD))
-                              : make_float2(-INFINITY, 0.f);
-            top = fmaxf(top, ml[p].x);
-          }
-          const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-          for (int p = 0; p < FEW_PARTS; ++p) {
-            ml[p].x = exp2_fast(ml[p].x - base);
-            total = __fmaf_rn(ml[p].x, ml[p].y, total);
-          }
-          const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-          if (h0 + h >= group) continue;
-#pragma unroll
-          for (int t = 0; t < 8 * NB; ++t) {
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int p = 0; p < FEW_PARTS; ++p)
-              if (p < parts) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + 8 * t + cc));
-                s0 = __fmaf_rn(ml[p].x, v.x, s0);
-                s1 = __fmaf_rn(ml[p].x, v.y, s1);
-              }
-            if (8 * t + cc < c.hd) {
-              out[(int64_t)h * c.hd + 8 * t + cc] = (TQ)(s0 * inv);
-              out[(int64_t)h * c.hd + 8 * t + cc + 1] = (TQ)(s1 * inv);
-            }
-          }
-        }
+          for (int e = 0; e < 2; ++e)
+            if (8 * t + cc + e < c.hd) out[(int64_t)h * c.hd + 8 * t + cc + e] = (TQ)(o[t][2 * rr + e] * inv);
       }
       continue;
     }
-    __syncthreads();
-    if (last_sh) {
-      __threadfence();
-      // First every part's share of each head's result (a warp per head, the
-      // parts over its lanes), then the sums over the parts.
-      float* share = merge;  // [HT][parts]
-      for (int h = warp; h < HT; h += W) {
-        float2 ml[DEC_MAX_PARTS / 32];
-        float top = -INFINITY, total = 0.f;
+    // The last segment's part goes where the ring was: its loads have all come.
+    const int which = have ? 0 : 1;
+    float* to = which ? reinterpret_cast<float*>(slots) : firsts + warp * HT * LD;
 #pragma unroll
-        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
-          const int p = lane + 32 * u;
-          ml[u] = p < parts ? __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + S::HD))
-                            : make_float2(-INFINITY, 0.f);
-          top = fmaxf(top, ml[u].x);
-        }
+    for (int rr = 0; rr < RH; ++rr) {
+      float* row = to + (r0 + 8 * rr) * LD;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
-          ml[u].x = exp2_fast(ml[u].x - base);
-          total = __fmaf_rn(ml[u].x, ml[u].y, total);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-#pragma unroll
-        for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
-          if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
-      }
-      __syncthreads();
-      constexpr int QUADS = HT * S::HD / 4;
-      for (int x = tid; x < QUADS; x += 32 * W) {
-        const int h = x / (S::HD / 4), y = 4 * (x - h * (S::HD / 4));
-        if (h0 + h >= group || y >= c.hd) continue;
-        float4 sum4 = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int p = 0; p < parts; ++p) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p) + h * LD + y));
-          const float w = share[h * parts + p];
-          sum4.x = __fmaf_rn(w, v.x, sum4.x);
-          sum4.y = __fmaf_rn(w, v.y, sum4.y);
-          sum4.z = __fmaf_rn(w, v.z, sum4.z);
-          sum4.w = __fmaf_rn(w, v.w, sum4.w);
-        }
-        TQ* to = out + (int64_t)h * c.hd + y;
-        to[0] = (TQ)sum4.x;
-        to[1] = (TQ)sum4.y;
-        to[2] = (TQ)sum4.z;
-        to[3] = (TQ)sum4.w;
-      }
+      for (int t = 0; t < 8 * NB; ++t)
+        *reinterpret_cast<float2*>(row + 8 * t + cc) = make_float2(o[t][2 * rr], o[t][2 * rr + 1]);
+      if ((lane & 3) == 0) *reinterpret_cast<float2*>(row + S::HD) = make_float2(m[rr], l[rr]);
     }
-    __syncthreads();  // last_sh is read before the next segment writes it
+    if (lane == 0) parts_sh[2 * warp + which] = DecPart{1, at.i, at.unit, at.n_unit, at.unit_at};
   }
-  // A failed wait leaves loads in flight: they land before the block ends.
+  // A failed wait leaves loads in flight: they land before the block goes on.
   if (!ok)
     for (; used < issued; ++used) mbar_wait(&full[warp][used % ST], (used / ST) & 1, c.status, W_ATT_DEC);
+
+  // ---- the block's parts, unit by unit in the order of the line --------------------
+  __syncthreads();
+  auto part_at = [&](int x) {
+    return x & 1 ? reinterpret_cast<const float*>(ring + (x >> 1) * ST * S::CHUNK) : firsts + (x >> 1) * HT * LD;
+  };
+  // What each part counts for in its unit; the unit's maximum and sum (by its
+  // first part).
+  float2(*unit_sh)[HT] = reinterpret_cast<float2(*)[HT]>(ring + HT * LD * 4);
+  float(*share_sh)[HT] = reinterpret_cast<float(*)[HT]>(ring + HT * LD * 4 + 2 * W * HT * 8);
+  unsigned held, heads;  // entries that hold a part; that hold their unit's first
+  {
+    const bool have_part = lane < 2 * W && parts_sh[lane & (2 * W - 1)].have;
+    held = __ballot_sync(0xffffffffu, have_part);
+    const int before_me = 31 - __clz(held & ((1u << lane) - 1));
+    const DecPart* me = parts_sh + (lane & (2 * W - 1));
+    const DecPart* prev = parts_sh + max(before_me, 0);
+    heads = __ballot_sync(0xffffffffu,
+                          have_part && (before_me < 0 || prev->i != me->i || prev->unit != me->unit));
+  }
+  // Entries of the unit that begins at e: those before the next one's first.
+  auto unit_of = [&](int e) {
+    const unsigned later = heads & ~((2u << e) - 1);
+    return held & ~((1u << e) - 1) & (later ? (later & -later) - 1 : 0xffffffffu);
+  };
+  if (tid < 2 * W * HT) {  // (whole warps)
+    const int e = tid & (2 * W - 1), h = tid / (2 * W);
+    const bool mine_held = held >> e & 1;
+    const float2 ml = mine_held ? *reinterpret_cast<const float2*>(part_at(e) + h * LD + S::HD)
+                                : make_float2(-INFINITY, 0.f);
+    const int e0 = 31 - __clz(heads & ((2u << e) - 1));
+    const unsigned all_of = mine_held ? unit_of(e0) : 0;
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2 * W; ++k) {
+      const float v = __shfl_sync(0xffffffffu, ml.x, k, 2 * W);
+      if (all_of >> k & 1) top = fmaxf(top, v);
+    }
+    const float share = mine_held ? exp2_fast(ml.x - (top == -INFINITY ? 0.f : top)) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 2 * W; ++k) {
+      const float v = __shfl_sync(0xffffffffu, share * ml.y, k, 2 * W);
+      if (all_of >> k & 1) total += v;
+    }
+    if (mine_held) {
+      share_sh[e][h] = share;
+      if (e == e0) unit_sh[e][h] = make_float2(top, total);
+    }
+  }
+  __syncthreads();
+  constexpr int QUADS = HT * S::HD / 4;
+  int cut[2] = {-1, -1};  // units that other blocks hold too: their first entry
+  for (unsigned left = heads; left; left &= left - 1) {
+    const int e = __ffs(left) - 1;
+    const unsigned all_of = unit_of(e);
+    const DecPart g = parts_sh[e];
+    const bool whole = g.unit_at >= block_at && g.unit_at + g.n_unit <= block_at + per;
+    const int kvh = g.unit / tiles, h0 = (g.unit - kvh * tiles) * HT;
+    TQ* out = static_cast<TQ*>(a.out) + (int64_t)g.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
+    // A cut unit's place: 0 if it is the block's first, else 1.
+    const int slot = g.unit_at <= block_at ? 0 : 1;
+    if (!whole) cut[slot] = e;
+    for (int x = tid; x < QUADS; x += 32 * W) {
+      const int h = x / (S::HD / 4), y = 4 * (x - h * (S::HD / 4));
+      const float2 ml = unit_sh[e][h];
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (unsigned k = all_of; k; k &= k - 1) {
+        const int at_k = __ffs(k) - 1;
+        const float4 u = *reinterpret_cast<const float4*>(part_at(at_k) + h * LD + y);
+        const float w = share_sh[at_k][h];
+        v.x = __fmaf_rn(w, u.x, v.x);
+        v.y = __fmaf_rn(w, u.y, v.y);
+        v.z = __fmaf_rn(w, u.z, v.z);
+        v.w = __fmaf_rn(w, u.w, v.w);
+      }
+      if (whole) {
+        if (h0 + h >= group || y >= c.hd) continue;
+        const float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
+        TQ* to = out + (int64_t)h * c.hd + y;
+        to[0] = (TQ)(v.x * inv);
+        to[1] = (TQ)(v.y * inv);
+        to[2] = (TQ)(v.z * inv);
+        to[3] = (TQ)(v.w * inv);
+      } else {
+        float* to = d.part + ((int64_t)(2 * blockIdx.x + slot) * HT + h) * LD;
+        *reinterpret_cast<float4*>(to + y) = v;
+        if (y == 0) *reinterpret_cast<float2*>(to + S::HD) = ml;
+      }
+    }
+  }
+  if (cut[0] < 0 && cut[1] < 0) return;
+
+  // ---- units of several blocks: the last to come joins the parts ---------------------
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    last_sh[tid] = 0;
+    if (cut[tid] >= 0) {
+      const DecPart g = parts_sh[cut[tid]];
+      const int b0 = (int)(g.unit_at / per), b1 = (int)((g.unit_at + g.n_unit - 1) / per);
+      last_sh[tid] = atomicAdd(d.count + b0, 1) == b1 - b0;
+      if (last_sh[tid]) d.count[b0] = 0;
+    }
+  }
+  __syncthreads();
+  for (int side = 0; side < 2; ++side) {
+    if (!last_sh[side]) continue;
+    __threadfence();
+    const DecPart g = parts_sh[cut[side]];
+    const int b0 = (int)(g.unit_at / per), parts = (int)((g.unit_at + g.n_unit - 1) / per) - b0 + 1;
+    const int kvh = g.unit / tiles, h0 = (g.unit - kvh * tiles) * HT;
+    TQ* out = static_cast<TQ*>(a.out) + (int64_t)g.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
+    // Parts in block order; the unit is the first of every block but b0, where
+    // it is unless it begins inside the block's range.
+    const int first = 2 * b0 + (g.unit_at == b0 * per ? 0 : 1);
+    auto part_of = [&](int p) { return d.part + (int64_t)(p == 0 ? first : 2 * (b0 + p)) * HT * LD; };
+    // First every part's share of each head's result (a warp per head, the
+    // parts over its lanes), then the sums over the parts.
+    float* share = firsts;  // [HT][parts]
+    __syncthreads();
+    for (int h = warp; h < HT; h += W) {
+      float2 ml[DEC_MAX_PARTS / 32];
+      float top = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
+        const int p = lane + 32 * u;
+        ml[u] = p < parts ? __ldcg(reinterpret_cast<const float2*>(part_of(p) + h * LD + S::HD))
+                          : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[u].x);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int u = 0; u < DEC_MAX_PARTS / 32; ++u) {
+        ml[u].x = exp2_fast(ml[u].x - base);
+        total = __fmaf_rn(ml[u].x, ml[u].y, total);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+#pragma unroll
+      for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
+        if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
+    }
+    __syncthreads();
+    for (int x = tid; x < QUADS; x += 32 * W) {
+      const int h = x / (S::HD / 4), y = 4 * (x - h * (S::HD / 4));
+      if (h0 + h >= group || y >= c.hd) continue;
+      float4 sum4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int p = 0; p < parts; ++p) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p) + h * LD + y));
+        const float w = share[h * parts + p];
+        sum4.x = __fmaf_rn(w, v.x, sum4.x);
+        sum4.y = __fmaf_rn(w, v.y, sum4.y);
+        sum4.z = __fmaf_rn(w, v.z, sum4.z);
+        sum4.w = __fmaf_rn(w, v.w, sum4.w);
+      }
+      TQ* to = out + (int64_t)h * c.hd + y;
+      to[0] = (TQ)sum4.x;
+      to[1] = (TQ)sum4.y;
+      to[2] = (TQ)sum4.z;
+      to[3] = (TQ)sum4.w;
+    }
+  }
 }
 
 size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 4) * sizeof(float); }
@@ -717,9 +732,10 @@ static int launch_decode(const DecArgs& d, const KvMaps& maps, cudaStream_t st) 
   static_assert(S::ST >= 2 && S::SMEM <= 226 * 1024, "two stages fit");
   static PerDeviceOnce attr;
   if (smem_attr_once(attr, attn_decode_kernel<TQ, TKV, NB, HT>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
-  // One block per SM, fewer when the tables hold less than a chunk per warp of each.
   const int64_t units = (int64_t)d.a.n * d.a.c.nkv * ((d.a.nh / d.a.c.nkv + HT - 1) / HT);
   const int64_t most = (int64_t)d.a.c.max_pages * d.a.c.page / DC;
+  if (most * (units / d.a.n) > INT32_MAX - 8 * num_sms()) return KC_ERR_SHAPE;  // chunks of a sequence, all heads
+  // One block per SM, fewer when the tables hold less than a chunk per warp of each.
   const int grid = (int)std::min<int64_t>(std::min(num_sms(), DEC_MAX_PARTS), units * ((most + S::W - 1) / S::W));
   launch_k(attn_decode_kernel<TQ, TKV, NB, HT>, grid, 32 * S::W, S::SMEM, st, d, maps);
   return KC_OK;
