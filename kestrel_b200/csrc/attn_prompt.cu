@@ -319,14 +319,18 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       // takes longer than the product it is for.)
       auto scores = [&](int w, uint32_t k) {
         const uint64_t kd = sw128_desc(k);
+        // Rests first: the tensor cores cut a sum's last bits off at every step,
+        // which costs the less the smaller the sum still is (f32 results over
+        // 4096 positions are 1.9e-6 off otherwise).
 #pragma unroll
-        for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
+        for (int part = kSplit ? 1 : 0; part >= 0; --part) {
           const uint64_t qd = sw128_desc(qa + ((TWO ? w : 0) * (kSplit ? 2 : 1) + part) * S::QB);
 #pragma unroll
           for (int ks = 0; ks < 4 * NB; ++ks)
             if (ks < ksteps)
               tc_mma(tmem + 128 * w, qd + ((ks >> 2) * PM * 128 + 32 * (ks & 3)) / 16,
-                     kd + ((ks >> 2) * BN * 128 + 32 * (ks & 3)) / 16, id_s, part > 0 || ks > 0);
+                     kd + ((ks >> 2) * BN * 128 + 32 * (ks & 3)) / 16, id_s,
+                     part < (kSplit ? 1 : 0) || ks > 0);
         }
         tc_commit(&s_full[w]);
       };
