@@ -44,7 +44,7 @@ namespace kc {
 constexpr int PM = 128;  // rows of a tile
 constexpr int P_STAGES_MAX = 8;
 constexpr int P_SPLITS_MAX = 8;  // blocks an item's positions are split over, at most
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * 168, "within the registers of the launch");
 
 template <typename TQ, int NB, bool TWO>
@@ -64,11 +64,20 @@ struct PromptShape {
   // Two streams: three warpgroups of 168 registers a thread at launch, of which
   // the third (loads, MMAs) gives the softmax warps 32 a thread.
   static constexpr int THREADS = 128 * NS + 128;
-  static constexpr int T_O = 256;                  // TMEM columns: S of stream w at 128 w, its O at T_O + HD w
+  // TMEM columns. Two streams with 16-bit weights share the scores' columns:
+  // they are free again as soon as they are in registers, so that the next
+  // scores are there when a softmax ends and its warps never wait for their own
+  // products (8192 rows of 32 heads: 478 us with scores and weights in the same
+  // columns, 464 so). Weights of two operands leave no room for that.
+  static constexpr bool kShared = NS == 2 && !kSplit;
+  static constexpr int T_S = kShared ? 0 : 128;    // scores of stream w at T_S w
+  static constexpr int T_P = kShared ? 128 : 0;    // its weights at T_P + (kShared ? 64 : 128) w
+  static constexpr int T_PW = kShared ? 64 : 128;
+  static constexpr int T_O = 256;                  // its accumulator at T_O + HD w
   // A split item's part: per four columns the rows' values ([HD / 4][PM][4]),
   // then the rows' maxima and sums ([PM][2]).
   static constexpr int PART = PM * (HD + 2);
-  static_assert(!TWO || NS == 2, "two row tiles need two streams");
+  static_assert(!TWO || kShared, "two row tiles: two streams of 16-bit weights");
   static_assert(ST >= 2 && T_O + NS * HD <= 512, "fits");
 };
 
@@ -182,12 +191,13 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   constexpr float kLift = std::is_same_v<TKV, __half> ? 7.f : 0.f;
   constexpr float kGrow = 8.f;
   constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1, W_AUX = W_TMA + 2;  // W_AUX: and the next
-  constexpr int AHEAD = TWO ? 1 : NS;  // K tiles loaded before the first V
+  constexpr bool kShared = S::kShared;
+  constexpr int AHEAD = NS;  // K tiles loaded before the first V
   if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : &q_map);
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
-  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], p_half[NS], p_full[NS], o_full[NS],
-      o_empty[NS];
+  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], s_free[NS], p_half[NS], p_full[NS],
+      pv_done[NS], o_empty[NS];
   __shared__ __align__(8) uint64_t q_raw, q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint32_t tmem_sh;
   __shared__ Item items[2];
@@ -212,7 +222,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       mbar_init(&s_full[w], 1);
       mbar_init(&p_half[w], 128);
       mbar_init(&p_full[w], 128);
-      mbar_init(&o_full[w], 1);
+      mbar_init(&s_free[w], 128);
+      mbar_init(&pv_done[w], 1);
       mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
     mbar_init(&q_raw, 1);
@@ -305,11 +316,12 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       const uint32_t id_s = tc_idesc<TKV>(BN, false), id_o = tc_idesc<TKV>(hd16, true);
       const int ksteps = hd16 / 16;
       const uint32_t qa = smem_u32(q_sm), ra = smem_u32(ring);
-      int it = 0;         // next stage of the ring, in the order of its loads
-      int kp[NS];         // weight tiles of each stream so far
-      int used = 0;       // items with products so far
+      int ring_at = 0;  // loads before this item's
+      int kp[NS];       // weight tiles of each stream so far
+      int used = 0;     // items with products so far
+#pragma unroll
       for (int w = 0; w < NS; ++w) kp[w] = 0;
-      auto stage_wait = [&]() {
+      auto stage = [&](int it) {
         wait(&kv_full[it % ST], it / ST);
         tc_fence_after();
         return ra + (it % ST) * S::KV;
@@ -328,7 +340,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 #pragma unroll
           for (int ks = 0; ks < 4 * NB; ++ks)
             if (ks < ksteps)
-              tc_mma(tmem + 128 * w, qd + ((ks >> 2) * PM * 128 + 32 * (ks & 3)) / 16,
+              tc_mma(tmem + S::T_S * w, qd + ((ks >> 2) * PM * 128 + 32 * (ks & 3)) / 16,
                      kd + ((ks >> 2) * BN * 128 + 32 * (ks & 3)) / 16, id_s,
                      part < (kSplit ? 1 : 0) || ks > 0);
         }
@@ -336,28 +348,29 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       };
       // The weights come in two halves, so that the first half's products run
       // beside the exponentials of the second.
-      auto values = [&](int w, uint32_t v, bool add) {
+      auto values = [&](int w, int k, uint32_t v, bool add) {
         const uint64_t vd = sw128_desc_mn(v, BN * 128);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          wait(half ? &p_full[w] : &p_half[w], kp[w]);
+          wait(half ? &p_full[w] : &p_half[w], k);
           if (!ok) return;
           tc_fence_after();
 #pragma unroll
           for (int part = 0; part < (kSplit ? 2 : 1); ++part)
 #pragma unroll
             for (int ks = half * (BN / 32); ks < (half + 1) * (BN / 32); ++ks)
-              tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + 128 * w + part * (BN / 2) + 8 * ks, vd + ks * 2048 / 16,
-                        id_o, add || half > 0 || part > 0 || ks > 0);
+              tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + S::T_P + S::T_PW * w + part * (BN / 2) + 8 * ks,
+                        vd + ks * 2048 / 16, id_o, add || half > 0 || part > 0 || ks > 0);
         }
-        ++kp[w];
+        tc_commit(&pv_done[w]);
       };
-      // Before an item's first products into the accumulators: the last item's
-      // results have been read from them.
+      // Before an item's first products into an accumulator: the last item's
+      // results have been read from it.
       auto results_read = [&](int w) {
         if (used > 0) wait(&o_empty[w], used - 1);
         tc_fence_after();
       };
+      int claims = 0, claim_w = 0, claim_k = 0;  // the scores issued last: whose they are
       for (int n = 0; ok; ++n) {
         if (!item_wait(n)) break;
         const int valid = items[n & 1].valid, nt = items[n & 1].t1 - items[n & 1].t0;
@@ -367,69 +380,62 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         wait(&q_full, used);
         if (!ok) break;
         tc_fence_after();
-        if constexpr (TWO) {
-          uint32_t k = stage_wait();
-          if (!ok) break;
-          scores(0, k);
-          scores(1, k);
-          tc_commit(&kv_empty[it % ST]);
-          ++it;
-          if (nt == 1) tc_commit(&q_empty);
-          for (int t = 0; t < nt && ok; ++t) {
-            const int v_it = it;
-            const uint32_t v = stage_wait();
-            ++it;
-            const bool more = t + 1 < nt;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (t == 0) results_read(w);
-              values(w, v, t > 0);
+        // Loads come as K 0, K 1, V 0, K 2, V 1 ...
+        auto k_at = [&](int t) { return ring_at + (NS == 2 ? max(2 * t - 1, 0) : 2 * t); };
+        auto v_at = [&](int t) { return ring_at + (NS == 2 ? min(2 * t + 2, 2 * nt - 1) : 2 * t + 1); };
+        if constexpr (kShared) {
+          // Steps: (tile, stream) pairs in turn. Scores of step i + 1, then the
+          // products of step i - 1.
+          const int steps = TWO ? 2 * nt : nt;
+          for (int i = -1; i <= steps && ok; ++i) {
+            if (i + 1 < steps) {
+              const int w = (i + 1) & 1, t = TWO ? (i + 1) >> 1 : i + 1;
+              const uint32_t k = stage(k_at(t));
+              // The last scores have been read.
+              if (claims++ > 0) wait(&s_free[claim_w], claim_k);
               if (!ok) break;
-              if (w == 1) tc_commit(&kv_empty[v_it % ST]);
-              if (!more) {
-                tc_commit(&o_full[w]);
-                continue;
-              }
-              if (w == 0) k = stage_wait();
-              if (!ok) break;
+              tc_fence_after();
               scores(w, k);
+              claim_w = w;
+              claim_k = kp[w] + (TWO ? t : t >> 1);
+              if (!TWO || w == 1) tc_commit(&kv_empty[k_at(t) % ST]);
+              if (i + 2 == steps) tc_commit(&q_empty);
             }
-            if (ok && more) {
-              tc_commit(&kv_empty[it % ST]);
-              ++it;
-              if (t + 2 == nt) tc_commit(&q_empty);
+            if (i >= 1) {
+              const int w = (i - 1) & 1, t = TWO ? (i - 1) >> 1 : i - 1, k = TWO ? t : t >> 1;
+              const uint32_t v = stage(v_at(t));
+              if (k == 0) results_read(w);
+              values(w, kp[w] + k, v, k > 0);
+              if (!ok) break;
+              if (!TWO || w == 1) tc_commit(&kv_empty[v_at(t) % ST]);
             }
           }
+          if (!TWO && nt == 1) results_read(1);  // (each item's phase is waited for)
+#pragma unroll
+          for (int w = 0; w < NS; ++w) kp[w] += TWO ? nt : (nt - w + 1) >> 1;
         } else {
-          for (int w = 0; w < NS && w < nt && ok; ++w) {
-            const uint32_t k = stage_wait();
-            if (!ok) break;
-            scores(w, k);
-            tc_commit(&kv_empty[it % ST]);
-            ++it;
-          }
-          if (ok && nt <= NS) tc_commit(&q_empty);
+          auto step_scores = [&](int t) {
+            const uint32_t k = stage(k_at(t));
+            if (!ok) return;
+            scores(t % NS, k);
+            tc_commit(&kv_empty[k_at(t) % ST]);
+            if (t + 1 == nt) tc_commit(&q_empty);
+          };
+          for (int t = 0; t < NS && t < nt && ok; ++t) step_scores(t);
 #pragma unroll
           for (int w = 0; w < NS; ++w) results_read(w);
           for (int t = 0; t < nt && ok; ++t) {
             const int w = t % NS;
-            const uint32_t v = stage_wait();
-            values(w, v, t >= NS);
+            const uint32_t v = stage(v_at(t));
+            values(w, kp[w] + t / NS, v, t >= NS);
             if (!ok) break;
-            tc_commit(&kv_empty[it % ST]);
-            ++it;
-            if (t + NS < nt) {
-              const uint32_t k = stage_wait();
-              if (!ok) break;
-              scores(w, k);
-              tc_commit(&kv_empty[it % ST]);
-              ++it;
-              if (t + NS + 1 == nt) tc_commit(&q_empty);
-            } else {
-              tc_commit(&o_full[w]);
-            }
+            tc_commit(&kv_empty[v_at(t) % ST]);
+            if (t + NS < nt) step_scores(t + NS);
           }
+#pragma unroll
+          for (int w = 0; w < NS; ++w) kp[w] += (nt - w + NS - 1) / NS;
         }
+        ring_at += 2 * nt;
         ++used;
       }
       // The tensor cores are done with TMEM and shared memory.
@@ -676,10 +682,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // ---- softmax: stream w, a thread per row ---------------------------------
     const int w = warp >> 2, r = tid & 127, my_tile = TWO ? w : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_t = tmem + lanes + 128 * w;
+    const uint32_t s_t = tmem + lanes + S::T_S * w, p_t = tmem + lanes + S::T_P + S::T_PW * w;
     const float unit = flip == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     int ks = 0, used = 0, ring_at = 0;  // score tiles, items with products, loads before this item's
-    int full[NS] = {}, parts = 0;       // results of each stream, split items before this one
+    int done[NS] = {}, parts = 0;       // tiles of each stream, split items before this one's
     for (int n = 0;; ++n) {
       item_wait(n);
       ok = __all_sync(0xffffffffu, ok);
@@ -715,6 +721,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 #pragma unroll
         for (int e = 0; e < BN; e += 32) tmem_ld32(s_t + e, s + e);
         tmem_wait_ld();
+        if constexpr (kShared) {
+          tc_fence_before();
+          mbar_arrive(&s_free[w]);
+        }
         if (j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks)) {
           // A bit per position: up to the row's own, and not before its window
           // unless among the first tokens.
@@ -757,8 +767,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         auto hand_over = [&](int half, const uint32_t* p, const uint32_t* rest) {
 #pragma unroll
           for (int e = 0; e < BN / 4; e += 16) {
-            tmem_st16(s_t + half * (BN / 4) + e, p + e);
-            if constexpr (kSplit) tmem_st16(s_t + BN / 2 + half * (BN / 4) + e, rest + e);
+            tmem_st16(p_t + half * (BN / 4) + e, p + e);
+            if constexpr (kSplit) tmem_st16(p_t + BN / 2 + half * (BN / 4) + e, rest + e);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -780,9 +790,14 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         float sum = 0.f;
         if constexpr (!kSplit) sum = weigh(0, m, p, rest);
         const bool grow = top > m + kGrow;
+        // This stream's last products are complete (with scores of its own that
+        // followed them they are anyway): the weights' columns are free, and
+        // until it has these the accumulator is this warp's.
+        if (kShared && ks > 0) {
+          wait(&pv_done[w], ks - 1);
+          tc_fence_after();
+        }
         if (__any_sync(0xffffffffu, grow)) {
-          // The products before these scores are complete, and the next ones
-          // wait for these weights: the accumulator is this warp's for now.
           const float shrink = grow ? exp2_fast(m - top) : 1.f;
           if (grow) m = top;
           l *= shrink;
@@ -815,7 +830,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       if (nt > 0) {
 #pragma unroll
         for (int v = 0; v < NS; ++v)
-          if (TWO ? v == w : v < nt) wait(&o_full[v], full[v]++);
+          if (TWO ? v == w : v < nt) {
+            done[v] += TWO ? nt : (nt - v + NS - 1) / NS;
+            wait(&pv_done[v], done[v] - 1);
+          }
         if constexpr (kJoin) {
           join_sh[used & 1][w][r] = make_float2(m, l);
           mbar_arrive(&join_full);
