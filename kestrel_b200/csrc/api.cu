@@ -3099,7 +3099,7 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
       return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: page of %d positions (16, 32, 64, 128 or 256)", page);
     if (head_dim < 8 || head_dim > 256 || head_dim % 8)
       return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: head_dim %d (a multiple of 8 up to 256)", head_dim);
-    if ((int64_t)max_pages * page > INT32_MAX || (int64_t)n_seq * max_pages > INT32_MAX ||
+    if ((int64_t)max_pages * page > INT32_MAX - 1024 || (int64_t)n_seq * max_pages > INT32_MAX ||
         (int64_t)n_layer * n_pages > INT32_MAX || n_head_kv > 4096)
       return fail(ctx, KC_ERR_SHAPE, "kc_kv_cache: sizes past 32 bits (max_pages * page, n_seq * max_pages or "
                                      "n_layer * n_pages)");

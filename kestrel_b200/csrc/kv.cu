@@ -244,7 +244,12 @@ __global__ void __launch_bounds__(KV_BLOCK) kv_extend_kernel(KvView c, const int
 // Rows 0 .. rows[i]-1 (null rows: all) of page src[i] to page dst[i], every
 // layer and head, k and v. No dst is a src. A unit is one page of one layer of
 // k or v; a block takes units in turn.
+// Bound by the memory rate (each byte read and written once). Four 16-byte
+// pieces of a thread under way and sixteen blocks per SM: 1.72 GB of pages in
+// 285 us, 6.0 TB/s, 93% of a plain copy (one piece 299, eight blocks and four
+// pieces 286, four blocks and eight 305).
 constexpr int COPY_THREADS = 256;
+constexpr int COPY_AHEAD = 4;  // 16-byte pieces of a thread under way
 __global__ void __launch_bounds__(COPY_THREADS) kv_copy_kernel(KvView c, bool whole, int32_t* table_remap,
                                                                const int* __restrict__ n_live) {
   pdl_enter();
@@ -268,18 +273,27 @@ __global__ void __launch_bounds__(COPY_THREADS) kv_copy_kernel(KvView c, bool wh
     uint4* pool = reinterpret_cast<uint4*>(w & 1 ? c.v : c.k) + (int64_t)(w >> 1) * c.n_pages * page_vec;
     const uint4* from = pool + c.src[i] * page_vec;
     uint4* to = pool + c.dst[i] * page_vec;
-    const int per = whole ? head_vec : c.rows[i] * row_vec;
-    for (int j = threadIdx.x; j < per * c.nkv; j += COPY_THREADS) {
-      const int h = j / per;
-      const int64_t at = (int64_t)h * head_vec + (j - h * per);
-      to[at] = from[at];
+    // A head's rows lie together; whole pages altogether.
+    const int per = whole ? (int)page_vec : c.rows[i] * row_vec, n_vec = whole ? (int)page_vec : per * c.nkv;
+    for (int j0 = threadIdx.x; j0 < n_vec; j0 += COPY_AHEAD * COPY_THREADS) {
+      uint4 v[COPY_AHEAD];
+      int64_t at[COPY_AHEAD];
+#pragma unroll
+      for (int k = 0; k < COPY_AHEAD; ++k) {
+        const int j = j0 + k * COPY_THREADS, h = j / per;
+        at[k] = (int64_t)h * head_vec + (j - h * per);
+        if (j < n_vec) v[k] = __ldcs(from + at[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < COPY_AHEAD; ++k)
+        if (j0 + k * COPY_THREADS < n_vec) __stcs(to + at[k], v[k]);
     }
   }
 }
 
 static void launch_copies(const KvView& c, int most, bool whole, int32_t* remap, const int* n_live, cudaStream_t st) {
   const int64_t units = (int64_t)most * c.n_layer * 2;
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(units, 1), 8 * (int64_t)num_sms());
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(units, 1), 16 * (int64_t)num_sms());
   launch_k(kv_copy_kernel, grid, COPY_THREADS, 0, st, c, whole, remap, n_live);
 }
 
