@@ -536,3 +536,50 @@ def test_weights_of_many_positions(ctx):
     ctx.attn_prompt_dev(c.id, 0, q, ints([0, 40]), out, scale=1.0)
     ctx.sync()
     close(wide(out), c.expected(0, wide(q), [0], [40], 1.0, 0, 0), F32)
+
+
+def test_offsets_past_32_bits(ctx):
+    """Pools of more than 2^31 elements, with the sequence's pages at their end:
+    every call addresses them."""
+    page, n_kv, hd = 256, 8, 128
+    n_pages = (1 << 31) // (page * n_kv * hd) + 40
+    k, v = (torch.empty((1, n_pages, n_kv, page, hd), dtype=F16, device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = 900
+    ids = [n_pages - 1, n_pages - 30, n_pages - 2, n_pages - 29]
+    table = torch.full((2, 5), -1, dtype=torch.int32, device="cuda")
+    table[0, :4] = ints(ids)
+    length, refs = ints([n - 1, 0]), torch.ones(n_pages, dtype=torch.int32, device="cuda")
+    refs[n_pages - 5:n_pages - 2] = 0
+    ctx.kv_cache(9999, k, v, table, length, refs)
+    rows_k, rows_v = (torch.randn((n, n_kv, hd), generator=g, device="cuda", dtype=F16) for _ in range(2))
+    ctx.kv_write_dev(9999, 0, rows_k[:n - 1], rows_v[:n - 1], row_start=ints([0, n - 1]))
+    ctx.kv_fork_dev(9999, ints([0]), ints([1]))
+    ctx.kv_extend_dev(9999, ints([1]), ints([1]))  # copies the last page into the pool's last free ones
+    ctx.kv_write_dev(9999, 0, rows_k[n - 1:], rows_v[n - 1:], seqs=ints([1]))
+    ctx.sync()
+    assert table[1].tolist() == ids[:3] + [n_pages - 5, -1] and length.tolist() == [n - 1, n]
+    for heads, t in (((16, 8), F32), ((8, 8), F16)):
+        q = queries(40, heads[0], hd, t, 2)
+        want = attention(wide(q), wide(rows_k), wide(rows_v), n - 40, hd ** -0.5)
+        out = torch.empty_like(q.contiguous())
+        ctx.attn_prompt_dev(9999, 0, q, ints([0, 40]), out, seqs=ints([1]))
+        one = torch.empty_like(out[:1])
+        ctx.attn_decode_dev(9999, 0, q[39:], one, seqs=ints([1]))
+        ctx.sync()
+        close(wide(out), want, t)
+        close(wide(one), want[39:], t)
+    ctx.kv_drop(9999)
+
+
+@pytest.mark.parametrize("args", [dict(), dict(window=100, sinks=4, page=16, prompt=500, chunk=130),
+                                  dict(sequences=1, branches=5, prompt=40, steps=6)], ids=str)
+def test_example(args):
+    """kestrel_b200.paged_example: the operators as a server calls them. The two
+    kernels' f32 results differ by at most twice an f32 result's tolerance."""
+    from kestrel_b200 import paged_example
+    got = paged_example.run(**args)
+    assert got["finite"] and got["same_after_compaction"]
+    assert got["kernels_differ"] <= 2 * TOL[F32]
+    assert got["pages_live"] < got["pages_without_sharing"]
+    assert got["pages_after_compaction"] < got["pages_live"]
