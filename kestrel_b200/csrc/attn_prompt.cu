@@ -13,7 +13,7 @@
 //   softmax warps  four per stream, a thread per row: scores from TMEM, the
 //                  mask where the tile needs it, weights back to TMEM as the
 //                  16-bit A operand of the second product. The accumulator is
-//                  rescaled only when a row's maximum has grown by 2^8.
+//                  rescaled only when a row's weights have grown too large.
 //   a TMA warp     K and V tiles, a box per page, through one ring.
 //   an MMA warp    S = Q K^T (both in shared memory), O += P V (P in TMEM).
 //   two more       find the next item and bring its queries, while the others
@@ -94,6 +94,9 @@ __device__ __forceinline__ bool normalise16(float (&v)[16], float f) {
   }
   return f2(odd).x + f2(odd).y != 0.f;
 }
+
+// Keeps a branch's code out of the way of what runs for every tile.
+__device__ __forceinline__ bool rarely(bool c) { return __builtin_expect(c, 0); }
 
 // The lowest n bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t low_bits(int n) {
@@ -187,9 +190,12 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   using S = PromptShape<TQ, NB, TWO>;
   constexpr int BN = S::BN, NS = S::NS, ST = S::ST;
   constexpr bool kSplit = S::kSplit;
-  // Weights reach 2^(lift + 8): small ones of f16 keep their bits.
-  constexpr float kLift = std::is_same_v<TKV, __half> ? 7.f : 0.f;
-  constexpr float kGrow = 8.f;
+  // Weights are 2^lift for a score at the reference, so that small ones of f16
+  // keep their bits; f16's range ends at 2^16, and rescaling starts from sums of
+  // kMost. (Two f16 operands: rescaling starts 2^8 past the reference.)
+  constexpr bool kF16 = std::is_same_v<TKV, __half>;
+  constexpr float kLift = kSplit ? 7.f : kF16 ? 3.f : 0.f;
+  constexpr float kMost = kF16 ? 32768.f : 1.1e9f;
   constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1, W_AUX = W_TMA + 2;  // W_AUX: and the next
   constexpr bool kShared = S::kShared;
   constexpr int AHEAD = NS;  // K tiles loaded before the first V
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
   __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], s_free[NS], p_half[NS], p_full[NS],
-      pv_done[NS], o_empty[NS];
+      half_done[NS], pv_done[NS], o_empty[NS];
   __shared__ __align__(8) uint64_t q_raw, q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint32_t tmem_sh;
   __shared__ Item items[2];
@@ -223,6 +229,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       mbar_init(&p_half[w], 128);
       mbar_init(&p_full[w], 128);
       mbar_init(&s_free[w], 128);
+      mbar_init(&half_done[w], 1);
       mbar_init(&pv_done[w], 1);
       mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
@@ -361,6 +368,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             for (int ks = half * (BN / 32); ks < (half + 1) * (BN / 32); ++ks)
               tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + S::T_P + S::T_PW * w + part * (BN / 2) + 8 * ks,
                         vd + ks * 2048 / 16, id_o, add || half > 0 || part > 0 || ks > 0);
+          if (!kSplit && half == 0) tc_commit(&half_done[w]);
         }
         tc_commit(&pv_done[w]);
       };
@@ -725,7 +733,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           tc_fence_before();
           mbar_arrive(&s_free[w]);
         }
-        if (j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks)) {
+        if (rarely(j0 + BN - 1 > t_at0 || (j0 < t_lo1 && j0 + BN > a.sinks))) {
           // A bit per position: up to the row's own, and not before its window
           // unless among the first tokens.
           const int hi = at - j0, from = lo - j0, first = a.sinks - j0;
@@ -736,7 +744,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             for (int e = 0; e < 32; ++e) s[y + e] = see >> e & 1 ? s[y + e] : -INFINITY;
           }
         }
-        if (j0 + BN > x.len) {
+        if (rarely(j0 + BN > x.len)) {
           // Rows past the sequence's end hold whatever the page held before:
           // zeros in their place (only the last tile has such rows; its V is
           // the item's last load).
@@ -751,18 +759,27 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         auto weigh = [&](int half, float mx, uint32_t* p, uint32_t* rest) {
           const float base = kLift - (mx == -INFINITY ? 0.f : mx);
           const uint64_t cq2 = f2(cq, cq), base2 = f2(base, base);
-          uint64_t sum = 0;
+          uint64_t sums[4] = {0, 0, 0, 0};
+          // In stretches of independent steps, so that none waits for the last.
 #pragma unroll
-          for (int e = 0; e < BN / 4; ++e) {
-            const int i = half * (BN / 2) + 2 * e;
-            float2 y = f2(fma2(f2(s[i], s[i + 1]), cq2, base2));
-            y.x = exp2_fast(y.x);
-            y.y = exp2_fast(y.y);
-            sum = add2(sum, f2(y.x, y.y));
-            p[e] = pack2<TKV>(y.x, y.y);
-            if constexpr (kSplit) rest[e] = rest2<TKV>(y.x, y.y, p[e]);
+          for (int e0 = 0; e0 < BN / 4; e0 += 4) {
+            float2 y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = half * (BN / 2) + 2 * (e0 + e);
+              y[e] = f2(fma2(f2(s[i], s[i + 1]), cq2, base2));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = make_float2(exp2_fast(y[e].x), exp2_fast(y[e].y));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sums[e & 3] = add2(sums[e & 3], f2(y[e].x, y[e].y));
+              p[e0 + e] = pack2<TKV>(y[e].x, y[e].y);
+              if constexpr (kSplit) rest[e0 + e] = rest2<TKV>(y[e].x, y[e].y, p[e0 + e]);
+            }
           }
-          return f2(sum).x + f2(sum).y;
+          const float2 sum = f2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+          return sum.x + sum.y;
         };
         auto hand_over = [&](int half, const uint32_t* p, const uint32_t* rest) {
 #pragma unroll
@@ -774,30 +791,23 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           tc_fence_before();
           mbar_arrive(half ? &p_full[w] : &p_half[w]);
         };
-        float tops[8];
+        // Largest of positions from .. from + n - 1, in exponents of 2.
+        auto top_of = [&](int from, int n) {
+          float tops[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tops[e] = s[e];
+          for (int e = 0; e < 8; ++e) tops[e] = s[from + e];
 #pragma unroll
-        for (int e = 8; e < BN; e += 2) tops[e / 2 & 7] = max3(tops[e / 2 & 7], s[e], s[e + 1]);
-        float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
-        top = top == -INFINITY ? top : top * cq;
-        if (k == 0) m = top;
-        // 16-bit weights of the first half are computed against the maximum so
-        // far while this tile's is found, and again in the rare case that it has
-        // grown too much. (With two operands that takes more registers than
-        // there are.)
-        uint32_t p[BN / 4], rest[kSplit ? BN / 4 : 1];
-        float sum = 0.f;
-        if constexpr (!kSplit) sum = weigh(0, m, p, rest);
-        const bool grow = top > m + kGrow;
-        // This stream's last products are complete (with scores of its own that
-        // followed them they are anyway): the weights' columns are free, and
-        // until it has these the accumulator is this warp's.
-        if (kShared && ks > 0) {
-          wait(&pv_done[w], ks - 1);
+          for (int e = 8; e < n; e += 2) tops[e / 2 & 7] = max3(tops[e / 2 & 7], s[from + e], s[from + e + 1]);
+          const float top =
+              max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
+          return top == -INFINITY ? top : top * cq;
+        };
+        // A larger maximum: what has been summed so far is rescaled. The
+        // accumulator is this warp's once `done` has come to `phase` (its
+        // products so far; the next ones wait for weights).
+        auto rescale = [&](float top, bool grow, uint64_t* done, int phase) {
+          if (phase >= 0) wait(done, phase);
           tc_fence_after();
-        }
-        if (__any_sync(0xffffffffu, grow)) {
           const float shrink = grow ? exp2_fast(m - top) : 1.f;
           if (grow) m = top;
           l *= shrink;
@@ -809,13 +819,43 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             for (int e = 0; e < 16; ++e) o[e] *= shrink;
             tmem_st16(o_t + e0, o);
           }
-          if constexpr (!kSplit) sum = weigh(0, m, p, rest);
+          tmem_wait_st();
+        };
+        uint32_t p[BN / 4], rest[kSplit ? BN / 4 : 1];
+        if constexpr (kSplit) {
+          const float top = top_of(0, BN);
+          if (k == 0) m = top;
+          const bool grow = top > m + 8.f;
+          if (__any_sync(0xffffffffu, grow)) rescale(top, grow, nullptr, -1);
+          float sum = weigh(0, m, p, rest);
+          hand_over(0, p, rest);
+          sum += weigh(1, m, p, rest);
+          hand_over(1, p, rest);
+          l += sum;
+        } else {
+          // No maximum is looked for after the first tile: while a half's weights
+          // add up to less than kMost, none of them is past the 16-bit type's
+          // range, and any reference does. (8192 rows of 32 heads: 471 us with
+          // every tile's maximum, 465 so.)
+          if (rarely(k == 0)) m = top_of(0, BN);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float sum = weigh(half, m, p, rest);
+            if (rarely(__any_sync(0xffffffffu, !(sum < kMost) || m == -INFINITY))) {
+              const float top = top_of(half * (BN / 2), BN / 2);
+              const bool grow = top > m && (!(sum < kMost) || m == -INFINITY);
+              if (__any_sync(0xffffffffu, grow)) {
+                if (half == 0) rescale(top, grow, &pv_done[w], ks - 1);
+                else rescale(top, grow, &half_done[w], ks);
+                sum = weigh(half, m, p, rest);
+              }
+            }
+            // The weights' columns are free once the last products are complete.
+            if (kShared && half == 0 && ks > 0) wait(&pv_done[w], ks - 1);
+            hand_over(half, p, rest);
+            l += sum;
+          }
         }
-        if constexpr (kSplit) sum = weigh(0, m, p, rest);
-        hand_over(0, p, rest);
-        sum += weigh(1, m, p, rest);
-        hand_over(1, p, rest);
-        l += sum;
       }
 
       // ---- the item's result -------------------------------------------------------
