@@ -447,8 +447,9 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
    allocation, so decode steps with them can be captured into CUDA graphs.
    Lists of sequences, counts and pages are device arrays too; what only the
    device can see wrong in them (an index out of range or given twice, too few
-   free pages, a bad table entry) is left out and reported by kc_sync. `seqs`
-   NULL means sequences 0 .. n-1; n is at most n_seq. A context's calls share
+   free pages) is left out and reported by kc_sync, as is a table entry outside
+   the pool (results of that sequence are then undefined). `seqs` NULL means
+   sequences 0 .. n-1; n is at most n_seq. A context's calls share
    one workspace: after kc_set_stream the caller orders the new stream behind
    the old one.
 

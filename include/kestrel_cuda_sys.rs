@@ -11,7 +11,8 @@
 //! return type says otherwise; the message of the last failure is
 //! `kc_last_error(ctx)` (ctx may be null for `kc_init`'s errors). Pointers
 //! are host memory for the plain calls and device memory for the `_dev`
-//! calls and `kc_route_noalloc`; the library copies what it keeps.
+//! calls and `kc_route_noalloc`; the library copies what it keeps, except for
+//! `kc_kv_cache`, whose device buffers stay the caller's until `kc_kv_drop`.
 #![allow(non_camel_case_types)]
 
 use std::ffi::{c_char, c_int, c_void, CStr};

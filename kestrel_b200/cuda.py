@@ -4,7 +4,8 @@ The Python mirror of the calls Kestrel's engine makes on its MoE path:
 `Context.moe_ffn` is Transformer::moe_ffn (crates/kestrel-engine/src/
 transformer.rs:513-589), `Context.matmul` is quant::matmul (quant.rs:229-339),
 `Context.upload_experts` is ExpertStore::preload_all into HBM (crates/
-kestrel-memory/src/expert.rs:620-641). Failures raise `KestrelCudaError`
+kestrel-memory/src/expert.rs:620-641). The paged key-value cache and its attention
+(`Context.kv_*`, `Context.attn_*`) are additions for servers. Failures raise `KestrelCudaError`
 carrying the library's status code and message (the analogue of
 EngineError, transformer.rs:15-27); there is no CPU fallback: if the CUDA
 library is missing or fails to load, importing this module raises.
