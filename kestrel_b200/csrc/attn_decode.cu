@@ -75,6 +75,12 @@ __device__ __forceinline__ Span dec_span(int len, int window, int sinks) {
   return s;
 }
 
+// a / b for a >= 0, b > 0: in 32 bits where they fit (a 64-bit division takes
+// several times as long, and half a dozen stand before the first load).
+__device__ __forceinline__ long long div_ll(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
 // A warp's range of the line, segment by segment (one segment: consecutive
 // chunks of one unit, a unit being a sequence's key-value head and head tile).
 struct SegIter {
@@ -202,12 +208,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // needs no join. (A segment's end and a join take about as long as two and
   // four more rounds of chunks: 32 sequences of 2048 positions took 37 us in
   // equal ranges and 29 in one part each.)
-  long long per = max((line + gridDim.x - 1) / gridDim.x, (long long)W);
+  long long per = max(div_ll(line + gridDim.x - 1, gridDim.x), (long long)W);
   per = (per + W - 1) / W * W;
   const long long all = (long long)a.n * units;
   int pad = 0;
   if (all <= gridDim.x) {
-    const int parts = (int)(gridDim.x / all);
+    const int parts = (int)(gridDim.x / (uint32_t)all);
     const int q = ((most + parts - 1) / parts + W - 1) / W * W;
     if (q <= per + (parts == 1 ? 6 : 2) * W) {
       per = q;
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // The sequence in which each warp's range begins: the last whose first chunk
   // is at or before it.
   if (pad) {
-    at.i = (int)(at.pos / ((long long)pad * units));
+    at.i = (int)div_ll(at.pos, (long long)pad * units);
     at.base = (long long)at.i * pad * units;
   } else {
     // Exactly one sequence holds each position.
@@ -283,20 +289,34 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // a load takes as long as those.
   const int r0 = lane >> 2, cc = 2 * (lane & 3);  // fragment row and first column
   constexpr bool kAhead = NB <= 2;
-  TQ raw[RH][4 * NB][4];
+  alignas(8) TQ raw[RH][4 * NB][4];
+  using Pair = std::conditional_t<sizeof(TQ) == 4, float2, uint32_t>;
+  const bool pairs = !((uintptr_t)a.q % sizeof(Pair)) && a.q_stride % 2 == 0;  // two columns a load
   auto ask = [&](const SegIter& g) {
     const int kvh = g.unit / tiles, h0 = (g.unit - kvh * tiles) * HT;
     const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)g.i * a.q_stride + (int64_t)(kvh * group + h0) * c.hd;
 #pragma unroll
     for (int rr = 0; rr < RH; ++rr) {
       const bool real = h0 + r0 + 8 * rr < group;
+      const TQ* row = q + (real ? (int64_t)(r0 + 8 * rr) * c.hd : 0) + cc;
+      if (pairs) {
 #pragma unroll
-      for (int ks = 0; ks < 4 * NB; ++ks)
+        for (int ks = 0; ks < 4 * NB; ++ks)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = 16 * ks + cc + (e & 1) + 8 * (e >> 1);
-          raw[rr][ks][e] = real && x < c.hd ? q[(int64_t)(r0 + 8 * rr) * c.hd + x] : (TQ)0.f;
-        }
+          for (int e = 0; e < 2; ++e) {
+            Pair v{};
+            if (real && 16 * ks + 8 * e + cc < c.hd) v = *reinterpret_cast<const Pair*>(row + 16 * ks + 8 * e);
+            *reinterpret_cast<Pair*>(&raw[rr][ks][2 * e]) = v;
+          }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 4 * NB; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = 16 * ks + (e & 1) + 8 * (e >> 1);
+            raw[rr][ks][e] = real && x + cc < c.hd ? row[x] : (TQ)0.f;
+          }
+      }
     }
   };
   SegIter ahead = at;  // what is loaded next
@@ -662,7 +682,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     last_sh[tid] = 0;
     if (cut[tid] >= 0) {
       const DecPart g = parts_sh[cut[tid]];
-      const int b0 = (int)(g.unit_at / per), b1 = (int)((g.unit_at + g.n_unit - 1) / per);
+      const int b0 = (int)div_ll(g.unit_at, per), b1 = (int)div_ll(g.unit_at + g.n_unit - 1, per);
       last_sh[tid] = atomicAdd(d.count + b0, 1) == b1 - b0;
       if (last_sh[tid]) d.count[b0] = 0;
     }
@@ -672,7 +692,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     if (!last_sh[side]) continue;
     __threadfence();
     const DecPart g = parts_sh[cut[side]];
-    const int b0 = (int)(g.unit_at / per), parts = (int)((g.unit_at + g.n_unit - 1) / per) - b0 + 1;
+    const int b0 = (int)div_ll(g.unit_at, per), parts = (int)div_ll(g.unit_at + g.n_unit - 1, per) - b0 + 1;
     const int kvh = g.unit / tiles, h0 = (g.unit - kvh * tiles) * HT;
     TQ* out = static_cast<TQ*>(a.out) + (int64_t)g.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;
     // Parts in block order; the unit is the first of every block but b0, where
@@ -713,14 +733,20 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       const int h = x / (S::HD / 4), y = 4 * (x - h * (S::HD / 4));
       if (h0 + h >= group || y >= c.hd) continue;
       float4 sum4 = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p) + h * LD + y));
-        const float w = share[h * parts + p];
-        sum4.x = __fmaf_rn(w, v.x, sum4.x);
-        sum4.y = __fmaf_rn(w, v.y, sum4.y);
-        sum4.z = __fmaf_rn(w, v.z, sum4.z);
-        sum4.w = __fmaf_rn(w, v.w, sum4.w);
+      for (int p0 = 0; p0 < parts; p0 += 16) {  // sixteen parts' loads at once
+        float4 v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          v[k] = p0 + k < parts ? __ldcg(reinterpret_cast<const float4*>(part_of(p0 + k) + h * LD + y))
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float w = p0 + k < parts ? share[h * parts + p0 + k] : 0.f;
+          sum4.x = __fmaf_rn(w, v[k].x, sum4.x);
+          sum4.y = __fmaf_rn(w, v[k].y, sum4.y);
+          sum4.z = __fmaf_rn(w, v[k].z, sum4.z);
+          sum4.w = __fmaf_rn(w, v[k].w, sum4.w);
+        }
       }
       TQ* to = out + (int64_t)h * c.hd + y;
       to[0] = (TQ)sum4.x;
