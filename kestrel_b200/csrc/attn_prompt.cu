@@ -31,10 +31,10 @@
 // tensor cores cut their sums off, see below).
 //
 // Measured on a B200, 32 query and 4 key-value heads of 128, f16: 8192 rows from
-// the first (550 GFLOP) in 461 us over 60 calls and 536 us kept up (1.02
+// the first (550 GFLOP) in 449 us over 60 calls and 536 us kept up (1.02
 // PFLOP/s, under the power cap, where the measured matrix rate is 1.43); two
 // prompts of 6001 and 7400 rows with 8 heads under a window of 2048, bf16 (422
-// GFLOP of visible pairs) in 380 and 477 us. At 4096 rows the tensor pipe is
+// GFLOP of visible pairs) in 376 and 477 us. At 4096 rows the tensor pipe is
 // busy for 50% of the active cycles, and so is the unit of the exponentials: a
 // stream's tile takes its warps about 2600 cycles beside the other stream's,
 // and the two products and their hand-overs 1650 a step. Tried and not kept: a
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : &q_map);
   pdl_enter();
   extern __shared__ uint8_t prompt_raw[];
-  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], s_free[NS], p_half[NS], p_full[NS],
-      half_done[NS], pv_done[NS], o_empty[NS];
+  __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], s_full[NS], s_free[NS], p_full[NS], pv_done[NS],
+      o_empty[NS];
   __shared__ __align__(8) uint64_t q_raw, q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint32_t tmem_sh;
   __shared__ Item items[2];
@@ -239,10 +239,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     }
     for (int w = 0; w < NS; ++w) {
       mbar_init(&s_full[w], 1);
-      mbar_init(&p_half[w], 128);
       mbar_init(&p_full[w], 128);
       mbar_init(&s_free[w], 128);
-      mbar_init(&half_done[w], 1);
       mbar_init(&pv_done[w], 1);
       mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
@@ -366,23 +364,17 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         }
         tc_commit(&s_full[w]);
       };
-      // The weights come in two halves, so that the first half's products run
-      // beside the exponentials of the second.
       auto values = [&](int w, int k, uint32_t v, bool add) {
         const uint64_t vd = sw128_desc_mn(v, BN * 128);
+        wait(&p_full[w], k);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          wait(half ? &p_full[w] : &p_half[w], k);
-          if (!ok) return;
-          tc_fence_after();
+        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
 #pragma unroll
-          for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll
-            for (int ks = half * (BN / 32); ks < (half + 1) * (BN / 32); ++ks)
-              tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + S::T_P + S::T_PW * w + part * (BN / 2) + 8 * ks,
-                        vd + ks * 2048 / 16, id_o, add || half > 0 || part > 0 || ks > 0);
-          if (!kSplit && half == 0) tc_commit(&half_done[w]);
-        }
+          for (int ks = 0; ks < BN / 16; ++ks)
+            tc_mma_ts(tmem + S::T_O + w * S::HD, tmem + S::T_P + S::T_PW * w + part * (BN / 2) + 8 * ks,
+                      vd + ks * 2048 / 16, id_o, add || part > 0 || ks > 0);
         tc_commit(&pv_done[w]);
       };
       // Before an item's first products into an accumulator: the last item's
@@ -794,32 +786,28 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           const float2 sum = f2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
           return sum.x + sum.y;
         };
-        auto hand_over = [&](int half, const uint32_t* p, const uint32_t* rest) {
+        auto put = [&](int half, const uint32_t* p, const uint32_t* rest) {
 #pragma unroll
           for (int e = 0; e < BN / 4; e += 16) {
             tmem_st16(p_t + half * (BN / 4) + e, p + e);
             if constexpr (kSplit) tmem_st16(p_t + BN / 2 + half * (BN / 4) + e, rest + e);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(half ? &p_full[w] : &p_half[w]);
         };
-        // Largest of positions from .. from + n - 1, in exponents of 2.
-        auto top_of = [&](int from, int n) {
+        // Largest of the row's scores, in exponents of 2.
+        auto largest = [&]() {
           float tops[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tops[e] = s[from + e];
+          for (int e = 0; e < 8; ++e) tops[e] = s[e];
 #pragma unroll
-          for (int e = 8; e < n; e += 2) tops[e / 2 & 7] = max3(tops[e / 2 & 7], s[from + e], s[from + e + 1]);
+          for (int e = 8; e < BN; e += 2) tops[e / 2 & 7] = max3(tops[e / 2 & 7], s[e], s[e + 1]);
           const float top =
               max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
           return top == -INFINITY ? top : top * cq;
         };
-        // A larger maximum: what has been summed so far is rescaled. The
-        // accumulator is this warp's once `done` has come to `phase` (its
-        // products so far; the next ones wait for weights).
-        auto rescale = [&](float top, bool grow, uint64_t* done, int phase) {
-          if (phase >= 0) wait(done, phase);
+        // A larger reference: what has been summed so far is rescaled. The
+        // products so far are complete, and the next ones wait for weights: the
+        // accumulator is this warp's.
+        auto rescale = [&](float top, bool grow) {
           tc_fence_after();
           const float shrink = grow ? exp2_fast(m - top) : 1.f;
           if (grow) m = top;
@@ -832,43 +820,46 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             for (int e = 0; e < 16; ++e) o[e] *= shrink;
             tmem_st16(o_t + e0, o);
           }
-          tmem_wait_st();
         };
         uint32_t p[BN / 4], rest[kSplit ? BN / 4 : 1];
+        float sum;
         if constexpr (kSplit) {
-          const float top = top_of(0, BN);
+          const float top = largest();
           if (k == 0) m = top;
           const bool grow = top > m + 8.f;
-          if (__any_sync(0xffffffffu, grow)) rescale(top, grow, nullptr, -1);
-          float sum = weigh(0, m, p, rest);
-          hand_over(0, p, rest);
+          if (__any_sync(0xffffffffu, grow)) rescale(top, grow);
+          sum = weigh(0, m, p, rest);
+          put(0, p, rest);
           sum += weigh(1, m, p, rest);
-          hand_over(1, p, rest);
-          l += sum;
         } else {
-          // No maximum is looked for after the first tile: while a half's weights
+          // No maximum is looked for after the first tile: while a tile's weights
           // add up to less than kMost, none of them is past the 16-bit type's
           // range, and any reference does. (8192 rows of 32 heads: 471 us with
-          // every tile's maximum, 465 so.)
-          if (rarely(k == 0)) m = top_of(0, BN);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float sum = weigh(half, m, p, rest);
-            if (rarely(__any_sync(0xffffffffu, !(sum < kMost) || m == -INFINITY))) {
-              const float top = top_of(half * (BN / 2), BN / 2);
-              const bool grow = top > m && (!(sum < kMost) || m == -INFINITY);
-              if (__any_sync(0xffffffffu, grow)) {
-                if (half == 0) rescale(top, grow, &pv_done[w], ks - 1);
-                else rescale(top, grow, &half_done[w], ks);
-                sum = weigh(half, m, p, rest);
-              }
+          // every tile's maximum, 461 so.) The weights are handed over once: in two
+          // halves, whose first products could start earlier, it took 4% more.
+          if (rarely(k == 0)) m = largest();
+          sum = weigh(0, m, p, rest);
+          // The weights' columns are free once the last products are complete.
+          if (kShared && ks > 0) wait(&pv_done[w], ks - 1);
+          put(0, p, rest);
+          sum += weigh(1, m, p, rest);
+          if (rarely(__any_sync(0xffffffffu, !(sum < kMost) || m == -INFINITY))) {
+            const float top = largest();
+            const bool grow = top > m && (!(sum < kMost) || m == -INFINITY);
+            if (__any_sync(0xffffffffu, grow)) {
+              if (!kShared && ks > 0) wait(&pv_done[w], ks - 1);
+              rescale(top, grow);
+              sum = weigh(0, m, p, rest);
+              put(0, p, rest);
+              sum += weigh(1, m, p, rest);
             }
-            // The weights' columns are free once the last products are complete.
-            if (kShared && half == 0 && ks > 0) wait(&pv_done[w], ks - 1);
-            hand_over(half, p, rest);
-            l += sum;
           }
         }
+        put(1, p, rest);
+        l += sum;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
       }
 
       // ---- the item's result -------------------------------------------------------
