@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       mbar_init(&o_empty[w], TWO ? 128 : 128 * NS);
     }
     mbar_init(&q_raw, 1);
-    mbar_init(&q_full, 2);
+    mbar_init(&q_full, kSplit && d.q_map ? 4 * NS : 2);
     mbar_init(&q_empty, 1);
     mbar_init(&drained, 1);
     mbar_init(&join_full, 128 * NS);
@@ -271,6 +271,40 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   };
   auto wait = [&](uint64_t* bar, int phase) {
     if (ok && !mbar_wait(bar, phase & 1, c.status, W_ATT_PROMPT)) ok = false;
+  };
+
+  // Eight values of each 64 of a query row, lane `part` of the row's eight, to
+  // the operands of row tile `tile`.
+  constexpr int TILE_Q = (kSplit ? 2 : 1) * S::QB;
+  auto operands = [&](const float (&v)[NB][8], int rr, int tile, int part, int buf) {
+    float f = 1.f;
+    if constexpr (kSplit) {
+      // A power of two puts the row's largest value in [2^14, 2^15).
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[j][e]));
+#pragma unroll
+      for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      f = pow2_factor(amax);
+      if (part == 0) factor_sh[buf][tile][rr] = f;
+    }
+    f *= flip;
+    uint8_t* to = q_sm + tile * TILE_Q + rr * 128 + ((part ^ (rr & 7)) << 4);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      uint32_t hi[4], rest[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z0 = v[j][2 * e] * f, z1 = v[j][2 * e + 1] * f;
+        hi[e] = pack2<TKV>(z0, z1);
+        if constexpr (kSplit) rest[e] = rest2<TKV>(z0, z1, hi[e]);
+      }
+      *reinterpret_cast<uint4*>(to + j * PM * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (kSplit)
+        *reinterpret_cast<uint4*>(to + S::QB + j * PM * 128) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+    }
   };
 
   if (warp >= W_TMA) {
@@ -595,7 +629,6 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       const RowMap rm(x.row0, group);
       const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride + (int64_t)x.kvh * group * c.hd;
       const int loader = tid - 32 * W_AUX;
-      constexpr int TILE_Q = (kSplit ? 2 : 1) * S::QB;
       if (d.q_map && finder && lane == 0) {
         // A box per tile and 128 bytes of columns. (Rows past the entry's are
         // another's or zeros; nothing comes of them.)
@@ -611,19 +644,12 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         if (!finder && lane == 0) mbar_arrive(&q_full);
         continue;
       }
-      const bool staged = kSplit && d.q_map;
-      if (staged) {
-        wait(&q_raw, used - 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
+      if (kSplit && d.q_map) continue;  // the softmax warps make operands of them
       {
-        // Eight lanes per row, eight values of each 64 a lane. f32 rows that TMA
-        // brought lie where their two operands go, row for row: a warp reads its
-        // rows whole before it writes them.
+        // Eight lanes per row, eight values of each 64 a lane.
         const bool wide = !((uintptr_t)a.q % 16) && a.q_stride * sizeof(TQ) % 16 == 0;
         const int part = loader & 7;
-        constexpr int BATCH = NB <= 2 ? 4 : 1;  // rows of a lane under way
+        constexpr int BATCH = NB > 2 ? 1 : kSplit ? 2 : 4;  // rows of a lane under way
         for (int f0 = loader >> 3; f0 < S::QT * PM; f0 += 8 * BATCH) {
           float v[BATCH][NB][8];
 #pragma unroll
@@ -633,15 +659,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
               const bool real = f < x.rows && 64 * j + 8 * part < c.hd;
-              if (staged) {
-                const uint8_t* raw = q_sm + (f >> 7) * TILE_Q + (2 * j + (part >> 2)) * PM * 128 + (f & (PM - 1)) * 128;
-                const int c0 = 2 * (part & 3), sw = f & 7, flip_c = part >> 2;  // (bank order)
-                const float4 u = *reinterpret_cast<const float4*>(raw + (((c0 + flip_c) ^ sw) << 4));
-                const float4 w = *reinterpret_cast<const float4*>(raw + (((c0 + 1 - flip_c) ^ sw) << 4));
-                const float4 lo4 = flip_c ? w : u, hi4 = flip_c ? u : w;
-                v[y][j][0] = lo4.x; v[y][j][1] = lo4.y; v[y][j][2] = lo4.z; v[y][j][3] = lo4.w;
-                v[y][j][4] = hi4.x; v[y][j][5] = hi4.y; v[y][j][6] = hi4.z; v[y][j][7] = hi4.w;
-              } else if (real && wide) {
+              if (real && wide) {
                 load8(from + 64 * j, v[y][j]);
               } else {
 #pragma unroll
@@ -650,44 +668,16 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             }
           }
 #pragma unroll
-          for (int y = 0; y < BATCH; ++y) {
-            const int rr = (f0 + 8 * y) & (PM - 1), tile = (f0 + 8 * y) >> 7;
-            float f = 1.f;
-            if constexpr (kSplit) {
-              // A power of two puts the row's largest value in [2^14, 2^15).
-              float amax = 0.f;
-#pragma unroll
-              for (int j = 0; j < NB; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[y][j][e]));
-#pragma unroll
-              for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-              f = pow2_factor(amax);
-              if (part == 0) factor_sh[(used - 1) & 1][tile][rr] = f;
-            }
-            f *= flip;
-            if (y == 0) __syncwarp();
-            uint8_t* to = q_sm + tile * TILE_Q + rr * 128 + ((part ^ (rr & 7)) << 4);
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-              uint32_t hi[4], rest[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float z0 = v[y][j][2 * e] * f, z1 = v[y][j][2 * e + 1] * f;
-                hi[e] = pack2<TKV>(z0, z1);
-                if constexpr (kSplit) rest[e] = rest2<TKV>(z0, z1, hi[e]);
-              }
-              *reinterpret_cast<uint4*>(to + j * PM * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if constexpr (kSplit)
-                *reinterpret_cast<uint4*>(to + S::QB + j * PM * 128) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-            }
-          }
+          for (int y = 0; y < BATCH; ++y)
+            operands(v[y], (f0 + 8 * y) & (PM - 1), (f0 + 8 * y) >> 7, part, (used - 1) & 1);
         }
       }
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
     }
+    // Every load lands before the block may end.
+    if (kSplit && finder && d.q_map && used > 0) mbar_wait(&q_raw, (used - 1) & 1, c.status, W_ATT_PROMPT);
     // The last block to find nothing left puts the counters back.
     if (finder && lane == 0 && atomicAdd(d.next + 1, 1) == (int)gridDim.x - 1) d.next[0] = d.next[1] = 0;
   } else {
@@ -710,6 +700,42 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       const bool real = f < x.rows;
       const int at = real ? at_base + rm.token(f) : -1;
       const int lo = a.window > 0 ? at - a.window + 1 : 0;
+      if constexpr (kSplit) {
+        if (d.q_map && nt > 0) {
+          // The rows that TMA brought lie where their two operands go, row for
+          // row: a warp reads its rows whole before it writes them. Eight lanes
+          // per row, eight values of each 64 a lane. (By two warps, beside the
+          // last item's end: 33 rows at 545 took 28 us from a cold L2, 26 so, 256
+          // at 4096 68 and 62, 8192 from the first 852 and 845.)
+          wait(&q_raw, used);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int part = tid & 7;
+          constexpr int STEP = 16 * NS;                   // rows of all threads at a time
+          constexpr int BATCH = NB <= 2 ? PM / STEP : 1;  // those of a thread under way
+          for (int f0 = tid >> 3; f0 < PM; f0 += STEP * BATCH) {
+            float v[BATCH][NB][8];
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y)
+#pragma unroll
+              for (int j = 0; j < NB; ++j) {
+                const int row = f0 + STEP * y, c0 = 2 * (part & 3), sw = row & 7, flip_c = part >> 2;  // (bank order)
+                const uint8_t* raw = q_sm + (2 * j + (part >> 2)) * PM * 128 + row * 128;
+                const float4 u = *reinterpret_cast<const float4*>(raw + (((c0 + flip_c) ^ sw) << 4));
+                const float4 z = *reinterpret_cast<const float4*>(raw + (((c0 + 1 - flip_c) ^ sw) << 4));
+                const float4 lo4 = flip_c ? z : u, hi4 = flip_c ? u : z;
+                v[y][j][0] = lo4.x; v[y][j][1] = lo4.y; v[y][j][2] = lo4.z; v[y][j][3] = lo4.w;
+                v[y][j][4] = hi4.x; v[y][j][5] = hi4.y; v[y][j][6] = hi4.z; v[y][j][7] = hi4.w;
+              }
+            __syncwarp();
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y) operands(v[y], f0 + STEP * y, 0, part, used & 1);
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full);
+        }
+      }
       // Tiles whose positions every row of this tile sees need no mask.
       const int t_at0 = at_base + rm.token(my_tile * PM);
       const int t_lo1 = a.window > 0 ? at_base + rm.token(min(x.rows, (my_tile + 1) * PM) - 1) - a.window + 1 : 0;

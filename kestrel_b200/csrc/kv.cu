@@ -245,9 +245,10 @@ __global__ void __launch_bounds__(KV_BLOCK) kv_extend_kernel(KvView c, const int
 // layer and head, k and v. No dst is a src. A unit is one page of one layer of
 // k or v; a block takes units in turn.
 // Bound by the memory rate (each byte read and written once). Four 16-byte
-// pieces of a thread under way and sixteen blocks per SM: 1.72 GB of pages in
-// 285 us, 6.0 TB/s, 93% of a plain copy (one piece 299, eight blocks and four
-// pieces 286, four blocks and eight 305).
+// pieces of a thread under way and sixteen blocks per SM: a compaction that moves
+// 1.72 GB of pages takes 297 us as a whole, 5.8 TB/s, 90% of a plain copy (one
+// piece and eight blocks 311, four and eight 298, eight pieces and four blocks
+// 317).
 constexpr int COPY_THREADS = 256;
 constexpr int COPY_AHEAD = 4;  // 16-byte pieces of a thread under way
 __global__ void __launch_bounds__(COPY_THREADS) kv_copy_kernel(KvView c, bool whole, int32_t* table_remap,
