@@ -20,9 +20,9 @@
 // more than eight heads with 16-bit queries use all sixteen rows for heads.
 //
 // Measured on a B200 (plain copy 6.46 TB/s): 96 sequences of 1500 to 8192 under
-// a window of 4096, 8 key-value heads of 128, 1.37 GB in 227 us (6.0 TB/s); one
-// of 131071, 4 heads, 268 MB in 55 us (4.9); 32 of 200 to 4096, 126 MB in 35 us
-// (3.6). What is not reading: about 5 us until the first chunks are asked for
+// a window of 4096, 8 key-value heads of 128, 1.37 GB in 232 us (5.9 TB/s); one
+// of 131071, 4 heads, 268 MB in 56 us (4.8); 32 of 200 to 4096, 126 MB in 34 us
+// (3.7). What is not reading: about 5 us until the first chunks are asked for
 // (launch, lengths, ranges, page ids) and 5 to 8 at the end (the last warp, the
 // parts, their join through L2).
 #include <algorithm>

@@ -31,13 +31,13 @@
 // tensor cores cut their sums off, see below).
 //
 // Measured on a B200, 32 query and 4 key-value heads of 128, f16: 8192 rows from
-// the first (550 GFLOP) in 449 us over 60 calls and 536 us kept up (1.02
+// the first (550 GFLOP) in 449 us over 60 calls and 535 us kept up (1.03
 // PFLOP/s, under the power cap, where the measured matrix rate is 1.43); two
 // prompts of 6001 and 7400 rows with 8 heads under a window of 2048, bf16 (422
-// GFLOP of visible pairs) in 376 and 477 us. At 4096 rows the tensor pipe is
-// busy for 50% of the active cycles, and so is the unit of the exponentials: a
+// GFLOP of visible pairs) in 376 and 475 us. At 4096 rows the tensor pipe is
+// busy for 52% of the active cycles, and so is the unit of the exponentials: a
 // stream's tile takes its warps about 2600 cycles beside the other stream's,
-// and the two products and their hand-overs 1650 a step. Tried and not kept: a
+// and the two products and their hand-overs 1550 a step. Tried and not kept: a
 // share of the exponentials as cubics on the FMA pipes (a quarter: 4% slower),
 // the MMA warp's code per stream or run by the whole warp (5% slower).
 #include <cuda.h>
