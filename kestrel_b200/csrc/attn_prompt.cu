@@ -492,16 +492,25 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   } else if (warp >= W_AUX) {
     // ---- the next item, and its queries -----------------------------------------
     const bool finder = warp == W_AUX;
-    // Row tiles of an entry (0 where its rows are out of order).
-    auto tiles_of = [&](int i, int& lo, int& hi) {
-      lo = hi = 0;
-      if (i < a.n) {
-        lo = a.row_start[i];
-        hi = a.row_start[i + 1];
-        if (lo < 0 || hi < lo || hi > a.n_rows) {
-          if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
-          lo = hi = 0;
-        }
+    // Row tiles of entry i, the lane's of 32 consecutive ones, in whose order the
+    // warp calls this; 0 where its rows are out of order: an entry begins where
+    // every earlier one has begun or later, so that no two share a row and the
+    // tiles of all of them are no more than the launch reckons with. `last`: the
+    // largest beginning before these 32, and then up to them.
+    auto tiles_of = [&](int i, int& last, int& lo, int& hi) {
+      lo = i < a.n ? a.row_start[i] : 0;
+      hi = i < a.n ? a.row_start[i + 1] : 0;
+      int top = lo;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, top, o);
+        if (lane >= o) top = max(top, y);
+      }
+      top = max(top, last);
+      last = __shfl_sync(0xffffffffu, top, 31);
+      if (lo < top || hi < lo || hi > a.n_rows) {
+        if (i < a.n && blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
+        lo = hi = 0;
       }
       return (int)(((int64_t)(hi - lo) * group + S::QT * PM - 1) / (S::QT * PM));
     };
@@ -528,13 +537,16 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         }
         for (int j = 0; j < 32; ++j)
           if (__shfl_sync(0xffffffffu, rank, j) == lane) e_i = j;
-        const int m = tiles_of(e_i, e_lo, e_hi);
+        int last = 0;
+        const int m = tiles_of(lane, last, e_lo, e_hi);
+        e_lo = __shfl_sync(0xffffffffu, e_lo, e_i);
+        e_hi = __shfl_sync(0xffffffffu, e_hi, e_i);
         e_len = __shfl_sync(0xffffffffu, len, e_i);
-        e_sum = scan(m);
+        e_sum = scan(__shfl_sync(0xffffffffu, m, e_i));
         tiles = __shfl_sync(0xffffffffu, e_sum, 31);
       } else {
-        int m = 0, lo, hi;
-        for (int b = 0; b < a.n; b += 32) m += tiles_of(b + lane, lo, hi);
+        int m = 0, last = 0, lo, hi;
+        for (int b = 0; b < a.n; b += 32) m += tiles_of(b + lane, last, lo, hi);
         tiles = __shfl_sync(0xffffffffu, scan(m), 31);
       }
     }
@@ -566,9 +578,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             x.len = __shfl_sync(0xffffffffu, e_len, l);
             if (l > 0) t -= __shfl_sync(0xffffffffu, e_sum, l - 1);
           } else {
+            int last = 0;
             for (int b = 0; b < a.n; b += 32) {
               int lo, hi;
-              const int m = tiles_of(b + lane, lo, hi), y = scan(m);
+              const int m = tiles_of(b + lane, last, lo, hi), y = scan(m);
               const unsigned at = __ballot_sync(0xffffffffu, t < y);
               if (at) {
                 l = __ffs(at) - 1;

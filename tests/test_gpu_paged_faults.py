@@ -1,0 +1,61 @@
+"""Calls of the paged cache and its attention that must be refused, left out or
+answered as the definition says where numbers end (run with -m gpu).
+
+Tolerances are test_gpu_paged's: with u the unit roundoff of the query / output
+type, 2 u max|v| for 16-bit results and 2^-15 max|v| for f32 ones, values of
+unit normal size (max|v| <= 6).
+"""
+import numpy as np
+import pytest
+
+from test_gpu_paged import BF16, F16, F32, PAIRS, Cache, close, ctx, ints, queries, torch, wide  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def pair_id(p):
+    return f"{p[0]}-{p[1]}".replace("torch.", "")
+
+
+def reported(c, code, text):
+    from kestrel_b200.cuda import KestrelCudaError
+    with pytest.raises(KestrelCudaError, match=text) as e:
+        c.sync()
+    assert e.value.code == code
+    c.sync()  # told once
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=pair_id)
+@pytest.mark.parametrize("n", [9, 41])
+def test_rows_given_to_several_entries(ctx, pair, n):
+    """row_start 0, N, 0, N, ...: the first entry has the N rows, the others
+    begin before it or end before they begin. Only the first is computed, and
+    the context's workspace holds what it should afterwards."""
+    rows = 1280
+    c = Cache(ctx, [1300] + [1100] * (n - 1), 128, 1, 64, pair[1], n_layer=1, seed=n)
+    q = queries(rows + 4, 1, 64, pair[0], 3)
+    out = torch.full_like(q.contiguous(), 7.0)
+    ctx.attn_prompt_dev(c.id, 0, q, ints([rows * (i % 2) for i in range(n + 1)]), out)
+    reported(ctx, 1, "rows that do not ascend")
+    want = c.expected(0, wide(q)[:rows], [0], [rows], 0.125, 0, 0)
+    close(wide(out)[:rows], want, pair[0])
+    assert (out[rows:] == 7).all()
+    # An entry after a later one's beginning, and one that goes on in order.
+    out.fill_(7)
+    start = [0] * n + [0]
+    start[1:4] = [40, 20, 60]
+    start[4:] = [60] * (n - 3)
+    ctx.attn_prompt_dev(c.id, 0, q, ints(start), out)  # entries 0: 0 .. 40, 1: 40 .. 20, 2: 20 .. 60
+    reported(ctx, 1, "rows that do not ascend")
+    close(wide(out)[:40], c.expected(0, wide(q)[:40], [0], [40], 0.125, 0, 0), pair[0])
+    assert (out[40:] == 7).all()
+    # What came after is as it was before.
+    again = torch.full_like(out, 7.0)
+    for o in (out, again):
+        ctx.attn_prompt_dev(c.id, 0, q, ints([0] + [rows] * n), o)
+        one = torch.empty_like(q[:n].contiguous())
+        ctx.attn_decode_dev(c.id, 0, q[:n], one)
+    ctx.sync()
+    close(wide(out)[:rows], want, pair[0])
+    assert torch.equal(out, again)
+    close(wide(one), c.expected(0, wide(q)[:n], range(n), [1] * n, 0.125, 0, 0), pair[0])
