@@ -489,7 +489,8 @@ KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, cons
    j <= i and (j > i - window or j < sinks); window 0: every j <= i. out =
    sum p_j v_j / sum p_j with p_j = exp(scale q.k_j - max); zeros where nothing
    is visible. What is not visible does not reach the result, whatever it holds
-   (stale rows of a page, NaN). q and out: rows of n_head * head_dim, the row
+   (stale rows of a page, NaN); infinities and NaN in what is visible give what
+   the formula gives. (Only scores of minus infinity: zeros.) q and out: rows of n_head * head_dim, the row
    strides in elements; type t is the cache's, or KC_F32 over a KC_F16 cache;
    n_head a multiple of n_head_kv (at most 128 query heads to one). Softmax and
    sums are f32 for every type.

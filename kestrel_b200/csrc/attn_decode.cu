@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            tt[rr][2 * t + e] = (kSplit ? sc[t][e] + sc[t][e + 2] : sc[t][e + 2 * rr]) * cq[rr];
+            tt[rr][2 * t + e] = (kSplit ? with_rest(sc[t][e], sc[t][e + 2]) : sc[t][e + 2 * rr]) * cq[rr];
       const bool edge = p0 + DC > at.len || (p0 < at.span.lo && p0 + DC > a.sinks);
       if (edge) {
         // Positions that the row does not see: no weight, and zeros in place of
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint32_t hi = pack2<TKV>(p[2 * t], p[2 * t + 1]);
+          const uint32_t hi = pack_weights<TKV>(p[2 * t], p[2 * t + 1]);
           if constexpr (kSplit) {
             pa[2 * t] = hi;
             pa[2 * t + 1] = rest2<TKV>(p[2 * t], p[2 * t + 1], hi);
@@ -548,8 +548,8 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     if constexpr (kSplit)
 #pragma unroll
       for (int t = 0; t < 8 * NB; ++t) {
-        o[t][0] += o[t][2];
-        o[t][1] += o[t][3];
+        o[t][0] = with_rest(o[t][0], o[t][2]);
+        o[t][1] = with_rest(o[t][1], o[t][3]);
       }
     if (!pad && at.c0 == 0 && at.c1 == at.n_unit) {
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)at.i * a.out_stride + (int64_t)(kvh * group + h0) * c.hd;

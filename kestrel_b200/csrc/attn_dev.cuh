@@ -62,6 +62,30 @@ __device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t pair) {
   return pack2<T>(lo - a, hi - b);
 }
 
+// Two weights (not negative) as a pair of T. One that f16 would round to zero
+// becomes its smallest value instead, 2^-24, so that an infinite value still
+// makes the result infinite, not NaN (0 times it); the rest takes what is too
+// much off again, and without a rest 2^-24 against weights of up to 2^15 is
+// below what the type of the result holds.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  uint32_t r = pack2<T>(lo, hi);
+  if constexpr (std::is_same_v<T, __half>) {
+    const uint32_t least = min(__float_as_uint(lo), 1u) | min(__float_as_uint(hi), 1u) << 16;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(least));
+  }
+  return r;
+}
+
+// A sum carried by values and rests. Of an infinite or NaN one the values' sum is
+// right by itself: it meets the rests as 0 times it, or with the other sign.
+// (Values are zero only where what they carry is, or is below 2^-39 of its
+// row's largest.)
+__device__ __forceinline__ float with_rest(float value, float rest) {
+  const float s = value + rest;
+  return fabsf(value) < INFINITY ? s : value;
+}
+
 // The power of two that puts a row's largest magnitude in [2^14, 2^15), within
 // f16's range (1 for a row of zeros or one that is not finite).
 __device__ __forceinline__ float pow2_factor(float amax) {

@@ -59,3 +59,57 @@ def test_rows_given_to_several_entries(ctx, pair, n):
     close(wide(out)[:rows], want, pair[0])
     assert torch.equal(out, again)
     close(wide(one), c.expected(0, wide(q)[:n], range(n), [1] * n, 0.125, 0, 0), pair[0])
+
+
+def same_numbers(got, want, t):
+    """NaN and infinities where they belong, the rest within the tolerance."""
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)].astype(got.dtype))
+    close(np.where(fine, got, 0.0), np.where(fine, want, 0.0), t)
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 64), (8, 2, 64), (20, 1, 64), (6, 2, 40), (3, 1, 256), (16, 1, 128)], ids=str)
+@pytest.mark.parametrize("pair", PAIRS, ids=pair_id)
+def test_infinities_in_view(ctx, heads, pair):
+    """Keys and values that hold infinities, seen by the row: a score of minus
+    infinity gives no weight, one of plus infinity NaN, an infinite value an
+    infinity (or NaN with no weight or beside one of the other sign). A weight
+    of exp(-40) is a weight. Short sequences and ones of many parts."""
+    nh, nkv, hd = heads
+    lens = [40, 3000, 9, 700]
+    c = Cache(ctx, lens, 16, nkv, hd, pair[1], n_layer=1, seed=nh)
+    at = lambda s, j: (0, c.m.table[s][j // 16], slice(None), j % 16)
+    for s, n in enumerate(lens):
+        c.k[at(s, 2)][:, 5] = float("inf")       # scores of both infinities, by the head
+        c.v[at(s, 3)][:, 9] = float("inf")
+        c.v[at(s, 4)][:, 10] = float("-inf")
+        c.v[at(s, n - 1)][:, 11] = float("inf")
+        c.v[at(s, 3)][:, 11] = float("-inf")
+        c.v[at(s, 2)][:, 12] = float("inf")      # where the score is minus infinity: NaN
+        c.k[at(s, 6)] = 0                        # a score of -40
+        c.k[at(s, 6)][:, 7] = -40
+        c.v[at(s, 6)][:, 13] = float("inf")
+    for s, n in enumerate(lens):
+        for j in range(n):
+            if j != 6:
+                c.k[at(s, j)][:, 7] = 0
+    c.m.k, c.m.v = wide(c.k), wide(c.v)
+    q = 0.3 * queries(len(lens), nh, hd, F32, 5)
+    q[..., 7] = 1
+    q[:, ::2, 5] = -q[:, ::2, 5].abs() - 0.01    # these heads leave position 2 out
+    q[:, 1::2, 5] = q[:, 1::2, 5].abs() + 0.01   # these come to NaN
+    q = q.to(pair[0])
+    with np.errstate(invalid="ignore"):
+        want = c.expected(0, wide(q), range(len(lens)), [1] * len(lens), 1.0, 0, 0)
+    assert np.isnan(want[:, 1::2]).all() and np.isposinf(want[:, ::2, [9, 13]]).all()
+    assert np.isneginf(want[:, ::2, 10]).all() and np.isnan(want[:, ::2, 11:13]).all()
+    assert np.isfinite(want[:, ::2, 14:]).all() and np.isfinite(want[:, ::2, :9]).all()
+    out = torch.full_like(q, 7.0)
+    ctx.attn_decode_dev(c.id, 0, q, out, scale=1.0)
+    ctx.sync()
+    same_numbers(wide(out), want, pair[0])
+    out.fill_(7)
+    ctx.attn_prompt_dev(c.id, 0, q, ints(range(len(lens) + 1)), out, scale=1.0)
+    ctx.sync()
+    same_numbers(wide(out), want, pair[0])
