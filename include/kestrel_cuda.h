@@ -466,6 +466,7 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
    kc_kv_write_dev: rows row_start[i] .. row_start[i+1]-1 of k and v (row
    strides in elements, heads contiguous; type KC_F32 or the cache's) become
    the last positions of sequence i in one layer; row_start NULL: one row each.
+   Of a sequence given twice either entry's rows may be written; it is reported.
    kc_kv_free_dev: forget positions from keep[i] on (NULL: all) and release the
    pages that hold none of the kept ones.
    kc_kv_compact_dev: live pages move to ids 0 .. live-1 (the i-th live page at

@@ -428,12 +428,48 @@ __global__ void __launch_bounds__(WRITE_THREADS) kv_write_kernel(KvView c, int l
                                                                  const int32_t* __restrict__ row_start, int n,
                                                                  int n_rows, const S* __restrict__ k,
                                                                  const S* __restrict__ v, int64_t k_stride,
-                                                                 int64_t v_stride, bool aligned) {
+                                                                 int64_t v_stride, bool aligned, int blocks) {
   pdl_enter();
+  if (blockIdx.x >= blocks) {
+    // One block more where a list could name a sequence twice: it tells, beside
+    // the others' writing (32 x 256 rows of 4 heads of 128 take 12.4 us as they did
+    // without it, 1000 x 1 3.3 against 2.6, 4096 x 1 11.9 against 5.6; leaving the
+    // second entry out would hold every write up: 14.5, 3.4 and 9.8). The marks
+    // are -1 between calls.
+    auto each = [&](auto&& fn) {  // eight entries of a thread under way
+      for (int i0 = threadIdx.x; i0 < n; i0 += 8 * WRITE_THREADS) {
+        int s[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s[u] = i0 + u * WRITE_THREADS < n ? __ldg(seqs + i0 + u * WRITE_THREADS) : -1;
+        fn(i0, s);
+      }
+      __syncthreads();
+    };
+    const auto real = [&](int s) { return s >= 0 && s < c.n_seq; };
+    each([&](int i0, const int(&s)[8]) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (real(s[u])) atomicMax(c.mark + s[u], i0 + u * WRITE_THREADS);
+    });
+    each([&](int i0, const int(&s)[8]) {
+      int last[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) last[u] = real(s[u]) ? __ldcg(c.mark + s[u]) : 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (real(s[u]) && last[u] != i0 + u * WRITE_THREADS) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
+    });
+    each([&](int, const int(&s)[8]) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (real(s[u])) c.mark[s[u]] = -1;
+    });
+    return;
+  }
   const int row_vec = c.hd / 8, per = c.nkv * row_vec;  // 16-byte pieces of a head's row, of a row of k or v
   const int64_t pieces = (int64_t)n_rows * 2 * per;
   for (int64_t x = (int64_t)blockIdx.x * WRITE_THREADS + threadIdx.x; x < pieces;
-       x += (int64_t)gridDim.x * WRITE_THREADS) {
+       x += (int64_t)blocks * WRITE_THREADS) {
     const int r = (int)(x / (2 * per)), y = (int)(x - (int64_t)r * 2 * per);
     const bool is_v = y >= per;
     const int e = is_v ? y - per : y, h = e / row_vec, j = e - h * row_vec;
@@ -475,8 +511,8 @@ static void write_rows(const KvView& c, int layer, const int32_t* seqs, const in
   const int grid = (int)std::min<int64_t>((pieces + WRITE_THREADS - 1) / WRITE_THREADS, 16 * (int64_t)num_sms());
   const int64_t el = 16 / sizeof(S);
   const bool aligned = !((uintptr_t)k & 15) && !((uintptr_t)v & 15) && ks % el == 0 && vs % el == 0;
-  launch_k(kv_write_kernel<S, D>, grid, WRITE_THREADS, 0, st, c, layer, seqs, row_start, n, n_rows,
-           static_cast<const S*>(k), static_cast<const S*>(v), ks, vs, aligned);
+  launch_k(kv_write_kernel<S, D>, grid + (seqs && n > 1), WRITE_THREADS, 0, st, c, layer, seqs, row_start, n, n_rows,
+           static_cast<const S*>(k), static_cast<const S*>(v), ks, vs, aligned, grid);
 }
 
 void launch_kv_write(const KvView& c, int layer, const int32_t* seqs, const int32_t* row_start, int n, int n_rows,

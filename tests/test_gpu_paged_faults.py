@@ -113,3 +113,42 @@ def test_infinities_in_view(ctx, heads, pair):
     ctx.attn_prompt_dev(c.id, 0, q, ints(range(len(lens) + 1)), out, scale=1.0)
     ctx.sync()
     same_numbers(wide(out), want, pair[0])
+
+
+@pytest.mark.parametrize("n_kv,hd", [(1, 8), (3, 40), (4, 128)])
+def test_write_to_a_sequence_given_twice(ctx, n_kv, hd):
+    """It is reported; the rows of all other sequences are written, and nothing
+    else is touched."""
+    n_seq = 70
+    lens = [40 + s for s in range(n_seq)]
+    c = Cache(ctx, lens, 16, n_kv, hd, F16, n_layer=1, spare=1, poison=False)
+    rng = np.random.default_rng(hd)
+    for counts in (None, [int(x) for x in rng.integers(1, 40, n_seq)]):
+        for n, pairs in ((n_seq, ((69, 3), (40, 39), (36, 0), (20, 3))), (5, ((4, 2),)), (2, ((1, 0),))):
+            rows = (counts or [1] * n_seq)[:n]
+            seqs = [int(s) for s in rng.permutation(n_seq)][:n]
+            for a, b in pairs:
+                seqs[a] = seqs[b]
+            x = torch.randn((2, sum(rows), n_kv, hd), device="cuda")
+            start = None if counts is None else ints([0] + list(np.cumsum(rows)))
+            ctx.kv_write_dev(c.id, 0, x[0], x[1], seqs=ints(seqs), row_start=start)
+            reported(ctx, 1, "given twice")
+            at = 0
+            for s, m in zip(seqs, rows):
+                if seqs.count(s) == 1:
+                    c.m.write(0, [s], [m], wide(x[0, at:at + m].half()), wide(x[1, at:at + m].half()))
+                at += m
+            # Either entry's rows: taken over into the model.
+            for s in {s for s in seqs if seqs.count(s) > 1}:
+                most = max(m for t, m in zip(seqs, rows) if t == s)
+                for j in range(lens[s] - most, lens[s]):
+                    p = c.m.table[s][j // 16]
+                    c.m.k[0, p, :, j % 16], c.m.v[0, p, :, j % 16] = wide(c.k[0, p, :, j % 16]), wide(c.v[0, p, :, j % 16])
+            c.same()
+            # The marks are clear again: each once is no error.
+            once = [int(s) for s in rng.permutation(n_seq)][:n]
+            ctx.kv_write_dev(c.id, 0, x[0], x[1], seqs=ints(once), row_start=start)
+            c.m.write(0, once, rows, wide(x[0].half()), wide(x[1].half()))
+            c.same()
+            ctx.kv_extend_dev(c.id, ints(once), ints([0] * n))
+            c.same()
