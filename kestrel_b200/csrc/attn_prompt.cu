@@ -140,52 +140,125 @@ struct Item {
   __device__ int pos(int t, int bn) const { return (t < head ? t : t - head + w0) * bn; }
 };
 
-// One row computed position by position by a warp: what the products cannot
-// give when a value that the row does not see is not finite (0 * NaN). Columns
-// col0 .. col1-1 are written.
+// One row computed by a warp, 32 positions at a time: what the products cannot
+// give when a value that the row does not see is not finite (0 * NaN). A lane
+// takes one position's score, then eight columns of every fourth position's
+// values, so that the loads of 64 columns are all under way together (32 rows
+// at 8192 positions, 8 heads of 64, all of them so: 18 ms; position by position
+// 219). Columns col0 .. col1-1 are written. `alive` is the time at which it last
+// moved on, for those who wait for it.
 template <typename TQ, typename TKV>
-__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int at, const TQ* q, TQ* out, int col0, int col1) {
-  const KvView& c = a.c;
-  const int lane = threadIdx.x & 31, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
-  float x[8], o[8], m = -INFINITY, l = 0.f;
+__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int at, const TQ* q, TQ* out, int col0,
+                                        int col1, volatile uint64_t* alive) {
+  const KvView c = a.c;
+  const int lane = threadIdx.x & 31, sub = lane & 7, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
+  const float scale = a.scale;
+  float x[8], o[4][8], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    x[u] = lane + 32 * u < c.hd ? (float)q[lane + 32 * u] : 0.f;
-    o[u] = 0.f;
-  }
-  for (int j = 0; j <= at; ++j) {
-    if (j < lo && j >= a.sinks) {
-      j = lo - 1;
+  for (int u = 0; u < 8; ++u) x[u] = lane + 32 * u < c.hd ? (float)q[lane + 32 * u] : 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[g][i] = 0.f;
+  for (int j0 = 0, steps = 0; j0 <= at; j0 += 32) {
+    if (j0 + 32 <= lo && j0 >= a.sinks) {
+      j0 = lo / 32 * 32 - 32;
       continue;
     }
-    const int id = c.table[(int64_t)s * c.max_pages + (j >> c.page_log2)];
-    if (id < 0 || id >= c.n_pages) continue;
-    const int64_t e =
-        ((((int64_t)a.layer * c.n_pages + id) * c.nkv + kvh) * c.page + (j & (c.page - 1))) * (int64_t)c.hd;
-    const TKV* k = reinterpret_cast<const TKV*>(c.k) + e;
-    const TKV* v = reinterpret_cast<const TKV*>(c.v) + e;
+    const int j = j0 + lane;
+    bool see = j <= at && (j >= lo || j < a.sinks);
+    long long e = 0;
+    if (see) {
+      const int id = c.table[(int64_t)s * c.max_pages + (j >> c.page_log2)];
+      see = id >= 0 && id < c.n_pages;
+      if (see) e = ((((int64_t)a.layer * c.n_pages + id) * c.nkv + kvh) * c.page + (j & (c.page - 1))) * (int64_t)c.hd;
+    }
+    const unsigned seen = __ballot_sync(0xffffffffu, see);
     float t = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (lane + 32 * u < c.hd) t = __fmaf_rn(x[u], (float)k[lane + 32 * u], t);
+    for (int g = 0; g < 4; ++g)
+      if (64 * g < c.hd) {
+        uint4 k[8];
 #pragma unroll
-    for (int w = 16; w; w >>= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
-    t *= a.scale;
-    if (t != t) {  // every result is NaN
-      l = t;
+        for (int w = 0; w < 8; ++w)
+          k[w] = see && 64 * g + 8 * w < c.hd
+                     ? reinterpret_cast<const uint4*>(reinterpret_cast<const TKV*>(c.k) + e)[8 * g + w]
+                     : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          alignas(16) TKV y[8];
+          *reinterpret_cast<uint4*>(y) = k[w];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            t = __fmaf_rn(__shfl_sync(0xffffffffu, x[2 * g + (w >> 2)], 8 * (w & 3) + i), (float)y[i], t);
+        }
+      }
+    t = see ? t * scale : -INFINITY;
+    if (__any_sync(0xffffffffu, !(t < INFINITY))) {  // a score of NaN or infinity: every result is NaN
+      l = NAN;
       break;
     }
-    const float mn = fmaxf(m, t), shrink = mn == -INFINITY ? 1.f : expf(m - mn);
-    const float p = mn == -INFINITY ? 0.f : expf(t - mn);
-    m = mn;
-    l = __fmaf_rn(l, shrink, p);
+    float top = t;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (lane + 32 * u < c.hd) o[u] = __fmaf_rn(p, (float)v[lane + 32 * u], o[u] * shrink);
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float mn = fmaxf(m, top), shrink = mn == -INFINITY ? 1.f : expf(m - mn);
+    const float p = mn == -INFINITY ? 0.f : expf(t - mn);
+    float sum = p;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    m = mn;
+    l = __fmaf_rn(l, shrink, sum);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (64 * g < c.hd) {
+        uint4 v[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const int from = 4 * y + (lane >> 3);
+          const long long e_y = __shfl_sync(0xffffffffu, e, from);
+          v[y] = seen >> from & 1 && 64 * g + 8 * sub < c.hd
+                     ? reinterpret_cast<const uint4*>(reinterpret_cast<const TKV*>(c.v) + e_y)[8 * g + sub]
+                     : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[g][i] *= shrink;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float p_y = __shfl_sync(0xffffffffu, p, 4 * y + (lane >> 3));
+          alignas(16) TKV z[8];
+          *reinterpret_cast<uint4*>(z) = v[y];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[g][i] = __fmaf_rn(p_y, (float)z[i], o[g][i]);
+        }
+      }
+    if (!(++steps & 31) && lane == 0) *alive = globaltimer();
   }
 #pragma unroll
-  for (int u = 0; u < 8; ++u)
-    if (lane + 32 * u >= col0 && lane + 32 * u < col1) out[lane + 32 * u] = (TQ)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(o[u], l));
+  for (int g = 0; g < 4; ++g)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float r = o[g][i];
+      r += __shfl_xor_sync(0xffffffffu, r, 8);
+      r += __shfl_xor_sync(0xffffffffu, r, 16);
+      const int col = 64 * g + 8 * sub + i;
+      if (lane < 8 && col >= col0 && col < col1) out[col] = (TQ)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(r, l));
+    }
+}
+
+// mbar_wait whose limit counts from the last time that a row computed by itself
+// moved on (it takes as long as it is).
+__device__ __forceinline__ bool prompt_wait(uint64_t* bar, uint32_t parity, int* status,
+                                            const volatile uint64_t* alive) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity)) {
+    const uint64_t now = globaltimer();
+    if (now - t0 > kWaitLimitNs && (int64_t)(now - *alive) > (int64_t)kWaitLimitNs) {
+      report(status, KC_ERR_TIMEOUT | (W_ATT_PROMPT << 8));
+      return false;
+    }
+  }
+  return true;
 }
 
 struct PromptArgs {
@@ -224,6 +297,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   __shared__ float factor_sh[2][S::QT][PM];  // what a row's queries were multiplied with (f32 queries)
   __shared__ float2 join_sh[2][NS][PM];      // maximum and sum of a stream's rows
   __shared__ int last_sh;
+  __shared__ uint64_t alive_sh;  // (prompt_row)
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -233,6 +307,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   uint8_t* q_sm = prompt_raw + ((1024 - (smem_u32(prompt_raw) & 1023)) & 1023);
   uint8_t* ring = q_sm + S::Q_ALL;
   if (tid == 0) {
+    alive_sh = 0;
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
@@ -266,11 +341,11 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   // Item n of this block, for every role but the one that finds it. A role
   // gives it back once it has read what it needs of it.
   auto item_wait = [&](int n) -> bool {
-    if (ok && !mbar_wait(&item_full[n & 1], (n >> 1) & 1, c.status, W_ATT_PROMPT)) ok = false;
+    if (ok && !prompt_wait(&item_full[n & 1], (n >> 1) & 1, c.status, &alive_sh)) ok = false;
     return ok;
   };
   auto wait = [&](uint64_t* bar, int phase) {
-    if (ok && !mbar_wait(bar, phase & 1, c.status, W_ATT_PROMPT)) ok = false;
+    if (ok && !prompt_wait(bar, phase & 1, c.status, &alive_sh)) ok = false;
   };
 
   // Eight values of each 64 of a query row, lane `part` of the row's eight, to
@@ -1052,7 +1127,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         prompt_row<TQ, TKV>(a, x.s, x.kvh, at_base + rm.token(f1),
                             static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride +
                                 (int64_t)x.kvh * group * c.hd + rm.offset(f1, a.q_stride, c.hd),
-                            out + rm.offset(f1, a.out_stride, c.hd), col0, min(col1, c.hd));
+                            out + rm.offset(f1, a.out_stride, c.hd), col0, min(col1, c.hd), &alive_sh);
       }
       if (!ok) break;
       __syncwarp();

@@ -152,3 +152,27 @@ def test_write_to_a_sequence_given_twice(ctx, n_kv, hd):
             c.same()
             ctx.kv_extend_dev(c.id, ints(once), ints([0] * n))
             c.same()
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=pair_id)
+def test_rows_computed_alone_over_a_long_cache(ctx, pair):
+    """An infinite value near the beginning of 160000 positions makes every row
+    one that is computed by itself: that takes its time, and no wait expires."""
+    n, rows, nh, hd, page = 160000, 32, 4, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k, v = (torch.randn((1, n // page, 1, page, hd), generator=g, device="cuda").to(pair[1]) for _ in range(2))
+    v[0, 2, 0, 5, 9], v[0, 2, 0, 6, 10] = float("inf"), float("nan")
+    ctx.kv_cache(9998, k, v, torch.arange(n // page, dtype=torch.int32, device="cuda")[None], ints([n]),
+                 torch.ones(n // page, dtype=torch.int32, device="cuda"))
+    q = queries(rows, nh, hd, pair[0], 9)
+    out = torch.empty_like(q.contiguous())
+    ctx.attn_prompt_dev(9998, 0, q, ints([0, rows]), out)
+    ctx.sync()
+    kk, vv = k.reshape(n, hd).double(), v.reshape(n, hd).double()
+    score = torch.einsum("rhd,jd->rhj", q.double(), kk) * hd ** -0.5
+    hidden = torch.arange(n, device="cuda") > (n - rows + torch.arange(rows, device="cuda"))[:, None, None]
+    want = torch.softmax(score.masked_fill(hidden, float("-inf")), -1) @ vv
+    # (The hidden positions are finite: their weight of zero adds nothing.)
+    same_numbers(wide(out), want.cpu().numpy(), pair[0])
+    assert torch.isinf(out[..., 9]).all() and torch.isnan(out[..., 10]).all() and torch.isfinite(out[..., 11:]).all()
+    ctx.kv_drop(9998)
