@@ -392,6 +392,9 @@ int check_status(kc_ctx* ctx) {
     // would not be ordered before the next call's kernels, whose bounded
     // waits read the word and return early on KC_ERR_STATE).
     CK(cudaMemsetAsync(ctx->status, 0, sizeof(int), ctx->stream));
+    // A block of an attention kernel that gave up waiting has not counted: what
+    // the others counted would make a later call join its parts too early.
+    if (ctx->kv.count) CK(cudaMemsetAsync(ctx->kv.count, 0, ctx->kv.count_bytes, ctx->stream));
     CK(cudaStreamSynchronize(ctx->stream));
     static const char* sites[] = {"unknown", "decode producer (empty stage)", "decode consumer (full stage)",
                                   "decode drain", "tcgen05 producer (raw stage)", "tcgen05 producer (operand stage)",
@@ -3134,6 +3137,7 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
       CK(cudaMalloc(&p, all));
       ctx->kv.part = static_cast<float*>(p);
       ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + part);
+      ctx->kv.count_bytes = (int64_t)cnt;
       ctx->kv.bytes = (int64_t)all;
       CK(cudaMemsetAsync(ctx->kv.count, 0, cnt, ctx->stream));
     }

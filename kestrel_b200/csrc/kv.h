@@ -55,7 +55,8 @@ struct KvState {
   std::map<int, KvCache> caches;
   float* part = nullptr;  // parts to be joined: the larger of the two kernels' needs
   int* count = nullptr;   // arrival counts, zero between launches
-  int64_t bytes = 0;
+  int64_t count_bytes = 0;
+  int64_t bytes = 0;      // of both
 };
 
 int64_t kv_workspace_ints(const KvView& c);

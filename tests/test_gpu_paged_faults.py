@@ -176,3 +176,49 @@ def test_rows_computed_alone_over_a_long_cache(ctx, pair):
     same_numbers(wide(out), want.cpu().numpy(), pair[0])
     assert torch.isinf(out[..., 9]).all() and torch.isnan(out[..., 10]).all() and torch.isfinite(out[..., 11:]).all()
     ctx.kv_drop(9998)
+
+
+def arrival_counts(c):
+    """The attention kernels' arrival counts in a context's workspace, as an
+    int32 CUDA tensor: their place is found in the context by what surrounds it
+    (parts, counts behind them, the bytes of the counts and of both)."""
+    with open("/proc/self/mem", "rb", 0) as mem:
+        mem.seek(c.h.value if hasattr(c.h, "value") else c.h)
+        words = np.frombuffer(mem.read(1 << 13), dtype=np.int64)
+    at = [i for i in range(len(words) - 3) if words[i] and words[i + 1] > words[i] and 0 < words[i + 2] < 1 << 16 and
+          words[i + 1] - words[i] + words[i + 2] == words[i + 3]]
+    assert len(at) == 1
+    address, size = int(words[at[0] + 1]), int(words[at[0] + 2]) // 4
+
+    class Counts:
+        __cuda_array_interface__ = {"shape": (size,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+    return torch.as_tensor(Counts(), device="cuda")
+
+
+def test_counts_after_an_expired_wait(ctx):
+    """What an attention call that gave up waiting leaves in the arrival counts is
+    cleared with the status, so that later calls join their parts in full. (The
+    counts are set here, and the status by an index out of range.)"""
+    c = Cache(ctx, [3000, 2500], 64, 1, 64, F16, seed=3)
+    q = queries(2 * 40, 4, 64, F32, 4)
+    one = torch.empty_like(q[:2].contiguous())
+    rows = torch.empty_like(q.contiguous())
+    counts = arrival_counts(ctx)
+    ctx.attn_decode_dev(c.id, 0, q[:2], one)
+    ctx.attn_prompt_dev(c.id, 0, q, ints([0, 40, 80]), rows)
+    ctx.sync()
+    assert not counts.any()  # put back by the kernels
+    want = one.clone(), rows.clone()
+    close(wide(one), c.expected(0, wide(q[:2]), [0, 1], [1, 1], 0.125, 0, 0), F32)
+    for left in (1, 3):
+        counts.fill_(left)
+        ctx.attn_decode_dev(c.id, 0, q[:1], one[:1], seqs=ints([99]))
+        reported(ctx, 1, "out of range")
+        assert not counts.any()
+        one.fill_(7)
+        rows.fill_(7)
+        ctx.attn_decode_dev(c.id, 0, q[:2], one)
+        ctx.attn_prompt_dev(c.id, 0, q, ints([0, 40, 80]), rows)
+        ctx.sync()
+        assert torch.equal(one, want[0]) and torch.equal(rows, want[1])
