@@ -500,7 +500,8 @@ KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, cons
    positions of sequence i, in order (already extended and written); row_start
    [n + 1] ascends within 0 .. n_rows. An entry that begins before an earlier
    one does, ends before it begins or ends past n_rows is left out and
-   reported. Rows in no sequence's range are not written. */
+   reported. Rows in no sequence's range are not written, nor (in both calls)
+   those of a sequence index out of range; a sequence may be given twice. */
 KC_API int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, int n_head, int t,
                               const void* q, int64_t q_stride, float scale, int window, int sinks, void* out,
                               int64_t out_stride);

@@ -164,9 +164,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     bool none = false;
     if (i < a.n) {
       const int s = a.seqs ? a.seqs[i] : i;
-      if (s >= 0 && s < c.n_seq) here = dec_span(kv_len(c, s), a.window, a.sinks).n;
+      const bool real = s >= 0 && s < c.n_seq;
+      if (real) here = dec_span(kv_len(c, s), a.window, a.sinks).n;
       else if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
-      none = here == 0 && i % gridDim.x == blockIdx.x;
+      none = real && here == 0 && i % gridDim.x == blockIdx.x;
     }
     for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)(i0 + __ffs(rows) - 1) * a.out_stride;

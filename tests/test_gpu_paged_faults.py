@@ -222,3 +222,19 @@ def test_counts_after_an_expired_wait(ctx):
         ctx.attn_prompt_dev(c.id, 0, q, ints([0, 40, 80]), rows)
         ctx.sync()
         assert torch.equal(one, want[0]) and torch.equal(rows, want[1])
+
+
+def test_rows_of_a_sequence_out_of_range(ctx):
+    """Both kernels leave them as they are, and zero those of an empty one."""
+    c = Cache(ctx, [70, 0, 33], 16, 1, 64, F16, seed=1)
+    q = queries(5, 2, 64, F32, 2)
+    out = torch.full_like(q.contiguous(), 7.0)
+    ctx.attn_decode_dev(c.id, 0, q[:3], out[:3], seqs=ints([2, 3, 1]))
+    reported(ctx, 1, "out of range")
+    close(wide(out)[:1], c.expected(0, wide(q)[:1], [2], [1], 0.125, 0, 0), F32)
+    assert (out[1] == 7).all() and (out[2] == 0).all()
+    out.fill_(7)
+    ctx.attn_prompt_dev(c.id, 0, q, ints([0, 2, 4, 5]), out, seqs=ints([2, -1, 1]))
+    reported(ctx, 1, "out of range")
+    close(wide(out)[:2], c.expected(0, wide(q)[:2], [2], [2], 0.125, 0, 0), F32)
+    assert (out[2:4] == 7).all() and (out[4] == 0).all()
