@@ -3077,8 +3077,10 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.scale = scale;
-    a.window = window;
-    a.sinks = window > 0 ? sinks : 0;
+    // A window as long as a table row hides nothing. (Positions less a longer one
+    // could also leave 32 bits.)
+    a.window = (int64_t)window < (int64_t)c.max_pages * c.page ? window : 0;
+    a.sinks = a.window > 0 ? sinks : 0;
     const int rc = prompt ? launch_attn_prompt(a, kv.tiles, ctx->kv.part, ctx->kv.count, ctx->stream)
                           : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
     return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);

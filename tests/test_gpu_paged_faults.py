@@ -238,3 +238,22 @@ def test_rows_of_a_sequence_out_of_range(ctx):
     reported(ctx, 1, "out of range")
     close(wide(out)[:2], c.expected(0, wide(q)[:2], [2], [2], 0.125, 0, 0), F32)
     assert (out[2:4] == 7).all() and (out[4] == 0).all()
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=pair_id)
+def test_windows_and_sinks_of_any_size(ctx, pair):
+    """Up to the largest int, longer than the sequence, and with more rows than
+    positions (the first rows then see nothing)."""
+    most = 2 ** 31 - 1
+    c = Cache(ctx, [40, 200, 1, 0], 16, 1, 64, pair[1], seed=2)
+    counts = [90, 200, 3, 2]
+    q = queries(sum(counts), 2, 64, pair[0], 3)
+    for window, sinks in ((most, 0), (most, most), (most - 5, 3), (c.table.shape[1] * 16, 1),
+                          (c.table.shape[1] * 16 - 1, 1), (30, most), (1, most), (200, 300), (199, 0)):
+        out = torch.full_like(q.contiguous(), 7.0)
+        ctx.attn_prompt_dev(c.id, 0, q, ints([0] + list(np.cumsum(counts))), out, window=window, sinks=sinks)
+        one = torch.full_like(q[:4].contiguous(), 7.0)
+        ctx.attn_decode_dev(c.id, 0, q[:4], one, window=window, sinks=sinks)
+        ctx.sync()
+        close(wide(out), c.expected(0, wide(q), range(4), counts, 0.125, window, sinks), pair[0])
+        close(wide(one), c.expected(0, wide(q)[:4], range(4), [1] * 4, 0.125, window, sinks), pair[0])
