@@ -401,9 +401,6 @@ void launch_kv_copy_pages(const KvView& c, const int32_t* src, const int32_t* ds
 }
 
 // ---- write -------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
-
 // Eight consecutive values of a row as cache values, in one 16-byte piece.
 template <typename S, typename D>
 __device__ __forceinline__ uint4 convert8(const S* p, bool aligned) {

@@ -8,7 +8,6 @@
 #include <stdint.h>
 
 #include <map>
-#include <string>
 
 namespace kc {
 

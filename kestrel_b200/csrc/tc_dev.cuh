@@ -111,8 +111,5 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const float* v) {
   for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i]);
   tmem_st16(t, u);
 }
-__device__ __forceinline__ void named_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 
 }  // namespace kc
