@@ -523,13 +523,21 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
       {
         const int pr = (lane & 7) + 8 * ((lane >> 3) & 1), g = lane >> 4;
+        // Added here, rounded to nearest: products that add to the sum cut its last
+        // bits off, 2^-24 of it per chunk, always towards zero (32 sequences of
+        // 131071, 1800 chunks a warp: 6e-5 where f32 sums are 2e-7 off, as here).
 #pragma unroll
         for (int t = 0; t < 4 * NB; ++t) {
           const int u = 2 * (t & 3) + g;
           uint32_t b[4];
           ldsm4t(b, vb + (t >> 2) * DC * 128 + pr * 128 + ((u ^ (pr & 7)) << 4));
-          mma16816<TKV>(o[2 * t], pa, b[0], b[1]);
-          mma16816<TKV>(o[2 * t + 1], pa, b[2], b[3]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float d[4];
+            mma16816_only<TKV>(d, pa, b[2 * y], b[2 * y + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * t + y][e] += d[e];
+          }
         }
       }
       __syncwarp();
