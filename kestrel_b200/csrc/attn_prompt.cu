@@ -26,9 +26,10 @@
 // block that finishes last joins the parts in their order.
 //
 // f32 queries are carried by two f16 operands (value and rest), and so are
-// their weights: twice the products, f32-grade results over a 16-bit cache
-// (2.7e-6 off at up to 4000 positions, where f32 arithmetic is 1.1e-6: the
-// tensor cores cut their sums off, see below).
+// their weights: twice the products, f32-grade results over a 16-bit cache (at
+// most 8e-6 off however long it is, 4e-6 for values of mean 0, where f32
+// arithmetic is 1e-6: the tensor cores cut their sums off, see KEEP). Weights
+// under 16-bit queries are rounded to the cache's type; their sum is not.
 //
 // Measured on a B200, 32 query and 4 key-value heads of 128, f16: 8192 rows from
 // the first (550 GFLOP) in 449 us over 60 calls and 535 us kept up (1.03
@@ -57,6 +58,7 @@ namespace kc {
 constexpr int PM = 128;  // rows of a tile
 constexpr int P_STAGES_MAX = 8;
 constexpr int P_SPLITS_MAX = 8;  // blocks an item's positions are split over, at most
+constexpr int KEPT_COLUMNS = 264;  // of both streams, or one, and their maxima
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * 168, "within the registers of the launch");
 
@@ -90,8 +92,19 @@ struct PromptShape {
   // A split item's part: per four columns the rows' values ([HD / 4][PM][4]),
   // then the rows' maxima and sums ([PM][2]).
   static constexpr int PART = PM * (HD + 2);
+  // An accumulator begins anew after so many tiles, and what it held is kept in
+  // memory: the tensor cores cut a sum's last bits off with every 16 positions
+  // (and operand), always towards zero, about 2^-24.5 of the final sum a step when
+  // nothing cancels. 1024 rows at 131072 positions, f32: 3.4e-4 off when they go
+  // on adding, 8e-6 with 12 tiles (192 steps; 6 x 256 rows at 300 to 4000 134 us
+  // and 129 without), 5.4e-6 with 8 (139 us), 1.1e-5 with 16 (131 us). Where results
+  // are rounded to 16 bits, 1024 steps.
+  static constexpr int KEEP = (kSplit ? 1536 : 16384) / BN;
+  // What a stream keeps: the maxima that the values count from (every fourth
+  // place), then the values, as in a part.
+  static constexpr int KEPT = PM * (HD + 4);
   static_assert(!TWO || kShared, "two row tiles: two streams of 16-bit weights");
-  static_assert(ST >= 2 && T_O + NS * HD <= 512, "fits");
+  static_assert(ST >= 2 && T_O + NS * HD <= 512 && NS * (HD + 4) <= KEPT_COLUMNS, "fits");
 };
 
 // 16 values times f; whether any of them was infinite or NaN (times 0 it is NaN).
@@ -261,10 +274,40 @@ __device__ __forceinline__ bool prompt_wait(uint64_t* bar, uint32_t parity, int*
   return true;
 }
 
+// A row's accumulator (hd16 columns at o_t of TMEM; reference m) and what is kept
+// of it in memory (its reference, values from 4 * PM on): put there, added to it,
+// or added back to the accumulator. Whole warps; out of the way of the tiles that
+// do not need it.
+enum { KEEP_FIRST, KEEP_ADD, KEEP_RETURN };
+__device__ __noinline__ void keep_sums(uint32_t o_t, int hd16, float* kept, float m, int how) {
+  const float before = how == KEEP_FIRST ? m : __ldcg(kept), shrink = before == m ? 1.f : exp2_fast(before - m);
+  for (int e0 = 0; e0 < hd16; e0 += 16) {
+    float4* at = reinterpret_cast<float4*>(kept + (e0 + 4) * PM);
+    float4 y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = how == KEEP_FIRST ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(at + e * PM);
+    float o[16];
+    tmem_ld16(o_t + e0, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e].x = __fmaf_rn(y[e].x, shrink, o[4 * e]);
+      y[e].y = __fmaf_rn(y[e].y, shrink, o[4 * e + 1]);
+      y[e].z = __fmaf_rn(y[e].z, shrink, o[4 * e + 2]);
+      y[e].w = __fmaf_rn(y[e].w, shrink, o[4 * e + 3]);
+      if (how != KEEP_RETURN) __stcg(at + e * PM, y[e]);
+    }
+    if (how == KEEP_RETURN) tmem_st16(o_t + e0, reinterpret_cast<const float*>(y));
+  }
+  if (how != KEEP_RETURN) __stcg(kept, m);
+  tmem_wait_st();
+}
+
 struct PromptArgs {
   AttnArgs a;
   int splits;   // blocks an item's positions may be split over
   float* part;  // [unit][split][PART]
+  float* kept;  // [block][stream][KEPT]
   int* count;   // per unit, zero between launches
   int* next;    // [2] items dealt beyond one per block, blocks done: zero between launches
   bool q_map;   // queries come by TMA
@@ -527,7 +570,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
               const int w = (i - 1) & 1, t = TWO ? (i - 1) >> 1 : i - 1, k = TWO ? t : t >> 1;
               const uint32_t v = stage(v_at(t));
               if (k == 0) results_read(w);
-              values(w, kp[w] + k, v, k > 0);
+              values(w, kp[w] + k, v, k % S::KEEP != 0);
               if (!ok) break;
               if (!TWO || w == 1) tc_commit(&kv_empty[v_at(t) % ST]);
             }
@@ -549,7 +592,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           for (int t = 0; t < nt && ok; ++t) {
             const int w = t % NS;
             const uint32_t v = stage(v_at(t));
-            values(w, kp[w] + t / NS, v, t >= NS);
+            values(w, kp[w] + t / NS, v, t / NS % S::KEEP != 0);
             if (!ok) break;
             tc_commit(&kv_empty[v_at(t) % ST]);
             if (t + NS < nt) step_scores(t + NS);
@@ -773,6 +816,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // ---- softmax: stream w, a thread per row ---------------------------------
     const int w = warp >> 2, r = tid & 127, my_tile = TWO ? w : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    float* kept = d.kept + (int64_t)(blockIdx.x * NS + w) * S::KEPT + 4 * r;
     const uint32_t s_t = tmem + lanes + S::T_S * w, p_t = tmem + lanes + S::T_P + S::T_PW * w;
     const float unit = flip == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     int ks = 0, used = 0, ring_at = 0;  // score tiles, items with products, loads before this item's
@@ -842,6 +886,19 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           break;
         }
         tc_fence_after();
+        if (rarely(k > 0 && k % S::KEEP == 0)) {
+          // The products so far are complete (with the scores, or are waited for),
+          // and the next ones do not add to them.
+          if constexpr (kShared) {
+            wait(&pv_done[w], ks - 1);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          keep_sums(o_t, hd16, kept, m, k == S::KEEP ? KEEP_FIRST : KEEP_ADD);
+        }
         if constexpr (kSplit)
           if (k == 0) cq = __fdiv_rn(unit, factor_sh[used & 1][my_tile][r]);
         float s[BN];
@@ -992,6 +1049,13 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             done[v] += TWO ? nt : (nt - v + NS - 1) / NS;
             wait(&pv_done[v], done[v] - 1);
           }
+        if (rarely(mine > S::KEEP)) {
+          // What was kept goes back to the accumulator.
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          if (ok) keep_sums(o_t, hd16, kept, m, KEEP_RETURN);
+          tc_fence_before();
+        }
         if constexpr (kJoin) {
           join_sh[used & 1][w][r] = make_float2(m, l);
           mbar_arrive(&join_full);
@@ -1142,7 +1206,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
 // Parts of split items: what 192 items of 128 rows take at a head size of 128.
 constexpr size_t PROMPT_PART_BYTES = (size_t)192 * PM * (128 + 2) * sizeof(float);
 constexpr int PROMPT_MAX_UNITS = 192;
-size_t attn_prompt_part_bytes() { return PROMPT_PART_BYTES; }
+// Behind them, what the streams of every block keep of sums over many tiles.
+size_t attn_prompt_part_bytes() {
+  return PROMPT_PART_BYTES + (size_t)num_sms() * PM * KEPT_COLUMNS * sizeof(float);
+}
 int attn_prompt_counts() { return PROMPT_MAX_UNITS + 2; }
 
 template <typename TQ, typename TKV, int NB, bool TWO>
@@ -1198,7 +1265,7 @@ static int launch_prompt_hd(const PromptArgs& d, const KvMaps& maps, cudaStream_
 int attn_prompt_box_rows(int page, int hd) { return std::min(page, hd <= 128 ? 128 : 64); }
 
 int launch_attn_prompt(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
-  const PromptArgs d{a, 1, part, count, count + PROMPT_MAX_UNITS, false};
+  const PromptArgs d{a, 1, part, part + PROMPT_PART_BYTES / sizeof(float), count, count + PROMPT_MAX_UNITS, false};
   if (a.c.type == T_BF16) return launch_prompt_hd<__nv_bfloat16, __nv_bfloat16>(d, maps, st);
   if (a.t_q == T_F32) return launch_prompt_hd<float, __half>(d, maps, st);
   return launch_prompt_hd<__half, __half>(d, maps, st);
