@@ -96,10 +96,11 @@ struct PromptShape {
   // memory: the tensor cores cut a sum's last bits off with every 16 positions
   // (and operand), always towards zero, about 2^-24.5 of the final sum a step when
   // nothing cancels. 1024 rows at 131072 positions, f32: 3.4e-4 off when they go
-  // on adding, 8e-6 with 12 tiles (192 steps; 6 x 256 rows at 300 to 4000 134 us
-  // and 129 without), 5.4e-6 with 8 (139 us), 1.1e-5 with 16 (131 us). Where results
-  // are rounded to 16 bits, 1024 steps.
-  static constexpr int KEEP = (kSplit ? 1536 : 16384) / BN;
+  // on adding, 8e-6 with 12 tiles (192 steps), 5.4e-6 with 8, 1.1e-5 with 16. 6 x
+  // 256 rows at 300 to 4000 take 129 us without, 134, 139 and 131 so, the 1024 at
+  // 131072 3.8 ms without and 4.2 with 12 or 16. Where results are rounded to 16
+  // bits, 2048 steps, 1e-4.
+  static constexpr int KEEP = (kSplit ? 1536 : 32768) / BN;
   // What a stream keeps: the maxima that the values count from (every fourth
   // place), then the values, as in a part.
   static constexpr int KEPT = PM * (HD + 4);
