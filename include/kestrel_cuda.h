@@ -446,8 +446,9 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
    change them in stream order, with no host synchronisation and no device
    allocation, so decode steps with them can be captured into CUDA graphs.
    Lists of sequences, counts and pages are device arrays too; what only the
-   device can see wrong in them (an index out of range or given twice, too few
-   free pages) is left out and reported by kc_sync, as is a table entry outside
+   device can see wrong in them (an index out of range, or given twice to a call
+   that changes it, too few free pages) is left out, unless a call says
+   otherwise, and reported by kc_sync, as is a table entry outside
    the pool (results of that sequence are then undefined). `seqs` NULL means
    sequences 0 .. n-1; n is at most n_seq. A context's calls share
    one workspace: after kc_set_stream the caller orders the new stream behind
@@ -493,8 +494,11 @@ KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, cons
    (stale rows of a page, NaN); infinities and NaN in what is visible give what
    the formula gives. (Only scores of minus infinity: zeros.) q and out: rows of n_head * head_dim, the row
    strides in elements; type t is the cache's, or KC_F32 over a KC_F16 cache;
-   n_head a multiple of n_head_kv (at most 128 query heads to one). Softmax and
-   sums are f32 for every type.
+   n_head a multiple of n_head_kv (at most 128 query heads to one). Maxima and
+   sums are f32 for every type. Weights: under KC_F32 queries good to 22 bits;
+   under 16-bit ones rounded to the cache's type in kc_attn_prompt_dev, and in
+   kc_attn_decode_dev where more than 8 query heads share one (22 bits, or 16 of
+   KC_BF16, otherwise).
    kc_attn_decode_dev: row i is the last position of sequence i.
    kc_attn_prompt_dev: rows row_start[i] .. row_start[i+1]-1 are the last
    positions of sequence i, in order (already extended and written); row_start

@@ -17,12 +17,15 @@
 // product. f32 queries and the f32 weights are each carried by two 16-bit rows
 // (value and rest, 22 bits for f16), which fill the product's other eight rows
 // at no cost: results are f32-grade although the cache is 16-bit. Groups of
-// more than eight heads with 16-bit queries use all sixteen rows for heads.
+// more than eight heads with 16-bit queries use all sixteen rows for heads (their
+// weights are rounded to the cache's type).
 //
 // Measured on a B200 (plain copy 6.46 TB/s): 96 sequences of 1500 to 8192 under
-// a window of 4096, 8 key-value heads of 128, 1.37 GB in 232 us (5.9 TB/s); one
-// of 131071, 4 heads, 268 MB in 56 us (4.8); 32 of 200 to 4096, 126 MB in 34 us
-// (3.7). What is not reading: about 5 us until the first chunks are asked for
+// a window of 4096, 8 key-value heads of 128, 1.37 GB in 234 us (5.9 TB/s); one
+// of 131071, 4 heads, 268 MB in 56 us (4.8); 32 of 200 to 4096, 126 MB in 34.6 us
+// (3.6). Past one round of a block's threads (256 sequences; 128 at head sizes
+// past 128) every block walks the list of lengths twice: 1000 of 64, 131 MB in 40
+// us (3.3). What is not reading: about 5 us until the first chunks are asked for
 // (launch, lengths, ranges, page ids) and 5 to 8 at the end (the last warp, the
 // parts, their join through L2).
 #include <algorithm>

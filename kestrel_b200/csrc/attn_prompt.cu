@@ -9,7 +9,8 @@
 // The rows of a key-value head (tokens outermost, then the heads of its group)
 // are cut into tiles of 128, the M of an MMA, so that the group shares every
 // key and value. Positions pass in tiles of BN. One block per SM takes items
-// (row tiles of a head) as it comes to them, those that see most first. Roles:
+// (row tiles of a head) as it comes to them, those that see most first (in the
+// list's order where it has more than 32 entries). Roles:
 //   softmax warps  four per stream, a thread per row: scores from TMEM, the
 //                  mask where the tile needs it, weights back to TMEM as the
 //                  16-bit A operand of the second product. The accumulator is
@@ -19,8 +20,8 @@
 //   two more       find the next item and bring its queries, while the others
 //                  are at the last one.
 // Two streams take turns on the tensor cores, so that one's exponentials run
-// beside the other's products (an MMA tile of 128 x 128 x 128 takes as long as
-// its 16384 exponentials): either two row tiles over the same positions, or
+// beside the other's products (the two of a tile, 128 x 128 x 128 each, take as
+// long as its 16384 exponentials, 1024 cycles): either two row tiles over the same positions, or
 // one row tile whose position tiles alternate, joined at the end. With fewer
 // items than SMs their positions are split further, over several blocks; the
 // block that finishes last joins the parts in their order.
@@ -32,10 +33,9 @@
 // under 16-bit queries are rounded to the cache's type; their sum is not.
 //
 // Measured on a B200, 32 query and 4 key-value heads of 128, f16: 8192 rows from
-// the first (550 GFLOP) in 449 us over 60 calls and 535 us kept up (1.03
-// PFLOP/s, under the power cap, where the measured matrix rate is 1.43); two
-// prompts of 6001 and 7400 rows with 8 heads under a window of 2048, bf16 (422
-// GFLOP of visible pairs) in 376 and 475 us. At 4096 rows the tensor pipe is
+// the first (550 GFLOP) in 533 us kept up (1.03 PFLOP/s, under the power cap,
+// where the measured matrix rate is 1.43); two prompts of 6001 and 7400 rows with 8
+// heads under a window of 2048, bf16 (422 GFLOP of visible pairs) in 476 us. At 4096 rows the tensor pipe is
 // busy for 52% of the active cycles, and so is the unit of the exponentials: a
 // stream's tile takes its warps about 2600 cycles beside the other stream's,
 // and the two products and their hand-overs 1550 a step. Tried and not kept: a
@@ -1245,7 +1245,12 @@ static int launch_prompt(PromptArgs d, const KvMaps& maps, cudaStream_t st) {
 template <typename TQ, typename TKV>
 static int launch_prompt_hd(const PromptArgs& d, const KvMaps& maps, cudaStream_t st) {
   // Two row tiles per item read every key and value once for both; with few
-  // rows, or f32 queries (two operands each), an item is one.
+  // rows, or f32 queries (two operands each), an item is one. f16, 32 and 4 heads
+  // of 128, two tiles and one, us: 5 x 256 rows at 2048 (160 pairs) 69 and 66, 6 x
+  // 256 at 300 to 4000 (192) 85 and 74, 8 x 256 at 2048 (256) 73 and 88, 10 x 256
+  // (320) 103 and 109, 2048 from the first (256) 56 and 63, 8192 (1024) 527 and 606.
+  // (Below two rounds of pairs one tile evens the rounds out better; the rule does
+  // not count them.)
   const AttnArgs& a = d.a;
   const int64_t pairs = ((int64_t)a.n_rows * (a.nh / a.c.nkv) + 2 * PM - 1) / (2 * PM) * a.c.nkv;
   const bool two = sizeof(TQ) == 2 && pairs >= num_sms();

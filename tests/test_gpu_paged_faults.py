@@ -143,7 +143,8 @@ def test_write_to_a_sequence_given_twice(ctx, n_kv, hd):
                 most = max(m for t, m in zip(seqs, rows) if t == s)
                 for j in range(lens[s] - most, lens[s]):
                     p = c.m.table[s][j // 16]
-                    c.m.k[0, p, :, j % 16], c.m.v[0, p, :, j % 16] = wide(c.k[0, p, :, j % 16]), wide(c.v[0, p, :, j % 16])
+                    c.m.k[0, p, :, j % 16] = wide(c.k[0, p, :, j % 16])
+                    c.m.v[0, p, :, j % 16] = wide(c.v[0, p, :, j % 16])
             c.same()
             # The marks are clear again: each once is no error.
             once = [int(s) for s in rng.permutation(n_seq)][:n]

@@ -70,9 +70,9 @@ def test_decode_of_long_batches(ctx, heads, types, mean):
 
 @pytest.mark.parametrize("mean", [0.0, 1.0])
 @pytest.mark.parametrize("types", [(F32, F16), (F16, F16), (BF16, BF16)], ids=str)
-@pytest.mark.parametrize("heads,rows,n", [((32, 4, 128), 1500, 40000), ((8, 2, 64), 40, 70000), ((16, 2, 64), 5000, 20000),
-                                          ((12, 3, 96), 2000, 33001), ((8, 2, 256), 1300, 20000), ((6, 2, 200), 33, 50000)],
-                         ids=str)
+@pytest.mark.parametrize("heads,rows,n", [((32, 4, 128), 1500, 40000), ((8, 2, 64), 40, 70000),
+                                          ((16, 2, 64), 5000, 20000), ((12, 3, 96), 2000, 33001),
+                                          ((8, 2, 256), 1300, 20000), ((6, 2, 200), 33, 50000)], ids=str)
 def test_prompts_over_long_caches(ctx, heads, rows, n, types, mean):
     """Items of one and two row tiles, of two streams and of one, whole and split
     over their positions."""
