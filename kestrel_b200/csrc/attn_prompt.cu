@@ -615,21 +615,31 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // warp calls this; 0 where its rows are out of order: an entry begins where
     // every earlier one has begun or later, so that no two share a row and the
     // tiles of all of them are no more than the launch reckons with. `last`: the
-    // largest beginning before these 32, and then up to them.
+    // largest beginning before these 32, and then up to them (0 until something is
+    // out of order). The first time over the list says whether anything is.
+    bool ascend = true, known = false;
     auto tiles_of = [&](int i, int& last, int& lo, int& hi) {
-      lo = i < a.n ? a.row_start[i] : 0;
-      hi = i < a.n ? a.row_start[i + 1] : 0;
-      int top = lo;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, top, o);
-        if (lane >= o) top = max(top, y);
+      lo = hi = last;
+      if (i < a.n) {
+        lo = a.row_start[i];
+        hi = a.row_start[i + 1];
       }
-      top = max(top, last);
-      last = __shfl_sync(0xffffffffu, top, 31);
-      if (lo < top || hi < lo || hi > a.n_rows) {
-        if (i < a.n && blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
-        lo = hi = 0;
+      bool wrong = lo < last || hi < lo || hi > a.n_rows;
+      // (If none is wrong by itself they ascend: each begins where the last ends.)
+      if (!ascend || (!known && __any_sync(0xffffffffu, wrong))) {
+        ascend = false;
+        int top = max(lo, last);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, top, o);
+          if (lane >= o) top = max(top, y);
+        }
+        last = __shfl_sync(0xffffffffu, top, 31);
+        wrong |= lo < top;
+        if (wrong) {
+          if (i < a.n && blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
+          lo = hi = 0;
+        }
       }
       return (int)(((int64_t)(hi - lo) * group + S::QT * PM - 1) / (S::QT * PM));
     };
@@ -669,6 +679,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         tiles = __shfl_sync(0xffffffffu, scan(m), 31);
       }
     }
+    known = true;
     const int64_t total = (int64_t)tiles * c.nkv * d.splits;
     int used = 0;
     int64_t idx = blockIdx.x;  // the block's first item; the rest as it comes to them
