@@ -183,9 +183,15 @@ def arrival_counts(c):
     """The attention kernels' arrival counts in a context's workspace, as an
     int32 CUDA tensor: their place is found in the context by what surrounds it
     (parts, counts behind them, the bytes of the counts and of both)."""
+    start, data = c.h.value if hasattr(c.h, "value") else c.h, b""
     with open("/proc/self/mem", "rb", 0) as mem:
-        mem.seek(c.h.value if hasattr(c.h, "value") else c.h)
-        words = np.frombuffer(mem.read(1 << 13), dtype=np.int64)
+        try:
+            for at in range(start, start + (1 << 13), 256):
+                mem.seek(at)
+                data += mem.read(256)
+        except OSError:  # past the heap's end
+            pass
+    words = np.frombuffer(data[:len(data) // 8 * 8], dtype=np.int64)
     at = [i for i in range(len(words) - 3) if words[i] and words[i + 1] > words[i] and 0 < words[i + 2] < 1 << 16 and
           words[i + 1] - words[i] + words[i + 2] == words[i + 3]]
     assert len(at) == 1
