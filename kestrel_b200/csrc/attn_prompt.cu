@@ -108,9 +108,13 @@ struct PromptShape {
   static_assert(ST >= 2 && T_O + NS * HD <= 512 && NS * (HD + 4) <= KEPT_COLUMNS, "fits");
 };
 
-// 16 values times f; whether any of them was infinite or NaN (times 0 it is NaN).
+// Keeps a branch's code out of the way of what runs for every tile.
+__device__ __forceinline__ bool rarely(bool c) { return __builtin_expect(c, 0); }
+
+// 16 values times f; whether any of them is NaN. (An infinity is one that the row
+// sees, with a weight: beyond its mask it would be NaN, 0 times it.)
 __device__ __forceinline__ bool normalise16(float (&v)[16], float f) {
-  uint64_t odd = 0;
+  uint64_t odd = 0;  // infinite and NaN values times 0 are NaN
 #pragma unroll
   for (int e = 0; e < 16; e += 2) {
     const uint64_t x = f2(v[e], v[e + 1]);
@@ -119,11 +123,13 @@ __device__ __forceinline__ bool normalise16(float (&v)[16], float f) {
     v[e] = y.x;
     v[e + 1] = y.y;
   }
-  return f2(odd).x + f2(odd).y != 0.f;
+  bool nan = false;
+  if (rarely(f2(odd).x + f2(odd).y != 0.f)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) nan |= v[e] != v[e];
+  }
+  return nan;
 }
-
-// Keeps a branch's code out of the way of what runs for every tile.
-__device__ __forceinline__ bool rarely(bool c) { return __builtin_expect(c, 0); }
 
 // The lowest n bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t low_bits(int n) {
@@ -1196,8 +1202,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           }
         }
       }
-      // A row that a value beyond its mask has spoilt (or that sees one that is
-      // not finite) is computed again by itself.
+      // A row that a value beyond its mask has spoilt (or that sees a NaN, or an
+      // infinity against a weight's rest) is computed again by itself.
       for (unsigned again = __ballot_sync(0xffffffffu, ok && write && real && bad); again; again &= again - 1) {
         const int f1 = my_tile * PM + 32 * (warp & 3) + __ffs(again) - 1;
         prompt_row<TQ, TKV>(a, x.s, x.kvh, at_base + rm.token(f1),
