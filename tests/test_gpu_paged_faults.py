@@ -264,3 +264,31 @@ def test_windows_and_sinks_of_any_size(ctx, pair):
         ctx.sync()
         close(wide(out), c.expected(0, wide(q), range(4), counts, 0.125, window, sinks), pair[0])
         close(wide(one), c.expected(0, wide(q)[:4], range(4), [1] * 4, 0.125, window, sinks), pair[0])
+
+
+def test_write_to_thousands_of_sequences(ctx):
+    """A list of more sequences than the looking block holds at a time: one given
+    twice is found wherever the two are, and none where each is given once."""
+    n = 2500
+    k = torch.zeros((1, n, 1, 16, 8), dtype=F16, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    ctx.kv_cache(9997, k, v, table, torch.ones(n, dtype=torch.int32, device="cuda"),
+                 torch.ones(n, dtype=torch.int32, device="cuda"))
+    x = torch.randn((2, n, 1, 8), device="cuda").half()
+    order = torch.randperm(n).int()
+    for a, b in ((None, None), (2499, 0), (1025, 1024), (1300, 70), (None, None)):
+        seqs = order.clone()
+        if a is not None:
+            seqs[a] = seqs[b]
+        k.zero_()
+        ctx.kv_write_dev(9997, 0, x[0], x[1], seqs=seqs.cuda())
+        if a is None:
+            ctx.sync()
+            at = order.long().cuda()
+            assert torch.equal(k[0, at, :, 0], x[0]) and torch.equal(v[0, at, :, 0], x[1])
+        else:
+            reported(ctx, 1, "given twice")
+            alone = torch.tensor([i for i in range(n) if i not in (a, b)])
+            assert torch.equal(k[0, order[alone].long().cuda(), :, 0], x[0][alone.cuda()])
+    ctx.kv_drop(9997)
