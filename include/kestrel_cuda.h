@@ -427,6 +427,39 @@ KC_API int kc_load_gguf(kc_ctx* ctx, const char* path, int n_ctx, char* info_jso
    sizes and strides) into out (cap bytes). Errors: kc_last_error(NULL). */
 KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
 
+/* ---- rotary positions ------------------------------------------------------
+   kc_rope registers a rotation under an id >= 0 (host memory only; an id used
+   before is replaced). Of a head's first `dim` values (even, up to 256), pair i
+   at position p turns by the angle p w_i,
+     (a, b) -> gain (a cos - b sin, a sin + b cos),
+   pairs being (2i, 2i + 1) under KC_ROPE_INTERLEAVED and (i, i + dim / 2) under
+   KC_ROPE_HALF; the values behind them stay. w_i = base^(-2 i / dim), divided by
+   freq_factors[i] (host, [dim / 2], as a GGUF file's rope_freqs.weight; NULL: 1)
+   and scaled for contexts past the `original` one:
+     KC_ROPE_NONE    as it is (factor, original, low and high are not read)
+     KC_ROPE_LINEAR  w_i / factor
+     KC_ROPE_YARN    w_i (r / factor + 1 - r), r rising from 0 at pair
+                     max(0, floor(c(high))) to 1 at pair min(dim - 1, ceil(c(low)))
+                     with c(x) = dim ln(original / (2 pi x)) / (2 ln base): pairs
+                     that turn more than `high` times in the original context stay
+                     (usual: low 1, high 32)
+     KC_ROPE_BANDS   w_i (z + (1 - z) / factor), z = (original w_i / (2 pi) - low) /
+                     (high - low) within 0 .. 1 (usual: low 1, high 4)
+   gain 0 is the scaling's own: 1 + 0.1 ln(factor) under KC_ROPE_YARN, else 1.
+   Angles are exact to 2^-33 of a turn at every int32 position, negative ones
+   included; products are f32, each result rounded once.
+
+   kc_rope_dev: rows of n_head heads of head_dim (even; heads contiguous, strides
+   in elements; KC_F32, KC_F16 or KC_BF16) at positions[row] (device), to rows of
+   out, which is x with x's stride or shares nothing with it. Queries and keys
+   that lie side by side in a fused row are one call. */
+enum { KC_ROPE_INTERLEAVED = 0, KC_ROPE_HALF = 1 };
+enum { KC_ROPE_NONE = 0, KC_ROPE_LINEAR = 1, KC_ROPE_YARN = 2, KC_ROPE_BANDS = 3 };
+KC_API int kc_rope(kc_ctx* ctx, int rope, int dim, int layout, float base, int scaling, float factor, int original,
+                   float low, float high, float gain, const float* freq_factors);
+KC_API int kc_rope_dev(kc_ctx* ctx, int rope, const int32_t* positions, int n_rows, int n_head, int head_dim, int t,
+                       const void* x, int64_t x_stride, void* out, int64_t out_stride);
+
 /* ---- paged key-value cache and its attention ------------------------------
    No counterpart in Kestrel, whose Transformer holds one contiguous cache per
    sequence (transformer.rs:147-272). A cache is a pool of pages of `page`
@@ -468,6 +501,12 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
    strides in elements, heads contiguous; type KC_F32 or the cache's) become
    the last positions of sequence i in one layer; row_start NULL: one row each.
    Of a sequence given twice either entry's rows may be written; it is reported.
+   kc_kv_append_dev: kc_kv_write_dev with every key turned by its position in its
+   sequence (the rotation `rope` of kc_rope, whose dim is at most head_dim); the
+   values stay as they are. Queries beside them (n_head heads; 0: none) are turned
+   to the rows of q_out, which has their type t and is q with q's stride or shares
+   nothing with the rows of q, k and v. Of a row that is reported neither a key
+   nor a query is written (of a table entry outside the pool the query is).
    kc_kv_free_dev: forget positions from keep[i] on (NULL: all) and release the
    pages that hold none of the kept ones.
    kc_kv_compact_dev: live pages move to ids 0 .. live-1 (the i-th live page at
@@ -483,6 +522,9 @@ KC_API int kc_kv_fork_dev(kc_ctx* ctx, int cache, const int32_t* src, const int3
 KC_API int kc_kv_extend_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* n_new, int n);
 KC_API int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
                            int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride);
+KC_API int kc_kv_append_dev(kc_ctx* ctx, int cache, int layer, int rope, const int32_t* seqs, const int32_t* row_start,
+                            int n, int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                            int n_head, const void* q, int64_t q_stride, void* q_out, int64_t out_stride);
 KC_API int kc_kv_free_dev(kc_ctx* ctx, int cache, const int32_t* seqs, const int32_t* keep, int n);
 KC_API int kc_kv_compact_dev(kc_ctx* ctx, int cache, int32_t* n_live);
 KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, const int32_t* dst, int n);

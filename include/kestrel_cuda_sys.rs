@@ -86,6 +86,14 @@ pub const KC_N_STAGES: c_int = 11;
 pub const KC_OPT_F32_PREFILL: c_int = 1;
 pub const KC_OPT_LOOKAHEAD: c_int = 2;
 
+// rotary positions (kc_rope layout and scaling)
+pub const KC_ROPE_INTERLEAVED: c_int = 0;
+pub const KC_ROPE_HALF: c_int = 1;
+pub const KC_ROPE_NONE: c_int = 0;
+pub const KC_ROPE_LINEAR: c_int = 1;
+pub const KC_ROPE_YARN: c_int = 2;
+pub const KC_ROPE_BANDS: c_int = 3;
+
 // model architectures
 pub const KC_ARCH_LLAMA: c_int = 0;
 pub const KC_ARCH_QWEN2: c_int = 1;
@@ -199,6 +207,10 @@ unsafe extern "C" {
         cap: i64) -> c_int;
     pub fn kc_gguf_inspect(path: *const c_char, out: *mut c_char, cap: i64) -> c_int;
     // paged key-value cache and its attention (device buffers)
+    pub fn kc_rope(ctx: *mut kc_ctx, rope: c_int, dim: c_int, layout: c_int, base: f32, scaling: c_int, factor: f32,
+        original: c_int, low: f32, high: f32, gain: f32, freq_factors: *const f32) -> c_int;
+    pub fn kc_rope_dev(ctx: *mut kc_ctx, rope: c_int, positions: *const i32, n_rows: c_int, n_head: c_int,
+        head_dim: c_int, t: c_int, x: *const c_void, x_stride: i64, out: *mut c_void, out_stride: i64) -> c_int;
     pub fn kc_kv_cache(ctx: *mut kc_ctx, cache: c_int, t: c_int, n_layer: c_int, n_pages: c_int, page: c_int,
         n_head_kv: c_int, head_dim: c_int, n_seq: c_int, max_pages: c_int, k: *mut c_void, v: *mut c_void,
         table: *mut i32, len: *mut i32, refs: *mut i32) -> c_int;
@@ -209,6 +221,9 @@ unsafe extern "C" {
     pub fn kc_kv_write_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32, row_start: *const i32,
         n: c_int, n_rows: c_int, t: c_int, k: *const c_void, v: *const c_void, k_stride: i64,
         v_stride: i64) -> c_int;
+    pub fn kc_kv_append_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, rope: c_int, seqs: *const i32,
+        row_start: *const i32, n: c_int, n_rows: c_int, t: c_int, k: *const c_void, v: *const c_void, k_stride: i64,
+        v_stride: i64, n_head: c_int, q: *const c_void, q_stride: i64, q_out: *mut c_void, out_stride: i64) -> c_int;
     pub fn kc_kv_free_dev(ctx: *mut kc_ctx, cache: c_int, seqs: *const i32, keep: *const i32, n: c_int) -> c_int;
     pub fn kc_kv_compact_dev(ctx: *mut kc_ctx, cache: c_int, n_live: *mut i32) -> c_int;
     pub fn kc_kv_copy_pages_dev(ctx: *mut kc_ctx, cache: c_int, src: *const i32, dst: *const i32,

@@ -18,6 +18,7 @@
 #include "ep.h"
 #include "kernels.h"
 #include "kv.h"
+#include "rope.h"
 #include "mma.h"
 #include "loader.h"
 #include "model.h"
@@ -219,6 +220,7 @@ struct kc_ctx {
   EpBufs epb;
   Prof prof;
   KvState kv;  // registered paged caches (kc_kv_*)
+  std::map<int, RopeParams> ropes;  // registered rotations (kc_rope)
 };
 
 namespace {
@@ -3087,6 +3089,25 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
   });
 }
 
+// Whether rows of a and b (n_rows of `width` bytes, strides in bytes) share a
+// byte. (False answers are never wrong; true ones may be, of strides that differ.)
+bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b, int64_t b_stride, int64_t b_width,
+                  int n_rows) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  if (x + (n_rows - 1) * a_stride + a_width <= y || y + (n_rows - 1) * b_stride + b_width <= x) return false;
+  if (a_stride != b_stride) return true;
+  // Of one stride: the columns in turn.
+  const int64_t off = ((int64_t)(y - x) % a_stride + a_stride) % a_stride;
+  return off < a_width || off + b_width > a_stride;
+}
+
+int find_rope(kc_ctx* ctx, int rope, const char* what, const RopeParams** r) {
+  const auto it = ctx->ropes.find(rope);
+  if (it == ctx->ropes.end()) return fail(ctx, KC_ERR_STATE, "%s: rope %d not registered", what, rope);
+  *r = &it->second;
+  return KC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -3212,6 +3233,102 @@ int kc_kv_write_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, cons
     const size_t el = t == T_F32 ? 4 : 2;
     if ((uintptr_t)k % el || (uintptr_t)v % el) return fail(ctx, KC_ERR_ARG, "kc_kv_write: misaligned buffer");
     launch_kv_write(c, layer, seqs, row_start, n, n_rows, t, k, v, k_stride, v_stride, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_rope(kc_ctx* ctx, int rope, int dim, int layout, float base, int scaling, float factor, int original, float low,
+            float high, float gain, const float* freq_factors) {
+  return kv_guard(ctx, "kc_rope", [&]() -> int {
+    if (rope < 0) return fail(ctx, KC_ERR_ARG, "kc_rope: rope id %d", rope);
+    if (dim < 2 || dim > ROPE_MAX_DIM || dim % 2)
+      return fail(ctx, KC_ERR_SHAPE, "kc_rope: dim %d (even, 2 to %d)", dim, ROPE_MAX_DIM);
+    if (layout != KC_ROPE_INTERLEAVED && layout != KC_ROPE_HALF)
+      return fail(ctx, KC_ERR_ARG, "kc_rope: layout %d", layout);
+    if (scaling < ROPE_NONE || scaling > ROPE_BANDS) return fail(ctx, KC_ERR_ARG, "kc_rope: scaling %d", scaling);
+    const auto positive = [](float x) { return x > 0.f && x < INFINITY; };
+    if (!positive(base)) return fail(ctx, KC_ERR_ARG, "kc_rope: base %g", base);
+    if (scaling != ROPE_NONE && !positive(factor)) return fail(ctx, KC_ERR_ARG, "kc_rope: factor %g", factor);
+    if (scaling == ROPE_YARN || scaling == ROPE_BANDS) {
+      if (original < 1 || !positive(low) || !positive(high) || !(scaling == ROPE_YARN ? low <= high : low < high))
+        return fail(ctx, KC_ERR_ARG, "kc_rope: original context %d, low %g and high %g", original, low, high);
+      if (scaling == ROPE_YARN && base <= 1.f)
+        return fail(ctx, KC_ERR_ARG, "kc_rope: base %g (above 1 for YaRN)", base);
+    }
+    if (!(gain > -INFINITY && gain < INFINITY)) return fail(ctx, KC_ERR_ARG, "kc_rope: gain is not finite");
+    for (int i = 0; freq_factors && i < dim / 2; ++i)
+      if (!positive(freq_factors[i])) return fail(ctx, KC_ERR_ARG, "kc_rope: freq_factors[%d] is %g", i, freq_factors[i]);
+    ctx->ropes[rope] = make_rope(dim, layout == KC_ROPE_INTERLEAVED, base, scaling, factor, original, low, high, gain,
+                                 freq_factors);
+    return KC_OK;
+  });
+}
+
+int kc_rope_dev(kc_ctx* ctx, int rope, const int32_t* positions, int n_rows, int n_head, int head_dim, int t,
+                const void* x, int64_t x_stride, void* out, int64_t out_stride) {
+  return kv_guard(ctx, "kc_rope_dev", [&]() -> int {
+    const RopeParams* r;
+    RC(find_rope(ctx, rope, "kc_rope_dev", &r));
+    if (n_rows < 0) return fail(ctx, KC_ERR_ARG, "kc_rope_dev: n_rows=%d", n_rows);
+    if (t != T_F32 && t != T_F16 && t != T_BF16)
+      return fail(ctx, KC_ERR_TYPE, "kc_rope_dev: type %d (F32, F16 or BF16)", t);
+    if (n_head < 1 || head_dim < r->dim || head_dim % 2 || (int64_t)n_head * head_dim > INT32_MAX)
+      return fail(ctx, KC_ERR_SHAPE, "kc_rope_dev: %d heads of %d (even, at least the rope's %d)", n_head, head_dim,
+                  r->dim);
+    if (n_rows == 0) return KC_OK;
+    if (!positions || !x || !out) return fail(ctx, KC_ERR_ARG, "kc_rope_dev: null buffer");
+    const int64_t row = (int64_t)n_head * head_dim, el = t == T_F32 ? 4 : 2;
+    if (x_stride < row || out_stride < row)
+      return fail(ctx, KC_ERR_SHAPE, "kc_rope_dev: row strides %lld / %lld below n_head * head_dim",
+                  (long long)x_stride, (long long)out_stride);
+    if ((uintptr_t)x % el || (uintptr_t)out % el || (uintptr_t)positions % 4)
+      return fail(ctx, KC_ERR_ARG, "kc_rope_dev: misaligned buffer");
+    if (!(x == out && x_stride == out_stride) &&
+        rows_overlap(x, x_stride * el, row * el, out, out_stride * el, row * el, n_rows))
+      return fail(ctx, KC_ERR_ARG, "kc_rope_dev: out overlaps x without being x");
+    launch_rope(*r, positions, n_rows, n_head, head_dim, t, x, x_stride, out, out_stride, ctx->stream);
+    CKL();
+    return KC_OK;
+  });
+}
+
+int kc_kv_append_dev(kc_ctx* ctx, int cache, int layer, int rope, const int32_t* seqs, const int32_t* row_start, int n,
+                     int n_rows, int t, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int n_head,
+                     const void* q, int64_t q_stride, void* q_out, int64_t out_stride) {
+  return kv_call(ctx, cache, "kc_kv_append", [&](const KvCache& kv) -> int {
+    const KvView& c = kv.view;
+    const RopeParams* r;
+    RC(find_rope(ctx, rope, "kc_kv_append", &r));
+    if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "kc_kv_append: layer %d of %d", layer, c.n_layer);
+    if (n < 0 || n > c.n_seq || n_rows < 0 || (!row_start && n_rows != n))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_append: n=%d (of %d sequences), n_rows=%d", n, c.n_seq, n_rows);
+    if (t != T_F32 && t != c.type)
+      return fail(ctx, KC_ERR_TYPE, "kc_kv_append: rows of type %d into a cache of type %d (its type or F32)", t, c.type);
+    if (r->dim > c.hd)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: the rope turns %d values, a head has %d", r->dim, c.hd);
+    if (n_head < 0 || (int64_t)n_head * c.hd > INT32_MAX || (q && !n_head))
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: %d query heads", n_head);
+    if (n == 0 || n_rows == 0) return KC_OK;
+    if (!k || !v || (n_head && (!q || !q_out))) return fail(ctx, KC_ERR_ARG, "kc_kv_append: null buffer");
+    const int64_t row = (int64_t)c.nkv * c.hd, q_row = (int64_t)n_head * c.hd, el = t == T_F32 ? 4 : 2;
+    if (k_stride < row || v_stride < row)
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: row strides %lld / %lld below n_head_kv * head_dim",
+                  (long long)k_stride, (long long)v_stride);
+    if (n_head && (q_stride < q_row || out_stride < q_row))
+      return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: row strides %lld / %lld below n_head * head_dim",
+                  (long long)q_stride, (long long)out_stride);
+    if ((uintptr_t)k % el || (uintptr_t)v % el || (n_head && ((uintptr_t)q % el || (uintptr_t)q_out % el)))
+      return fail(ctx, KC_ERR_ARG, "kc_kv_append: misaligned buffer");
+    if (n_head) {
+      const auto over = [&](const void* x, int64_t stride, int64_t width) {
+        return rows_overlap(x, stride * el, width * el, q_out, out_stride * el, q_row * el, n_rows);
+      };
+      if ((!(q == q_out && q_stride == out_stride) && over(q, q_stride, q_row)) || over(k, k_stride, row) ||
+          over(v, v_stride, row))
+        return fail(ctx, KC_ERR_ARG, "kc_kv_append: q_out overlaps k, v, or q without being q");
+    }
+    const AppendArgs a{c, layer, seqs, row_start, n, n_rows, n_head, q, k, v, q_out, q_stride, k_stride, v_stride, out_stride};
+    launch_kv_append(a, *r, t, ctx->stream);
     return KC_OK;
   });
 }

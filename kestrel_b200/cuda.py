@@ -75,11 +75,14 @@ SIGNATURES = {
     "kc_expert_prefetch": (I, [P, I, P, I]),
     "kc_expert_cache_stats": (I, [P, P, I]),
     "kc_expert_cache_decay": (I, [P]),
+    "kc_rope": (I, [P, I, I, I, F, I, F, I, F, F, F, P]),
+    "kc_rope_dev": (I, [P, I, P, I, I, I, I, P, I64, P, I64]),
     "kc_kv_cache": (I, [P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]),
     "kc_kv_drop": (I, [P, I]),
     "kc_kv_fork_dev": (I, [P, I, P, P, I]),
     "kc_kv_extend_dev": (I, [P, I, P, P, I]),
     "kc_kv_write_dev": (I, [P, I, I, P, P, I, I, I, P, P, I64, I64]),
+    "kc_kv_append_dev": (I, [P, I, I, I, P, P, I, I, I, P, P, I64, I64, I, P, I64, P, I64]),
     "kc_kv_free_dev": (I, [P, I, P, P, I]),
     "kc_kv_compact_dev": (I, [P, I, P]),
     "kc_kv_copy_pages_dev": (I, [P, I, P, P, I]),
@@ -96,6 +99,9 @@ XS_COUNTERS = ["capacity", "cached", "requests", "hits", "late", "misses", "scra
                "prefetch_issued", "prefetch_used", "prefetch_wasted", "evictions", "lookahead_predicted",
                "lookahead_correct", "reads", "forced", "scratch", "spec", "spec_pauses"]
 ARCH_LLAMA, ARCH_QWEN2, ARCH_QWEN3 = 0, 1, 2
+# Rotary positions (kc_rope).
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2, "bands": 3}
 (T_ATTN_NORM, T_ATTN_Q, T_ATTN_K, T_ATTN_V, T_ATTN_OUT, T_ATTN_Q_BIAS, T_ATTN_K_BIAS, T_ATTN_V_BIAS,
  T_ATTN_Q_NORM, T_ATTN_K_NORM, T_FFN_NORM, T_FFN_GATE, T_FFN_UP, T_FFN_DOWN) = range(14)
 T_TOKEN_EMBD, T_OUTPUT_NORM, T_OUTPUT = 0, 1, 2
@@ -469,6 +475,33 @@ class Context:
         self._n_vocab = int(info.get("n_vocab", getattr(self, "_n_vocab", 0)))
         return info
 
+    # ---- rotary positions --------------------------------------------------------
+    def rope(self, rope: int, dim: int, layout: str = "half", base: float = 10000.0, scaling: str = "none",
+             factor: float = 1.0, original: int = 0, low: float = 0.0, high: float = 0.0, gain: float = 0.0,
+             freq_factors=None):
+        """Register a rotation of the first `dim` values of a head under an id:
+        layout "half" or "interleaved", scaling "none", "linear", "yarn" or
+        "bands" (formulas: kc_rope in include/kestrel_cuda.h); freq_factors:
+        dim / 2 host values that divide the frequencies."""
+        if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+            raise ValueError(f"layout is one of {list(ROPE_LAYOUTS)}, scaling of {list(ROPE_SCALINGS)}")
+        ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, dtype=np.float32)
+        if ff is not None and ff.size != dim // 2:
+            raise ValueError(f"freq_factors holds {ff.size} values, {dim // 2} needed")
+        self._check(lib().kc_rope(self.h, rope, dim, ROPE_LAYOUTS[layout], base, ROPE_SCALINGS[scaling], factor,
+                                  original, low, high, gain, _ptr(ff)))
+
+    def rope_dev(self, rope: int, x, positions, out=None):
+        """Rows x [rows, heads, head_dim] turned by positions [rows] (int32 CUDA
+        tensor), to out (None: in place)."""
+        out = x if out is None else out
+        xs, os_ = _dev_rows("x", x), _dev_rows("out", out)
+        rows, nh, hd = x.shape
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must have x's shape and type")
+        self._check(lib().kc_rope_dev(self.h, rope, _dev_ints("positions", positions, rows), rows, nh, hd,
+                                      _float_type("x", x), x.data_ptr(), xs, out.data_ptr(), os_))
+
     # ---- paged key-value cache (torch CUDA tensors) ------------------------------
     def kv_cache(self, cache: int, k, v, table, length, refs):
         """Register the caller's tensors as paged cache `cache`: k and v
@@ -523,6 +556,30 @@ class Context:
         self._check(lib().kc_kv_write_dev(self.h, cache, layer, _dev_ints("seqs", seqs, n),
                                           _dev_ints("row_start", row_start), n, rows, _float_type("k", k),
                                           k.data_ptr(), v.data_ptr(), ks, vs))
+
+    def kv_append_dev(self, cache: int, layer: int, rope: int, k, v, q=None, q_out=None, seqs=None, row_start=None):
+        """kv_write_dev with the keys turned by their positions (a rotation that
+        `rope` registered); q [rows, n_head, head_dim], if given, is turned to
+        q_out (None: in place)."""
+        _, n_kv, hd = self._kv_shape(cache)
+        ks, vs = _dev_rows("k", k, n_kv, hd), _dev_rows("v", v, n_kv, hd)
+        rows = k.shape[0]
+        if v.shape[0] != rows or v.dtype != k.dtype:
+            raise ValueError("k and v differ in rows or type")
+        n = rows if row_start is None else row_start.numel() - 1
+        nh = qs = os_ = 0
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            qs, os_ = _dev_rows("q", q, None, hd), _dev_rows("q_out", q_out, None, hd)
+            nh = q.shape[1]
+            if q.shape[0] != rows or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != q.dtype:
+                raise ValueError("q and q_out must have k's rows and type, and each other's shape")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        self._check(lib().kc_kv_append_dev(self.h, cache, layer, rope, _dev_ints("seqs", seqs, n),
+                                           _dev_ints("row_start", row_start), n, rows, _float_type("k", k),
+                                           k.data_ptr(), v.data_ptr(), ks, vs, nh, q.data_ptr() if nh else None, qs,
+                                           q_out.data_ptr() if nh else None, os_))
 
     def kv_free_dev(self, cache: int, seqs=None, keep=None):
         """Forget positions keep[i] and on (None: all) of each of `seqs` (None:
