@@ -3272,7 +3272,7 @@ int kc_rope_dev(kc_ctx* ctx, int rope, const int32_t* positions, int n_rows, int
     if (n_rows < 0) return fail(ctx, KC_ERR_ARG, "kc_rope_dev: n_rows=%d", n_rows);
     if (t != T_F32 && t != T_F16 && t != T_BF16)
       return fail(ctx, KC_ERR_TYPE, "kc_rope_dev: type %d (F32, F16 or BF16)", t);
-    if (n_head < 1 || head_dim < r->dim || head_dim % 2 || (int64_t)n_head * head_dim > INT32_MAX)
+    if (n_head < 1 || head_dim < r->dim || head_dim % 2 || (int64_t)n_head * head_dim > 1 << 24)
       return fail(ctx, KC_ERR_SHAPE, "kc_rope_dev: %d heads of %d (even, at least the rope's %d)", n_head, head_dim,
                   r->dim);
     if (n_rows == 0) return KC_OK;
@@ -3306,7 +3306,7 @@ int kc_kv_append_dev(kc_ctx* ctx, int cache, int layer, int rope, const int32_t*
       return fail(ctx, KC_ERR_TYPE, "kc_kv_append: rows of type %d into a cache of type %d (its type or F32)", t, c.type);
     if (r->dim > c.hd)
       return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: the rope turns %d values, a head has %d", r->dim, c.hd);
-    if (n_head < 0 || (int64_t)n_head * c.hd > INT32_MAX || (q && !n_head))
+    if (n_head < 0 || (int64_t)n_head * c.hd > 1 << 24 || (q && !n_head))
       return fail(ctx, KC_ERR_SHAPE, "kc_kv_append: %d query heads", n_head);
     if (n == 0 || n_rows == 0) return KC_OK;
     if (!k || !v || (n_head && (!q || !q_out))) return fail(ctx, KC_ERR_ARG, "kc_kv_append: null buffer");

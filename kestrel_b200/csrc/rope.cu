@@ -8,15 +8,24 @@
 // point. The quadrant is its top two bits; what is left, within an eighth of a
 // turn either way, goes to sincospif, good to its last bits.
 //
-// Both calls are bound by the memory rate (3 operations a value). A thread takes
-// the same columns of several heads of a row, so that their cos and sin are
-// computed once for all of these: 8 columns (16 bytes of 16-bit values) at a time
-// where dim and head_dim allow it, in both halves if those are paired.
+// Both calls are bound by the memory rate (3 operations a value). A block takes a
+// few rows: it looks up where each stands and goes, computes the rows' cos and sin
+// once into shared memory, and then streams through their heads, 16 bytes of
+// 16-bit values a thread at a time (32 of f32) where dim and head_dim allow it, in
+// both halves if those are paired. A thread's first loads go out before all that,
+// the next ones before the last are turned.
+//
+// Measured on a B200 (plain copy 6.56 TB/s): 8192 rows of 36 heads of 128, bf16,
+// 151 MB in 37.3 us (4.0 TB/s); 24 x 256 rows of 32 and 4 heads of 128, f32 into
+// an f16 cache, 239 MB in 45.0 us (5.3). Angles by each thread for up to eight
+// heads of its own took 43.6 and 66.8 us, places by division instead of steps 46.4
+// and 47.7.
 #include <math.h>
 
 #include <algorithm>
 #include <type_traits>
 
+#include "attn_dev.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "kv.h"
@@ -28,6 +37,8 @@
 namespace kc {
 
 constexpr int ROPE_THREADS = 128;
+constexpr int ROPE_ROWS = 8;                 // rows of a block, at most
+constexpr int ROPE_PAIRS = ROPE_ROWS * 64;   // and their angles
 
 RopeParams make_rope(int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
                      float high, float gain, const float* freq_factors) {
@@ -71,206 +82,259 @@ __device__ __forceinline__ float2 cos_sin(uint64_t phase, float gain) {
   return make_float2((quarter + 1) & 2 ? -x * gain : x * gain, quarter & 2 ? -y * gain : y * gain);
 }
 
+// VEC values as they are in memory.
 template <int VEC, typename S>
-__device__ __forceinline__ void load_vec(const S* p, float (&v)[VEC], bool aligned) {
-  alignas(16) S in[VEC];
+struct alignas(VEC * sizeof(S) < 16 ? VEC * sizeof(S) : 16) Raw {
+  S v[VEC];
+};
+template <int VEC, typename S>
+__device__ __forceinline__ Raw<VEC, S> load_vec(const S* p, bool aligned) {
+  Raw<VEC, S> r;
   constexpr int BYTES = VEC * sizeof(S);
-  if (aligned && BYTES >= 4) {
+  if (aligned) {
     if constexpr (BYTES >= 16) {
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(in)[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(in) = *reinterpret_cast<const uint2*>(p);
-    } else if constexpr (BYTES == 4) {
-      *reinterpret_cast<uint32_t*>(in) = *reinterpret_cast<const uint32_t*>(p);
+      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      r = *reinterpret_cast<const Raw<VEC, S>*>(p);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) in[i] = p[i];
+    for (int i = 0; i < VEC; ++i) r.v[i] = p[i];
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = (float)in[i];
+  return r;
 }
 template <int VEC, typename D>
 __device__ __forceinline__ void store_vec(D* p, const float (&v)[VEC], bool aligned) {
-  alignas(16) D o[VEC];
+  Raw<VEC, D> r;
+  if constexpr (sizeof(D) == 2 && VEC > 1) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) o[i] = (D)v[i];
+    for (int i = 0; i < VEC / 2; ++i) reinterpret_cast<uint32_t*>(&r)[i] = pack2<D>(v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = (D)v[i];
+  }
   constexpr int BYTES = VEC * sizeof(D);
-  if (aligned && BYTES >= 4) {
+  if (aligned) {
     if constexpr (BYTES >= 16) {
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(o)[i];
-    } else if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(o);
-    } else if constexpr (BYTES == 4) {
-      *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(o);
+      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&r)[i];
+    } else {
+      *reinterpret_cast<Raw<VEC, D>*>(p) = r;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = o[i];
+    for (int i = 0; i < VEC; ++i) p[i] = r.v[i];
   }
 }
 
-// What a thread has of each head of its chunk: VEC columns from `col` on, and if
-// halves are paired VEC more from col2 on (-1: none), turned or as they are.
+// What a thread has of a head: VEC columns from `col` on, and if halves are paired
+// VEC more from col + dim / 2 on. Lanes of a head: those that turn, then those of
+// the columns behind.
 template <int VEC, bool HALF>
 struct RopeLane {
-  static constexpr int ANGLES = HALF ? VEC : (VEC + 1) / 2;
-  int col, col2;
-  bool turns;
-  float2 cs[ANGLES];
-
-  // Lanes of a head: those that turn, then those of the columns behind.
+  int col, first;  // first: the pair whose angle the first column has; -1: none
   static __host__ __device__ int turning(int dim) { return HALF ? dim / 2 / VEC : dim / VEC; }
   static __host__ __device__ int count(int dim, int hd) { return turning(dim) + (hd - dim) / VEC; }
-
-  __device__ __forceinline__ void place(int lane, int dim) {
+  __device__ __forceinline__ RopeLane(int lane, int dim) {
     const int t = turning(dim);
-    turns = lane < t;
-    col = turns ? lane * VEC : dim + (lane - t) * VEC;
-    col2 = HALF && turns ? dim / 2 + lane * VEC : -1;
-  }
-  __device__ __forceinline__ void angles(const RopeParams& r, int position) {
-    const int first = HALF ? col : col / 2;
-#pragma unroll
-    for (int i = 0; i < ANGLES; ++i) cs[i] = cos_sin((uint64_t)(int64_t)position * r.turn[first + i], r.gain);
-  }
-  template <typename S>
-  __device__ __forceinline__ void load(const S* head, float (&x)[VEC], float (&y)[VEC], bool aligned) const {
-    load_vec<VEC>(head + col, x, aligned);
-    if (HALF && col2 >= 0) load_vec<VEC>(head + col2, y, aligned);
-  }
-  __device__ __forceinline__ void turn(float (&x)[VEC], float (&y)[VEC]) const {
-    if constexpr (HALF) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float a = x[i], b = y[i];
-        x[i] = __fmaf_rn(a, cs[i].x, -(b * cs[i].y));
-        y[i] = __fmaf_rn(a, cs[i].y, b * cs[i].x);
-      }
-    } else if constexpr (VEC > 1) {
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2) {
-        const float a = x[i], b = x[i + 1];
-        x[i] = __fmaf_rn(a, cs[i / 2].x, -(b * cs[i / 2].y));
-        x[i + 1] = __fmaf_rn(a, cs[i / 2].y, b * cs[i / 2].x);
-      }
-    }
-  }
-  template <typename D>
-  __device__ __forceinline__ void store(D* head, const float (&x)[VEC], const float (&y)[VEC], bool aligned) const {
-    store_vec<VEC>(head + col, x, aligned);
-    if (HALF && col2 >= 0) store_vec<VEC>(head + col2, y, aligned);
+    col = lane < t ? lane * VEC : dim + (lane - t) * VEC;
+    first = lane < t ? (HALF ? col : col / 2) : -1;
   }
 };
 
-// `heads` heads from head(0), head(1) .. to to(0), to(1) ..: loads of two at once.
-template <int VEC, bool HALF, typename Head, typename To>
-__device__ __forceinline__ void rope_heads(const RopeLane<VEC, HALF>& lane, int heads, bool turns, bool in_aligned,
-                                           bool out_aligned, Head head, To to) {
-  for (int h = 0; h < heads; h += 2) {
-    float x[2][VEC], y[2][VEC];
+// One thread's values of a head, as they are in memory.
+template <int VEC, bool HALF, typename S>
+struct RopeValues {
+  Raw<VEC, S> x, y;
+  __device__ __forceinline__ void load(const S* head, const RopeLane<VEC, HALF>& l, int half, bool aligned) {
+    x = load_vec<VEC>(head + l.col, aligned);
+    if (HALF && l.first >= 0) y = load_vec<VEC>(head + l.col + half, aligned);
+  }
+  // cos, sin: of the row's pairs.
+  template <typename D>
+  __device__ __forceinline__ void put(D* head, const RopeLane<VEC, HALF>& l, int half, bool turns, const float* cos,
+                                      const float* sin, bool aligned) const {
+    float a[VEC], b[VEC];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (h + u < heads) lane.load(head(h + u), x[u], y[u], in_aligned);
+    for (int i = 0; i < VEC; ++i) {
+      a[i] = (float)x.v[i];
+      b[i] = HALF ? (float)y.v[i] : 0.f;
+    }
+    if (turns) {
+      if constexpr (HALF) {
+        const Raw<VEC, float> c = load_vec<VEC>(cos + l.first, true), s = load_vec<VEC>(sin + l.first, true);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (h + u < heads) {
-        if (turns) lane.turn(x[u], y[u]);
-        lane.store(to(h + u), x[u], y[u], out_aligned);
+        for (int i = 0; i < VEC; ++i) {
+          const float p = a[i], q = b[i];
+          a[i] = __fmaf_rn(p, c.v[i], -(q * s.v[i]));
+          b[i] = __fmaf_rn(p, s.v[i], q * c.v[i]);
+        }
+      } else {
+        const Raw<VEC / 2, float> c = load_vec<VEC / 2>(cos + l.first, true), s = load_vec<VEC / 2>(sin + l.first, true);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          const float p = a[i], q = a[i + 1];
+          a[i] = __fmaf_rn(p, c.v[i / 2], -(q * s.v[i / 2]));
+          a[i + 1] = __fmaf_rn(p, s.v[i / 2], q * c.v[i / 2]);
+        }
       }
+    }
+    store_vec<VEC>(head + l.col, a, aligned);
+    if (HALF && l.first >= 0) store_vec<VEC>(head + l.col + half, b, aligned);
+  }
+};
+
+// A launch's rows and how they are cut: `rows` rows a block, a row's heads into
+// `cuts` blocks.
+struct RopeCut {
+  int rows, cuts;
+};
+
+// The block's work: heads h0 .. h1-1 of rows r0 .. r1-1, angles by `angles`, from
+// from(row, head) by put(row, head, values, lane).
+template <int VEC, bool HALF, typename S, class From, class Angles, class Put>
+__device__ __forceinline__ void rope_block(int dim, int hd, int rows, int h0, int h1, bool aligned, From from,
+                                           Angles angles, Put put) {
+  const int lanes = RopeLane<VEC, HALF>::count(dim, hd), heads = h1 - h0, half = dim / 2;
+  // A thread's place, and how far the next one is: steps with carries, since
+  // divisions would take longer than the rotation.
+  const uint32_t part = threadIdx.x / (uint32_t)lanes, step = ROPE_THREADS / (uint32_t)lanes;
+  int l = threadIdx.x - part * lanes, row = part / (uint32_t)heads, h = part - row * heads;
+  const int dl = ROPE_THREADS - step * lanes, dr = step / (uint32_t)heads, dh = step - dr * heads;
+  RopeValues<VEC, HALF, S> now;
+  if (row < rows) now.load(from(row, h0 + h), RopeLane<VEC, HALF>(l, dim), half, aligned);
+  angles();
+  while (row < rows) {
+    const int row0 = row, head0 = h0 + h;
+    const RopeLane<VEC, HALF> lane(l, dim);
+    l += dl;
+    h += dh;
+    row += dr;
+    if (l >= lanes) {
+      l -= lanes;
+      ++h;
+    }
+    if (h >= heads) {
+      h -= heads;
+      ++row;
+    }
+    RopeValues<VEC, HALF, S> next;
+    if (row < rows) next.load(from(row, h0 + h), RopeLane<VEC, HALF>(l, dim), half, aligned);
+    put(row0, head0, now, lane);
+    now = next;
+  }
+}
+
+// cos and sin of the block's rows into shared memory: [rows][dim / 2] each.
+template <class Position>
+__device__ __forceinline__ void rope_angles(const RopeParams& r, int rows, float* cos, float* sin, Position position) {
+  const int half = r.dim / 2;
+  for (int x = threadIdx.x; x < rows * half; x += ROPE_THREADS) {
+    const int row = (uint32_t)x / (uint32_t)half;
+    const float2 cs = cos_sin((uint64_t)(int64_t)position(row) * r.turn[x - row * half], r.gain);
+    cos[x] = cs.x;
+    sin[x] = cs.y;
   }
 }
 
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ RopeParams r,
                                                             const int32_t* positions, int n_rows, int n_head, int hd,
-                                                            int chunk, const T* x, int64_t xs, T* out, int64_t os,
+                                                            RopeCut cut, const T* x, int64_t xs, T* out, int64_t os,
                                                             bool x_aligned, bool out_aligned) {
+  __shared__ __align__(16) float cos_sh[ROPE_PAIRS], sin_sh[ROPE_PAIRS];
   pdl_enter();
-  const int lanes = RopeLane<VEC, HALF>::count(r.dim, hd), chunks = (n_head + chunk - 1) / chunk;
-  const int64_t all = (int64_t)n_rows * chunks * lanes;
-  for (int64_t i = (int64_t)blockIdx.x * ROPE_THREADS + threadIdx.x; i < all; i += (int64_t)gridDim.x * ROPE_THREADS) {
-    const int64_t part = i / lanes;
-    const int row = (int)(part / chunks), h0 = (int)(part - (int64_t)row * chunks) * chunk;
-    RopeLane<VEC, HALF> lane;
-    lane.place((int)(i - part * lanes), r.dim);
-    if (lane.turns) lane.angles(r, positions[row]);
-    const T* from = x + row * xs + (int64_t)h0 * hd;
-    T* to = out + row * os + (int64_t)h0 * hd;
-    rope_heads(lane, min(chunk, n_head - h0), lane.turns, x_aligned, out_aligned,
-               [&](int h) { return from + (int64_t)h * hd; }, [&](int h) { return to + (int64_t)h * hd; });
-  }
+  const int half = r.dim / 2, h0 = (int)((int64_t)n_head * blockIdx.y / cut.cuts),
+            h1 = (int)((int64_t)n_head * (blockIdx.y + 1) / cut.cuts);
+  const int64_t r0 = (int64_t)blockIdx.x * cut.rows;
+  const int rows = (int)min((int64_t)cut.rows, n_rows - r0);
+  rope_block<VEC, HALF, T>(
+      r.dim, hd, rows, h0, h1, x_aligned, [&](int row, int h) { return x + (r0 + row) * xs + (int64_t)h * hd; },
+      [&] {
+        rope_angles(r, rows, cos_sh, sin_sh, [&](int row) { return positions[r0 + row]; });
+        __syncthreads();
+      },
+      [&](int row, int h, const RopeValues<VEC, HALF, T>& v, const RopeLane<VEC, HALF>& l) {
+        v.put(out + (r0 + row) * os + (int64_t)h * hd, l, half, l.first >= 0, cos_sh + row * half, sin_sh + row * half,
+              out_aligned);
+      });
 }
 
 // Rows of k and v into the pages as kv_write_kernel puts them (kv.cu), the keys
 // turned by their positions, and the queries beside them to rows of their own.
-// Chunks of a row: the queries' heads, the keys', the values'.
+// Heads of a row: the queries', the keys', the values'.
 template <typename S, typename D, int VEC, bool HALF>
 __global__ void __launch_bounds__(ROPE_THREADS) kv_append_kernel(const AppendArgs a,
-                                                                 const __grid_constant__ RopeParams r, int chunk,
+                                                                 const __grid_constant__ RopeParams r, RopeCut cut,
                                                                  bool in_aligned, bool out_aligned, int blocks) {
+  __shared__ __align__(16) float cos_sh[ROPE_PAIRS], sin_sh[ROPE_PAIRS];
+  __shared__ int pos_sh[ROPE_ROWS], page_sh[ROPE_ROWS];  // a row's position and page; -1: none
   pdl_enter();
   const KvView& c = a.c;
   if (blockIdx.x >= blocks) {
-    kv_report_repeats<ROPE_THREADS>(c, a.seqs, a.n);
+    if (blockIdx.y == 0) kv_report_repeats<ROPE_THREADS>(c, a.seqs, a.n);
     return;
   }
-  const int lanes = RopeLane<VEC, HALF>::count(r.dim, c.hd);
-  const int of_q = (a.nh + chunk - 1) / chunk, of_k = (c.nkv + chunk - 1) / chunk, chunks = of_q + 2 * of_k;
-  const int64_t all = (int64_t)a.n_rows * chunks * lanes;
-  for (int64_t x = (int64_t)blockIdx.x * ROPE_THREADS + threadIdx.x; x < all; x += (int64_t)blocks * ROPE_THREADS) {
-    const int64_t part = x / lanes;
-    const int row = (int)(part / chunks), l = (int)(x - part * lanes);
-    int at = (int)(part - (int64_t)row * chunks);
-    const bool tell = at == chunks - 1 && l == 0;  // (one thread a row reports)
-    int i = row, back = 1;  // the row is `back` positions from its sequence's end
-    if (a.row_start) {
-      i = kv_row_owner(a.row_start, a.n, row);
-      if (i < 0) {
-        if (tell) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
-        continue;
-      }
-      back = a.row_start[i + 1] - row;
-    }
-    const int s = a.seqs ? a.seqs[i] : i;
-    if (s < 0 || s >= c.n_seq) {
-      if (tell) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
-      continue;
-    }
-    const int pos = kv_len(c, s) - back;
-    if (pos < 0) {
-      if (tell) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
-      continue;
-    }
-    RopeLane<VEC, HALF> lane;
-    lane.place(l, r.dim);
-    const bool is_v = at >= of_q + of_k, turns = lane.turns && !is_v;
-    if (turns) lane.angles(r, pos);
-    if (at < of_q) {
-      const int h0 = at * chunk;
-      const S* from = static_cast<const S*>(a.q) + row * a.q_stride + (int64_t)h0 * c.hd;
-      S* to = static_cast<S*>(a.q_out) + row * a.out_stride + (int64_t)h0 * c.hd;
-      rope_heads(lane, min(chunk, a.nh - h0), turns, in_aligned, out_aligned,
-                 [&](int h) { return from + (int64_t)h * c.hd; }, [&](int h) { return to + (int64_t)h * c.hd; });
-      continue;
-    }
-    const int id = c.table[(int64_t)s * c.max_pages + (pos >> c.page_log2)];
-    if (id < 0 || id >= c.n_pages) {
-      if (tell) report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
-      continue;
-    }
-    at -= is_v ? of_q + of_k : of_q;
-    const int h0 = at * chunk;
-    const S* from = (is_v ? static_cast<const S*>(a.v) + row * a.v_stride : static_cast<const S*>(a.k) + row * a.k_stride) +
-                    (int64_t)h0 * c.hd;
-    const int64_t step = (int64_t)c.page * c.hd;  // from a head's row to the next one's
-    D* to = reinterpret_cast<D*>(is_v ? c.v : c.k) + (((int64_t)a.layer * c.n_pages + id) * c.nkv + h0) * step +
-            (int64_t)(pos & (c.page - 1)) * c.hd;
-    rope_heads(lane, min(chunk, c.nkv - h0), turns, in_aligned, true,
-               [&](int h) { return from + (int64_t)h * c.hd; }, [&](int h) { return to + h * step; });
-  }
+  const int half = r.dim / 2, heads = a.nh + 2 * c.nkv, h0 = (int)((int64_t)heads * blockIdx.y / cut.cuts),
+            h1 = (int)((int64_t)heads * (blockIdx.y + 1) / cut.cuts);
+  const int64_t r0 = (int64_t)blockIdx.x * cut.rows;
+  const int rows = (int)min((int64_t)cut.rows, a.n_rows - r0);
+  rope_block<VEC, HALF, S>(
+      r.dim, c.hd, rows, h0, h1, in_aligned,
+      [&](int row, int h) {
+        const int64_t at = r0 + row;
+        if (h < a.nh) return static_cast<const S*>(a.q) + at * a.q_stride + (int64_t)h * c.hd;
+        if (h < a.nh + c.nkv) return static_cast<const S*>(a.k) + at * a.k_stride + (int64_t)(h - a.nh) * c.hd;
+        return static_cast<const S*>(a.v) + at * a.v_stride + (int64_t)(h - a.nh - c.nkv) * c.hd;
+      },
+      [&] {
+        if (threadIdx.x < rows) {
+          const int row = (int)r0 + threadIdx.x;
+          int i = row, back = 1, wrong = 0, pos = -1, id = -1;  // the row is `back` positions from its sequence's end
+          if (a.row_start) {
+            i = kv_row_owner(a.row_start, a.n, row);
+            if (i < 0) wrong = W_KV_ROWS;
+            else back = a.row_start[i + 1] - row;
+          }
+          const int s = wrong ? -1 : a.seqs ? a.seqs[i] : i;
+          if (!wrong && (s < 0 || s >= c.n_seq)) wrong = W_KV_SEQ;
+          if (!wrong) {
+            pos = kv_len(c, s) - back;
+            if (pos < 0) {
+              pos = -1;
+              wrong = W_KV_ROWS;
+            } else {
+              id = c.table[(int64_t)s * c.max_pages + (pos >> c.page_log2)];
+              if (id < 0 || id >= c.n_pages) {
+                id = -1;
+                wrong = W_KV_PAGE;
+              }
+            }
+          }
+          if (wrong && blockIdx.y == 0) report(c.status, KC_ERR_ARG | (wrong << 8));
+          pos_sh[threadIdx.x] = pos;
+          page_sh[threadIdx.x] = id;
+        }
+        __syncthreads();
+        rope_angles(r, rows, cos_sh, sin_sh, [&](int row) { return pos_sh[row]; });
+        __syncthreads();
+      },
+      [&](int row, int h, const RopeValues<VEC, HALF, S>& v, const RopeLane<VEC, HALF>& l) {
+        const float *cos = cos_sh + row * half, *sin = sin_sh + row * half;
+        const int pos = pos_sh[row], id = page_sh[row];
+        if (h < a.nh) {
+          if (pos >= 0)
+            v.put(static_cast<S*>(a.q_out) + (r0 + row) * a.out_stride + (int64_t)h * c.hd, l, half, l.first >= 0, cos,
+                  sin, out_aligned);
+          return;
+        }
+        if (id < 0) return;
+        const bool is_v = h >= a.nh + c.nkv;
+        D* pool = reinterpret_cast<D*>(is_v ? c.v : c.k);
+        const int64_t head = ((int64_t)a.layer * c.n_pages + id) * c.nkv + (h - a.nh - (is_v ? c.nkv : 0));
+        v.put(pool + (head * c.page + (pos & (c.page - 1))) * c.hd, l, half, l.first >= 0 && !is_v, cos, sin, true);
+      });
 }
 
 // Columns a thread takes at a time.
@@ -279,12 +343,18 @@ static int rope_vec(const RopeParams& r, int hd) {
   return unit % 8 == 0 && (hd - r.dim) % 8 == 0 ? 8 : unit % 2 == 0 ? 2 : 1;
 }
 
-// Heads of a thread: more where there are threads enough without, since their
-// angles are computed once.
-static int rope_chunk(int64_t threads, int most) {
-  int chunk = 1;
-  while (chunk < most && chunk < 8 && threads / (2 * chunk) >= (int64_t)num_sms() * 1024) chunk *= 2;
-  return chunk;
+// Rows a block takes: up to six loads a thread, while that leaves two blocks an SM
+// (8192 rows of 36 heads of 128, bf16: one row 39.8 us, two 37.3, four 42.2, eight
+// 45.8; 24 x 256 rows of 32 and 4 heads, f32 to f16: 47.1, 45.0, 51.2 and 51.1); a
+// row's heads over several blocks where there are fewer rows than SMs.
+static RopeCut rope_cut(int n_rows, int heads, int lanes, int dim) {
+  const int per = heads * lanes, sms = num_sms();  // (a row has at most 2^24 values)
+  RopeCut c{1, 1};
+  while (2 * c.rows <= ROPE_ROWS && 2 * c.rows * (dim / 2) <= ROPE_PAIRS && 2 * c.rows * per <= 6 * ROPE_THREADS &&
+         n_rows / (2 * c.rows) >= 2 * sms)
+    c.rows *= 2;
+  if (n_rows < sms) c.cuts = std::max(1, std::min({sms / n_rows, per / ROPE_THREADS, heads}));
+  return c;
 }
 static bool rows_aligned(const void* p, int64_t stride, int hd, size_t el, int vec) {
   const size_t bytes = std::min<size_t>(16, vec * el);
@@ -294,13 +364,10 @@ static bool rows_aligned(const void* p, int64_t stride, int hd, size_t el, int v
 template <int VEC, bool HALF, typename T>
 static void rope_run(const RopeParams& r, const int32_t* positions, int n_rows, int n_head, int hd, const void* x,
                      int64_t xs, void* out, int64_t os, cudaStream_t st) {
-  const int lanes = RopeLane<VEC, HALF>::count(r.dim, hd);
-  const int chunk = rope_chunk((int64_t)n_rows * n_head * lanes, n_head);
-  const int64_t all = (int64_t)n_rows * ((n_head + chunk - 1) / chunk) * lanes;
-  const int grid = (int)std::min<int64_t>((all + ROPE_THREADS - 1) / ROPE_THREADS, 32 * (int64_t)num_sms());
-  launch_k(rope_kernel<T, VEC, HALF>, grid, ROPE_THREADS, 0, st, r, positions, n_rows, n_head, hd, chunk,
-           static_cast<const T*>(x), xs, static_cast<T*>(out), os, rows_aligned(x, xs, hd, sizeof(T), VEC),
-           rows_aligned(out, os, hd, sizeof(T), VEC));
+  const RopeCut cut = rope_cut(n_rows, n_head, RopeLane<VEC, HALF>::count(r.dim, hd), r.dim);
+  launch_k(rope_kernel<T, VEC, HALF>, dim3((n_rows + cut.rows - 1) / cut.rows, cut.cuts), ROPE_THREADS, 0, st, r,
+           positions, n_rows, n_head, hd, cut, static_cast<const T*>(x), xs, static_cast<T*>(out), os,
+           rows_aligned(x, xs, hd, sizeof(T), VEC), rows_aligned(out, os, hd, sizeof(T), VEC));
 }
 
 // fn<VEC, HALF>() for a rotation and head size. (Interleaved pairs are at least
@@ -334,15 +401,12 @@ void launch_rope(const RopeParams& r, const int32_t* positions, int n_rows, int 
 template <int VEC, bool HALF, typename S, typename D>
 static void append_run(const AppendArgs& a, const RopeParams& r, cudaStream_t st) {
   const KvView& c = a.c;
-  const int lanes = RopeLane<VEC, HALF>::count(r.dim, c.hd);
-  const int chunk = rope_chunk((int64_t)a.n_rows * (a.nh + 2 * c.nkv) * lanes, c.nkv);
-  const int chunks = (a.nh + chunk - 1) / chunk + 2 * ((c.nkv + chunk - 1) / chunk);
-  const int64_t all = (int64_t)a.n_rows * chunks * lanes;
-  const int grid = (int)std::min<int64_t>((all + ROPE_THREADS - 1) / ROPE_THREADS, 32 * (int64_t)num_sms());
+  const RopeCut cut = rope_cut(a.n_rows, a.nh + 2 * c.nkv, RopeLane<VEC, HALF>::count(r.dim, c.hd), r.dim);
+  const int grid = (a.n_rows + cut.rows - 1) / cut.rows;
   bool aligned = rows_aligned(a.k, a.k_stride, c.hd, sizeof(S), VEC) && rows_aligned(a.v, a.v_stride, c.hd, sizeof(S), VEC);
   if (a.nh) aligned = aligned && rows_aligned(a.q, a.q_stride, c.hd, sizeof(S), VEC);
-  launch_k(kv_append_kernel<S, D, VEC, HALF>, grid + (a.seqs && a.n > 1), ROPE_THREADS, 0, st, a, r, chunk, aligned,
-           a.nh && rows_aligned(a.q_out, a.out_stride, c.hd, sizeof(S), VEC), grid);
+  launch_k(kv_append_kernel<S, D, VEC, HALF>, dim3(grid + (a.seqs && a.n > 1), cut.cuts), ROPE_THREADS, 0, st, a, r,
+           cut, aligned, a.nh && rows_aligned(a.q_out, a.out_stride, c.hd, sizeof(S), VEC), grid);
 }
 
 void launch_kv_append(const AppendArgs& a, const RopeParams& r, int t, cudaStream_t st) {
