@@ -555,6 +555,30 @@ KC_API int kc_attn_prompt_dev(kc_ctx* ctx, int cache, int layer, const int32_t* 
                               int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale, int window,
                               int sinks, void* out, int64_t out_stride);
 
+/* ---- sampling ---------------------------------------------------------------
+   One token for each of n rows of logits (KC_F32, KC_F16 or KC_BF16; n_vocab up to
+   393216, rows `stride` elements apart, 0 for draws from one row) by the settings of its row. All arrays are
+   device memory of n values; those of settings may be NULL:
+     u            uniform numbers in [0, 1), the caller's
+     temperature  T (NULL: 1). Not above 0: the first maximum, whatever u
+     top_k        NULL, not above 0, or n_vocab and more: off
+     top_p        NULL or not below 1: off
+     min_p        NULL or not above 0: off
+   w_j = exp((l_j - max l) / T); tokens rank by their logit, equal ones by their
+   index. Kept are the top_k first; of these the shortest run from the first whose
+   sum reaches top_p times all of theirs (one at least); of these those with w_j >=
+   min_p (min_p above 1: 1). tokens[i] is the first in the order of the indices at
+   which the running sum of what is kept exceeds u times their sum; probs[i] (NULL:
+   not wanted) its share of that sum. Weights and sums are good to 2e-13, so rows
+   whose border lies further off get the token that exact arithmetic gives.
+   A logit that is not a number counts as minus infinity; of infinite ones each
+   weighs 1 and the others nothing; a row with nothing else than minus infinity gets
+   token -1 and share 0. u below 0 or not a number counts as 0, 1 and above as the
+   largest below 1. (The greedy calls kc_model_* take the same first maximum.) */
+KC_API int kc_sample_dev(kc_ctx* ctx, int t, const void* logits, int64_t stride, int n, int n_vocab, const float* u,
+                         const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                         int32_t* tokens, float* probs);
+
 /* ---- expert parallelism (one process per GPU, NCCL over NVLink) -------- */
 
 /* 128-byte NCCL unique id, created on one rank and shared by the host. */

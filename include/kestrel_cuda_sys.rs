@@ -235,6 +235,9 @@ unsafe extern "C" {
         row_start: *const i32, n: c_int, n_rows: c_int, n_head: c_int, t: c_int, q: *const c_void, q_stride: i64,
         scale: f32, window: c_int, sinks: c_int, out: *mut c_void, out_stride: i64) -> c_int;
     // expert parallelism (one process per GPU)
+    pub fn kc_sample_dev(ctx: *mut kc_ctx, t: c_int, logits: *const c_void, stride: i64, n: c_int, n_vocab: c_int,
+        u: *const f32, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32,
+        tokens: *mut i32, probs: *mut f32) -> c_int;
     pub fn kc_ep_unique_id(out: *mut c_char) -> c_int; // out: 128 bytes
     pub fn kc_ep_init(ctx: *mut kc_ctx, rank: c_int, world: c_int, uid: *const c_char) -> c_int; // uid: 128 bytes
     pub fn kc_ep_reserve(ctx: *mut kc_ctx, max_tokens: c_int) -> c_int;

@@ -19,6 +19,7 @@
 #include "kernels.h"
 #include "kv.h"
 #include "rope.h"
+#include "sample.h"
 #include "mma.h"
 #include "loader.h"
 #include "model.h"
@@ -3329,6 +3330,30 @@ int kc_kv_append_dev(kc_ctx* ctx, int cache, int layer, int rope, const int32_t*
     }
     const AppendArgs a{c, layer, seqs, row_start, n, n_rows, n_head, q, k, v, q_out, q_stride, k_stride, v_stride, out_stride};
     launch_kv_append(a, *r, t, ctx->stream);
+    return KC_OK;
+  });
+}
+
+int kc_sample_dev(kc_ctx* ctx, int t, const void* logits, int64_t stride, int n, int n_vocab, const float* u,
+                  const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                  int32_t* tokens, float* probs) {
+  return kv_guard(ctx, "kc_sample_dev", [&]() -> int {
+    if (t != T_F32 && t != T_F16 && t != T_BF16)
+      return fail(ctx, KC_ERR_TYPE, "kc_sample_dev: type %d (F32, F16 or BF16)", t);
+    if (n < 0 || n > INT32_MAX / 8) return fail(ctx, KC_ERR_ARG, "kc_sample_dev: n=%d", n);
+    if (n_vocab < 1 || n_vocab > SAMPLE_MAX_VOCAB || stride < 0)
+      return fail(ctx, KC_ERR_SHAPE, "kc_sample_dev: rows of %d (1 to %d), %lld apart", n_vocab, SAMPLE_MAX_VOCAB,
+                  (long long)stride);
+    if (n == 0) return KC_OK;
+    if (!logits || !u || !tokens) return fail(ctx, KC_ERR_ARG, "kc_sample_dev: null buffer");
+    if ((uintptr_t)logits % (t == T_F32 ? 4 : 2) ||
+        ((uintptr_t)u | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p |
+         (uintptr_t)tokens | (uintptr_t)probs) % 4)
+      return fail(ctx, KC_ERR_ARG, "kc_sample_dev: misaligned buffer");
+    const SampleArgs a{logits, stride, n, n_vocab, u, temperature, top_k, top_p, min_p, tokens, probs};
+    const int rc = launch_sample(a, t, ctx->stream);
+    if (rc != KC_OK) return fail(ctx, rc, "kc_sample_dev: launch set-up failed");
+    CKL();
     return KC_OK;
   });
 }

@@ -77,6 +77,7 @@ SIGNATURES = {
     "kc_expert_cache_decay": (I, [P]),
     "kc_rope": (I, [P, I, I, I, F, I, F, I, F, F, F, P]),
     "kc_rope_dev": (I, [P, I, P, I, I, I, I, P, I64, P, I64]),
+    "kc_sample_dev": (I, [P, I, P, I64, I, I, P, P, P, P, P, P, P]),
     "kc_kv_cache": (I, [P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]),
     "kc_kv_drop": (I, [P, I]),
     "kc_kv_fork_dev": (I, [P, I, P, P, I]),
@@ -202,6 +203,21 @@ def _dev_rows(name: str, a, heads: int | None = None, head_dim: int | None = Non
     if (hd > 1 and stride[2] != 1) or (nh > 1 and stride[1] != hd):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
     return stride[0] if rows > 1 else nh * hd
+
+
+_FLOAT32 = set()  # torch.float32, once seen
+
+
+def _dev_floats(name: str, a, size: int):
+    """A contiguous float32 CUDA tensor of `size` values."""
+    if a is None:
+        return None
+    if not _is_dev(a) or not (a.dtype in _FLOAT32 or str(a.dtype) == "torch.float32") or not a.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 CUDA tensor")
+    _FLOAT32.add(a.dtype)
+    if a.numel() != size:
+        raise ValueError(f"{name} holds {a.numel()} values, {size} needed")
+    return a.data_ptr()
 
 
 class Context:
@@ -624,6 +640,22 @@ class Context:
                                              _dev_ints("row_start", row_start), n, rows, nh, _float_type("q", q),
                                              q.data_ptr(), qs, hd ** -0.5 if scale is None else scale, window, sinks,
                                              out.data_ptr(), os_))
+
+    # ---- sampling ------------------------------------------------------------------
+    def sample_dev(self, logits, u, tokens, probs=None, temperature=None, top_k=None, top_p=None, min_p=None):
+        """One token per row of logits [n, n_vocab] (float32, float16 or bfloat16)
+        to tokens [n] (int32), its share to probs [n], from the uniform numbers u
+        [n] and each row's settings [n] (kc_sample_dev; None: off)."""
+        if not _is_dev(logits) or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise ValueError("logits must be a CUDA tensor [rows, vocabulary] of contiguous rows")
+        if u is None or tokens is None:
+            raise ValueError("u and tokens are needed")
+        n, vocab = logits.shape
+        self._check(lib().kc_sample_dev(self.h, _float_type("logits", logits), logits.data_ptr(),
+                                        logits.stride(0) if n > 1 else vocab, n, vocab, _dev_floats("u", u, n),
+                                        _dev_floats("temperature", temperature, n), _dev_ints("top_k", top_k, n),
+                                        _dev_floats("top_p", top_p, n), _dev_floats("min_p", min_p, n),
+                                        _dev_ints("tokens", tokens, n), _dev_floats("probs", probs, n)))
 
     def ep_reserve(self, max_tokens: int):
         """Collective: map the peer exchange arenas for up to max_tokens tokens
