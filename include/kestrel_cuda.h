@@ -547,13 +547,26 @@ KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, cons
    [n + 1] ascends within 0 .. n_rows. An entry that begins before an earlier
    one does, ends before it begins or ends past n_rows is left out and
    reported. Rows in no sequence's range are not written, nor (in both calls)
-   those of a sequence index out of range; a sequence may be given twice. */
+   those of a sequence index out of range; a sequence may be given twice.
+   kc_attn_shared_dev: kc_attn_decode_dev without a window, for entries in groups
+   whose sequences begin with the same pages (branches of one prompt): entries
+   group_start[g] .. group_start[g+1]-1 are a group, group_start [n_groups + 1]
+   ascending within 0 .. n. The leading pages that the tables of all of a group's
+   sequences that hold positions name alike, and behind which each holds another
+   position, are read once for the group; the device looks them up, so the results
+   are kc_attn_decode_dev's (within the roundings above, weights of 16-bit queries
+   rounded as in kc_attn_prompt_dev) whatever the groups are. An entry in no group
+   is by itself; a list that does not ascend is reported, and nothing is shared. */
 KC_API int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, int n_head, int t,
                               const void* q, int64_t q_stride, float scale, int window, int sinks, void* out,
                               int64_t out_stride);
 KC_API int kc_attn_prompt_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,
                               int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale, int window,
                               int sinks, void* out, int64_t out_stride);
+
+KC_API int kc_attn_shared_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, const int32_t* group_start,
+                              int n_groups, int n_head, int t, const void* q, int64_t q_stride, float scale, void* out,
+                              int64_t out_stride);
 
 /* ---- sampling ---------------------------------------------------------------
    One token for each of n rows of logits (KC_F32, KC_F16 or KC_BF16; n_vocab up to

@@ -231,6 +231,9 @@ unsafe extern "C" {
     pub fn kc_attn_decode_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32, n: c_int,
         n_head: c_int, t: c_int, q: *const c_void, q_stride: i64, scale: f32, window: c_int, sinks: c_int,
         out: *mut c_void, out_stride: i64) -> c_int;
+    pub fn kc_attn_shared_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32, n: c_int,
+        group_start: *const i32, n_groups: c_int, n_head: c_int, t: c_int, q: *const c_void, q_stride: i64,
+        scale: f32, out: *mut c_void, out_stride: i64) -> c_int;
     pub fn kc_attn_prompt_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32,
         row_start: *const i32, n: c_int, n_rows: c_int, n_head: c_int, t: c_int, q: *const c_void, q_stride: i64,
         scale: f32, window: c_int, sinks: c_int, out: *mut c_void, out_stride: i64) -> c_int;

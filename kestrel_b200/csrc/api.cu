@@ -3040,9 +3040,10 @@ int kv_call(kc_ctx* ctx, int cache, const char* what, Fn&& fn) {
   });
 }
 
+// prompt: rows of row_start; shared: row_start are the groups' first entries, n_groups + 1.
 int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t* seqs, const int32_t* row_start,
               bool prompt, int n, int n_rows, int n_head, int t, const void* q, int64_t q_stride, float scale,
-              int window, int sinks, void* out, int64_t out_stride) {
+              int window, int sinks, void* out, int64_t out_stride, bool shared = false, int n_groups = 0) {
   return kv_call(ctx, cache, what, [&](const KvCache& kv) -> int {
     const KvView& c = kv.view;
     if (layer < 0 || layer >= c.n_layer) return fail(ctx, KC_ERR_ARG, "%s: layer %d of %d", what, layer, c.n_layer);
@@ -3051,7 +3052,9 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
                   n_rows, window, sinks);
     if (!(scale > -INFINITY && scale < INFINITY)) return fail(ctx, KC_ERR_ARG, "%s: scale is not finite", what);
     if (n == 0 || n_rows == 0) return KC_OK;
-    if (!q || !out || (prompt && !row_start)) return fail(ctx, KC_ERR_ARG, "%s: null buffer", what);
+    if (!q || !out || ((prompt || n_groups) && !row_start)) return fail(ctx, KC_ERR_ARG, "%s: null buffer", what);
+    if (n_groups < 0 || n_groups > c.n_seq)
+      return fail(ctx, KC_ERR_ARG, "%s: %d groups (of %d sequences)", what, n_groups, c.n_seq);
     if (n_head <= 0 || n_head % c.nkv || n_head / c.nkv > 128)
       return fail(ctx, KC_ERR_SHAPE, "%s: %d query heads over %d key-value heads (1 to 128 each)", what, n_head,
                   c.nkv);
@@ -3070,7 +3073,7 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     a.c = c;
     a.layer = layer;
     a.seqs = seqs;
-    a.row_start = row_start;
+    a.row_start = prompt ? row_start : nullptr;
     a.n = n;
     a.n_rows = n_rows;
     a.nh = n_head;
@@ -3084,8 +3087,16 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     // could also leave 32 bits.)
     a.window = (int64_t)window < (int64_t)c.max_pages * c.page ? window : 0;
     a.sinks = a.window > 0 ? sinks : 0;
-    const int rc = prompt ? launch_attn_prompt(a, kv.tiles, ctx->kv.part, ctx->kv.count, ctx->stream)
-                          : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
+    SharedArgs sh{};
+    sh.group_start = row_start;
+    sh.n_groups = n_groups;
+    sh.of_entry = c.both;
+    sh.of_group = c.both_group;
+    sh.lead = c.lead;
+    const int rc = prompt   ? launch_attn_prompt(a, kv.tiles, ctx->kv.part, ctx->kv.count, ctx->stream)
+                   : shared ? launch_attn_shared(a, sh, kv.rows16, kv.tiles, ctx->kv.part, ctx->kv.count,
+                                                 ctx->kv.shared, ctx->stream)
+                            : launch_attn_decode(a, kv.rows16, ctx->kv.part, ctx->kv.count, ctx->stream);
     return rc == KC_OK ? KC_OK : fail(ctx, rc, "%s: launch set-up failed", what);
   });
 }
@@ -3156,11 +3167,13 @@ int kc_kv_cache(kc_ctx* ctx, int cache, int t, int n_layer, int n_pages, int pag
       return fail(ctx, KC_ERR_CUDA, "kc_kv_cache: cuTensorMapEncodeTiled refused the pools");
     if (!ctx->kv.part) {
       const size_t part = std::max(attn_decode_part_bytes(), attn_prompt_part_bytes());
-      const size_t cnt = (size_t)std::max(num_sms(), attn_prompt_counts()) * sizeof(int), all = part + cnt;
+      const size_t cnt = (size_t)(std::max(num_sms(), attn_prompt_counts()) + attn_shared_counts()) * sizeof(int);
+      const size_t all = part + attn_shared_part_bytes() + cnt;
       void* p = nullptr;
       CK(cudaMalloc(&p, all));
       ctx->kv.part = static_cast<float*>(p);
-      ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + part);
+      ctx->kv.shared = ctx->kv.part + part / sizeof(float);
+      ctx->kv.count = reinterpret_cast<int*>(static_cast<uint8_t*>(p) + part + attn_shared_part_bytes());
       ctx->kv.count_bytes = (int64_t)cnt;
       ctx->kv.bytes = (int64_t)all;
       CK(cudaMemsetAsync(ctx->kv.count, 0, cnt, ctx->stream));
@@ -3390,6 +3403,13 @@ int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, i
                        int64_t out_stride) {
   return attn_call(ctx, cache, "kc_attn_decode", layer, seqs, nullptr, false, n, n, n_head, t, q, q_stride, scale,
                    window, sinks, out, out_stride);
+}
+
+int kc_attn_shared_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, const int32_t* group_start,
+                       int n_groups, int n_head, int t, const void* q, int64_t q_stride, float scale, void* out,
+                       int64_t out_stride) {
+  return attn_call(ctx, cache, "kc_attn_shared", layer, seqs, group_start, false, n, n, n_head, t, q, q_stride, scale, 0,
+                   0, out, out_stride, true, n_groups);
 }
 
 int kc_attn_prompt_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, const int32_t* row_start, int n,

@@ -62,18 +62,36 @@ struct DecArgs {
   AttnArgs a;
   float* part;  // [grid][2][HT][LD]
   int* count;   // [grid], zero between launches
+  SharedArgs sh;  // of calls with prefixes that are computed elsewhere
 };
+
+// Entry i's sequence, and the positions before its own part (SHARED).
+template <bool SHARED>
+__device__ __forceinline__ int dec_seq(const DecArgs& d, int i) {
+  return d.a.seqs ? d.a.seqs[i] : SHARED ? d.sh.e0 + i : i;
+}
+template <bool SHARED>
+__device__ __forceinline__ int dec_before(const DecArgs& d, int i) {
+  return SHARED ? d.sh.of_entry[d.sh.e0 + i] : 0;
+}
 
 // Chunks of the visible positions of a sequence of `len` positions as seen from
 // its last one: `head` chunks of the first tokens, then those from w0 on.
 struct Span {
   int head, w0, n, lo;
 };
-__device__ __forceinline__ Span dec_span(int len, int window, int sinks) {
+template <bool SHARED>
+__device__ __forceinline__ Span dec_span(int len, int window, int sinks, int before) {
   Span s;
-  s.lo = window > 0 ? max(0, len - window) : 0;
-  s.head = (min(sinks, s.lo) + DC - 1) / DC;
-  s.w0 = max(s.lo / DC, s.head);
+  if constexpr (SHARED) {
+    // (A prefix is whole pages, and of a sequence that goes on behind it.)
+    s.lo = s.head = 0;
+    s.w0 = before / DC;
+  } else {
+    s.lo = window > 0 ? max(0, len - window) : 0;
+    s.head = (min(sinks, s.lo) + DC - 1) / DC;
+    s.w0 = max(s.lo / DC, s.head);
+  }
   s.n = len > 0 ? s.head + (len + DC - 1) / DC - s.w0 : 0;
   return s;
 }
@@ -96,19 +114,23 @@ struct SegIter {
   long long unit_at;  // line position of the unit's first chunk
 };
 
-__device__ __forceinline__ void seg_sequence(SegIter& t, const AttnArgs& a) {
-  t.s = a.seqs ? a.seqs[t.i] : t.i;
+template <bool SHARED>
+__device__ __forceinline__ void seg_sequence(SegIter& t, const DecArgs& d) {
+  const AttnArgs& a = d.a;
+  t.s = dec_seq<SHARED>(d, t.i);
   t.len = t.s >= 0 && t.s < a.c.n_seq ? kv_len(a.c, t.s) : 0;
-  t.span = dec_span(t.len, a.window, a.sinks);
+  t.span = dec_span<SHARED>(t.len, a.window, a.sinks, dec_before<SHARED>(d, t.i));
 }
-__device__ __forceinline__ bool seg_next(SegIter& t, const AttnArgs& a, int units) {
+template <bool SHARED>
+__device__ __forceinline__ bool seg_next(SegIter& t, const DecArgs& d, int units) {
+  const AttnArgs& a = d.a;
   while (t.pos < t.end) {
     const int np = t.pad ? t.pad : t.span.n;
     const long long off = t.pos - t.base;  // (a sequence's stretch fits 31 bits: the host sees to it)
     if (off >= np * units) {
       t.base += np * units;
       if (++t.i >= a.n) return false;
-      seg_sequence(t, a);
+      seg_sequence<SHARED>(t, d);
       continue;
     }
     t.unit = (int)((uint32_t)off / (uint32_t)np);
@@ -129,7 +151,59 @@ struct DecPart {
   long long unit_at;
 };
 
-template <typename TQ, typename TKV, int NB, int HT>
+// The prefix parts of an entry's head: `n` of them, `step` floats apart, each the
+// result, then its maximum (in exponents of 2) and sum at LD - 4.
+struct PrefixParts {
+  const float* row;
+  int64_t step;
+  int n, at;  // at: LD - 4
+  __device__ __forceinline__ float2 state(int p) const { return __ldcg(reinterpret_cast<const float2*>(row + p * step + at)); }
+  // What a part's result counts for against maximum `base`. (Never quite nothing,
+  // so that an infinite result stays what the formula gives.)
+  __device__ __forceinline__ float share(int p, float base) const {
+    const float2 ml = state(p);
+    return ml.y == 0.f ? 0.f : fmaxf(exp2_fast(ml.x - base), 1e-37f) * ml.y;
+  }
+};
+template <int LD>
+__device__ __forceinline__ PrefixParts prefix_parts(const DecArgs& d, int i, int head) {
+  const int both = d.sh.of_entry[d.sh.e0 + i], n = d.sh.e1 - d.sh.e0;
+  PrefixParts x;
+  x.step = (int64_t)n * d.a.nh * LD;
+  x.row = d.sh.part + ((int64_t)i * d.a.nh + head) * LD;
+  x.n = both > 0 ? shared_splits(both, d.a.c.hd, d.sh.splits) : 0;
+  x.at = LD - 4;
+  return x;
+}
+// Joins an entry's own part (maximum m, sum l) with its prefix: the maximum that
+// shares count from, 1 / the sum, and what the own values count for.
+struct PrefixJoin {
+  float base, inv, own;
+};
+__device__ __forceinline__ PrefixJoin prefix_join(const PrefixParts& x, float m, float l) {
+  PrefixJoin j;
+  j.base = m;
+  for (int p = 0; p < x.n; ++p) j.base = fmaxf(j.base, x.state(p).x);
+  if (j.base == -INFINITY) j.base = 0.f;
+  j.own = l == 0.f ? 0.f : fmaxf(exp2_fast(m - j.base), 1e-37f);
+  float sum = l * j.own;
+  for (int p = 0; p < x.n; ++p) sum += x.share(p, j.base);
+  j.inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+  return j;
+}
+__device__ __forceinline__ float4 prefix_add(const PrefixParts& x, const PrefixJoin& j, int y, float4 v) {
+  for (int p = 0; p < x.n; ++p) {
+    const float w = x.share(p, j.base) * j.inv;
+    const float4 u = __ldcg(reinterpret_cast<const float4*>(x.row + p * x.step + y));
+    v.x = __fmaf_rn(w, u.x, v.x);
+    v.y = __fmaf_rn(w, u.y, v.y);
+    v.z = __fmaf_rn(w, u.z, v.z);
+    v.w = __fmaf_rn(w, u.w, v.w);
+  }
+  return v;
+}
+
+template <typename TQ, typename TKV, int NB, int HT, bool SHARED>
 __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     attn_decode_kernel(const DecArgs d, const __grid_constant__ KvMaps maps) {
   using S = DecShape<NB, HT>;
@@ -144,6 +218,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   __shared__ int found[W];
   __shared__ DecPart parts_sh[2 * W];  // per warp: of its range's first segment, and of its last
   __shared__ int last_sh[2];
+  __shared__ PrefixJoin join_sh[SHARED ? HT : 1];
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -166,9 +241,9 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     here = 0;
     bool none = false;
     if (i < a.n) {
-      const int s = a.seqs ? a.seqs[i] : i;
+      const int s = dec_seq<SHARED>(d, i);
       const bool real = s >= 0 && s < c.n_seq;
-      if (real) here = dec_span(kv_len(c, s), a.window, a.sinks).n;
+      if (real) here = dec_span<SHARED>(kv_len(c, s), a.window, a.sinks, dec_before<SHARED>(d, i)).n;
       else if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
       none = real && here == 0 && i % gridDim.x == blockIdx.x;
     }
@@ -259,8 +334,8 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         const int i = b + tid;
         int n = 0;
         if (i < a.n) {
-          const int s = a.seqs ? a.seqs[i] : i;
-          if (s >= 0 && s < c.n_seq) n = dec_span(kv_len(c, s), a.window, a.sinks).n;
+          const int s = dec_seq<SHARED>(d, i);
+          if (s >= 0 && s < c.n_seq) n = dec_span<SHARED>(kv_len(c, s), a.window, a.sinks, dec_before<SHARED>(d, i)).n;
         }
         long long x = n;
 #pragma unroll
@@ -284,7 +359,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     at.base = found_at[warp];
     if (at.i >= a.n) at.pos = at.end;
   }
-  if (at.pos < at.end) seg_sequence(at, a);
+  if (at.pos < at.end) seg_sequence<SHARED>(at, d);
 
   // ---- queries ------------------------------------------------------------------
   // A segment's, as this lane holds them in A fragments (row r0, and r0 + 8 in
@@ -324,7 +399,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     }
   };
   SegIter ahead = at;  // what is loaded next
-  bool more = seg_next(ahead, a, units), have = more;
+  bool more = seg_next<SHARED>(ahead, d, units), have = more;
   SegIter to_come = ahead;  // the segment after the one at hand
   if (kAhead && have) ask(to_come);
 
@@ -335,7 +410,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // The next chunk: first position, sequence and head. False when there is none.
   auto plan = [&](int& p, int& s, int& head) {
     while (more && next >= ahead.c1) {
-      more = seg_next(ahead, a, units);
+      more = seg_next<SHARED>(ahead, d, units);
       next = ahead.c0 + mine;
     }
     if (!more) return false;
@@ -417,7 +492,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
           }
         }
     }
-    have = seg_next(to_come, a, units);
+    have = seg_next<SHARED>(to_come, d, units);
     if (kAhead && have) ask(to_come);
     float m[RH], l[RH], o[8 * NB][4];
 #pragma unroll
@@ -569,7 +644,31 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       for (int rr = 0; rr < RH; ++rr) {
         const int h = r0 + 8 * rr;
         if (h0 + h >= group) continue;
-        const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
+        float inv;
+        if constexpr (SHARED) {
+          const PrefixParts x = prefix_parts<LD>(d, at.i, kvh * group + h0 + h);
+          const PrefixJoin j = prefix_join(x, m[rr] - kLift, l[rr]);
+          inv = j.own * j.inv;
+          if (x.n) {
+#pragma unroll
+            for (int t = 0; t < 8 * NB; ++t) {
+              o[t][2 * rr] *= inv;
+              o[t][2 * rr + 1] *= inv;
+            }
+            for (int p = 0; p < x.n; ++p) {
+              const float w = x.share(p, j.base) * j.inv;
+#pragma unroll
+              for (int t = 0; t < 8 * NB; ++t) {
+                const float2 u = __ldcg(reinterpret_cast<const float2*>(x.row + p * x.step + 8 * t + cc));
+                o[t][2 * rr] = __fmaf_rn(w, u.x, o[t][2 * rr]);
+                o[t][2 * rr + 1] = __fmaf_rn(w, u.y, o[t][2 * rr + 1]);
+              }
+            }
+            inv = 1.f;
+          }
+        } else {
+          inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
+        }
 #pragma unroll
         for (int t = 0; t < 8 * NB; ++t)
 #pragma unroll
@@ -672,7 +771,16 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
       if (whole) {
         if (h0 + h >= group || y >= c.hd) continue;
-        const float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
+        float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
+        if constexpr (SHARED) {
+          const PrefixParts px = prefix_parts<LD>(d, g.i, kvh * group + h0 + h);
+          if (px.n) {
+            const PrefixJoin j = prefix_join(px, ml.x - kLift, ml.y);
+            const float own = j.own * j.inv;
+            v = prefix_add(px, j, y, make_float4(v.x * own, v.y * own, v.z * own, v.w * own));
+            inv = 1.f;
+          }
+        }
         TQ* to = out + (int64_t)h * c.hd + y;
         to[0] = (TQ)(v.x * inv);
         to[1] = (TQ)(v.y * inv);
@@ -735,7 +843,13 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+      float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+      if constexpr (SHARED) {
+        const PrefixParts px = prefix_parts<LD>(d, g.i, kvh * group + min(h0 + h, group - 1));
+        const PrefixJoin j = prefix_join(px, top - kLift, total);
+        inv = j.own * j.inv;
+        if (lane == 0) join_sh[h] = j;
+      }
 #pragma unroll
       for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
         if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
@@ -760,6 +874,8 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
           sum4.w = __fmaf_rn(w, v[k].w, sum4.w);
         }
       }
+      if constexpr (SHARED)
+        sum4 = prefix_add(prefix_parts<LD>(d, g.i, kvh * group + h0 + h), join_sh[h], y, sum4);
       TQ* to = out + (int64_t)h * c.hd + y;
       to[0] = (TQ)sum4.x;
       to[1] = (TQ)sum4.y;
@@ -771,39 +887,50 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
 
 size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 4) * sizeof(float); }
 
-template <typename TQ, typename TKV, int NB, int HT>
+template <typename TQ, typename TKV, int NB, int HT, bool SHARED>
 static int launch_decode(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
   using S = DecShape<NB, HT>;
   static_assert(S::ST >= 2 && S::SMEM <= 226 * 1024, "two stages fit");
   static PerDeviceOnce attr;
-  if (smem_attr_once(attr, attn_decode_kernel<TQ, TKV, NB, HT>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
+  if (smem_attr_once(attr, attn_decode_kernel<TQ, TKV, NB, HT, SHARED>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
   const int64_t units = (int64_t)d.a.n * d.a.c.nkv * ((d.a.nh / d.a.c.nkv + HT - 1) / HT);
   const int64_t most = (int64_t)d.a.c.max_pages * d.a.c.page / DC;
   if (most * (units / d.a.n) > INT32_MAX - 8 * num_sms()) return KC_ERR_SHAPE;  // chunks of a sequence, all heads
   // One block per SM, fewer when the tables hold less than a chunk per warp of each.
   const int grid = (int)std::min<int64_t>(std::min(num_sms(), DEC_MAX_PARTS), units * ((most + S::W - 1) / S::W));
-  launch_k(attn_decode_kernel<TQ, TKV, NB, HT>, grid, 32 * S::W, S::SMEM, st, d, maps);
+  launch_k(attn_decode_kernel<TQ, TKV, NB, HT, SHARED>, grid, 32 * S::W, S::SMEM, st, d, maps);
   return KC_OK;
 }
 
-template <typename TQ, typename TKV, int HT>
+template <typename TQ, typename TKV, int HT, bool SHARED>
 static int launch_decode_hd(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
   switch ((d.a.c.hd + 63) / 64) {
-    case 1: return launch_decode<TQ, TKV, 1, HT>(d, maps, st);
-    case 2: return launch_decode<TQ, TKV, 2, HT>(d, maps, st);
-    case 3: return launch_decode<TQ, TKV, 3, HT>(d, maps, st);
-    default: return launch_decode<TQ, TKV, 4, HT>(d, maps, st);
+    case 1: return launch_decode<TQ, TKV, 1, HT, SHARED>(d, maps, st);
+    case 2: return launch_decode<TQ, TKV, 2, HT, SHARED>(d, maps, st);
+    case 3: return launch_decode<TQ, TKV, 3, HT, SHARED>(d, maps, st);
+    default: return launch_decode<TQ, TKV, 4, HT, SHARED>(d, maps, st);
   }
 }
 
-int launch_attn_decode(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
-  const DecArgs d{a, part, count};
+template <bool SHARED>
+static int launch_decode_types(const DecArgs& d, const KvMaps& maps, cudaStream_t st) {
+  const AttnArgs& a = d.a;
   const bool many = a.nh / a.c.nkv > 8;
   if (a.c.type == T_BF16)
-    return many ? launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 16>(d, maps, st)
-                : launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 8>(d, maps, st);
-  if (a.t_q == T_F32) return launch_decode_hd<float, __half, 8>(d, maps, st);
-  return many ? launch_decode_hd<__half, __half, 16>(d, maps, st) : launch_decode_hd<__half, __half, 8>(d, maps, st);
+    return many ? launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 16, SHARED>(d, maps, st)
+                : launch_decode_hd<__nv_bfloat16, __nv_bfloat16, 8, SHARED>(d, maps, st);
+  if (a.t_q == T_F32) return launch_decode_hd<float, __half, 8, SHARED>(d, maps, st);
+  return many ? launch_decode_hd<__half, __half, 16, SHARED>(d, maps, st)
+              : launch_decode_hd<__half, __half, 8, SHARED>(d, maps, st);
+}
+
+int launch_attn_decode(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
+  return launch_decode_types<false>(DecArgs{a, part, count, {}}, maps, st);
+}
+
+int launch_attn_own(const AttnArgs& a, const SharedArgs& sh, const KvMaps& maps, float* part, int* count,
+                    cudaStream_t st) {
+  return launch_decode_types<true>(DecArgs{a, part, count, sh}, maps, st);
 }
 
 }  // namespace kc

@@ -167,9 +167,11 @@ struct Item {
 // at 8192 positions, 8 heads of 64, all of them so: 18 ms; position by position
 // 219). Columns col0 .. col1-1 are written. `alive` is the time at which it last
 // moved on, for those who wait for it.
-template <typename TQ, typename TKV>
-__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int at, const TQ* q, TQ* out, int col0,
-                                        int col1, volatile uint64_t* alive) {
+// Positions `from` .. `at` (SHARED: a part of a prefix, whose maximum, in exponents
+// of 2, and sum go to `state` with column 0).
+template <typename TQ, typename TKV, typename TO, bool SHARED>
+__device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int from, int at, const TQ* q, TO* out,
+                                        int col0, int col1, float* state, volatile uint64_t* alive) {
   const KvView c = a.c;
   const int lane = threadIdx.x & 31, sub = lane & 7, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
   const float scale = a.scale;
@@ -180,7 +182,7 @@ __device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int a
   for (int g = 0; g < 4; ++g)
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[g][i] = 0.f;
-  for (int j0 = 0, steps = 0; j0 <= at; j0 += 32) {
+  for (int j0 = SHARED ? from : 0, steps = 0; j0 <= at; j0 += 32) {
     if (j0 + 32 <= lo && j0 >= a.sinks) {
       j0 = lo / 32 * 32 - 32;
       continue;
@@ -261,8 +263,9 @@ __device__ __noinline__ void prompt_row(const AttnArgs& a, int s, int kvh, int a
       r += __shfl_xor_sync(0xffffffffu, r, 8);
       r += __shfl_xor_sync(0xffffffffu, r, 16);
       const int col = 64 * g + 8 * sub + i;
-      if (lane < 8 && col >= col0 && col < col1) out[col] = (TQ)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(r, l));
+      if (lane < 8 && col >= col0 && col < col1) out[col] = (TO)(l == 0.f ? 0.f : l != l ? l : __fdiv_rn(r, l));
     }
+  if (SHARED && col0 == 0 && lane == 0) *reinterpret_cast<float2*>(state) = make_float2(m * 1.4426950408889634f, l);
 }
 
 // mbar_wait whose limit counts from the last time that a row computed by itself
@@ -318,9 +321,13 @@ struct PromptArgs {
   int* count;   // per unit, zero between launches
   int* next;    // [2] items dealt beyond one per block, blocks done: zero between launches
   bool q_map;   // queries come by TMA
+  SharedArgs sh;  // SHARED
 };
 
-template <typename TQ, typename TKV, int NB, bool TWO>
+// SHARED: an entry is a group of sequences, its rows one query of each; every row
+// sees all positions that the group has in common, and what comes of them is left
+// for the join (attn_decode.cu).
+template <typename TQ, typename TKV, int NB, bool TWO, bool SHARED>
 __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     attn_prompt_kernel(const PromptArgs d, const __grid_constant__ KvMaps maps, const __grid_constant__ KvMap q_map) {
   using S = PromptShape<TQ, NB, TWO>;
@@ -625,6 +632,14 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // out of order). The first time over the list says whether anything is.
     bool ascend = true, known = false;
     auto tiles_of = [&](int i, int& last, int& lo, int& hi) {
+      if constexpr (SHARED) {
+        lo = hi = 0;
+        if (i < a.n && d.sh.of_group[i] > 0) {
+          lo = max(a.row_start[i], d.sh.e0);
+          hi = max(lo, min(a.row_start[i + 1], d.sh.e1));
+        }
+        return (int)(((int64_t)(hi - lo) * group + S::QT * PM - 1) / (S::QT * PM));
+      }
       lo = hi = last;
       if (i < a.n) {
         lo = a.row_start[i];
@@ -663,8 +678,13 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     const bool sorted = a.n <= 32;
     if (finder) {
       if (sorted) {
-        const int s = lane < a.n ? (a.seqs ? a.seqs[lane] : lane) : -1;
-        const int len = s >= 0 && s < c.n_seq ? kv_len(c, s) : 0;
+        int len;
+        if constexpr (SHARED) {
+          len = lane < a.n ? d.sh.of_group[lane] : 0;
+        } else {
+          const int s = lane < a.n ? (a.seqs ? a.seqs[lane] : lane) : -1;
+          len = s >= 0 && s < c.n_seq ? kv_len(c, s) : 0;
+        }
         int rank = 0;
         for (int j = 0; j < 32; ++j) {
           const int other = __shfl_sync(0xffffffffu, len, j);
@@ -731,15 +751,16 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             }
           }
           x.row0 = t * S::QT * PM;
-          x.s = a.seqs ? a.seqs[i] : i;
+          x.s = SHARED ? d.sh.lead[i] : a.seqs ? a.seqs[i] : i;
           if (x.s < 0 || x.s >= c.n_seq) {
             if (lane == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
             continue;
           }
-          if (!sorted) x.len = kv_len(c, x.s);
+          if (!sorted) x.len = SHARED ? d.sh.of_group[i] : kv_len(c, x.s);
           x.rows = min(S::QT * PM, x.count * group - x.row0);
           // Positions of the first and last row, and the tiles they see.
-          const int at0 = x.len - x.count + x.row0 / group, at1 = x.len - x.count + (x.row0 + x.rows - 1) / group;
+          const int at0 = SHARED ? x.len - 1 : x.len - x.count + x.row0 / group,
+                    at1 = SHARED ? x.len - 1 : x.len - x.count + (x.row0 + x.rows - 1) / group;
           x.head = x.w0 = x.nt = 0;
           if (at1 >= 0) {
             const int lo = a.window > 0 ? max(0, at0 - a.window + 1) : 0;
@@ -848,7 +869,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       const RowMap rm(x.row0, group);
       const int f = my_tile * PM + r, nt = x.t1 - x.t0, at_base = x.len - x.count;
       const bool real = f < x.rows;
-      const int at = real ? at_base + rm.token(f) : -1;
+      const int at = !real ? -1 : SHARED ? x.len - 1 : at_base + rm.token(f);
       const int lo = a.window > 0 ? at - a.window + 1 : 0;
       if constexpr (kSplit) {
         if (d.q_map && nt > 0) {
@@ -887,7 +908,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         }
       }
       // Tiles whose positions every row of this tile sees need no mask.
-      const int t_at0 = at_base + rm.token(my_tile * PM);
+      const int t_at0 = SHARED ? x.len - 1 : at_base + rm.token(my_tile * PM);
       const int t_lo1 = a.window > 0 ? at_base + rm.token(min(x.rows, (my_tile + 1) * PM) - 1) - a.window + 1 : 0;
       float m = -INFINITY, l = 0.f;
       // Stream w's k-th tile is k (two row tiles) or NS k + w.
@@ -1091,13 +1112,19 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
-      const bool split = x.splits > 1;
+      const bool split = !SHARED && x.splits > 1;
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)x.start * a.out_stride + (int64_t)x.kvh * group * c.hd;
       const uint32_t grain = (uint32_t)((uintptr_t)a.out | (uint64_t)a.out_stride * sizeof(TQ) | c.hd * sizeof(TQ));
       float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
       bool bad = l != l || l == INFINITY;
       TQ* to_row = out + rm.offset(real ? f : 0, a.out_stride, c.hd);
       float* part_row = d.part + ((int64_t)x.unit * d.splits + x.split) * S::PART + 4 * r;
+      // SHARED: the row of its (split, entry, head) for the join.
+      constexpr int JOIN_LD = S::HD + 4;
+      float* join_row = nullptr;
+      if constexpr (SHARED)
+        join_row = d.sh.part + (((int64_t)x.split * (d.sh.e1 - d.sh.e0) + x.start - d.sh.e0) * a.nh + x.kvh * group) * JOIN_LD +
+                   rm.offset(real ? f : 0, (int64_t)a.nh * JOIN_LD, JOIN_LD);
       for (int e0 = col0; e0 < col1; e0 += 32) {
         float o[2][16];
         const uint32_t o_0 = tmem + lanes + S::T_O + (TWO ? w : 0) * S::HD + e0;
@@ -1124,6 +1151,15 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         for (int y = 0; y < 2; ++y) {
           if (y && !both) break;
           const int e1 = e0 + 16 * y;
+          if constexpr (SHARED) {
+            bad |= normalise16(o[y], inv);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(join_row + e1 + e) =
+                  make_float4(o[y][e], o[y][e + 1], o[y][e + 2], o[y][e + 3]);
+            if (e1 == 0) *reinterpret_cast<float2*>(join_row + S::HD) = make_float2(m - kLift, l);
+            continue;
+          }
           if (split) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -1206,10 +1242,18 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       // infinity against a weight's rest) is computed again by itself.
       for (unsigned again = __ballot_sync(0xffffffffu, ok && write && real && bad); again; again &= again - 1) {
         const int f1 = my_tile * PM + 32 * (warp & 3) + __ffs(again) - 1;
-        prompt_row<TQ, TKV>(a, x.s, x.kvh, at_base + rm.token(f1),
-                            static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride +
-                                (int64_t)x.kvh * group * c.hd + rm.offset(f1, a.q_stride, c.hd),
-                            out + rm.offset(f1, a.out_stride, c.hd), col0, min(col1, c.hd), &alive_sh);
+        const TQ* q_row = static_cast<const TQ*>(a.q) + (int64_t)x.start * a.q_stride + (int64_t)x.kvh * group * c.hd +
+                          rm.offset(f1, a.q_stride, c.hd);
+        if constexpr (SHARED) {
+          // (x.head is 0: position tile t begins at t BN.)
+          float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)join_row, __ffs(again) - 1));
+          prompt_row<TQ, TKV, float, true>(a, x.s, x.kvh, x.t0 * BN, min(x.t1 * BN, x.len) - 1, q_row, to, col0,
+                                           min(col1, c.hd), to + S::HD, &alive_sh);
+        } else {
+          prompt_row<TQ, TKV, TQ, false>(a, x.s, x.kvh, 0, at_base + rm.token(f1), q_row,
+                                         out + rm.offset(f1, a.out_stride, c.hd), col0, min(col1, c.hd), nullptr,
+                                         &alive_sh);
+        }
       }
       if (!ok) break;
       __syncwarp();
@@ -1230,18 +1274,18 @@ size_t attn_prompt_part_bytes() {
 }
 int attn_prompt_counts() { return PROMPT_MAX_UNITS + 2; }
 
-template <typename TQ, typename TKV, int NB, bool TWO>
+template <typename TQ, typename TKV, int NB, bool TWO, bool SHARED>
 static int launch_prompt(PromptArgs d, const KvMaps& maps, cudaStream_t st) {
   using S = PromptShape<TQ, NB, TWO>;
   const AttnArgs& a = d.a;
   static PerDeviceOnce attr;
-  if (smem_attr_once(attr, attn_prompt_kernel<TQ, TKV, NB, TWO>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
+  if (smem_attr_once(attr, attn_prompt_kernel<TQ, TKV, NB, TWO, SHARED>, S::SMEM) != cudaSuccess) return KC_ERR_CUDA;
   // Every sequence may leave its last tile partly filled.
   const int64_t rows = (int64_t)a.n_rows * (a.nh / a.c.nkv), tile = S::QT * PM;
   const int64_t most = (rows / tile + std::min(a.n, a.n_rows)) * a.c.nkv;
   if (most > INT32_MAX / 16) return KC_ERR_SHAPE;
-  d.splits = 1;
-  if (!TWO) {
+  d.splits = SHARED ? d.sh.splits : 1;
+  if (!TWO && !SHARED) {
     // Fewer items than SMs: their positions over as many blocks as there are,
     // within the workspace.
     const int64_t likely = std::max<int64_t>((rows + tile - 1) / tile, std::min(a.n, a.n_rows)) * a.c.nkv;
@@ -1255,11 +1299,11 @@ static int launch_prompt(PromptArgs d, const KvMaps& maps, cudaStream_t st) {
   const int group = a.nh / a.c.nkv;
   d.q_map = (S::kSplit || a.scale > 0.f) && PM % group == 0 && !((uintptr_t)a.q % 16) &&
             a.q_stride * sizeof(TQ) % 16 == 0 && make_q_map(a, q_map) == KC_OK;
-  launch_k(attn_prompt_kernel<TQ, TKV, NB, TWO>, grid, S::THREADS, S::SMEM, st, d, maps, q_map);
+  launch_k(attn_prompt_kernel<TQ, TKV, NB, TWO, SHARED>, grid, S::THREADS, S::SMEM, st, d, maps, q_map);
   return KC_OK;
 }
 
-template <typename TQ, typename TKV>
+template <typename TQ, typename TKV, bool SHARED>
 static int launch_prompt_hd(const PromptArgs& d, const KvMaps& maps, cudaStream_t st) {
   // Two row tiles per item read every key and value once for both; with few
   // rows, or f32 queries (two operands each), an item is one. f16, 32 and 4 heads
@@ -1270,28 +1314,41 @@ static int launch_prompt_hd(const PromptArgs& d, const KvMaps& maps, cudaStream_
   // not count them.)
   const AttnArgs& a = d.a;
   const int64_t pairs = ((int64_t)a.n_rows * (a.nh / a.c.nkv) + 2 * PM - 1) / (2 * PM) * a.c.nkv;
-  const bool two = sizeof(TQ) == 2 && pairs >= num_sms();
+  const bool two = sizeof(TQ) == 2 && !SHARED && pairs >= num_sms();
   switch ((a.c.hd + 63) / 64) {
     case 1:
       if constexpr (sizeof(TQ) == 2)
-        if (two) return launch_prompt<TQ, TKV, 1, true>(d, maps, st);
-      return launch_prompt<TQ, TKV, 1, false>(d, maps, st);
+        if (two) return launch_prompt<TQ, TKV, 1, true, false>(d, maps, st);
+      return launch_prompt<TQ, TKV, 1, false, SHARED>(d, maps, st);
     case 2:
       if constexpr (sizeof(TQ) == 2)
-        if (two) return launch_prompt<TQ, TKV, 2, true>(d, maps, st);
-      return launch_prompt<TQ, TKV, 2, false>(d, maps, st);
-    case 3: return launch_prompt<TQ, TKV, 3, false>(d, maps, st);
-    default: return launch_prompt<TQ, TKV, 4, false>(d, maps, st);
+        if (two) return launch_prompt<TQ, TKV, 2, true, false>(d, maps, st);
+      return launch_prompt<TQ, TKV, 2, false, SHARED>(d, maps, st);
+    case 3: return launch_prompt<TQ, TKV, 3, false, SHARED>(d, maps, st);
+    default: return launch_prompt<TQ, TKV, 4, false, SHARED>(d, maps, st);
   }
 }
 
 int attn_prompt_box_rows(int page, int hd) { return std::min(page, hd <= 128 ? 128 : 64); }
 
+template <bool SHARED>
+static int launch_prompt_types(const PromptArgs& d, const KvMaps& maps, cudaStream_t st) {
+  if (d.a.c.type == T_BF16) return launch_prompt_hd<__nv_bfloat16, __nv_bfloat16, SHARED>(d, maps, st);
+  if (d.a.t_q == T_F32) return launch_prompt_hd<float, __half, SHARED>(d, maps, st);
+  return launch_prompt_hd<__half, __half, SHARED>(d, maps, st);
+}
+
 int launch_attn_prompt(const AttnArgs& a, const KvMaps& maps, float* part, int* count, cudaStream_t st) {
-  const PromptArgs d{a, 1, part, part + PROMPT_PART_BYTES / sizeof(float), count, count + PROMPT_MAX_UNITS, false};
-  if (a.c.type == T_BF16) return launch_prompt_hd<__nv_bfloat16, __nv_bfloat16>(d, maps, st);
-  if (a.t_q == T_F32) return launch_prompt_hd<float, __half>(d, maps, st);
-  return launch_prompt_hd<__half, __half>(d, maps, st);
+  return launch_prompt_types<false>(
+      PromptArgs{a, 1, part, part + PROMPT_PART_BYTES / sizeof(float), count, count + PROMPT_MAX_UNITS, false, {}}, maps,
+      st);
+}
+
+int launch_attn_prefix(const AttnArgs& a, const SharedArgs& sh, const KvMaps& maps, float* part, int* count,
+                       cudaStream_t st) {
+  return launch_prompt_types<true>(
+      PromptArgs{a, 1, part, part + PROMPT_PART_BYTES / sizeof(float), count, count + PROMPT_MAX_UNITS, false, sh}, maps,
+      st);
 }
 
 }  // namespace kc

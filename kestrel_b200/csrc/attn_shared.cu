@@ -1,0 +1,150 @@
+// Attention of one new token per sequence where groups of sequences begin with the
+// same pages: what a group has in common is read and computed once for all of it.
+//
+// The softmax over a sequence's positions splits into that over the common prefix
+// and that over its own rest: with maxima m, sums l and results o of both,
+//   out = (l_1 2^(m_1 - m) o_1 + l_2 2^(m_2 - m) o_2) / (l_1 2^(m_1 - m) + l_2 2^(m_2 - m)).
+// The queries of a group against its prefix are a matrix product of many rows, so
+// the prompt kernel computes them on the tensor cores, split over the prefix where
+// there are few (attn_prompt.cu, SHARED); the decode kernel streams the rest and
+// joins (attn_decode.cu, SHARED). This file looks up what is common: the leading
+// pages that the tables of all of a group's sequences name alike, and that every
+// one of them goes on behind. Nothing is taken on trust, so the result is that of
+// kc_attn_decode_dev whatever the groups are.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kv.h"
+#include "kv_dev.cuh"
+
+namespace kc {
+
+constexpr int PREP_THREADS = 128;
+// Below so many positions a prefix is not worth the way of its results through
+// memory (of n_head heads against n_head_kv keys and values).
+constexpr int SHARED_LEAST = 64;
+constexpr int SHARED_SPLITS = 32;
+constexpr size_t SHARED_PART_BYTES = (size_t)24 << 20;
+
+size_t attn_shared_part_bytes() { return SHARED_PART_BYTES; }
+int attn_shared_counts() { return 1; }
+
+// A block per entry: the pages that its table has in common with that of the first
+// of its group that holds anything. The last block takes the least of each group.
+__global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, const int32_t* __restrict__ seqs, int n,
+                                                                   const int32_t* __restrict__ group_start,
+                                                                   int n_groups, int32_t* of_entry, int32_t* of_group,
+                                                                   int32_t* lead, int* done) {
+  pdl_enter();
+  __shared__ int differ, last, wrong;
+  const int i = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const auto seq = [&](int e) { return seqs ? seqs[e] : e; };
+  const auto holds = [&](int s) { return s >= 0 && s < c.n_seq ? kv_len(c, s) : 0; };
+  if (tid == 0) wrong = 0;
+  {
+    const int g = kv_row_owner(group_start, n_groups, i), s = seq(i), len = holds(s);
+    int pages = 0;
+    if (g >= 0 && len > 0) {
+      int first = max(group_start[g], 0);
+      while (first < i && holds(seq(first)) == 0) ++first;
+      const int s0 = seq(first);
+      pages = (min(len, holds(s0)) - 1) >> c.page_log2;  // (a position behind them is left)
+      if (tid == 0) differ = pages;
+      __syncthreads();
+      const int32_t *x = c.table + (int64_t)s0 * c.max_pages, *y = c.table + (int64_t)s * c.max_pages;
+      for (int p0 = 0; p0 < pages; p0 += 8 * PREP_THREADS) {
+        int at = INT_MAX;
+#pragma unroll
+        for (int u = 7; u >= 0; --u) {
+          const int p = p0 + u * PREP_THREADS + tid;
+          if (p < pages) {
+            const int a = x[p], b = y[p];
+            if (a != b || a < 0 || a >= c.n_pages) at = p;
+          }
+        }
+        if (at != INT_MAX) atomicMin(&differ, at);
+        if (__syncthreads_or(at != INT_MAX)) break;
+      }
+      __syncthreads();
+      pages = differ;
+    }
+    if (tid == 0) of_entry[i] = g < 0 ? 0 : len > 0 ? pages << c.page_log2 : -1;
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(done, 1) == n - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  if (tid == 0) *done = 0;
+  // Groups that do not ascend within the entries: nothing is common.
+  for (int g = tid; g <= n_groups; g += PREP_THREADS) {
+    const int at = group_start[g];
+    if (at < (g ? group_start[g - 1] : 0) || at > n) wrong = 1;
+  }
+  __syncthreads();
+  if (wrong) {
+    if (tid == 0) report(c.status, KC_ERR_ARG | (W_KV_ROWS << 8));
+    for (int e = tid; e < n; e += PREP_THREADS) of_entry[e] = 0;
+    for (int g = tid; g < n_groups; g += PREP_THREADS) of_group[g] = 0;
+    return;
+  }
+  for (int g = warp; g < n_groups; g += PREP_THREADS / 32) {
+    const int lo = group_start[g], hi = group_start[g + 1];
+    int least = INT_MAX, first = INT_MAX, held = 0;
+    for (int e = lo + lane; e < hi; e += 32) {
+      const int both = __ldcg(of_entry + e);
+      if (both < 0) continue;
+      least = min(least, both);
+      first = min(first, e);
+      ++held;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    first = __reduce_min_sync(0xffffffffu, first);
+    held = __reduce_add_sync(0xffffffffu, held);
+    const int both = held > 1 && least >= SHARED_LEAST ? least : 0;
+    for (int e = lo + lane; e < hi; e += 32) of_entry[e] = __ldcg(of_entry + e) < 0 ? 0 : both;
+    if (lane == 0) {
+      of_group[g] = both;
+      lead[g] = held ? seq(first) : 0;
+    }
+  }
+}
+
+int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, const KvMaps& tiles, float* part,
+                       int* count, float* shared_part, cudaStream_t st) {
+  const KvView& c = a.c;
+  const int64_t row = (int64_t)a.nh * shared_row_floats(c.hd), room = (int64_t)(SHARED_PART_BYTES / sizeof(float)) / row;
+  if (a.n < 2 || sh.n_groups < 1 || room < 2) return launch_attn_decode(a, rows16, part, count, st);
+  // Few row tiles: the prefixes are split over the SMs, within the workspace.
+  const int64_t group = a.nh / c.nkv;
+  const int64_t likely = std::max<int64_t>((a.n * group + 127) / 128, std::min(sh.n_groups, a.n / 2)) * c.nkv;
+  sh.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, SHARED_SPLITS, room / a.n}));
+  sh.part = shared_part;
+  int* done = count + std::max(num_sms(), attn_prompt_counts());
+  launch_k(shared_prep_kernel, a.n, PREP_THREADS, 0, st, c, a.seqs, a.n, sh.group_start, sh.n_groups, sh.of_entry,
+           sh.of_group, sh.lead, done);
+  // As many entries at a time as the workspace has room for.
+  const int step = (int)std::min<int64_t>(a.n, room / sh.splits);
+  const int64_t el = a.t_q == T_F32 ? 4 : 2;
+  for (sh.e0 = 0; sh.e0 < a.n; sh.e0 += step) {
+    sh.e1 = std::min(a.n, sh.e0 + step);
+    AttnArgs p = a, own = a;
+    p.seqs = nullptr;
+    p.row_start = sh.group_start;
+    p.n = sh.n_groups;
+    p.n_rows = a.n;
+    int rc = launch_attn_prefix(p, sh, tiles, part, count, st);
+    if (rc != KC_OK) return rc;
+    own.seqs = a.seqs ? a.seqs + sh.e0 : nullptr;
+    own.n = own.n_rows = sh.e1 - sh.e0;
+    own.q = static_cast<const uint8_t*>(a.q) + sh.e0 * a.q_stride * el;
+    own.out = static_cast<uint8_t*>(a.out) + sh.e0 * a.out_stride * el;
+    rc = launch_attn_own(own, sh, rows16, part, count, st);
+    if (rc != KC_OK) return rc;
+  }
+  return KC_OK;
+}
+
+}  // namespace kc

@@ -27,6 +27,7 @@ struct KvView {
   int *first;              // [n_seq] extend: its first entry of `fresh`
   int *fresh;              // [n_pages] extend: the pages it takes, ascending
   int *n_copy;             // entries of src / dst / rows
+  int *both, *both_group, *lead;  // [n_seq] attention over shared prefixes (SharedArgs)
   int *status;
 };
 
@@ -55,7 +56,8 @@ struct KvState {
   float* part = nullptr;  // parts to be joined: the larger of the two kernels' needs
   int* count = nullptr;   // arrival counts, zero between launches
   int64_t count_bytes = 0;
-  int64_t bytes = 0;      // of both
+  int64_t bytes = 0;      // of all
+  float* shared = nullptr;  // between parts and counts: results of shared prefixes
 };
 
 int64_t kv_workspace_ints(const KvView& c);
@@ -85,6 +87,26 @@ struct AttnArgs {
   float scale;
   int window, sinks;         // window 0: none
 };
+// Decode attention of groups of entries whose sequences begin with the same pages:
+// their prefix is computed once for a group (attn_prompt.cu's kernel, its rows the
+// group's queries), the rest entry by entry (attn_decode.cu's), which joins both.
+struct SharedArgs {
+  const int32_t* group_start;  // [n_groups + 1]
+  int n_groups;
+  int32_t* of_entry;           // [n] positions that an entry's group has in common (a multiple of the page; 0: none)
+  int32_t* of_group;           // [n_groups] the same of each group
+  int32_t* lead;               // [n_groups] a sequence of it
+  int e0, e1;                  // entries of this launch
+  int splits;                  // blocks a group's prefix may be split over
+  float* part;                 // [split][entry][head][64 * ceil(hd / 64) + 4]: result, maximum, sum
+};
+// Blocks that a prefix of `both` positions is split over: at least four tiles each.
+__host__ __device__ inline int shared_splits(int both, int hd, int most) {
+  const int tile = hd <= 128 ? 128 : 64, t = (both + tile - 1) / tile / 4;
+  return t < 1 ? 1 : t < most ? t : most;
+}
+__host__ __device__ inline int shared_row_floats(int hd) { return (hd + 63) / 64 * 64 + 4; }
+
 // The query rows of a call as [row][head][column], boxes of 128 (token, head)
 // rows of one key-value head's group (which divides 128) x 128 bytes of columns.
 int make_q_map(const AttnArgs& a, KvMap& map);
@@ -97,5 +119,15 @@ int attn_prompt_box_rows(int page, int hd);
 size_t attn_prompt_part_bytes();
 int attn_prompt_counts();
 int launch_attn_prompt(const AttnArgs& a, const KvMaps& tiles, float* part, int* count, cudaStream_t st);
+
+// (SharedArgs' e0, e1, splits and part are filled in here.)
+int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, const KvMaps& tiles, float* part,
+                       int* count, float* shared_part, cudaStream_t st);
+size_t attn_shared_part_bytes();
+int attn_shared_counts();
+int launch_attn_own(const AttnArgs& a, const SharedArgs& sh, const KvMaps& rows16, float* part, int* count,
+                    cudaStream_t st);
+int launch_attn_prefix(const AttnArgs& a, const SharedArgs& sh, const KvMaps& tiles, float* part, int* count,
+                       cudaStream_t st);
 
 }  // namespace kc

@@ -88,6 +88,7 @@ SIGNATURES = {
     "kc_kv_compact_dev": (I, [P, I, P]),
     "kc_kv_copy_pages_dev": (I, [P, I, P, P, I]),
     "kc_attn_decode_dev": (I, [P, I, I, P, I, I, I, P, I64, F, I, I, P, I64]),
+    "kc_attn_shared_dev": (I, [P, I, I, P, I, P, I, I, I, P, I64, F, P, I64]),
     "kc_attn_prompt_dev": (I, [P, I, I, P, P, I, I, I, I, P, I64, F, I, I, P, I64]),
 }
 
@@ -629,6 +630,15 @@ class Context:
                                              _float_type("q", q), q.data_ptr(), qs,
                                              hd ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
                                              os_))
+
+    def attn_shared_dev(self, cache: int, layer: int, q, group_start, out, seqs=None, scale: float | None = None):
+        """attn_decode_dev for entries in groups (group_start[g] .. group_start[g+1]-1)
+        whose sequences begin with the same pages: those are read once a group."""
+        n, nh, hd, qs, os_ = self._attn(cache, q, out)
+        self._check(lib().kc_attn_shared_dev(self.h, cache, layer, _dev_ints("seqs", seqs, n), n,
+                                             _dev_ints("group_start", group_start), group_start.numel() - 1, nh,
+                                             _float_type("q", q), q.data_ptr(), qs,
+                                             hd ** -0.5 if scale is None else scale, out.data_ptr(), os_))
 
     def attn_prompt_dev(self, cache: int, layer: int, q, row_start, out, seqs=None, scale: float | None = None,
                         window: int = 0, sinks: int = 0):
