@@ -151,56 +151,11 @@ struct DecPart {
   long long unit_at;
 };
 
-// The prefix parts of an entry's head: `n` of them, `step` floats apart, each the
-// result, then its maximum (in exponents of 2) and sum at LD - 4.
-struct PrefixParts {
-  const float* row;
-  int64_t step;
-  int n, at;  // at: LD - 4
-  __device__ __forceinline__ float2 state(int p) const { return __ldcg(reinterpret_cast<const float2*>(row + p * step + at)); }
-  // What a part's result counts for against maximum `base`. (Never quite nothing,
-  // so that an infinite result stays what the formula gives.)
-  __device__ __forceinline__ float share(int p, float base) const {
-    const float2 ml = state(p);
-    return ml.y == 0.f ? 0.f : fmaxf(exp2_fast(ml.x - base), 1e-37f) * ml.y;
-  }
-};
+// SHARED: results go to the join (attn_shared.cu) as f32 rows, behind the parts of
+// the prefix: the values, then at LD - 4 the maximum (in exponents of 2) and sum.
 template <int LD>
-__device__ __forceinline__ PrefixParts prefix_parts(const DecArgs& d, int i, int head) {
-  const int both = d.sh.of_entry[d.sh.e0 + i], n = d.sh.e1 - d.sh.e0;
-  PrefixParts x;
-  x.step = (int64_t)n * d.a.nh * LD;
-  x.row = d.sh.part + ((int64_t)i * d.a.nh + head) * LD;
-  x.n = both > 0 ? shared_splits(both, d.a.c.hd, d.sh.splits) : 0;
-  x.at = LD - 4;
-  return x;
-}
-// Joins an entry's own part (maximum m, sum l) with its prefix: the maximum that
-// shares count from, 1 / the sum, and what the own values count for.
-struct PrefixJoin {
-  float base, inv, own;
-};
-__device__ __forceinline__ PrefixJoin prefix_join(const PrefixParts& x, float m, float l) {
-  PrefixJoin j;
-  j.base = m;
-  for (int p = 0; p < x.n; ++p) j.base = fmaxf(j.base, x.state(p).x);
-  if (j.base == -INFINITY) j.base = 0.f;
-  j.own = l == 0.f ? 0.f : fmaxf(exp2_fast(m - j.base), 1e-37f);
-  float sum = l * j.own;
-  for (int p = 0; p < x.n; ++p) sum += x.share(p, j.base);
-  j.inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-  return j;
-}
-__device__ __forceinline__ float4 prefix_add(const PrefixParts& x, const PrefixJoin& j, int y, float4 v) {
-  for (int p = 0; p < x.n; ++p) {
-    const float w = x.share(p, j.base) * j.inv;
-    const float4 u = __ldcg(reinterpret_cast<const float4*>(x.row + p * x.step + y));
-    v.x = __fmaf_rn(w, u.x, v.x);
-    v.y = __fmaf_rn(w, u.y, v.y);
-    v.z = __fmaf_rn(w, u.z, v.z);
-    v.w = __fmaf_rn(w, u.w, v.w);
-  }
-  return v;
+__device__ __forceinline__ float* own_row(const DecArgs& d, int i, int head) {
+  return d.sh.part + (((int64_t)d.sh.splits * (d.sh.e1 - d.sh.e0) + i) * d.a.nh + head) * LD;
 }
 
 template <typename TQ, typename TKV, int NB, int HT, bool SHARED>
@@ -211,14 +166,16 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   constexpr bool kSplit = HT == 8;               // rows 8 .. 15 carry the rests
   constexpr bool kHalf = std::is_same_v<TKV, __half>;
   constexpr float kLift = kHalf ? 15.f : 0.f;    // f16 weights up to 2^15: small ones keep their bits
-  pdl_enter();
+  // SHARED: beside the prefixes' kernel, whose blocks have all seen the end of what
+  // came before it when these start; it is waited for at the end.
+  if constexpr (SHARED) pdl_trigger();
+  else pdl_enter();
   extern __shared__ uint8_t dec_raw[];
   __shared__ __align__(8) uint64_t full[W][ST];
   __shared__ long long red[3][W], found_at[W];
   __shared__ int found[W];
   __shared__ DecPart parts_sh[2 * W];  // per warp: of its range's first segment, and of its last
   __shared__ int last_sh[2];
-  __shared__ PrefixJoin join_sh[SHARED ? HT : 1];
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -248,6 +205,11 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       none = real && here == 0 && i % gridDim.x == blockIdx.x;
     }
     for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
+      if constexpr (SHARED) {
+        for (int h = lane; h < a.nh; h += 32)
+          *reinterpret_cast<float2*>(own_row<LD>(d, i0 + __ffs(rows) - 1, h) + S::HD) = make_float2(-INFINITY, 0.f);
+        continue;
+      }
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)(i0 + __ffs(rows) - 1) * a.out_stride;
       for (int x = lane; x < a.nh * c.hd; x += 32) out[x] = (TQ)0.f;
     }
@@ -279,7 +241,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     most = max(most, (int)red[1][w]);
   }
   line *= units;
-  if (line == 0) return;
+  if (line == 0) {
+    if constexpr (SHARED) pdl_wait();
+    return;
+  }
   // Equal ranges of at least one chunk per warp. When the units are few, each
   // is cut into the same whole number of parts instead (its stretch of the line
   // padded to `pad` chunks) where that is not slower: ranges that begin with
@@ -301,7 +266,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
     }
   }
   const long long block_at = blockIdx.x * per, block_end = min(line, block_at + per), share_of = per / W;
-  if (block_at >= block_end) return;
+  if (block_at >= block_end) {
+    if constexpr (SHARED) pdl_wait();
+    return;
+  }
   SegIter at;
   // A block of one unit's part deals its chunks to the warps in turn (so that
   // they read side by side: 131071 positions took 56.5 us, in stretches 57.2);
@@ -644,30 +612,14 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       for (int rr = 0; rr < RH; ++rr) {
         const int h = r0 + 8 * rr;
         if (h0 + h >= group) continue;
-        float inv;
+        const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
         if constexpr (SHARED) {
-          const PrefixParts x = prefix_parts<LD>(d, at.i, kvh * group + h0 + h);
-          const PrefixJoin j = prefix_join(x, m[rr] - kLift, l[rr]);
-          inv = j.own * j.inv;
-          if (x.n) {
+          float* row = own_row<LD>(d, at.i, kvh * group + h0 + h);
 #pragma unroll
-            for (int t = 0; t < 8 * NB; ++t) {
-              o[t][2 * rr] *= inv;
-              o[t][2 * rr + 1] *= inv;
-            }
-            for (int p = 0; p < x.n; ++p) {
-              const float w = x.share(p, j.base) * j.inv;
-#pragma unroll
-              for (int t = 0; t < 8 * NB; ++t) {
-                const float2 u = __ldcg(reinterpret_cast<const float2*>(x.row + p * x.step + 8 * t + cc));
-                o[t][2 * rr] = __fmaf_rn(w, u.x, o[t][2 * rr]);
-                o[t][2 * rr + 1] = __fmaf_rn(w, u.y, o[t][2 * rr + 1]);
-              }
-            }
-            inv = 1.f;
-          }
-        } else {
-          inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
+          for (int t = 0; t < 8 * NB; ++t)
+            *reinterpret_cast<float2*>(row + 8 * t + cc) = make_float2(o[t][2 * rr] * inv, o[t][2 * rr + 1] * inv);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(row + S::HD) = make_float2(m[rr] - kLift, l[rr]);
+          continue;
         }
 #pragma unroll
         for (int t = 0; t < 8 * NB; ++t)
@@ -771,15 +723,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
       if (whole) {
         if (h0 + h >= group || y >= c.hd) continue;
-        float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
+        const float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
         if constexpr (SHARED) {
-          const PrefixParts px = prefix_parts<LD>(d, g.i, kvh * group + h0 + h);
-          if (px.n) {
-            const PrefixJoin j = prefix_join(px, ml.x - kLift, ml.y);
-            const float own = j.own * j.inv;
-            v = prefix_add(px, j, y, make_float4(v.x * own, v.y * own, v.z * own, v.w * own));
-            inv = 1.f;
-          }
+          float* row = own_row<LD>(d, g.i, kvh * group + h0 + h);
+          *reinterpret_cast<float4*>(row + y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          if (y == 0) *reinterpret_cast<float2*>(row + S::HD) = make_float2(ml.x - kLift, ml.y);
+          continue;
         }
         TQ* to = out + (int64_t)h * c.hd + y;
         to[0] = (TQ)(v.x * inv);
@@ -793,7 +742,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
     }
   }
-  if (cut[0] < 0 && cut[1] < 0) return;
+  if (cut[0] < 0 && cut[1] < 0) {
+    if constexpr (SHARED) pdl_wait();
+    return;
+  }
 
   // ---- units of several blocks: the last to come joins the parts ---------------------
   __threadfence();
@@ -843,13 +795,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-      if constexpr (SHARED) {
-        const PrefixParts px = prefix_parts<LD>(d, g.i, kvh * group + min(h0 + h, group - 1));
-        const PrefixJoin j = prefix_join(px, top - kLift, total);
-        inv = j.own * j.inv;
-        if (lane == 0) join_sh[h] = j;
-      }
+      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+      if constexpr (SHARED)
+        if (lane == 0 && h0 + h < group)
+          *reinterpret_cast<float2*>(own_row<LD>(d, g.i, kvh * group + h0 + h) + S::HD) = make_float2(top - kLift, total);
 #pragma unroll
       for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
         if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
@@ -874,8 +823,10 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
           sum4.w = __fmaf_rn(w, v[k].w, sum4.w);
         }
       }
-      if constexpr (SHARED)
-        sum4 = prefix_add(prefix_parts<LD>(d, g.i, kvh * group + h0 + h), join_sh[h], y, sum4);
+      if constexpr (SHARED) {
+        *reinterpret_cast<float4*>(own_row<LD>(d, g.i, kvh * group + h0 + h) + y) = sum4;
+        continue;
+      }
       TQ* to = out + (int64_t)h * c.hd + y;
       to[0] = (TQ)sum4.x;
       to[1] = (TQ)sum4.y;
@@ -883,6 +834,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       to[3] = (TQ)sum4.w;
     }
   }
+  if constexpr (SHARED) pdl_wait();
 }
 
 size_t attn_decode_part_bytes() { return (size_t)num_sms() * 2 * 16 * (256 + 4) * sizeof(float); }

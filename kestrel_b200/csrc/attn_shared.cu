@@ -6,11 +6,14 @@
 //   out = (l_1 2^(m_1 - m) o_1 + l_2 2^(m_2 - m) o_2) / (l_1 2^(m_1 - m) + l_2 2^(m_2 - m)).
 // The queries of a group against its prefix are a matrix product of many rows, so
 // the prompt kernel computes them on the tensor cores, split over the prefix where
-// there are few (attn_prompt.cu, SHARED); the decode kernel streams the rest and
-// joins (attn_decode.cu, SHARED). This file looks up what is common: the leading
-// pages that the tables of all of a group's sequences name alike, and that every
-// one of them goes on behind. Nothing is taken on trust, so the result is that of
-// kc_attn_decode_dev whatever the groups are.
+// there are few (attn_prompt.cu, SHARED), and the decode kernel streams the rest
+// (attn_decode.cu, SHARED), beside it where SMs are free. This file looks up before
+// what is common: the leading pages that the tables of all of a group's sequences
+// name alike, and that every one of them goes on behind. Nothing is taken on trust,
+// so the result is that of kc_attn_decode_dev whatever the groups are. And it joins
+// the parts, a warp per head of an entry. (Joined by the decode kernel's blocks at
+// the end of each sequence, one read after the other, 64 entries at 32768 positions
+// took 145 us.)
 #include <algorithm>
 
 #include "common.cuh"
@@ -24,7 +27,7 @@ constexpr int PREP_THREADS = 128;
 // Below so many positions a prefix is not worth the way of its results through
 // memory (of n_head heads against n_head_kv keys and values).
 constexpr int SHARED_LEAST = 64;
-constexpr int SHARED_SPLITS = 32;
+constexpr int SHARED_SPLITS = 31;  // (a lane each in the join, and one for the own part)
 constexpr size_t SHARED_PART_BYTES = (size_t)24 << 20;
 
 size_t attn_shared_part_bytes() { return SHARED_PART_BYTES; }
@@ -112,21 +115,75 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
   }
 }
 
+// A warp per (entry, head): the parts' maxima and sums a lane each, then their
+// values, 16 bytes a lane, eight parts under way.
+template <typename T>
+__global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArgs a, const SharedArgs sh) {
+  pdl_enter();
+  const KvView& c = a.c;
+  const int lane = threadIdx.x & 31, ld = shared_row_floats(c.hd), n = sh.e1 - sh.e0;
+  const int64_t row = (int64_t)blockIdx.x * (PREP_THREADS / 32) + (threadIdx.x >> 5);
+  if (row >= (int64_t)n * a.nh) return;
+  const int i = (int)(row / a.nh), s = a.seqs ? a.seqs[sh.e0 + i] : sh.e0 + i;
+  if (s < 0 || s >= c.n_seq) return;
+  const int both = sh.of_entry[sh.e0 + i], splits = both > 0 ? shared_splits(both, c.hd, sh.splits) : 0;
+  const int64_t step = (int64_t)n * a.nh * ld;
+  // Lane p: part p of the prefix; lane `splits`: the own one.
+  const float* mine = sh.part + row * ld + (lane < splits ? lane : sh.splits) * step;
+  const float2 ml = lane <= splits ? __ldcg(reinterpret_cast<const float2*>(mine + ld - 4)) : make_float2(-INFINITY, 0.f);
+  float top = ml.y == 0.f ? -INFINITY : ml.x;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // (Never quite nothing, so that an infinite result stays what the formula gives.)
+  float share = ml.y == 0.f ? 0.f : fmaxf(exp2f(ml.x - (top == -INFINITY ? 0.f : top)), 1e-37f) * ml.y, sum = share;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  share = sum == 0.f ? 0.f : __fdiv_rn(share, sum);
+  T* out = static_cast<T*>(a.out) + (int64_t)(sh.e0 + i) * a.out_stride + (row - (int64_t)i * a.nh) * c.hd;
+  for (int y0 = 0; y0 < c.hd; y0 += 128) {
+    const int y = y0 + 4 * lane;
+    const bool mine_y = y < c.hd;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 <= splits; p0 += 8) {
+      float4 u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (p0 + k <= splits && mine_y)
+          u[k] = __ldcg(reinterpret_cast<const float4*>(sh.part + row * ld + (p0 + k < splits ? p0 + k : sh.splits) * step + y));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, share, min(p0 + k, 31));
+        if (p0 + k <= splits && mine_y && w != 0.f) {
+          v.x = __fmaf_rn(w, u[k].x, v.x);
+          v.y = __fmaf_rn(w, u[k].y, v.y);
+          v.z = __fmaf_rn(w, u[k].z, v.z);
+          v.w = __fmaf_rn(w, u[k].w, v.w);
+        }
+      }
+    }
+    if (!mine_y) continue;
+    out[y] = (T)v.x;
+    out[y + 1] = (T)v.y;
+    out[y + 2] = (T)v.z;
+    out[y + 3] = (T)v.w;
+  }
+}
+
 int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, const KvMaps& tiles, float* part,
                        int* count, float* shared_part, cudaStream_t st) {
   const KvView& c = a.c;
   const int64_t row = (int64_t)a.nh * shared_row_floats(c.hd), room = (int64_t)(SHARED_PART_BYTES / sizeof(float)) / row;
-  if (a.n < 2 || sh.n_groups < 1 || room < 2) return launch_attn_decode(a, rows16, part, count, st);
+  if (a.n < 2 || sh.n_groups < 1 || room < 4) return launch_attn_decode(a, rows16, part, count, st);
   // Few row tiles: the prefixes are split over the SMs, within the workspace.
   const int64_t group = a.nh / c.nkv;
   const int64_t likely = std::max<int64_t>((a.n * group + 127) / 128, std::min(sh.n_groups, a.n / 2)) * c.nkv;
-  sh.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, SHARED_SPLITS, room / a.n}));
+  sh.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, SHARED_SPLITS, room / a.n - 1}));
   sh.part = shared_part;
   int* done = count + std::max(num_sms(), attn_prompt_counts());
   launch_k(shared_prep_kernel, a.n, PREP_THREADS, 0, st, c, a.seqs, a.n, sh.group_start, sh.n_groups, sh.of_entry,
            sh.of_group, sh.lead, done);
   // As many entries at a time as the workspace has room for.
-  const int step = (int)std::min<int64_t>(a.n, room / sh.splits);
+  const int step = (int)std::min<int64_t>(a.n, room / (sh.splits + 1));
   const int64_t el = a.t_q == T_F32 ? 4 : 2;
   for (sh.e0 = 0; sh.e0 < a.n; sh.e0 += step) {
     sh.e1 = std::min(a.n, sh.e0 + step);
@@ -143,6 +200,11 @@ int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, c
     own.out = static_cast<uint8_t*>(a.out) + sh.e0 * a.out_stride * el;
     rc = launch_attn_own(own, sh, rows16, part, count, st);
     if (rc != KC_OK) return rc;
+    const int64_t rows = (int64_t)own.n * a.nh;
+    const int grid = (int)((rows + PREP_THREADS / 32 - 1) / (PREP_THREADS / 32));
+    if (a.t_q == T_F32) launch_k(shared_join_kernel<float>, grid, PREP_THREADS, 0, st, a, sh);
+    else if (a.t_q == T_F16) launch_k(shared_join_kernel<__half>, grid, PREP_THREADS, 0, st, a, sh);
+    else launch_k(shared_join_kernel<__nv_bfloat16>, grid, PREP_THREADS, 0, st, a, sh);
   }
   return KC_OK;
 }

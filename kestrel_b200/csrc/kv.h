@@ -98,7 +98,9 @@ struct SharedArgs {
   int32_t* lead;               // [n_groups] a sequence of it
   int e0, e1;                  // entries of this launch
   int splits;                  // blocks a group's prefix may be split over
-  float* part;                 // [split][entry][head][64 * ceil(hd / 64) + 4]: result, maximum, sum
+  // [split + 1][entry][head][64 * ceil(hd / 64) + 4]: result, maximum, sum; of the
+  // parts of the prefix, then of the entries' own
+  float* part;
 };
 // Blocks that a prefix of `both` positions is split over: at least four tiles each.
 __host__ __device__ inline int shared_splits(int both, int hd, int most) {
