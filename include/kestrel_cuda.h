@@ -325,7 +325,10 @@ enum {
   KC_OPT_F32_PREFILL = 1,
   /* value 1 (default): the whole-model path predicts the next host-streamed
      layer's experts and prefetches them (router lookahead); 0: off. */
-  KC_OPT_LOOKAHEAD = 2
+  KC_OPT_LOOKAHEAD = 2,
+  /* value 0 (default): kc_attn_shared_dev shares what a group has in common where
+     that is expected to take less time; 1: wherever there is a page of it. */
+  KC_OPT_SHARE_ALWAYS = 3
 };
 KC_API int kc_set_option(kc_ctx* ctx, int option, int value);
 

@@ -85,6 +85,7 @@ pub const KC_N_STAGES: c_int = 11;
 // kc_set_option options
 pub const KC_OPT_F32_PREFILL: c_int = 1;
 pub const KC_OPT_LOOKAHEAD: c_int = 2;
+pub const KC_OPT_SHARE_ALWAYS: c_int = 3;
 
 // rotary positions (kc_rope layout and scaling)
 pub const KC_ROPE_INTERLEAVED: c_int = 0;

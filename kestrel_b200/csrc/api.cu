@@ -2513,6 +2513,10 @@ int kc_set_option(kc_ctx* ctx, int option, int value) {
     ctx->xs.lookahead = value != 0;
     return KC_OK;
   }
+  if (option == KC_OPT_SHARE_ALWAYS) {
+    ctx->kv.share_always = value != 0;
+    return KC_OK;
+  }
 
   return fail(ctx, KC_ERR_ARG, "kc_set_option: unknown option %d", option);
 }
@@ -3093,6 +3097,8 @@ int attn_call(kc_ctx* ctx, int cache, const char* what, int layer, const int32_t
     sh.of_entry = c.both;
     sh.of_group = c.both_group;
     sh.lead = c.lead;
+    sh.plan = c.plan;
+    sh.always = ctx->kv.share_always;
     const int rc = prompt   ? launch_attn_prompt(a, kv.tiles, ctx->kv.part, ctx->kv.count, ctx->stream)
                    : shared ? launch_attn_shared(a, sh, kv.rows16, kv.tiles, ctx->kv.part, ctx->kv.count,
                                                  ctx->kv.shared, ctx->stream)

@@ -152,10 +152,10 @@ struct DecPart {
 };
 
 // SHARED: results go to the join (attn_shared.cu) as f32 rows, behind the parts of
-// the prefix: the values, then at LD - 4 the maximum (in exponents of 2) and sum.
-template <int LD>
+// the prefix: the values, then at HD the maximum (in exponents of 2) and sum.
+template <int HD>
 __device__ __forceinline__ float* own_row(const DecArgs& d, int i, int head) {
-  return d.sh.part + (((int64_t)d.sh.splits * (d.sh.e1 - d.sh.e0) + i) * d.a.nh + head) * LD;
+  return d.sh.part + (((int64_t)d.sh.splits * (d.sh.e1 - d.sh.e0) + i) * d.a.nh + head) * (HD + 8);
 }
 
 template <typename TQ, typename TKV, int NB, int HT, bool SHARED>
@@ -182,6 +182,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   uint8_t* ring = dec_raw + ((1024 - (smem_u32(dec_raw) & 1023)) & 1023);
   float* firsts = reinterpret_cast<float*>(ring + W * ST * S::CHUNK);
   const int group = a.nh / c.nkv, tiles = (group + HT - 1) / HT, units = c.nkv * tiles;
+  // SHARED: the other blocks' SMs are the prefixes'.
+  const int blocks = SHARED ? min((int)gridDim.x, d.sh.plan[PLAN_OWN]) : gridDim.x;
+  if (SHARED && blockIdx.x >= blocks) {
+    pdl_wait();
+    return;
+  }
   if (lane == 0) {
     for (int s = 0; s < ST; ++s) mbar_init(&full[warp][s], 1);
     fence_mbar_init();
@@ -202,12 +208,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       const bool real = s >= 0 && s < c.n_seq;
       if (real) here = dec_span<SHARED>(kv_len(c, s), a.window, a.sinks, dec_before<SHARED>(d, i)).n;
       else if (blockIdx.x == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
-      none = real && here == 0 && i % gridDim.x == blockIdx.x;
+      none = real && here == 0 && i % blocks == blockIdx.x;
     }
     for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
       if constexpr (SHARED) {
         for (int h = lane; h < a.nh; h += 32)
-          *reinterpret_cast<float2*>(own_row<LD>(d, i0 + __ffs(rows) - 1, h) + S::HD) = make_float2(-INFINITY, 0.f);
+          *reinterpret_cast<float2*>(own_row<S::HD>(d, i0 + __ffs(rows) - 1, h) + S::HD) = make_float2(-INFINITY, 0.f);
         continue;
       }
       TQ* out = static_cast<TQ*>(a.out) + (int64_t)(i0 + __ffs(rows) - 1) * a.out_stride;
@@ -252,12 +258,12 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   // needs no join. (A segment's end and a join take about as long as two and
   // four more rounds of chunks: 32 sequences of 2048 positions took 37 us in
   // equal ranges and 29 in one part each.)
-  long long per = max(div_ll(line + gridDim.x - 1, gridDim.x), (long long)W);
+  long long per = max(div_ll(line + blocks - 1, blocks), (long long)W);
   per = (per + W - 1) / W * W;
   const long long all = (long long)a.n * units;
   int pad = 0;
-  if (all <= gridDim.x) {
-    const int parts = (int)(gridDim.x / (uint32_t)all);
+  if (all <= blocks) {
+    const int parts = (int)((uint32_t)blocks / (uint32_t)all);
     const int q = ((most + parts - 1) / parts + W - 1) / W * W;
     if (q <= per + (parts == 1 ? 6 : 2) * W) {
       per = q;
@@ -614,7 +620,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         if (h0 + h >= group) continue;
         const float inv = l[rr] == 0.f ? 0.f : __fdiv_rn(1.f, l[rr]);
         if constexpr (SHARED) {
-          float* row = own_row<LD>(d, at.i, kvh * group + h0 + h);
+          float* row = own_row<S::HD>(d, at.i, kvh * group + h0 + h);
 #pragma unroll
           for (int t = 0; t < 8 * NB; ++t)
             *reinterpret_cast<float2*>(row + 8 * t + cc) = make_float2(o[t][2 * rr] * inv, o[t][2 * rr + 1] * inv);
@@ -725,7 +731,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         if (h0 + h >= group || y >= c.hd) continue;
         const float inv = ml.y == 0.f ? 0.f : __fdiv_rn(1.f, ml.y);
         if constexpr (SHARED) {
-          float* row = own_row<LD>(d, g.i, kvh * group + h0 + h);
+          float* row = own_row<S::HD>(d, g.i, kvh * group + h0 + h);
           *reinterpret_cast<float4*>(row + y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
           if (y == 0) *reinterpret_cast<float2*>(row + S::HD) = make_float2(ml.x - kLift, ml.y);
           continue;
@@ -798,7 +804,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
       const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
       if constexpr (SHARED)
         if (lane == 0 && h0 + h < group)
-          *reinterpret_cast<float2*>(own_row<LD>(d, g.i, kvh * group + h0 + h) + S::HD) = make_float2(top - kLift, total);
+          *reinterpret_cast<float2*>(own_row<S::HD>(d, g.i, kvh * group + h0 + h) + S::HD) = make_float2(top - kLift, total);
 #pragma unroll
       for (int u = 0; u < DEC_MAX_PARTS / 32; ++u)
         if (lane + 32 * u < parts) share[h * parts + lane + 32 * u] = ml[u].x * inv;
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
         }
       }
       if constexpr (SHARED) {
-        *reinterpret_cast<float4*>(own_row<LD>(d, g.i, kvh * group + h0 + h) + y) = sum4;
+        *reinterpret_cast<float4*>(own_row<S::HD>(d, g.i, kvh * group + h0 + h) + y) = sum4;
         continue;
       }
       TQ* to = out + (int64_t)h * c.hd + y;

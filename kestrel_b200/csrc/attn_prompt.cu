@@ -358,6 +358,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   const AttnArgs& a = d.a;
   const KvView& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // SHARED: as many blocks and parts of a prefix as the device has planned.
+  const int splits = SHARED ? d.sh.plan[PLAN_SPLITS] : d.splits;
+  const int blocks = SHARED ? min((int)gridDim.x, d.sh.plan[PLAN_PREFIX]) : gridDim.x;
+  if (SHARED && blockIdx.x >= blocks) return;
   const int group = a.nh / c.nkv;
   const int hd16 = (c.hd + 15) / 16 * 16;  // columns of the products that are computed
   const float flip = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;  // into the queries: score factors are positive
@@ -458,12 +462,9 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         if (lane >= pieces || t >= x.t1) return -1;
         const int p = x.pos(t, BN) + lane * piece;
         if (p >= x.len) return -1;
-        const int id = c.table[(int64_t)x.s * c.max_pages + (p >> c.page_log2)];
-        if (id < 0 || id >= c.n_pages) {
-          report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
-          return -1;
-        }
-        return id;
+        // (Looked at where it is used: the look-ups of the tiles ahead are under way
+        // together.)
+        return c.table[(int64_t)x.s * c.max_pages + (p >> c.page_log2)];
       };
       auto load = [&](const KvMap* map, int t, int id) {
         const int st = it % ST;
@@ -475,7 +476,9 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         __syncwarp();
         if (lane < pieces) {
           const int p = x.pos(t, BN) + lane * piece;
-          const int lp = id >= 0 ? a.layer * c.n_pages + id : c.n_layer * c.n_pages;  // past the pool: zeros
+          const bool in_pool = id >= 0 && id < c.n_pages;
+          if (!in_pool && p < x.len) report(c.status, KC_ERR_ARG | (W_KV_PAGE << 8));
+          const int lp = in_pool ? a.layer * c.n_pages + id : c.n_layer * c.n_pages;  // past the pool: zeros
 #pragma unroll
           for (int b = 0; b < NB; ++b)
             kv_load(to + b * BN * 128 + lane * piece * 128, map, 64 * b, p & (c.page - 1), x.kvh, lp, &kv_full[st]);
@@ -674,13 +677,20 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     };
     // Up to 32 entries are taken in the order of their positions, most last
     // (items are dealt from the end); this lane holds the lane-th of them.
-    int e_i = lane, e_lo = 0, e_hi = 0, e_len = 0, e_sum = 0, tiles = 0;
+    int e_i = lane, e_lo = 0, e_hi = 0, e_len = 0, e_sum = 0, tiles = 0, e_lead = 0;  // (e_lead: the lane-th entry's)
     const bool sorted = a.n <= 32;
     if (finder) {
       if (sorted) {
-        int len;
+        int len = 0, m = 0;
         if constexpr (SHARED) {
-          len = lane < a.n ? d.sh.of_group[lane] : 0;
+          if (lane < a.n) {
+            len = d.sh.of_group[lane];
+            e_lead = d.sh.lead[lane];
+            e_lo = max(a.row_start[lane], d.sh.e0);
+            e_hi = max(e_lo, min(a.row_start[lane + 1], d.sh.e1));
+          }
+          if (len == 0) e_lo = e_hi = 0;
+          m = (int)(((int64_t)(e_hi - e_lo) * group + S::QT * PM - 1) / (S::QT * PM));
         } else {
           const int s = lane < a.n ? (a.seqs ? a.seqs[lane] : lane) : -1;
           len = s >= 0 && s < c.n_seq ? kv_len(c, s) : 0;
@@ -693,7 +703,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
         for (int j = 0; j < 32; ++j)
           if (__shfl_sync(0xffffffffu, rank, j) == lane) e_i = j;
         int last = 0;
-        const int m = tiles_of(lane, last, e_lo, e_hi);
+        if constexpr (!SHARED) m = tiles_of(lane, last, e_lo, e_hi);
         e_lo = __shfl_sync(0xffffffffu, e_lo, e_i);
         e_hi = __shfl_sync(0xffffffffu, e_hi, e_i);
         e_len = __shfl_sync(0xffffffffu, len, e_i);
@@ -706,7 +716,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       }
     }
     known = true;
-    const int64_t total = (int64_t)tiles * c.nkv * d.splits;
+    const int64_t total = (int64_t)tiles * c.nkv * splits;
     int used = 0;
     int64_t idx = blockIdx.x;  // the block's first item; the rest as it comes to them
     bool dealt = false;
@@ -717,13 +727,13 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           if (dealt) {
             int more = 0;
             if (lane == 0) more = atomicAdd(d.next, 1);
-            idx = (int64_t)gridDim.x + __shfl_sync(0xffffffffu, more, 0);
+            idx = (int64_t)blocks + __shfl_sync(0xffffffffu, more, 0);
           }
           dealt = true;
           x.valid = idx < total;
           if (!x.valid) break;
-          x.split = (int)(idx % d.splits);
-          x.unit = (int)(total / d.splits - 1 - idx / d.splits);
+          x.split = (int)(idx % splits);
+          x.unit = (int)(total / splits - 1 - idx / splits);
           x.kvh = x.unit % c.nkv;
           int t = x.unit / c.nkv, l = 0, i = 0;
           if (sorted) {
@@ -751,7 +761,8 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             }
           }
           x.row0 = t * S::QT * PM;
-          x.s = SHARED ? d.sh.lead[i] : a.seqs ? a.seqs[i] : i;
+          if constexpr (SHARED) x.s = sorted ? __shfl_sync(0xffffffffu, e_lead, i & 31) : d.sh.lead[i];
+          else x.s = a.seqs ? a.seqs[i] : i;
           if (x.s < 0 || x.s >= c.n_seq) {
             if (lane == 0) report(c.status, KC_ERR_ARG | (W_KV_SEQ << 8));
             continue;
@@ -769,7 +780,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             x.nt = x.head + at1 / BN + 1 - x.w0;
           }
           // At least four tiles to a part: a join takes about as long.
-          x.splits = max(1, min(d.splits, x.nt / 4));
+          x.splits = SHARED ? shared_splits(x.len, c.hd, splits) : max(1, min(splits, x.nt / 4));
           if (x.split >= x.splits) continue;
           x.t0 = (int)((int64_t)x.nt * x.split / x.splits);
           x.t1 = (int)((int64_t)x.nt * (x.split + 1) / x.splits);
@@ -849,7 +860,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
     // Every load lands before the block may end.
     if (kSplit && finder && d.q_map && used > 0) mbar_wait(&q_raw, (used - 1) & 1, c.status, W_ATT_PROMPT);
     // The last block to find nothing left puts the counters back.
-    if (finder && lane == 0 && atomicAdd(d.next + 1, 1) == (int)gridDim.x - 1) d.next[0] = d.next[1] = 0;
+    if (finder && lane == 0 && atomicAdd(d.next + 1, 1) == blocks - 1) d.next[0] = d.next[1] = 0;
   } else {
     if constexpr (NS == 2) regs_up<kSoftmaxRegs>();
     // ---- softmax: stream w, a thread per row ---------------------------------
@@ -1120,7 +1131,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       TQ* to_row = out + rm.offset(real ? f : 0, a.out_stride, c.hd);
       float* part_row = d.part + ((int64_t)x.unit * d.splits + x.split) * S::PART + 4 * r;
       // SHARED: the row of its (split, entry, head) for the join.
-      constexpr int JOIN_LD = S::HD + 4;
+      constexpr int JOIN_LD = S::HD + 8, JOIN_GRAIN = JOIN_LD * 4;  // (rows of whole sectors)
       float* join_row = nullptr;
       if constexpr (SHARED)
         join_row = d.sh.part + (((int64_t)x.split * (d.sh.e1 - d.sh.e0) + x.start - d.sh.e0) * a.nh + x.kvh * group) * JOIN_LD +
@@ -1153,10 +1164,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           const int e1 = e0 + 16 * y;
           if constexpr (SHARED) {
             bad |= normalise16(o[y], inv);
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(join_row + e1 + e) =
-                  make_float4(o[y][e], o[y][e + 1], o[y][e + 2], o[y][e + 3]);
+            store16(join_row + e1, o[y], 16, JOIN_GRAIN);
             if (e1 == 0) *reinterpret_cast<float2*>(join_row + S::HD) = make_float2(m - kLift, l);
             continue;
           }

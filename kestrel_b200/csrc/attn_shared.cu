@@ -24,29 +24,80 @@
 namespace kc {
 
 constexpr int PREP_THREADS = 128;
-// Below so many positions a prefix is not worth the way of its results through
-// memory (of n_head heads against n_head_kv keys and values).
-constexpr int SHARED_LEAST = 64;
 constexpr int SHARED_SPLITS = 31;  // (a lane each in the join, and one for the own part)
 constexpr size_t SHARED_PART_BYTES = (size_t)24 << 20;
 
 size_t attn_shared_part_bytes() { return SHARED_PART_BYTES; }
 int attn_shared_counts() { return 1; }
 
+// What the two kernels take, in us, as measured on a B200: until their first
+// products and after their last, for a step of 128 (64) positions of a row tile, and
+// by the bytes that an SM, and all of them, take in.
+constexpr float PREFIX_FIXED = 9.f, ITEM_FIXED = 6.f, PREFIX_STEP = 1.15f, PREFIX_STEP_F32 = 1.8f;
+constexpr float OWN_FIXED = 16.f, DECODE_FIXED = 9.f, PREP_AND_JOIN = 12.f;
+constexpr float BESIDE_BYTES = 2.8e4f, SM_BYTES = 4.2e4f, ALL_BYTES = 5.8e6f, SEEN_BYTES = 8.5e6f;  // (of pages that L2 has seen before)
+
+// The plan, by one warp: a lane per number of SMs that the prefixes get, the last
+// one for all SMs to both in turn. False: not shared it takes no longer.
+struct PlanSums {
+  int units;    // row tiles of the prefixes, over the heads
+  int longest;  // tiles of the longest prefix
+  float steps;  // tiles of all units
+  float prefix, own, all;  // positions: of the prefixes, the own parts, and not shared
+};
+__device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, bool f32, int sms, int most, int32_t* plan) {
+  const int lane = threadIdx.x & 31;
+  const float bytes = 4.f * c.hd * c.nkv;
+  const bool turns = lane == 31;
+  const int g = turns ? sms : max(1, (lane + 1) * sms / 32), rest = turns ? sms : sms - g;
+  // A step alone, or with its part of the memory rate, which row tiles that read the
+  // same positions share.
+  float step = f32 ? PREFIX_STEP_F32 : PREFIX_STEP;
+  if (!turns) step = fmaxf(step, __fdividef(t.prefix * bytes, t.steps * BESIDE_BYTES));
+  // Items (units by parts) go over the g SMs in rounds.
+  int splits = 1;
+  float prefix = INFINITY;
+  const float units = t.units, longest = t.longest, per = __fdividef(1.f, (float)g);
+  for (int p = 1; p <= min(most, max(1, t.longest / 2)); ++p) {
+    const float took = PREFIX_FIXED + ceilf(units * p * per - 1e-3f) * (ITEM_FIXED + step * ceilf(__fdividef(longest, (float)p)));
+    if (took < prefix) {
+      prefix = took;
+      splits = p;
+    }
+  }
+  prefix = fmaxf(prefix, PREFIX_FIXED + t.prefix * bytes / ALL_BYTES);
+  // (Side by side they share the memory rate.)
+  const float own = OWN_FIXED + fmaxf(t.own * bytes / (rest * SM_BYTES), (t.own + (turns ? 0 : t.prefix)) * bytes / ALL_BYTES);
+  const float both = PREP_AND_JOIN + (turns ? prefix + own : fmaxf(prefix, own));
+  const unsigned best = __reduce_min_sync(0xffffffffu, __float_as_uint(both));
+  const unsigned who = __ballot_sync(0xffffffffu, __float_as_uint(both) == best);
+  if (lane == __ffs(who) - 1) {
+    plan[PLAN_SPLITS] = splits;
+    plan[PLAN_PREFIX] = g;
+    plan[PLAN_OWN] = rest;
+  }
+  return __uint_as_float(best) < DECODE_FIXED + t.all * bytes / SEEN_BYTES;
+}
+
 // A block per entry: the pages that its table has in common with that of the first
 // of its group that holds anything. The last block takes the least of each group.
 __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, const int32_t* __restrict__ seqs, int n,
                                                                    const int32_t* __restrict__ group_start,
                                                                    int n_groups, int32_t* of_entry, int32_t* of_group,
-                                                                   int32_t* lead, int* done) {
+                                                                   int32_t* lead, int* done, int group, bool f32,
+                                                                   int sms, int most, bool whole, bool always, int32_t* plan) {
   pdl_enter();
-  __shared__ int differ, last, wrong;
+  __shared__ int differ, last, wrong, shares;
+  __shared__ PlanSums sums;
   const int i = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const auto seq = [&](int e) { return seqs ? seqs[e] : e; };
   const auto holds = [&](int s) { return s >= 0 && s < c.n_seq ? kv_len(c, s) : 0; };
-  if (tid == 0) wrong = 0;
+  if (tid == 0) {
+    wrong = 0;
+    sums = PlanSums{};
+  }
   {
-    const int g = kv_row_owner(group_start, n_groups, i), s = seq(i), len = holds(s);
+    const int s = seq(i), len = holds(s), g = kv_row_owner(group_start, n_groups, i);
     int pages = 0;
     if (g >= 0 && len > 0) {
       int first = max(group_start[g], 0);
@@ -80,7 +131,11 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
   __syncthreads();
   if (!last) return;
   __threadfence();
-  if (tid == 0) *done = 0;
+  if (tid == 0) {
+    *done = 0;
+    plan[PLAN_SPLITS] = most;
+    plan[PLAN_PREFIX] = plan[PLAN_OWN] = sms;
+  }
   // Groups that do not ascend within the entries: nothing is common.
   for (int g = tid; g <= n_groups; g += PREP_THREADS) {
     const int at = group_start[g];
@@ -106,12 +161,49 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
     least = __reduce_min_sync(0xffffffffu, least);
     first = __reduce_min_sync(0xffffffffu, first);
     held = __reduce_add_sync(0xffffffffu, held);
-    const int both = held > 1 && least >= SHARED_LEAST ? least : 0;
+    const int both = held > 1 ? least : 0;
     for (int e = lo + lane; e < hi; e += 32) of_entry[e] = __ldcg(of_entry + e) < 0 ? 0 : both;
     if (lane == 0) {
       of_group[g] = both;
       lead[g] = held ? seq(first) : 0;
+      if (both) {
+        const int units = (int)(((int64_t)(hi - lo) * group + 127) / 128) * c.nkv, nt = (both + shared_tile(c.hd) - 1) / shared_tile(c.hd);
+        atomicAdd(&sums.units, units);
+        atomicMax(&sums.longest, nt);
+        atomicAdd(&sums.steps, (float)units * nt);  // (in any order: a plan, and its sums are whole)
+        atomicAdd(&sums.prefix, (float)both);
+      }
     }
+  }
+  if (!whole) return;
+  __syncthreads();
+  float own = 0.f, all = 0.f;
+  for (int e = tid; e < n; e += PREP_THREADS) {
+    const int len = holds(seq(e));
+    own += len - __ldcg(of_entry + e);
+    all += len;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    own += __shfl_xor_sync(0xffffffffu, own, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) {
+    atomicAdd(&sums.own, own);
+    atomicAdd(&sums.all, all);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const bool yes = sums.units > 0 && shared_plan(sums, c, f32, sms, most, plan);
+    if (lane == 0) shares = yes || always;
+  }
+  __syncthreads();
+  if (shares) return;
+  for (int e = tid; e < n; e += PREP_THREADS) of_entry[e] = 0;
+  for (int g = tid; g < n_groups; g += PREP_THREADS) of_group[g] = 0;
+  if (tid == 0) {
+    plan[PLAN_SPLITS] = plan[PLAN_PREFIX] = 1;
+    plan[PLAN_OWN] = sms;
   }
 }
 
@@ -126,11 +218,20 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArg
   if (row >= (int64_t)n * a.nh) return;
   const int i = (int)(row / a.nh), s = a.seqs ? a.seqs[sh.e0 + i] : sh.e0 + i;
   if (s < 0 || s >= c.n_seq) return;
-  const int both = sh.of_entry[sh.e0 + i], splits = both > 0 ? shared_splits(both, c.hd, sh.splits) : 0;
+  const int both = sh.of_entry[sh.e0 + i], splits = both > 0 ? shared_splits(both, c.hd, sh.plan[PLAN_SPLITS]) : 0;
   const int64_t step = (int64_t)n * a.nh * ld;
   // Lane p: part p of the prefix; lane `splits`: the own one.
   const float* mine = sh.part + row * ld + (lane < splits ? lane : sh.splits) * step;
-  const float2 ml = lane <= splits ? __ldcg(reinterpret_cast<const float2*>(mine + ld - 4)) : make_float2(-INFINITY, 0.f);
+  // (The first values are asked for beside the maxima and sums.)
+  const auto ask = [&](int p0, int y, float4(&u)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (p0 + k <= splits && y < c.hd)
+        u[k] = __ldcg(reinterpret_cast<const float4*>(sh.part + row * ld + (p0 + k < splits ? p0 + k : sh.splits) * step + y));
+  };
+  float4 u[8];
+  ask(0, 4 * lane, u);
+  const float2 ml = lane <= splits ? __ldcg(reinterpret_cast<const float2*>(mine + ld - 8)) : make_float2(-INFINITY, 0.f);
   float top = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -145,11 +246,7 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArg
     const bool mine_y = y < c.hd;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int p0 = 0; p0 <= splits; p0 += 8) {
-      float4 u[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (p0 + k <= splits && mine_y)
-          u[k] = __ldcg(reinterpret_cast<const float4*>(sh.part + row * ld + (p0 + k < splits ? p0 + k : sh.splits) * step + y));
+      if (y0 || p0) ask(p0, y, u);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float w = __shfl_sync(0xffffffffu, share, min(p0 + k, 31));
@@ -173,17 +270,22 @@ int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, c
                        int* count, float* shared_part, cudaStream_t st) {
   const KvView& c = a.c;
   const int64_t row = (int64_t)a.nh * shared_row_floats(c.hd), room = (int64_t)(SHARED_PART_BYTES / sizeof(float)) / row;
-  if (a.n < 2 || sh.n_groups < 1 || room < 4) return launch_attn_decode(a, rows16, part, count, st);
+  // Where the entries cannot hold so much that reading it takes longer than a plan, a
+  // prefix kernel's start and a join, there is nothing to plan. (4 at 300, 8 and 2
+  // heads of 64: 11.6 us, planned and shared 25.)
+  const double most = 4.0 * c.hd * c.nkv * a.n * std::min((int64_t)c.max_pages * c.page, (int64_t)c.n_pages * c.page);
+  const bool small = most / SEEN_BYTES < PREP_AND_JOIN + ITEM_FIXED;
+  if (a.n < 2 || sh.n_groups < 1 || room < 4 || (small && !sh.always))
+    return launch_attn_decode(a, rows16, part, count, st);
   // Few row tiles: the prefixes are split over the SMs, within the workspace.
-  const int64_t group = a.nh / c.nkv;
-  const int64_t likely = std::max<int64_t>((a.n * group + 127) / 128, std::min(sh.n_groups, a.n / 2)) * c.nkv;
-  sh.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / likely, SHARED_SPLITS, room / a.n - 1}));
+  const int64_t group = a.nh / c.nkv, units = (a.n * group + 127) / 128 * c.nkv;
+  sh.splits = (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / units, SHARED_SPLITS, room / a.n - 1}));
   sh.part = shared_part;
   int* done = count + std::max(num_sms(), attn_prompt_counts());
-  launch_k(shared_prep_kernel, a.n, PREP_THREADS, 0, st, c, a.seqs, a.n, sh.group_start, sh.n_groups, sh.of_entry,
-           sh.of_group, sh.lead, done);
   // As many entries at a time as the workspace has room for.
   const int step = (int)std::min<int64_t>(a.n, room / (sh.splits + 1));
+  launch_k(shared_prep_kernel, a.n, PREP_THREADS, 0, st, c, a.seqs, a.n, sh.group_start, sh.n_groups, sh.of_entry,
+           sh.of_group, sh.lead, done, (int)group, a.t_q == T_F32, num_sms(), sh.splits, step == a.n, sh.always, sh.plan);
   const int64_t el = a.t_q == T_F32 ? 4 : 2;
   for (sh.e0 = 0; sh.e0 < a.n; sh.e0 += step) {
     sh.e1 = std::min(a.n, sh.e0 + step);

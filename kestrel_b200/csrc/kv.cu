@@ -540,7 +540,7 @@ int make_q_map(const AttnArgs& a, KvMap& map) {
 // ---- workspace ---------------------------------------------------------------
 int64_t kv_workspace_ints(const KvView& c) {
   const int64_t m = std::max(c.n_seq, c.n_pages);
-  return 4 * m + 5 * (int64_t)c.n_seq + c.n_pages + 4;
+  return 4 * m + 5 * (int64_t)c.n_seq + c.n_pages + 4 + SHARED_PLAN;
 }
 
 cudaError_t kv_workspace_init(KvView& c, int* work, cudaStream_t st) {
@@ -556,6 +556,7 @@ cudaError_t kv_workspace_init(KvView& c, int* work, cudaStream_t st) {
   c.both = c.n_copy + 4;
   c.both_group = c.both + c.n_seq;
   c.lead = c.both_group + c.n_seq;
+  c.plan = c.lead + c.n_seq;
   cudaError_t e = cudaMemsetAsync(c.mark, 0xff, m * sizeof(int), st);
   if (e == cudaSuccess) e = cudaMemsetAsync(c.n_copy, 0, 4 * sizeof(int), st);
   return e;

@@ -27,7 +27,7 @@ struct KvView {
   int *first;              // [n_seq] extend: its first entry of `fresh`
   int *fresh;              // [n_pages] extend: the pages it takes, ascending
   int *n_copy;             // entries of src / dst / rows
-  int *both, *both_group, *lead;  // [n_seq] attention over shared prefixes (SharedArgs)
+  int *both, *both_group, *lead, *plan;  // attention over shared prefixes (SharedArgs)
   int *status;
 };
 
@@ -57,6 +57,7 @@ struct KvState {
   int* count = nullptr;   // arrival counts, zero between launches
   int64_t count_bytes = 0;
   int64_t bytes = 0;      // of all
+  bool share_always = false;  // KC_OPT_SHARE_ALWAYS
   float* shared = nullptr;  // between parts and counts: results of shared prefixes
 };
 
@@ -96,18 +97,25 @@ struct SharedArgs {
   int32_t* of_entry;           // [n] positions that an entry's group has in common (a multiple of the page; 0: none)
   int32_t* of_group;           // [n_groups] the same of each group
   int32_t* lead;               // [n_groups] a sequence of it
+  int32_t* plan;               // [SHARED_PLAN] what the device decides (below)
   int e0, e1;                  // entries of this launch
-  int splits;                  // blocks a group's prefix may be split over
-  // [split + 1][entry][head][64 * ceil(hd / 64) + 4]: result, maximum, sum; of the
+  int splits;                  // parts of a group's prefix, at most
+  bool always;                 // (KC_OPT_SHARE_ALWAYS)
+  // [split + 1][entry][head][64 * ceil(hd / 64) + 8]: result, maximum, sum; of the
   // parts of the prefix, then of the entries' own
   float* part;
 };
-// Blocks that a prefix of `both` positions is split over: at least four tiles each.
+// The plan: parts of a prefix (at most `splits`); blocks of the two kernels that
+// work, the others leave their SMs at once.
+enum { PLAN_SPLITS = 0, PLAN_PREFIX = 1, PLAN_OWN = 2, SHARED_PLAN = 4 };
+__host__ __device__ inline int shared_tile(int hd) { return hd <= 128 ? 128 : 64; }
+// Parts of a prefix of `both` positions: two tiles each at least, one a stream.
 __host__ __device__ inline int shared_splits(int both, int hd, int most) {
-  const int tile = hd <= 128 ? 128 : 64, t = (both + tile - 1) / tile / 4;
+  const int t = (both + shared_tile(hd) - 1) / shared_tile(hd) / 2;
   return t < 1 ? 1 : t < most ? t : most;
 }
-__host__ __device__ inline int shared_row_floats(int hd) { return (hd + 63) / 64 * 64 + 4; }
+// (Whole 32-byte sectors.)
+__host__ __device__ inline int shared_row_floats(int hd) { return (hd + 63) / 64 * 64 + 8; }
 
 // The query rows of a call as [row][head][column], boxes of 128 (token, head)
 // rows of one key-value head's group (which divides 128) x 128 bytes of columns.

@@ -95,6 +95,7 @@ SIGNATURES = {
 # Options (kc_set_option) and whole-model tensor kinds (kc_model_tensor).
 OPT_F32_PREFILL = 1
 OPT_LOOKAHEAD = 2
+OPT_SHARE_ALWAYS = 3
 # Expert-cache policies (kc_expert_cache_reserve) and counters (kc_expert_cache_stats).
 EXPERT_POLICY_LFRU, EXPERT_POLICY_LRU = 0, 1
 XS_COUNTERS = ["capacity", "cached", "requests", "hits", "late", "misses", "scratch_loads", "bytes_read",

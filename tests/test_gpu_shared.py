@@ -18,9 +18,10 @@ torch = pytest.importorskip("torch")
 def ctx():
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")
-    from kestrel_b200.cuda import Context
+    from kestrel_b200.cuda import OPT_SHARE_ALWAYS, Context
     c = Context(0)
     c.set_stream(torch.cuda.current_stream().cuda_stream)
+    c.set_option(OPT_SHARE_ALWAYS, 1)  # these sizes would not be shared for their time
     yield c
     c.close()
 
@@ -193,6 +194,24 @@ def test_strides_rows_and_graphs(ctx):
     graph.replay()
     ctx.sync()
     close(wide(out), c.expected(1, wide(q), range(5), [1] * 5, 0.125, 0, 0), BF16)
+
+
+def test_by_expected_time(ctx):
+    """Without the option: what is not worth it is not shared (the decode call's bits),
+    what is (64 x 24000 positions, 790 MB unshared) gives the same within tolerance."""
+    from kestrel_b200.cuda import OPT_SHARE_ALWAYS
+    ctx.set_option(OPT_SHARE_ALWAYS, 0)
+    try:
+        for pages, lens, same in ((5, [90, 81, 85], True), (375, [24001 + 61 * i for i in range(64)], False)):
+            c, start = branches(ctx, [(pages, lens)], 16 if same else 64, 2, 64, F16, poison=False)
+            q = queries(len(lens), 8, 64, F16, 5).contiguous()
+            out, alone = run(ctx, c, q, start), torch.empty_like(q)
+            ctx.attn_decode_dev(c.id, 1, q, alone)
+            ctx.sync()
+            assert torch.equal(out, alone) == same
+            assert (alone.double() - out.double()).norm() <= 2.0 ** -10 * alone.double().norm()
+    finally:
+        ctx.set_option(OPT_SHARE_ALWAYS, 1)
 
 
 def test_reports_and_refusals(ctx):
