@@ -41,9 +41,10 @@ constexpr int SMP_ALL = SMP_CLUSTER * SMP_WARPS;
 constexpr int SMP_COARSE = 128;   // bins of the histogram: four a lane
 constexpr int SMP_FINE = 128;     // and of one of them
 constexpr int SMP_BINS = SMP_COARSE * SMP_FINE;
-constexpr int SMP_LIST = 1024;    // tokens of a bin that one block looks through
-constexpr int SMP_SHORT = 512;    // tokens that top-k leaves to one block
-constexpr int SMP_TRIES = 40;     // bins looked at for top-p, at most
+constexpr int SMP_LIST = 512;     // tokens of a bin that one block looks through
+constexpr int SMP_SHORT = 256;    // tokens that top-k leaves to one block
+constexpr int SMP_NEAR = 1024;    // tokens of a coarse bin that a block keeps in mind
+constexpr int SMP_TRIES = 40;     // coarse bins looked at for top-p, at most
 constexpr float SMP_SPAN = 24.f;  // the histogram reaches so far below the maximum
 constexpr double SMP_UNIT = 17592186044416.0;  // 2^44: sums of a list in whole numbers
 
@@ -53,18 +54,24 @@ constexpr double SMP_UNIT = 17592186044416.0;  // 2^44: sums of a list in whole 
 struct alignas(16) SampleShared {
   union {
     uint32_t coarse[SMP_COARSE][32];  // a column a lane: no two of a warp meet in a bank
-    struct {
-      uint64_t comp[SMP_LIST];  // listed tokens (rank 0), once the histograms are through
+    struct {                          // once that histogram is through:
+      uint64_t weights[SMP_CLUSTER][SMP_FINE];  // the blocks' weights by bins of a coarse bin
+      uint64_t comp[SMP_LIST];                  // listed tokens (rank 0)
       uint64_t weight[SMP_LIST];
     };
   };
-  uint32_t fine[SMP_FINE];
-  uint16_t bins[2][SMP_CLUSTER][SMP_COARSE];  // the blocks' histograms (a block holds fewer than 2^16)
-  double part[2][4][SMP_ALL];                 // the warps' sums
+  uint64_t fine[SMP_FINE];
+  union {
+    uint16_t bins[2][SMP_CLUSTER][SMP_COARSE];  // the blocks' counts (a block holds fewer than 2^16)
+    uint32_t mass[SMP_CLUSTER][SMP_COARSE];     // or weights
+  };
+  double part[2][3][SMP_ALL];  // the warps' sums
+  uint16_t near[SMP_NEAR];     // places of tokens of a coarse bin in the block's stretch
+  int n_near;
   uint64_t span[SMP_CLUSTER][2];
   float top[SMP_CLUSTER], low[SMP_CLUSTER];
-  int first[SMP_CLUSTER];
-  int listed[SMP_TRIES + 1];  // (rank 0)
+  int first[SMP_CLUSTER];  // greedy: the blocks' first maxima
+  int listed[2];  // (rank 0)
   // From rank 0: the cut for k; then the stretch that holds the token.
   uint64_t cut;
   double left, total;
@@ -98,12 +105,12 @@ __device__ __forceinline__ double weight_of(double d, double c, const double* ta
   const double y = fma(d, c, 384.0);
   const int h = (__double2hiint(y) + 0x80) & ~0xff;
   const double r = y - __hiloint2double(h, 0);
-  double p = 1.3333558146428443e-3;       // ln 2 ^ 5 / 5!
-  p = fma(p, r, 9.6181291076284772e-3);   // ^ 4 / 4!
-  p = fma(p, r, 5.5504108664821580e-2);   // ^ 3 / 3!
-  p = fma(p, r, 2.4022650695910072e-1);   // ^ 2 / 2!
-  p = fma(p, r, 6.9314718055994531e-1);   // ln 2
-  p = fma(p, r, 1.0);
+  // (By halves: the steps wait for each other less.)
+  const double r2 = r * r;
+  const double lo = fma(6.9314718055994531e-1, r, 1.0);                      // ln 2
+  const double mid = fma(5.5504108664821580e-2, r, 2.4022650695910072e-1);   // its powers by n!
+  const double hi = fma(1.3333558146428443e-3, r, 9.6181291076284772e-3);
+  const double p = fma(r2, fma(r2, hi, mid), lo);
   const double w = table[(h >> 8) & 15] * p;
   return __hiloint2double(__double2hiint(w) + ((h << 8) & 0x0ff00000) - (128 << 20), __double2loint(w));
 }
@@ -189,14 +196,21 @@ struct SampleRow {
   double c;               // log2(e) / T
   float c32;
 
-  // fn(l, index) of four values a lane at a time, over the warp's stretch (whole warps).
+  // fn(l, index) of four values a lane at a time, over the warp's stretch (whole
+  // warps). The next ones are asked for before the last are at work.
   template <class Fn>
   __device__ __forceinline__ void each4(Fn fn) {
-    const int seg = chunk / SMP_WARPS;
-    for (int i = warp * seg + 4 * lane; i < (warp + 1) * seg; i += 128) {
-      float v[4];
-      load4(logits + i, v);
-      fn(v, at + i);
+    const int seg = chunk / SMP_WARPS, end = (warp + 1) * seg;
+    float v[4];
+    load4(logits + warp * seg + 4 * lane, v);
+    for (int i = warp * seg + 4 * lane; i < end;) {
+      float now[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) now[e] = v[e];
+      const int here = i;
+      i += 128;
+      if (i < end) load4(logits + i, v);
+      fn(now, at + here);
     }
   }
   // How far below the maximum, in bins; the bin.
@@ -210,10 +224,6 @@ struct SampleRow {
     const double w = weight_of((double)l - (double)m, c, s.table);
     const bool some = (m - l) * c32 < 100.f;
     return __hiloint2double(some ? __double2hiint(w) : 0, some ? __double2loint(w) : 0);
-  }
-  // What a bin's tokens weigh, by its middle (f32 is enough: it is checked).
-  __device__ __forceinline__ double guess(uint32_t n, float middle) const {
-    return n ? (double)n * exp2f(-middle / scale * c32) : 0.0;
   }
   // Sums of the lanes' v[y] over all blocks, in every lane, after a barrier.
   template <int N>
@@ -247,41 +257,31 @@ struct SampleRow {
       n[3] += y.y >> 16;
     }
   }
-  // Tokens by bins of one coarse bin, of all blocks; the f32 sums of all weights and
-  // of those above the coarse bin. Only logits from `floor` on.
-  __device__ __forceinline__ void fine_bins(int coarse, float floor, uint32_t (&n)[4], double& all, double& above) {
+  // Tokens by bins of one coarse bin, of all blocks.
+  __device__ __forceinline__ void fine_bins(int coarse, uint32_t (&n)[4]) {
     const float begins = coarse * SMP_FINE, ends = begins + SMP_FINE;
-    if (tid < SMP_FINE) s.fine[tid] = 0;
+    uint32_t* fine = reinterpret_cast<uint32_t*>(s.fine);
+    if (tid < SMP_FINE) fine[tid] = 0;
     __syncthreads();
-    float sum = 0.f, over = 0.f;
     each4([&](const float (&v)[4], int) {
-      float r[4], w[4];
+      float r[4];
       bool here = false;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        r[e] = v[e] >= floor ? depth(v[e]) : -1.f;
+        r[e] = depth(v[e]);
         here |= r[e] >= begins && r[e] < ends;
-        w[e] = exp2_fast((v[e] - m) * c32);
-        w[e] = r[e] >= 0.f && v[e] > -INFINITY ? w[e] : 0.f;
       }
-      sum += (w[0] + w[1]) + (w[2] + w[3]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = r[e] < begins ? w[e] : 0.f;
-      over += (w[0] + w[1]) + (w[2] + w[3]);
       if (__any_sync(0xffffffffu, here)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (r[e] >= begins && r[e] < ends) atomicAdd(&s.fine[whole(r[e]) & (SMP_FINE - 1)], 1u);
+          if (r[e] >= begins && r[e] < ends) atomicAdd(&fine[whole(r[e]) & (SMP_FINE - 1)], 1u);
       }
     });
     __syncthreads();
     for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
-      cluster.map_shared_rank(&s.bins[turn & 1][rank][0], y / SMP_FINE)[y % SMP_FINE] = (uint16_t)s.fine[y % SMP_FINE];
-    double v[2] = {sum, over};
-    totals(v);
-    all = v[0];
-    above = v[1];
-    gather_bins(turn - 1, n);
+      cluster.map_shared_rank(&s.bins[turn & 1][rank][0], y / SMP_FINE)[y % SMP_FINE] = (uint16_t)fine[y % SMP_FINE];
+    cluster.sync();
+    gather_bins(turn++, n);
   }
   // Adds a token to rank 0's list (whole warps; nothing past its end).
   __device__ __forceinline__ void list(bool mine, int which, uint64_t comp, double w) {
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (by_k || by_p)
     for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) s.coarse[i / 32][i % 32] = 0;
   if (tid < 16) s.table[tid] = exp2(tid / 16.0);
-  if (tid <= SMP_TRIES) s.listed[tid] = 0;
+  if (tid < 2) s.listed[tid] = 0;
   float top = -INFINITY, low = INFINITY;
   {
     const T* from = static_cast<const T*>(a.logits) + row * a.stride + x.at;
@@ -492,41 +492,36 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   const double draw = fminf(u > 0.f ? u : 0.f, 0x1.fffffep-1f);
 
   // ---- the histogram ------------------------------------------------------------------------
-  uint64_t cut = 0;   // kept: the places from it on
-  uint32_t count[4];  // tokens of coarse bins 4 lane ..
+  uint64_t cut = 0;  // kept: the places from it on
   const int seg = chunk / SMP_WARPS;
-  if (by_k || by_p) {
-    // What is below (1 - p) / n_vocab of the first adds up to less than 1 - p of
-    // all: top-p alone never reaches it. (A little further for roundings.)
-    const float reach =
-        by_k ? INFINITY : temperature * (logf((float)a.n_vocab) - logf(fmaxf(1.f - top_p, 1e-7f)) + 0.01f);
+  // Sums of a histogram's columns, told to all blocks: four threads a bin, eight
+  // columns each.
+  const auto tell_columns = [&](auto put) {
+    __syncthreads();
+    const int bin = tid / 4, col = 8 * (tid & 3);
+    uint32_t n = 0;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) n += s.coarse[bin][col + ((y + bin) & 7)];
+    n += __shfl_xor_sync(0xffffffffu, n, 1);
+    n += __shfl_xor_sync(0xffffffffu, n, 2);
+    for (int b = tid & 3; b < blocks; b += 4) put(b, bin, n);
+    cluster.sync();
+    ++x.turn;
+  };
+
+  // ---- top-k ------------------------------------------------------------------------------------
+  float floor = -INFINITY;  // (no token below it is kept)
+  if (by_k) {
     x.each4([&](const float (&v)[4], int) {
       int b[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) b[e] = x.whole(x.depth(v[e])) / SMP_FINE;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (top - v[e] <= reach) atomicAdd(&s.coarse[b[e]][lane], 1u);
+      for (int e = 0; e < 4; ++e) atomicAdd(&s.coarse[b[e]][lane], 1u);
     });
-    __syncthreads();
-    {
-      // Four threads a bin, eight columns each.
-      const int bin = tid / 4, col = 8 * (tid & 3);
-      uint32_t n = 0;
-#pragma unroll
-      for (int y = 0; y < 8; ++y) n += s.coarse[bin][col + ((y + bin) & 7)];
-      n += __shfl_xor_sync(0xffffffffu, n, 1);
-      n += __shfl_xor_sync(0xffffffffu, n, 2);
-      for (int b = tid & 3; b < blocks; b += 4) cluster.map_shared_rank(&s.bins[0][rank][0], b)[bin] = (uint16_t)n;
-    }
-    cluster.sync();
-    ++x.turn;
+    tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.bins[0][rank][0], b)[bin] = (uint16_t)n; });
+    uint32_t count[4];  // tokens of coarse bins 4 lane ..
     x.gather_bins(0, count);
-  }
-
-  // ---- top-k ------------------------------------------------------------------------------------
-  float floor = -INFINITY;  // (no token below it is kept)
-  if (by_k) {
     // (Whole numbers, exact in 64 bits.)
     Quad q;
 #pragma unroll
@@ -552,7 +547,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       uint64_t *placed = s.comp + SMP_SHORT, *kept = s.weight + SMP_SHORT;
       if (tid == 0) s.add[0] = 0;
       // The weights of those at a token's place and above, and in the low bits its
-      // rank (512 weights of 2^44 leave room). The k-th's are all of theirs.
+      // rank (256 weights of 2^44 leave room). The k-th's are all of theirs.
       x.pairs(
           members, [&](int i, int j) { return s.comp[j] >= s.comp[i] ? (s.weight[j] << 10) + 1 : 0ull; },
           [&](int i, uint64_t sum) {
@@ -581,14 +576,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     }
     // The bin that holds the k-th, then its place among the bin's.
     int rest = k - (int)Quad::of(coarse, [&](int e) { return q.upto(e) - q.v[e]; });
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int b = 4 * lane + e;
-      count[e] = b < coarse ? count[e] : b == coarse ? rest : 0;
-    }
     uint32_t n[4];
-    double none;
-    x.fine_bins(coarse, floor, n, none, none);
+    x.fine_bins(coarse, n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) q.v[e] = n[e];
     q.scan(lane);
@@ -626,76 +615,69 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   }
 
   // ---- weights: sums of what is kept, and the place at which top-p ends -----------------------------
-  // The warps' sums of what is kept: s.part[stretch & 1][3].
-  int stretch;
-  double sums[4] = {0, 0, 0, 0};  // of all, above the bin, in it, kept above it
+  int stretch;                 // the warps' sums of what is kept: s.part[stretch & 1][2]
+  double sums[3] = {0, 0, 0};  // of all, above a bin, kept
   if (by_p) {
-    // Bins gfrom .. gto are left in question. A coarse one is chosen by the counts'
-    // weights, then a bin by those of its own and f32 sums, which a pass checks in
-    // 64 bits: if the target is not reached there, the bins on that side are out.
-    int gfrom = 0, gto = SMP_BINS - 1, bin = 0, coarse = -1, tries = 0, last = 0, moves = 0;
-    uint32_t n[4] = {0, 0, 0, 0};  // tokens of the coarse bin's
-    Quad q, fq;                    // weights by the counts
-    double fix = 0;                // the sum above the coarse bin
+    // The coarse bins' weights, in 2^-16 of a token at each bin's beginning.
+    const float unit = x.c32 / x.scale;
+    if (by_k) {
+      for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) s.coarse[i / 32][i % 32] = 0;
+      __syncthreads();
+    }
+    for (int i = warp * seg + 4 * lane; i < (warp + 1) * seg; i += 256) {
+      // Eight values a lane under way.
+      float v[2][4];
+      load4(x.logits + i, v[0]);
+      if (i + 128 < (warp + 1) * seg) load4(x.logits + i + 128, v[1]);
+      else v[1][0] = v[1][1] = v[1][2] = v[1][3] = NAN;
+      int b[8];
+      uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q.v[e] = x.guess(count[e], (4 * lane + e + 0.5f) * SMP_FINE);
+      for (int e = 0; e < 8; ++e) {
+        const float r = x.depth(v[e / 4][e % 4]), begins = __fadd_rd(r * (1.f / SMP_FINE), 8388608.f);
+        b[e] = __float_as_int(begins) & (SMP_COARSE - 1);
+        const float part = exp2_fast(((begins - 8388608.f) * SMP_FINE - r) * unit);
+        w[e] = max(1, __float_as_int(__fadd_rn(part * 65536.f, 8388608.f)) & 0x1ffff);  // (none is lost)
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e / 4][e % 4] >= floor)  // (not of NAN)
+          atomicAdd(&s.coarse[b[e]][lane], w[e]);
+    }
+    tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.mass[rank][0], b)[bin] = n; });
+    Quad q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] = 0;
+    for (int b = 0; b < blocks; ++b) {
+      const uint4 y = *reinterpret_cast<const uint4*>(&s.mass[b][4 * lane]);
+      q.v[0] += y.x;
+      q.v[1] += y.y;
+      q.v[2] += y.z;
+      q.v[3] += y.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] *= exp2f(-((4 * lane + e) * SMP_FINE) * unit);
     q.scan(lane);
-    double target = p * Quad::of(SMP_COARSE - 1, [&](int e) { return q.upto(e); });
-    const auto coarse_open = [&](int e) {
-      const int b = 4 * lane + e;
-      return count[e] > 0 && b * SMP_FINE <= gto && (b + 1) * SMP_FINE > gfrom;
-    };
-    const auto fine_open = [&](int e) {
-      const int g = coarse * SMP_FINE + 4 * lane + e;
-      return n[e] > 0 && g >= gfrom && g <= gto;
-    };
-    while (true) {
-      int next = coarse;
-      if (coarse < 0) {
-        next = Quad::first(lane, [&](int e) { return coarse_open(e) && q.upto(e) >= target; });
-        if (next == INT_MAX) next = Quad::last(lane, coarse_open);
-      } else if (Quad::first(lane, fine_open) == INT_MAX) {
-        // None left in this one: the next one in the direction of the target.
-        next = Quad::first(lane, [&](int e) { return coarse_open(e) && 4 * lane + e > coarse; });
-        if (next == INT_MAX) next = Quad::last(lane, [&](int e) { return coarse_open(e) && 4 * lane + e < coarse; });
-      }
-      if (next < 0) break;  // (rounding: the last bin stands)
-      while (next != coarse) {
-        const int was = coarse;
-        coarse = next;
-        double all;
-        x.fine_bins(coarse, floor, n, all, fix);
+    // Coarse bins from .. to are left in question. The one in which the sum reaches the
+    // target is taken by these weights; a pass checks it in 64 bits, and has its bins'.
+    int from = 0, to = SMP_COARSE - 1, bin = 0;
+    double target = p * Quad::of(SMP_COARSE - 1, [&](int e) { return q.upto(e); }), rest = 0;
+    const auto open = [&](int e) { return q.v[e] > 0 && 4 * lane + e >= from && 4 * lane + e <= to; };
+    int coarse = Quad::first(lane, [&](int e) { return open(e) && q.upto(e) >= target; });
+    if (coarse == INT_MAX) coarse = Quad::last(lane, open);
+    coarse = max(coarse, 0);  // (the first token's bin, if its weight is lost in 2^-16)
+    Quad f;
+    for (int tries = 0;; ++tries) {
+      if (tid < SMP_FINE) s.fine[tid] = 0;
+      if (tid == 0) s.n_near = 0;
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) fq.v[e] = x.guess(n[e], coarse * SMP_FINE + 4 * lane + e + 0.5f);
-        fq.scan(lane);
-        if (tries == 0) {
-          target = p * all;
-          // The f32 sums may already say that it is another coarse bin.
-          const double here = Quad::of(SMP_FINE - 1, [&](int e) { return fq.upto(e); });
-          const bool high = fix >= target, low_of = fix + here < target;
-          if ((high || low_of) && moves++ < 4) {
-            const int to = high ? Quad::last(lane, [&](int e) { return coarse_open(e) && 4 * lane + e < coarse; })
-                                : Quad::first(lane, [&](int e) { return coarse_open(e) && 4 * lane + e > coarse; });
-            if (to >= 0 && to < SMP_COARSE && to != was) next = to;
-          }
-        }
-      }
-      int fine = Quad::first(lane, [&](int e) { return fine_open(e) && fix + fq.upto(e) >= target; });
-      if (fine == INT_MAX) fine = Quad::last(lane, fine_open);
-      if (fine < 0) {  // the coarse bin holds nothing in question
-        if (gfrom >= coarse * SMP_FINE) gfrom = max(gfrom, (coarse + 1) * SMP_FINE);
-        else gto = min(gto, coarse * SMP_FINE - 1);
-        continue;
-      }
-      bin = coarse * SMP_FINE + fine;
-      last = tries;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) sums[y] = 0;
+      for (int y = 0; y < 3; ++y) sums[y] = 0;
       const auto pass = [&](auto bounded, auto limited) {
-        const float begins = bin, ends = bin + 1;
+        const float begins = coarse * SMP_FINE, ends = begins + SMP_FINE;
         x.each4([&](const float (&v)[4], int i) {
-          double w[4];
-          bool here[4], over[4];
+          double w[4], over[4];
+          bool here[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = x.weight(v[e]);
 #pragma unroll
@@ -703,45 +685,128 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
             const float r = x.depth(v[e]);
             const bool keep = !decltype(bounded)::value || order_of(v[e], i + e) >= cut;
             here[e] = r >= begins && r < ends && keep;
-            over[e] = r < begins && keep;
-            if (keep) sums[0] += w[e];
-            if (over[e]) sums[1] += w[e];
-            if (decltype(limited)::value && over[e] && w[e] >= least) sums[3] += w[e];
+            if (!keep) w[e] = 0.0;
+            over[e] = r < begins ? w[e] : 0.0;
+          }
+          sums[0] += (w[0] + w[1]) + (w[2] + w[3]);
+          sums[1] += (over[0] + over[1]) + (over[2] + over[3]);
+          if (decltype(limited)::value) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (over[e] >= least) sums[2] += over[e];
           }
           if (__any_sync(0xffffffffu, here[0] || here[1] || here[2] || here[3])) {
+            // To what the block keeps in mind, a place in the order of the lanes.
+            unsigned who[4];
+            int at = 0, all = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if (here[e]) sums[2] += w[e];
-              x.list(here[e], 1 + tries, order_of(v[e], i + e), w[e]);
+              who[e] = __ballot_sync(0xffffffffu, here[e]);
+              at += __popc(who[e] & ((1u << lane) - 1));
+              all += __popc(who[e]);
             }
+            int base = 0;
+            if (lane == 0) base = atomicAdd(&s.n_near, all);
+            at += __shfl_sync(0xffffffffu, base, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (here[e]) {
+                if (at < SMP_NEAR) s.near[at] = (uint16_t)(i + e - x.at);
+                ++at;
+              }
           }
         });
-        if (!decltype(limited)::value) sums[3] = sums[1];
+        if (!decltype(limited)::value) sums[2] = sums[1];
       };
       using std::false_type;
       using std::true_type;
       if (by_k) pass(true_type{}, true_type{});
       else if (least > 0) pass(false_type{}, true_type{});
       else pass(false_type{}, false_type{});
-      stretch = x.turn;
-      x.totals(sums);
-      target = p * sums[0];
-      const bool high = !(sums[1] < target), low_of = sums[1] + sums[2] < target;
-      if (!(high || low_of) || tries + 1 >= SMP_TRIES) break;
-      const int was_from = gfrom, was_to = gto;
-      if (high) gto = bin - 1;
-      else gfrom = bin + 1;
-      const int others = Quad::last(lane, [&](int e) { return fine_open(e) || (coarse_open(e) && 4 * lane + e != coarse); });
-      if (others < 0) {
-        gfrom = was_from;
-        gto = was_to;
-        break;  // (rounding: the bin stands)
+      __syncthreads();
+      // The weights of the bins of the coarse one.
+      const auto weigh = [&](float l, int i) {
+        if (order_of(l, i) >= cut)
+          atomicAdd((unsigned long long*)&s.fine[x.whole(x.depth(l)) & (SMP_FINE - 1)],
+                    (unsigned long long)llrint(x.weight(l) * SMP_UNIT));
+      };
+      if (s.n_near <= SMP_NEAR) {
+        for (int j = tid; j < s.n_near; j += SMP_THREADS) weigh((float)x.logits[s.near[j]], x.at + s.near[j]);
+      } else {
+        const float begins = coarse * SMP_FINE, ends = begins + SMP_FINE;
+        x.each4([&](const float (&v)[4], int i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x.depth(v[e]) >= begins && x.depth(v[e]) < ends) weigh(v[e], i + e);
+        });
       }
-      // The sum up to the bin's beginning is known: the estimates count from there.
-      fix = sums[1] - Quad::of(fine, [&](int e) { return fq.upto(e) - fq.v[e]; });
-      ++tries;
+      __syncthreads();
+      for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
+        cluster.map_shared_rank(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
+      double total[2] = {sums[0], sums[1]};
+      x.totals(total);
+      uint64_t in[4] = {0, 0, 0, 0};
+      for (int b = 0; b < blocks; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) in[e] += s.weights[b][4 * lane + e];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[e] = (double)in[e] / SMP_UNIT;
+      f.scan(lane);
+      target = p * total[0];
+      rest = target - total[1];  // of the coarse bin's
+      const double inside = Quad::of(SMP_FINE - 1, [&](int e) { return f.upto(e); });
+      // Not the bin: the next one in the target's direction that holds anything.
+      const bool high = !(rest > 0), low_of = inside < rest;
+      if (!(high || low_of) || tries + 1 >= SMP_TRIES) break;
+      if (high) to = coarse - 1;
+      else from = coarse + 1;
+      const int next = high ? Quad::last(lane, open) : Quad::first(lane, open);
+      if (next < 0 || next >= SMP_COARSE) break;  // (rounding: the bin stands)
+      coarse = next;
+      cluster.sync();  // (all have read the weights)
     }
-    const int members = *cluster.map_shared_rank(&s.listed[1 + last], 0);
+    // The bin in which the sum reaches the target, and what it lacks at its beginning.
+    int fine = Quad::first(lane, [&](int e) { return f.v[e] > 0 && f.upto(e) >= rest; });
+    if (fine == INT_MAX) fine = max(0, Quad::last(lane, [&](int e) { return f.v[e] > 0; }));
+    rest -= Quad::of(fine, [&](int e) { return f.upto(e) - f.v[e]; });
+    bin = coarse * SMP_FINE + fine;
+    {
+      // Its tokens to rank 0's list, those above it to what their stretches keep.
+      const float begins = coarse * SMP_FINE, at_bin = bin, ends = bin + 1;
+      if (tid < SMP_ALL) s.add[tid] = 0;
+      __syncthreads();
+      const auto place = [&](float l, int i, bool real) {
+        const float r = x.depth(l);
+        const bool keep = real && order_of(l, i) >= cut, here = keep && r >= at_bin && r < ends;
+        const double w = x.weight(l);
+        if (keep && r >= begins && r < at_bin && w >= least)
+          atomicAdd((unsigned long long*)&s.add[(i - x.at) / seg], (unsigned long long)llrint(w * SMP_UNIT));
+        x.list(here, 1, order_of(l, i), w);
+      };
+      if (s.n_near <= SMP_NEAR) {
+        for (int j0 = 0; j0 < s.n_near; j0 += SMP_THREADS) {
+          const bool real = j0 + tid < s.n_near;
+          const int i = real ? s.near[j0 + tid] : 0;
+          place((float)x.logits[i], x.at + i, real);
+        }
+      } else {
+        x.each4([&](const float (&v)[4], int i) {
+          bool some = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) some |= x.depth(v[e]) >= begins && x.depth(v[e]) < ends;
+          if (__any_sync(0xffffffffu, some)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) place(v[e], i + e, true);
+          }
+        });
+      }
+      __syncthreads();
+      const double mine = warp_sum(sums[2]) + (double)s.add[warp] / SMP_UNIT;
+      stretch = x.turn++;
+      if (lane == 0) *cluster.map_shared_rank(&s.part[stretch & 1][2][rank * SMP_WARPS + warp], 0) = mine;
+      cluster.sync();
+    }
+    const int members = *cluster.map_shared_rank(&s.listed[1], 0);
     if (members <= SMP_LIST) {
       if (rank == 0) {
         // In whole units: the order of the list does not matter.
@@ -751,7 +816,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         }
         if (tid < SMP_ALL) s.add[tid] = 0;
         __syncthreads();
-        const double need = (target - sums[1]) * SMP_UNIT;
+        const double need = rest * SMP_UNIT;
         x.pairs(
             members, [&](int i, int j) { return s.comp[j] >= s.comp[i] ? s.weight[j] : 0ull; },
             [&](int i, uint64_t sum) {
@@ -767,17 +832,17 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
           if (s.comp[i] >= cut && (double)s.weight[i] >= least * SMP_UNIT)
             atomicAdd((unsigned long long*)&s.add[(int)~(uint32_t)s.comp[i] / seg], (unsigned long long)s.weight[i]);
         __syncthreads();
-        if (tid < blocks * SMP_WARPS) s.part[stretch & 1][3][tid] += (double)s.add[tid] / SMP_UNIT;
+        if (tid < blocks * SMP_WARPS) s.part[stretch & 1][2][tid] += (double)s.add[tid] / SMP_UNIT;
         __syncthreads();
       }
     } else {
-      cut = max(cut, x.halve(bin, cut, target - sums[1], [&](float l) { return x.weight(l); }));
-      double all_kept[4] = {0, 0, 0, 0};
+      cut = max(cut, x.halve(bin, cut, rest, [&](float l) { return x.weight(l); }));
+      double all_kept[3] = {0, 0, 0};
       x.each4([&](const float (&v)[4], int i) {
         for (int e = 0; e < 4; ++e)
           if (order_of(v[e], i + e) >= cut) {
             const double w = x.weight(v[e]);
-            if (w >= least) all_kept[3] += w;
+            if (w >= least) all_kept[2] += w;
           }
       });
       stretch = x.turn;
@@ -791,7 +856,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       for (int e = 0; e < 4; ++e) w[e] = x.weight(v[e]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (order_of(v[e], i + e) >= cut && w[e] >= least) sums[3] += w[e];
+        if (order_of(v[e], i + e) >= cut && w[e] >= least) sums[2] += w[e];
     });
     stretch = x.turn;
     x.totals(sums);
@@ -801,7 +866,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (rank == 0 && warp == 0) {
     Quad q;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q.v[e] = 4 * lane + e < blocks * SMP_WARPS ? s.part[stretch & 1][3][4 * lane + e] : 0.0;
+    for (int e = 0; e < 4; ++e) q.v[e] = 4 * lane + e < blocks * SMP_WARPS ? s.part[stretch & 1][2][4 * lane + e] : 0.0;
     q.scan(lane);
     const double total = Quad::of(SMP_ALL - 1, [&](int e) { return q.upto(e); }), want = draw * total;
     // The first stretch past whose end the sum exceeds it; if rounding leaves none,
@@ -819,28 +884,48 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   }
   cluster.sync();
   const int owner = s.owner;
-  if (owner / SMP_WARPS != rank || owner % SMP_WARPS != warp) return;
+  if (owner / SMP_WARPS != rank) return;
+  // The block's threads have a few tokens of the stretch each, in their order. (One
+  // warp for all of them took 10 us.)
   cut = s.cut;
-  double run = 0, w_last = 0;
-  int token = -1;  // the last kept one so far
-  for (int i0 = warp * seg; i0 < (warp + 1) * seg; i0 += 32) {
-    const float l = (float)x.logits[i0 + lane];
-    double w = order_of(l, x.at + i0 + lane) >= cut ? x.weight(l) : 0.0;
-    if (!(w >= least)) w = 0.0;
-    const unsigned some = __ballot_sync(0xffffffffu, w > 0);
-    if (!some) continue;
-    const double upto = warp_scan(w, lane);
-    const unsigned past = __ballot_sync(0xffffffffu, w > 0 && run + upto > s.left);
-    const int pick = past ? __ffs(past) - 1 : 31 - __clz(some);
-    token = x.at + i0 + pick;
-    w_last = __shfl_sync(0xffffffffu, w, pick);
-    if (past) break;
-    run += __shfl_sync(0xffffffffu, upto, 31);
+  const int per = (seg + SMP_THREADS - 1) / SMP_THREADS, first_at = (owner % SMP_WARPS) * seg + tid * per,
+            end_at = min(first_at + per, (owner % SMP_WARPS + 1) * seg);
+  const auto kept_weight = [&](int i) {
+    const float l = (float)x.logits[i];
+    const double w = order_of(l, x.at + i) >= cut ? x.weight(l) : 0.0;
+    return w >= least ? w : 0.0;
+  };
+  double own = 0;
+  for (int i = first_at; i < end_at; ++i) own += kept_weight(i);
+  double upto = warp_scan(own, lane);
+  double* sums_of = s.part[0][0];
+  __syncthreads();
+  if (lane == 31) sums_of[warp] = upto;
+  if (tid == 0) {
+    s.first[0] = INT_MAX;
+    s.first[1] = -1;
   }
-  if (lane == 0) {
-    a.tokens[row] = token;
-    if (a.probs) a.probs[row] = (float)(w_last / s.total);
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += sums_of[w];
+  if (own > 0) {
+    if (upto > s.left) atomicMin(&s.first[0], tid);
+    atomicMax(&s.first[1], tid);
   }
+  __syncthreads();
+  // (If rounding leaves none past it, the last that holds anything.)
+  if (tid != (s.first[0] != INT_MAX ? s.first[0] : s.first[1])) return;
+  double run = upto - own, w_last = 0;
+  int token = -1;
+  for (int i = first_at; i < end_at; ++i) {
+    const double w = kept_weight(i);
+    if (w == 0) continue;
+    token = x.at + i;
+    w_last = w;
+    run += w;
+    if (run > s.left) break;
+  }
+  a.tokens[row] = token;
+  if (a.probs) a.probs[row] = (float)(w_last / s.total);
 }
 
 template <typename T>
