@@ -36,6 +36,8 @@
  *   kc_model_generate        the greedy loop of Engine::generate with
  *                            SamplerConfig::greedy (crates/kestrel-engine/src/
  *                            lib.rs:116-145, sampler.rs:25-27, 104-112)
+ *   kc_model_sample          the same loop with the sampler's settings (Sampler::sample,
+ *                            sampler.rs:48), uniform numbers from the caller
  *   kc_model_truncate        Transformer::truncate (transformer.rs:276-278)
  *   kc_model_set_sequences / _prefill_seq / _decode_seqs / _generate_batch
  *                            n independent Engine::generate greedy loops
@@ -380,6 +382,12 @@ KC_API int kc_model_forward(kc_ctx* ctx, const uint32_t* tokens, int n, float* l
    fed to the next step from device memory (no host round trip per token).
    out_tokens [n_gen]. */
 KC_API int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, uint32_t* out_tokens);
+/* The same loop with every token drawn from its logits by kc_sample_dev's rules:
+   one setting of each kind for all, u [n_gen] uniform numbers and (optional) probs
+   [n_gen] the tokens' shares, host buffers. temperature 0: kc_model_generate's
+   tokens. */
+KC_API int kc_model_sample(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, float temperature, int top_k,
+                           float top_p, float min_p, const float* u, uint32_t* out_tokens, float* probs);
 /* Several independent sequences on one context, each with its own KV cache
    (sequence 0's is the one the calls above use), decoded in lockstep.
    kc_model_set_sequences: room for n_seq (1..32) sequences; growing it drops

@@ -201,6 +201,8 @@ unsafe extern "C" {
     pub fn kc_model_decode_seqs(ctx: *mut kc_ctx, n_seq: c_int, n_gen: c_int, out_tokens: *mut u32) -> c_int;
     pub fn kc_model_generate_batch(ctx: *mut kc_ctx, n_seq: c_int, prompts: *const u32,
         prompt_lens: *const c_int, n_gen: c_int, out_tokens: *mut u32) -> c_int;
+    pub fn kc_model_sample(ctx: *mut kc_ctx, prompt: *const u32, n_prompt: c_int, n_gen: c_int, temperature: f32,
+        top_k: c_int, top_p: f32, min_p: f32, u: *const f32, out_tokens: *mut u32, probs: *mut f32) -> c_int;
     pub fn kc_model_truncate(ctx: *mut kc_ctx, keep: c_int) -> c_int;
     pub fn kc_model_cached(ctx: *const kc_ctx) -> c_int;
     // GGUF / KGUF loading

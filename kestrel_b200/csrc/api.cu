@@ -2660,17 +2660,26 @@ int kc_model_forward(kc_ctx* ctx, const uint32_t* tokens, int n, float* logits, 
   return check_status(ctx);  // synchronises the stream
 }
 
-int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, uint32_t* out_tokens) {
-  if (!ctx) return KC_ERR_ARG;
-  ctx->err.clear();
-  if (!ctx->model) return fail(ctx, KC_ERR_STATE, "kc_model_generate: call kc_model_init first");
+// What kc_model_sample adds to the greedy loop: each token drawn from its logits.
+struct SampleSpec {
+  float temperature;
+  int32_t top_k;
+  float top_p, min_p;
+  const float* u;  // host, [n_gen]
+  float* probs;    // host, [n_gen] or null
+};
+
+// The loop of kc_model_generate, and of kc_model_sample (sample non-null).
+static int model_tokens(kc_ctx* ctx, const char* what, const uint32_t* prompt, int n_prompt, int n_gen,
+                        const SampleSpec* sample, uint32_t* out_tokens) {
+  if (!ctx->model) return fail(ctx, KC_ERR_STATE, "%s: call kc_model_init first", what);
   if (!prompt || n_prompt < 1 || n_gen < 0 || (n_gen > 0 && !out_tokens))
-    return fail(ctx, KC_ERR_ARG, "kc_model_generate: bad arguments");
+    return fail(ctx, KC_ERR_ARG, "%s: bad arguments", what);
   cudaSetDevice(ctx->device);
   Model& m = *ctx->model;
   if (!m.seq_pos.empty()) m.seq_pos[0] = -1;  // sequence 0 loses its pending token
   if (m.cached + n_prompt + std::max(0, n_gen - 1) > m.n_ctx)
-    return fail(ctx, KC_ERR_ARG, "kc_model_generate: context full (n_ctx = %d)", m.n_ctx);
+    return fail(ctx, KC_ERR_ARG, "%s: context full (n_ctx = %d)", what, m.n_ctx);
   RC(model_forward(ctx, prompt, false, n_prompt));
   if (n_gen == 0) {
     return check_status(ctx);  // synchronises the stream
@@ -2680,20 +2689,39 @@ int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_g
   // token. The first step runs eagerly (it also sizes every buffer for one
   // row); it is then captured once as a CUDA graph and replayed for the rest.
   uint32_t* hist = nullptr;
-  CK(cudaMalloc(&hist, (size_t)n_gen * 4));
+  CK(cudaMalloc(&hist, (size_t)n_gen * (sample ? 12 : 4) + 16));
   int rc = KC_OK;
+  // Sampling: behind the history the numbers, the shares and the settings; the
+  // token's index, in m.counters[0], says which number is its.
+  float *u = reinterpret_cast<float*>(hist + n_gen), *probs = u + n_gen, *settings = probs + n_gen;
+  auto draw = [&]() -> int {
+    SampleArgs a{m.logits, m.n_vocab, 1, m.n_vocab, u, settings, reinterpret_cast<int32_t*>(settings + 1), settings + 2,
+                 settings + 3, reinterpret_cast<int32_t*>(m.next), probs, m.counters};
+    return launch_sample(a, T_F32, ctx->stream);
+  };
   const int init[2] = {1, m.cached};
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t exec = nullptr;
   auto step = [&]() -> int {
     RC(model_chunk(ctx, m, 1, m.next, true));
+    if (sample) RC(draw());
     launch_advance(m.next, hist, m.counters, m.counters + 1, ctx->stream);
     CKL();
     return KC_OK;
   };
-  if (cudaMemcpyAsync(hist, m.next, 4, cudaMemcpyDeviceToDevice, ctx->stream) != cudaSuccess ||
-      cudaMemcpyAsync(m.counters, init, sizeof init, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess)
-    rc = fail(ctx, KC_ERR_CUDA, "kc_model_generate: copy failed");
+  if (sample) {
+    const int zero[2] = {0, 0};
+    if (cudaMemcpyAsync(u, sample->u, (size_t)n_gen * 4, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess ||
+        cudaMemcpyAsync(settings, sample, 16, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess ||
+        cudaMemcpyAsync(m.counters, zero, sizeof zero, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess ||
+        cudaStreamSynchronize(ctx->stream) != cudaSuccess)  // (`zero` and the counters' next values are host temporaries)
+      rc = fail(ctx, KC_ERR_CUDA, "%s: copy failed", what);
+    else if ((rc = draw()) != KC_OK)
+      fail(ctx, rc, "%s: launch set-up failed", what);
+  }
+  if (rc == KC_OK && (cudaMemcpyAsync(hist, m.next, 4, cudaMemcpyDeviceToDevice, ctx->stream) != cudaSuccess ||
+                      cudaMemcpyAsync(m.counters, init, sizeof init, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess))
+    rc = fail(ctx, KC_ERR_CUDA, "%s: copy failed", what);
   const bool graphs = ctx->ep.world <= 1 && !ctx->prof.on && ctx->xs.n_layers == 0 && model_graphs_enabled();
   for (int i = 1; i < n_gen && rc == KC_OK; ++i) {
     if (exec) {
@@ -2701,12 +2729,12 @@ int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_g
     } else if (i >= 2 && graphs) {
       // Capture on the context's own capture stream, replay on its stream.
       if (!ctx->cap && cudaStreamCreateWithFlags(&ctx->cap, cudaStreamNonBlocking) != cudaSuccess) {
-        rc = fail(ctx, KC_ERR_CUDA, "kc_model_generate: capture stream creation failed");
+        rc = fail(ctx, KC_ERR_CUDA, "%s: capture stream creation failed", what);
         break;
       }
       cudaStream_t run = ctx->stream;
       if (cudaStreamBeginCapture(ctx->cap, cudaStreamCaptureModeThreadLocal) != cudaSuccess) {
-        rc = fail(ctx, KC_ERR_CUDA, "kc_model_generate: stream capture failed");
+        rc = fail(ctx, KC_ERR_CUDA, "%s: stream capture failed", what);
         break;
       }
       ctx->stream = ctx->cap;
@@ -2718,7 +2746,7 @@ int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_g
         break;
       }
       if (ec != cudaSuccess || cudaGraphInstantiate(&exec, graph, 0) != cudaSuccess) {
-        rc = fail(ctx, KC_ERR_CUDA, "kc_model_generate: graph capture of a decode step failed");
+        rc = fail(ctx, KC_ERR_CUDA, "%s: graph capture of a decode step failed", what);
         break;
       }
       if (cudaGraphLaunch(exec, ctx->stream) != cudaSuccess) rc = fail(ctx, KC_ERR_CUDA, "cudaGraphLaunch failed");
@@ -2729,13 +2757,33 @@ int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_g
   }
   if (rc == KC_OK && cudaMemcpyAsync(out_tokens, hist, (size_t)n_gen * 4, cudaMemcpyDeviceToHost, ctx->stream) !=
                          cudaSuccess)
-    rc = fail(ctx, KC_ERR_CUDA, "kc_model_generate: copy failed");
+    rc = fail(ctx, KC_ERR_CUDA, "%s: copy failed", what);
+  if (rc == KC_OK && sample && sample->probs &&
+      cudaMemcpyAsync(sample->probs, probs, (size_t)n_gen * 4, cudaMemcpyDeviceToHost, ctx->stream) != cudaSuccess)
+    rc = fail(ctx, KC_ERR_CUDA, "%s: copy failed", what);
   cudaStreamSynchronize(ctx->stream);
   if (exec) cudaGraphExecDestroy(exec);
   if (graph) cudaGraphDestroy(graph);
   cudaFree(hist);
   if (rc != KC_OK) return rc;
   return check_status(ctx);
+}
+
+int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, uint32_t* out_tokens) {
+  if (!ctx) return KC_ERR_ARG;
+  ctx->err.clear();
+  return model_tokens(ctx, "kc_model_generate", prompt, n_prompt, n_gen, nullptr, out_tokens);
+}
+
+int kc_model_sample(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, float temperature, int top_k,
+                    float top_p, float min_p, const float* u, uint32_t* out_tokens, float* probs) {
+  if (!ctx) return KC_ERR_ARG;
+  ctx->err.clear();
+  if (n_gen > 0 && !u) return fail(ctx, KC_ERR_ARG, "kc_model_sample: no uniform numbers");
+  if (ctx->model && ctx->model->n_vocab > SAMPLE_MAX_VOCAB)
+    return fail(ctx, KC_ERR_SHAPE, "kc_model_sample: vocabulary of %d (up to %d)", ctx->model->n_vocab, SAMPLE_MAX_VOCAB);
+  const SampleSpec spec{temperature, top_k, top_p, min_p, u, probs};
+  return model_tokens(ctx, "kc_model_sample", prompt, n_prompt, n_gen, &spec, out_tokens);
 }
 
 // Caches, positions, logits and argmax slots for n_seq sequences (grown, never
@@ -3369,7 +3417,7 @@ int kc_sample_dev(kc_ctx* ctx, int t, const void* logits, int64_t stride, int n,
         ((uintptr_t)u | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p |
          (uintptr_t)tokens | (uintptr_t)probs) % 4)
       return fail(ctx, KC_ERR_ARG, "kc_sample_dev: misaligned buffer");
-    const SampleArgs a{logits, stride, n, n_vocab, u, temperature, top_k, top_p, min_p, tokens, probs};
+    const SampleArgs a{logits, stride, n, n_vocab, u, temperature, top_k, top_p, min_p, tokens, probs, nullptr};
     const int rc = launch_sample(a, t, ctx->stream);
     if (rc != KC_OK) return fail(ctx, rc, "kc_sample_dev: launch set-up failed");
     CKL();

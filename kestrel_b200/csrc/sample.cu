@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
                  tid, warp, lane, 0};
 
   // ---- the row into shared memory, its maximum and least value -------------------------
+  const int64_t number = row + (a.at ? *a.at : 0);  // the row's of u and probs
   const float temperature = a.temperature ? a.temperature[row] : 1.f;
   const int k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.f;
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (top == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
-      if (a.probs) a.probs[row] = 0.f;
+      if (a.probs) a.probs[number] = 0.f;
     }
     return;
   }
@@ -481,14 +482,14 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (rank == 0 && tid == 0) {
       for (int b = 0; b < blocks; ++b) first = min(first, s.first[b]);
       a.tokens[row] = first;
-      if (a.probs) a.probs[row] = 1.f;
+      if (a.probs) a.probs[number] = 1.f;
     }
     return;
   }
   x.c = 1.4426950408889634 / temperature;
   x.c32 = (float)fmin(x.c, 3e38);
   x.scale = (SMP_BINS - 1) / fmaxf(fminf(SMP_SPAN, top - low), 1e-30f);
-  const float u = a.u[row];
+  const float u = a.u[number];
   const double draw = fminf(u > 0.f ? u : 0.f, 0x1.fffffep-1f);
 
   // ---- the histogram ------------------------------------------------------------------------
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
           [&](int i, uint64_t sum) {
             if ((double)sum > want && (double)(sum - kept[i]) <= want && kept[i]) {
               a.tokens[row] = (int)~(uint32_t)s.comp[i];
-              if (a.probs) a.probs[row] = (float)((double)kept[i] / total);
+              if (a.probs) a.probs[number] = (float)((double)kept[i] / total);
             }
           });
       return;
@@ -925,7 +926,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (run > s.left) break;
   }
   a.tokens[row] = token;
-  if (a.probs) a.probs[row] = (float)(w_last / s.total);
+  if (a.probs) a.probs[number] = (float)(w_last / s.total);
 }
 
 template <typename T>

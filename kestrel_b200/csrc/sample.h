@@ -19,6 +19,7 @@ struct SampleArgs {
   const float* min_p;        // [n] or null: 0
   int32_t* tokens;           // [n]
   float* probs;              // [n] or null
+  const int* at;             // null: 0; else u and probs are those from *at on
 };
 int launch_sample(const SampleArgs& a, int t, cudaStream_t st);
 

@@ -62,6 +62,7 @@ SIGNATURES = {
     "kc_model_tensor": (I, [P, I, I, I, P, I64, I64, I]),
     "kc_model_forward": (I, [P, P, I, P, P]),
     "kc_model_generate": (I, [P, P, I, I, P]),
+    "kc_model_sample": (I, [P, P, I, I, F, I, F, F, P, P, P]),
     "kc_model_generate_batch": (I, [P, I, P, P, I, P]),
     "kc_model_set_sequences": (I, [P, I]),
     "kc_model_prefill_seq": (I, [P, I, P, I, P]),
@@ -450,6 +451,19 @@ class Context:
         out = np.zeros(max(1, n_gen), np.uint32)
         self._check(lib().kc_model_generate(self.h, _ptr(tk), tk.size, n_gen, _ptr(out)))
         return [int(t) for t in out[:n_gen]]
+
+    def model_sample(self, prompt, n_gen: int, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                     min_p: float = 0.0):
+        """kc_model_sample: n_gen tokens drawn with the uniform numbers u [n_gen]
+        (host); returns (tokens, their shares)."""
+        tk = np.ascontiguousarray(prompt, dtype=np.uint32)
+        u = np.ascontiguousarray(u, dtype=np.float32)
+        if u.size != n_gen:
+            raise ValueError(f"u holds {u.size} numbers, {n_gen} needed")
+        out, probs = np.zeros(max(1, n_gen), np.uint32), np.zeros(max(1, n_gen), np.float32)
+        self._check(lib().kc_model_sample(self.h, _ptr(tk), tk.size, n_gen, temperature, top_k, top_p, min_p, _ptr(u),
+                                          _ptr(out), _ptr(probs)))
+        return [int(t) for t in out[:n_gen]], [float(p) for p in probs[:n_gen]]
 
     def model_generate_batch(self, prompts, n_gen: int):
         """kc_model_generate_batch: greedy decode of len(prompts) independent
