@@ -225,17 +225,20 @@ struct SampleRow {
     const bool some = (m - l) * c32 < 100.f;
     return __hiloint2double(some ? __double2hiint(w) : 0, some ? __double2loint(w) : 0);
   }
-  // Sums of the lanes' v[y] over all blocks, in every lane, after a barrier.
+  // Sums of the lanes' v[y] over all blocks: told before a barrier, in every lane
+  // behind it.
   template <int N>
-  __device__ __forceinline__ void totals(double (&v)[N]) {
-    double(*part)[SMP_ALL] = s.part[turn & 1];
+  __device__ __forceinline__ void tell(double (&v)[N]) {
+    double(*part)[SMP_ALL] = s.part[turn++ & 1];
 #pragma unroll
     for (int y = 0; y < N; ++y) {
       v[y] = warp_sum(v[y]);
       if (lane < blocks) *cluster.map_shared_rank(&part[y][rank * SMP_WARPS + warp], lane) = v[y];
     }
-    cluster.sync();
-    ++turn;
+  }
+  template <int N>
+  __device__ __forceinline__ void gather(double (&v)[N]) {
+    double(*part)[SMP_ALL] = s.part[(turn - 1) & 1];
 #pragma unroll
     for (int y = 0; y < N; ++y) {
       double sum = 0;
@@ -309,12 +312,24 @@ struct SampleRow {
       if (i < members && tid % share == 0) done(i, sum);
     }
   }
+  // The blocks' s.fine, summed, after a barrier: four a lane.
+  __device__ __forceinline__ void gather_fine(uint64_t (&in)[4]) {
+    for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
+      cluster.map_shared_rank(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
+    cluster.sync();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) in[e] = 0;
+    for (int b = 0; b < blocks; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] += s.weights[b][4 * lane + e];
+  }
   // The highest place among those of `bin` (and at or past `from`) from which on
-  // `measure` of them reaches `want`, by halving the range of places: for bins of
-  // more tokens than a list holds. (The lowest, if rounding says that all of them
-  // do not.) The blocks take the same steps.
+  // `measure` of them (whole numbers) reaches `want`, for bins of more tokens than a
+  // list holds, as where many are equal: the range of places is cut into 128, again
+  // and again. (The lowest, if rounding says that all of them do not reach it.) The
+  // blocks take the same steps.
   template <class Measure>
-  __device__ uint64_t halve(int bin, uint64_t from, double want, Measure measure) {
+  __device__ uint64_t narrow(int bin, uint64_t from, double want, Measure measure) {
     uint64_t lo = ~0ull, hi = 0;
     const auto each = [&](auto fn) {
       each4([&](const float (&v)[4], int i) {
@@ -354,16 +369,27 @@ struct SampleRow {
       hi = max(hi, s.span[b][1]);
     }
     while (lo < hi) {
-      const uint64_t mid = lo + (hi - lo + 1) / 2;
-      double sum[1] = {0};
+      const int shift = max(0, 57 - __clzll((long long)(hi - lo)));  // (hi - lo) >> shift < 128
+      if (tid < SMP_FINE) s.fine[tid] = 0;
+      __syncthreads();
       each([&](float l, uint64_t o) {
-        if (o >= mid) sum[0] += measure(l);
+        if (o >= lo && o <= hi) atomicAdd((unsigned long long*)&s.fine[(o - lo) >> shift], (unsigned long long)measure(l));
       });
-      totals(sum);
-      if (sum[0] >= want) lo = mid;
-      else hi = mid - 1;
+      __syncthreads();
+      uint64_t in[4];
+      gather_fine(in);
+      Quad f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[e] = (double)in[e];
+      f.scan(lane);
+      const double all = Quad::of(SMP_FINE - 1, [&](int e) { return f.upto(e); });
+      int part = Quad::last(lane, [&](int e) { return f.v[e] > 0 && all - (f.upto(e) - f.v[e]) >= want; });
+      if (part < 0) part = max(0, Quad::first(lane, [&](int e) { return f.v[e] > 0; }) & (SMP_FINE - 1));
+      want -= all - Quad::of(part, [&](int e) { return f.upto(e); });
+      lo += (uint64_t)part << shift;
+      hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+      cluster.sync();  // (all have read the sums)
     }
-    cluster.sync();
     return lo;
   }
 };
@@ -610,7 +636,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       cluster.sync();
       cut = s.cut;
     } else {
-      cut = x.halve(bin, 0, rest, [](float) { return 1.0; });
+      cut = x.narrow(bin, 0, rest, [](float) { return 1ull; });
     }
     floor = order_value((uint32_t)(cut >> 32));
   }
@@ -742,14 +768,12 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         });
       }
       __syncthreads();
-      for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
-        cluster.map_shared_rank(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
+      // (One barrier for both.)
       double total[2] = {sums[0], sums[1]};
-      x.totals(total);
-      uint64_t in[4] = {0, 0, 0, 0};
-      for (int b = 0; b < blocks; ++b)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) in[e] += s.weights[b][4 * lane + e];
+      x.tell(total);
+      uint64_t in[4];
+      x.gather_fine(in);
+      x.gather(total);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f.v[e] = (double)in[e] / SMP_UNIT;
       f.scan(lane);
@@ -837,7 +861,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         __syncthreads();
       }
     } else {
-      cut = max(cut, x.halve(bin, cut, rest, [&](float l) { return x.weight(l); }));
+      cut = max(cut, x.narrow(bin, cut, rest * SMP_UNIT, [&](float l) { return llrint(x.weight(l) * SMP_UNIT); }));
       double all_kept[3] = {0, 0, 0};
       x.each4([&](const float (&v)[4], int i) {
         for (int e = 0; e < 4; ++e)
@@ -847,7 +871,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
           }
       });
       stretch = x.turn;
-      x.totals(all_kept);
+      x.tell(all_kept);
+      cluster.sync();
     }
   } else {
     x.each4([&](const float (&v)[4], int i) {
@@ -860,7 +885,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         if (order_of(v[e], i + e) >= cut && w[e] >= least) sums[2] += w[e];
     });
     stretch = x.turn;
-    x.totals(sums);
+    x.tell(sums);
+    cluster.sync();
   }
 
   // ---- the stretch that holds the token, then the token ------------------------------------------------
