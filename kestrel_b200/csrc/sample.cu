@@ -43,6 +43,7 @@ constexpr int SMP_FINE = 128;     // and of one of them
 constexpr int SMP_BINS = SMP_COARSE * SMP_FINE;
 constexpr int SMP_LIST = 512;     // tokens of a bin that one block looks through
 constexpr int SMP_SHORT = 256;    // tokens that top-k leaves to one block
+constexpr int SMP_FEW = 128;      // the largest k for which the threads' maxima are looked at first
 constexpr int SMP_NEAR = 1024;    // tokens of a coarse bin that a block keeps in mind
 constexpr int SMP_TRIES = 40;     // coarse bins looked at for top-p, at most
 constexpr float SMP_SPAN = 24.f;  // the histogram reaches so far below the maximum
@@ -71,7 +72,8 @@ struct alignas(16) SampleShared {
   uint64_t span[SMP_CLUSTER][2];
   float top[SMP_CLUSTER], low[SMP_CLUSTER];
   int first[SMP_CLUSTER];  // greedy: the blocks' first maxima
-  int listed[2];  // (rank 0)
+  int listed[3];  // (rank 0)
+  int listed_by[SMP_ALL];  // (by warps)
   // From rank 0: the cut for k; then the stretch that holds the token.
   uint64_t cut;
   double left, total;
@@ -213,6 +215,23 @@ struct SampleRow {
       fn(now, at + here);
     }
   }
+  // fn(l) of eight values a lane at a time, in no order; not a number where there is
+  // none. (For short work, so that more of it is under way.)
+  template <class Fn>
+  __device__ __forceinline__ void each8(Fn fn) {
+    const int seg = chunk / SMP_WARPS, end = (warp + 1) * seg;
+    for (int i = warp * seg + 4 * lane; i < end; i += 256) {
+      float v[8], w[4];
+      load4(logits + i, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = w[e];
+      const bool more = i + 128 < end;
+      if (more) load4(logits + i + 128, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 + e] = more ? w[e] : NAN;
+      fn(v);
+    }
+  }
   // How far below the maximum, in bins; the bin.
   __device__ __forceinline__ float depth(float l) const { return fminf((m - l) * scale, SMP_BINS - 1); }
   static __device__ __forceinline__ int whole(float depth) {
@@ -329,9 +348,19 @@ struct SampleRow {
   // and again. (The lowest, if rounding says that all of them do not reach it.) The
   // blocks take the same steps.
   template <class Measure>
-  __device__ uint64_t narrow(int bin, uint64_t from, double want, Measure measure) {
+  __device__ uint64_t narrow(int bin, uint64_t from, double want, bool near, Measure measure) {
     uint64_t lo = ~0ull, hi = 0;
+    // (`near`: the block keeps the bin's tokens in mind, if they are not too many.)
     const auto each = [&](auto fn) {
+      if (near && s.n_near <= SMP_NEAR) {
+        for (int j = tid; j < s.n_near; j += SMP_THREADS) {
+          const int i = s.near[j];
+          const float l = (float)logits[i];
+          const uint64_t o = order_of(l, at + i);
+          if (whole(depth(l)) == bin && o >= from) fn(l, o);
+        }
+        return;
+      }
       each4([&](const float (&v)[4], int i) {
         for (int e = 0; e < 4; ++e) {
           const uint64_t o = order_of(v[e], i + e);
@@ -416,7 +445,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (by_k || by_p)
     for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) s.coarse[i / 32][i % 32] = 0;
   if (tid < 16) s.table[tid] = exp2(tid / 16.0);
-  if (tid < 2) s.listed[tid] = 0;
+  if (tid < 3) s.listed[tid] = 0;
   float top = -INFINITY, low = INFINITY;
   {
     const T* from = static_cast<const T*>(a.logits) + row * a.stride + x.at;
@@ -451,6 +480,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     }
     for (int i = done + tid; i < chunk; i += SMP_THREADS) x.logits[i] = i < have ? (T)take((float)from[i]) : (T)-INFINITY;
   }
+  float thread_top = top;  // of the thread's own tokens
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -485,6 +515,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (top == INFINITY && !greedy) {
     // Infinite ones share everything.
     for (int i = tid; i < chunk; i += SMP_THREADS) x.logits[i] = (float)x.logits[i] == INFINITY ? (T)0.f : (T)-INFINITY;
+    thread_top = thread_top == INFINITY ? 0.f : -INFINITY;
     top = low = 0.f;
     __syncthreads();
   }
@@ -533,44 +564,39 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     n += __shfl_xor_sync(0xffffffffu, n, 2);
     for (int b = tid & 3; b < blocks; b += 4) put(b, bin, n);
     cluster.sync();
-    ++x.turn;
   };
 
   // ---- top-k ------------------------------------------------------------------------------------
   float floor = -INFINITY;  // (no token below it is kept)
   if (by_k) {
-    x.each4([&](const float (&v)[4], int) {
-      int b[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = x.whole(x.depth(v[e])) / SMP_FINE;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) atomicAdd(&s.coarse[b[e]][lane], 1u);
-    });
-    tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.bins[0][rank][0], b)[bin] = (uint16_t)n; });
-    uint32_t count[4];  // tokens of coarse bins 4 lane ..
-    x.gather_bins(0, count);
-    // (Whole numbers, exact in 64 bits.)
-    Quad q;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q.v[e] = count[e];
-    q.scan(lane);
-    const int coarse = Quad::first(lane, [&](int e) { return q.upto(e) >= k; });
-    const double through = Quad::of(coarse, [&](int e) { return q.upto(e); });
-    if (through <= SMP_SHORT) {
-      // Few enough: one block does the rest with them, pair by pair.
+    // The tokens down to a coarse bin to rank 0's list; how many there were. (Every
+    // block counts its own: rank 0's list is gone with rank 0.)
+    const auto list_down_to = [&](int coarse) {
       const float ends = (coarse + 1) * SMP_FINE;
+      int mine = 0;
       x.each4([&](const float (&v)[4], int i) {
         bool here[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) here[e] = x.depth(v[e]) < ends;
         if (__any_sync(0xffffffffu, here[0] || here[1] || here[2] || here[3])) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x.list(here[e], 0, order_of(v[e], i + e), x.weight(v[e]));
+          for (int e = 0; e < 4; ++e) {
+            mine += here[e];
+            x.list(here[e], 0, order_of(v[e], i + e), x.weight(v[e]));
+          }
         }
       });
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if (lane < blocks) *cluster.map_shared_rank(&s.listed_by[rank * SMP_WARPS + warp], lane) = mine;
       cluster.sync();
-      if (rank != 0) return;
-      const int members = s.listed[0];
+      int all = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * lane + e < blocks * SMP_WARPS) all += s.listed_by[4 * lane + e];
+      return (int)__reduce_add_sync(0xffffffffu, all);
+    };
+    // Few enough: rank 0 does the rest with them, pair by pair.
+    const auto finish = [&](int members) {
       uint64_t *placed = s.comp + SMP_SHORT, *kept = s.weight + SMP_SHORT;
       if (tid == 0) s.add[0] = 0;
       // The weights of those at a token's place and above, and in the low bits its
@@ -599,6 +625,52 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
               if (a.probs) a.probs[number] = (float)((double)kept[i] / total);
             }
           });
+    };
+    uint32_t count[4];  // of coarse bins 4 lane ..
+    Quad q;
+    if (k <= SMP_FEW) {
+      // The k-th largest of the threads' maxima is no more than the k-th largest
+      // token: the tokens down to its coarse bin are enough, and seldom many more. (A
+      // histogram of a value a thread instead of all: 256 rows of 151936 by top-k 40
+      // took 123 us with that of all.)
+      atomicAdd(&s.coarse[x.whole(x.depth(thread_top)) / SMP_FINE][lane], 1u);
+      tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.bins[0][rank][0], b)[bin] = (uint16_t)n; });
+      x.gather_bins(x.turn++, count);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q.v[e] = count[e];
+      q.scan(lane);
+      const int coarse = Quad::first(lane, [&](int e) { return q.upto(e) >= k; });
+      if (coarse < SMP_COARSE - 1) {
+        const int members = list_down_to(coarse);
+        if (members <= SMP_SHORT) {
+          if (rank == 0) finish(members);
+          return;
+        }
+      }
+      for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) s.coarse[i / 32][i % 32] = 0;
+      __syncthreads();
+    }
+    x.each4([&](const float (&v)[4], int) {
+      int b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = x.whole(x.depth(v[e])) / SMP_FINE;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) atomicAdd(&s.coarse[b[e]][lane], 1u);
+    });
+    const int counts = x.turn;
+    tell_columns([&](int b, int bin, uint32_t n) {
+      cluster.map_shared_rank(&s.bins[counts & 1][rank][0], b)[bin] = (uint16_t)n;
+    });
+    x.gather_bins(x.turn++, count);
+    // (Whole numbers, exact in 64 bits.)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.v[e] = count[e];
+    q.scan(lane);
+    const int coarse = Quad::first(lane, [&](int e) { return q.upto(e) >= k; });
+    const double through = Quad::of(coarse, [&](int e) { return q.upto(e); });
+    if (k > SMP_FEW && through <= SMP_SHORT) {
+      const int members = list_down_to(coarse);
+      if (rank == 0) finish(members);
       return;
     }
     // The bin that holds the k-th, then its place among the bin's.
@@ -620,11 +692,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       }
       if (__any_sync(0xffffffffu, here[0] || here[1] || here[2] || here[3])) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.list(here[e], 0, order_of(v[e], i + e), 0.0);
+        for (int e = 0; e < 4; ++e) x.list(here[e], 2, order_of(v[e], i + e), 0.0);
       }
     });
     cluster.sync();
-    const int members = *cluster.map_shared_rank(&s.listed[0], 0);
+    const int members = *cluster.map_shared_rank(&s.listed[2], 0);
     if (members <= SMP_LIST) {
       if (rank == 0)
         x.pairs(
@@ -636,7 +708,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       cluster.sync();
       cut = s.cut;
     } else {
-      cut = x.narrow(bin, 0, rest, [](float) { return 1ull; });
+      cut = x.narrow(bin, 0, rest, false, [](float) { return 1ull; });
     }
     floor = order_value((uint32_t)(cut >> 32));
   }
@@ -651,26 +723,20 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) s.coarse[i / 32][i % 32] = 0;
       __syncthreads();
     }
-    for (int i = warp * seg + 4 * lane; i < (warp + 1) * seg; i += 256) {
-      // Eight values a lane under way.
-      float v[2][4];
-      load4(x.logits + i, v[0]);
-      if (i + 128 < (warp + 1) * seg) load4(x.logits + i + 128, v[1]);
-      else v[1][0] = v[1][1] = v[1][2] = v[1][3] = NAN;
+    x.each8([&](const float (&v)[8]) {
       int b[8];
       uint32_t w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float r = x.depth(v[e / 4][e % 4]), begins = __fadd_rd(r * (1.f / SMP_FINE), 8388608.f);
+        const float r = x.depth(v[e]), begins = __fadd_rd(r * (1.f / SMP_FINE), 8388608.f);
         b[e] = __float_as_int(begins) & (SMP_COARSE - 1);
         const float part = exp2_fast(((begins - 8388608.f) * SMP_FINE - r) * unit);
         w[e] = max(1, __float_as_int(__fadd_rn(part * 65536.f, 8388608.f)) & 0x1ffff);  // (none is lost)
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (v[e / 4][e % 4] >= floor)  // (not of NAN)
-          atomicAdd(&s.coarse[b[e]][lane], w[e]);
-    }
+        if (v[e] >= floor) atomicAdd(&s.coarse[b[e]][lane], w[e]);  // (not of NAN)
+    });
     tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.mass[rank][0], b)[bin] = n; });
     Quad q;
 #pragma unroll
@@ -861,7 +927,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         __syncthreads();
       }
     } else {
-      cut = max(cut, x.narrow(bin, cut, rest * SMP_UNIT, [&](float l) { return llrint(x.weight(l) * SMP_UNIT); }));
+      cut = max(cut, x.narrow(bin, cut, rest * SMP_UNIT, true, [&](float l) { return llrint(x.weight(l) * SMP_UNIT); }));
       double all_kept[3] = {0, 0, 0};
       x.each4([&](const float (&v)[4], int i) {
         for (int e = 0; e < 4; ++e)
