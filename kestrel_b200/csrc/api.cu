@@ -3326,8 +3326,10 @@ int kc_rope(kc_ctx* ctx, int rope, int dim, int layout, float base, int scaling,
     if (!(gain > -INFINITY && gain < INFINITY)) return fail(ctx, KC_ERR_ARG, "kc_rope: gain is not finite");
     for (int i = 0; freq_factors && i < dim / 2; ++i)
       if (!positive(freq_factors[i])) return fail(ctx, KC_ERR_ARG, "kc_rope: freq_factors[%d] is %g", i, freq_factors[i]);
-    ctx->ropes[rope] = make_rope(dim, layout == KC_ROPE_INTERLEAVED, base, scaling, factor, original, low, high, gain,
-                                 freq_factors);
+    RopeParams r;
+    if (!make_rope(r, dim, layout == KC_ROPE_INTERLEAVED, base, scaling, factor, original, low, high, gain, freq_factors))
+      return fail(ctx, KC_ERR_ARG, "kc_rope: a frequency above %g (of base, factor and freq_factors)", ROPE_MAX_FREQUENCY);
+    ctx->ropes[rope] = r;
     return KC_OK;
   });
 }

@@ -167,9 +167,14 @@ __global__ void __launch_bounds__(32 * DecShape<NB, HT>::W, 1)
   constexpr bool kHalf = std::is_same_v<TKV, __half>;
   constexpr float kLift = kHalf ? 15.f : 0.f;    // f16 weights up to 2^15: small ones keep their bits
   // SHARED: beside the prefixes' kernel, whose blocks have all seen the end of what
-  // came before it when these start; it is waited for at the end.
-  if constexpr (SHARED) pdl_trigger();
-  else pdl_enter();
+  // came before it when these start (the fence: nor does this SM hold anything older);
+  // it is waited for at the end.
+  if constexpr (SHARED) {
+    pdl_trigger();
+    __threadfence();
+  } else {
+    pdl_enter();
+  }
   extern __shared__ uint8_t dec_raw[];
   __shared__ __align__(8) uint64_t full[W][ST];
   __shared__ long long red[3][W], found_at[W];

@@ -16,10 +16,10 @@
 // the next ones before the last are turned.
 //
 // Measured on a B200 (plain copy 6.56 TB/s): 8192 rows of 36 heads of 128, bf16,
-// 151 MB in 37.3 us (4.0 TB/s); 24 x 256 rows of 32 and 4 heads of 128, f32 into
-// an f16 cache, 239 MB in 45.0 us (5.3). Angles by each thread for up to eight
+// 151 MB in 29.8 us (5.1 TB/s); 24 x 256 rows of 32 and 4 heads of 128, f32 into
+// an f16 cache, 239 MB in 44.8 us (5.3). Angles by each thread for up to eight
 // heads of its own took 43.6 and 66.8 us, places by division instead of steps 46.4
-// and 47.7.
+// and 47.7, pairs turned one by one instead of two at a time 37.3 and 47.0.
 #include <math.h>
 
 #include <algorithm>
@@ -40,10 +40,10 @@ constexpr int ROPE_THREADS = 128;
 constexpr int ROPE_ROWS = 8;                 // rows of a block, at most
 constexpr int ROPE_PAIRS = ROPE_ROWS * 64;   // and their angles
 
-RopeParams make_rope(int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
-                     float high, float gain, const float* freq_factors) {
+bool make_rope(RopeParams& r, int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
+               float high, float gain, const float* freq_factors) {
   const long double two_pi = 2 * acosl(-1.0L), s = factor, len = original;
-  RopeParams r{};
+  r = RopeParams{};
   r.dim = dim;
   r.interleaved = interleaved;
   r.gain = gain != 0.f ? gain : scaling == ROPE_YARN ? (float)(1 + 0.1L * logl(s)) : 1.f;
@@ -65,11 +65,12 @@ RopeParams make_rope(int dim, bool interleaved, float base, int scaling, float f
       const long double z = std::min(1.0L, std::max(0.0L, (len * w / two_pi - low) / ((long double)high - low)));
       w *= z + (1 - z) / s;
     }
+    if (!(w <= ROPE_MAX_FREQUENCY)) return false;
     long double turn = w / two_pi;
     turn -= floorl(turn);  // whole turns a position change nothing
     r.turn[i] = (uint64_t)(int64_t)llrintl(ldexpl(turn - (turn >= 0.5L ? 1 : 0), 64));
   }
-  return r;
+  return true;
 }
 
 // gain * (cos, sin) of a phase in 64-bit fractions of a turn.
@@ -143,6 +144,17 @@ struct RopeLane {
   }
 };
 
+// Two consecutive values as an f32 pair, and back.
+template <typename S>
+__device__ __forceinline__ uint64_t widen2(const S* p) {
+  if constexpr (std::is_same_v<S, __nv_bfloat16>) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  } else {
+    return f2((float)p[0], (float)p[1]);
+  }
+}
+
 // One thread's values of a head, as they are in memory.
 template <int VEC, bool HALF, typename S>
 struct RopeValues {
@@ -151,32 +163,49 @@ struct RopeValues {
     x = load_vec<VEC>(head + l.col, aligned);
     if (HALF && l.first >= 0) y = load_vec<VEC>(head + l.col + half, aligned);
   }
-  // cos, sin: of the row's pairs.
+  // cos, sin: of the row's pairs. Halves of two columns or more are turned two pairs
+  // at a time.
   template <typename D>
   __device__ __forceinline__ void put(D* head, const RopeLane<VEC, HALF>& l, int half, bool turns, const float* cos,
                                       const float* sin, bool aligned) const {
     float a[VEC], b[VEC];
+    if constexpr (HALF && VEC > 1) {
+      const uint64_t minus = f2(-1.f, -1.f);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      a[i] = (float)x.v[i];
-      b[i] = HALF ? (float)y.v[i] : 0.f;
-    }
-    if (turns) {
-      if constexpr (HALF) {
-        const Raw<VEC, float> c = load_vec<VEC>(cos + l.first, true), s = load_vec<VEC>(sin + l.first, true);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float p = a[i], q = b[i];
-          a[i] = __fmaf_rn(p, c.v[i], -(q * s.v[i]));
-          b[i] = __fmaf_rn(p, s.v[i], q * c.v[i]);
+      for (int i = 0; i < VEC; i += 2) {
+        uint64_t p = widen2(x.v + i), q = widen2(y.v + i);
+        if (turns) {
+          const uint64_t c = *reinterpret_cast<const uint64_t*>(cos + l.first + i),
+                         s = *reinterpret_cast<const uint64_t*>(sin + l.first + i);
+          const uint64_t u = fma2(p, c, mul2(mul2(q, minus), s));
+          q = fma2(p, s, mul2(q, c));
+          p = u;
         }
-      } else {
-        const Raw<VEC / 2, float> c = load_vec<VEC / 2>(cos + l.first, true), s = load_vec<VEC / 2>(sin + l.first, true);
+        const float2 pf = f2(p), qf = f2(q);
+        a[i] = pf.x;
+        a[i + 1] = pf.y;
+        b[i] = qf.x;
+        b[i + 1] = qf.y;
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          const float p = a[i], q = a[i + 1];
-          a[i] = __fmaf_rn(p, c.v[i / 2], -(q * s.v[i / 2]));
-          a[i + 1] = __fmaf_rn(p, s.v[i / 2], q * c.v[i / 2]);
+      for (int i = 0; i < VEC; ++i) {
+        a[i] = (float)x.v[i];
+        b[i] = HALF ? (float)y.v[i] : 0.f;
+      }
+      if (turns) {
+        if constexpr (HALF) {
+          const float p = a[0], q = b[0], c = cos[l.first], s = sin[l.first];
+          a[0] = __fmaf_rn(p, c, -(q * s));
+          b[0] = __fmaf_rn(p, s, q * c);
+        } else {
+          const Raw<VEC / 2, float> c = load_vec<VEC / 2>(cos + l.first, true), s = load_vec<VEC / 2>(sin + l.first, true);
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            const float p = a[i], q = a[i + 1];
+            a[i] = __fmaf_rn(p, c.v[i / 2], -(q * s.v[i / 2]));
+            a[i + 1] = __fmaf_rn(p, s.v[i / 2], q * c.v[i / 2]);
+          }
         }
       }
     }
@@ -344,9 +373,9 @@ static int rope_vec(const RopeParams& r, int hd) {
 }
 
 // Rows a block takes: up to six loads a thread, while that leaves two blocks an SM
-// (8192 rows of 36 heads of 128, bf16: one row 39.8 us, two 37.3, four 42.2, eight
-// 45.8; 24 x 256 rows of 32 and 4 heads, f32 to f16: 47.1, 45.0, 51.2 and 51.1); a
-// row's heads over several blocks where there are fewer rows than SMs.
+// (8192 rows of 36 heads of 128, bf16: two 30.0 us, four 32.5; 24 x 256 rows of 32 and
+// 4 heads, f32 to f16: 45.0 and 46.3; blocks of 256 threads 31.0 and 50.3, of 64 32.3
+// and 46.0); a row's heads over several blocks where there are fewer rows than SMs.
 static RopeCut rope_cut(int n_rows, int heads, int lanes, int dim) {
   const int per = heads * lanes, sms = num_sms();  // (a row has at most 2^24 values)
   RopeCut c{1, 1};

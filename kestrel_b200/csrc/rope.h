@@ -23,9 +23,11 @@ struct RopeParams {
 
 enum : int { ROPE_NONE = 0, ROPE_LINEAR = 1, ROPE_YARN = 2, ROPE_BANDS = 3 };
 
-// The formulas of kc_rope, in the host's widest type.
-RopeParams make_rope(int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
-                     float high, float gain, const float* freq_factors);
+// The formulas of kc_rope, in the host's widest type. False: a frequency above
+// ROPE_MAX_FREQUENCY, past which the far positions' phases would not be exact.
+constexpr double ROPE_MAX_FREQUENCY = 4.0;
+bool make_rope(RopeParams& r, int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
+               float high, float gain, const float* freq_factors);
 
 // Rows of n_head heads of hd, strides in elements; out may be x.
 void launch_rope(const RopeParams& r, const int32_t* positions, int n_rows, int n_head, int hd, int t, const void* x,

@@ -135,7 +135,8 @@ def test_refusals(ctx):
                       (dict(dim=64, scaling="yarn", factor=2.0), 1), (dict(dim=64, gain=float("inf")), 1),
                       (dict(dim=64, scaling="bands", factor=2.0, original=99, low=4.0, high=4.0), 1),
                       (dict(dim=64, scaling="yarn", factor=2.0, original=99, low=1.0, high=9.0, base=1.0), 1),
-                      (dict(dim=4, freq_factors=[1.0, -1.0]), 1)):
+                      (dict(dim=4, freq_factors=[1.0, -1.0]), 1), (dict(dim=4, freq_factors=[0.2, 1.0]), 1),
+                      (dict(dim=64, base=1e-3), 1)):
         with pytest.raises(KestrelCudaError) as e:
             ctx.rope(7, **bad)
         assert e.value.code == code
