@@ -372,14 +372,14 @@ static int rope_vec(const RopeParams& r, int hd) {
   return unit % 8 == 0 && (hd - r.dim) % 8 == 0 ? 8 : unit % 2 == 0 ? 2 : 1;
 }
 
-// Rows a block takes: up to six loads a thread, while that leaves two blocks an SM
+// Rows a block takes: up to eight loads a thread, while that leaves two blocks an SM
 // (8192 rows of 36 heads of 128, bf16: two 30.0 us, four 32.5; 24 x 256 rows of 32 and
 // 4 heads, f32 to f16: 45.0 and 46.3; blocks of 256 threads 31.0 and 50.3, of 64 32.3
 // and 46.0); a row's heads over several blocks where there are fewer rows than SMs.
 static RopeCut rope_cut(int n_rows, int heads, int lanes, int dim) {
   const int per = heads * lanes, sms = num_sms();  // (a row has at most 2^24 values)
   RopeCut c{1, 1};
-  while (2 * c.rows <= ROPE_ROWS && 2 * c.rows * (dim / 2) <= ROPE_PAIRS && 2 * c.rows * per <= 6 * ROPE_THREADS &&
+  while (2 * c.rows <= ROPE_ROWS && 2 * c.rows * (dim / 2) <= ROPE_PAIRS && 2 * c.rows * per <= 8 * ROPE_THREADS &&
          n_rows / (2 * c.rows) >= 2 * sms)
     c.rows *= 2;
   if (n_rows < sms) c.cuts = std::max(1, std::min({sms / n_rows, per / ROPE_THREADS, heads}));

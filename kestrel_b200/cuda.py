@@ -186,9 +186,11 @@ def _dev_ints(name: str, a, size: int | None = None):
     """A contiguous int32 CUDA tensor of `size` values (None: any)."""
     if a is None:
         return None
-    if not _is_dev(a) or not (a.dtype in _INT32 or str(a.dtype) == "torch.int32") or not a.is_contiguous():
+    if not getattr(a, "is_cuda", False) or not (a.dtype in _INT32 or str(a.dtype) == "torch.int32") or \
+            not a.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
-    _INT32.add(a.dtype)
+    if not _INT32:
+        _INT32.add(a.dtype)
     if size is not None and a.numel() != size:
         raise ValueError(f"{name} holds {a.numel()} values, {size} needed")
     return a.data_ptr()
@@ -197,15 +199,17 @@ def _dev_ints(name: str, a, size: int | None = None):
 def _dev_rows(name: str, a, heads: int | None = None, head_dim: int | None = None):
     """Row stride (elements) of a CUDA tensor [rows, heads, head_dim] whose
     heads are contiguous within a row."""
-    shape = a.shape
-    if not _is_dev(a) or len(shape) != 3 or (heads is not None and shape[1] != heads) or \
-            (head_dim is not None and shape[2] != head_dim):
+    try:  # (on the per-call path: no helper calls)
+        rows, nh, hd = a.shape
+        ok = a.is_cuda
+    except (AttributeError, TypeError, ValueError):
+        ok = False
+    if not ok or (heads is not None and nh != heads) or (head_dim is not None and hd != head_dim):
         raise ValueError(f"{name} must be a CUDA tensor [rows, heads, head_dim]")
-    rows, nh, hd = shape
-    stride = a.stride()
-    if (hd > 1 and stride[2] != 1) or (nh > 1 and stride[1] != hd):
+    s0, s1, s2 = a.stride()
+    if (hd > 1 and s2 != 1) or (nh > 1 and s1 != hd):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
-    return stride[0] if rows > 1 else nh * hd
+    return s0 if rows > 1 else nh * hd
 
 
 _FLOAT32 = set()  # torch.float32, once seen
@@ -601,10 +605,14 @@ class Context:
         n = rows if row_start is None else row_start.numel() - 1
         nh = qs = os_ = 0
         if q is not None:
-            q_out = q if q_out is None else q_out
-            qs, os_ = _dev_rows("q", q, None, hd), _dev_rows("q_out", q_out, None, hd)
-            nh = q.shape[1]
-            if q.shape[0] != rows or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != q.dtype:
+            qs = os_ = _dev_rows("q", q, None, hd)
+            shape = q.shape
+            nh = shape[1]
+            if q_out is None:
+                q_out = q
+            elif q_out is not q:
+                os_ = _dev_rows("q_out", q_out, nh, hd)
+            if shape[0] != rows or q.dtype != k.dtype or q_out.shape[0] != rows or q_out.dtype != q.dtype:
                 raise ValueError("q and q_out must have k's rows and type, and each other's shape")
         elif q_out is not None:
             raise ValueError("q_out without q")
