@@ -803,6 +803,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
       }
       if (!x.valid) break;
       if (x.nt <= 0) continue;
+      // (Nothing would hold the queries of the items to come back for this warp: a
+      // wait that it enters two of them late sees a phase of the same parity under
+      // way, and after the last item for good.)
+      if (kSplit && d.q_map && !finder) continue;
       if (used > 0) wait(&q_empty, used - 1);
       ++used;
       ok = __all_sync(0xffffffffu, ok);
