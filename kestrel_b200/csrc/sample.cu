@@ -45,7 +45,6 @@ constexpr int SMP_LIST = 512;     // tokens of a bin that one block looks throug
 constexpr int SMP_SHORT = 256;    // tokens that top-k leaves to one block
 constexpr int SMP_FEW = 128;      // the largest k for which the threads' maxima are looked at first
 constexpr int SMP_NEAR = 1024;    // tokens of a coarse bin that a block keeps in mind
-constexpr int SMP_TRIES = 40;     // coarse bins looked at for top-p, at most
 constexpr float SMP_SPAN = 24.f;  // the histogram reaches so far below the maximum
 constexpr double SMP_UNIT = 17592186044416.0;  // 2^44: sums of a list in whole numbers
 
@@ -728,10 +727,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       uint32_t w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float r = x.depth(v[e]), begins = __fadd_rd(r * (1.f / SMP_FINE), 8388608.f);
+        const float t = (x.m - v[e]) * x.scale, begins = __fadd_rd(fminf(t, SMP_BINS - 1) * (1.f / SMP_FINE), 8388608.f);
         b[e] = __float_as_int(begins) & (SMP_COARSE - 1);
-        const float part = exp2_fast(((begins - 8388608.f) * SMP_FINE - r) * unit);
-        w[e] = max(1, __float_as_int(__fadd_rn(part * 65536.f, 8388608.f)) & 0x1ffff);  // (none is lost)
+        const float part = exp2_fast(((begins - 8388608.f) * SMP_FINE - t) * unit);
+        // (None is lost that has a weight; the last bin's many without any count nothing.)
+        w[e] = t * unit < 100.f ? max(1, __float_as_int(__fadd_rn(part * 65536.f, 8388608.f)) & 0x1ffff) : 0;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -846,13 +846,19 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       target = p * total[0];
       rest = target - total[1];  // of the coarse bin's
       const double inside = Quad::of(SMP_FINE - 1, [&](int e) { return f.upto(e); });
-      // Not the bin: the next one in the target's direction that holds anything.
+      // Not the bin: the next one in the target's direction that holds anything, and
+      // from the third on those in question are halved.
       const bool high = !(rest > 0), low_of = inside < rest;
-      if (!(high || low_of) || tries + 1 >= SMP_TRIES) break;
+      if (!(high || low_of)) break;
       if (high) to = coarse - 1;
       else from = coarse + 1;
-      const int next = high ? Quad::last(lane, open) : Quad::first(lane, open);
+      int next = high ? Quad::last(lane, open) : Quad::first(lane, open);
       if (next < 0 || next >= SMP_COARSE) break;  // (rounding: the bin stands)
+      if (tries > 1) {
+        const int half = (from + to) / 2;
+        next = Quad::last(lane, [&](int e) { return open(e) && 4 * lane + e <= half; });
+        if (next < 0) next = Quad::first(lane, open);
+      }
       coarse = next;
       cluster.sync();  // (all have read the weights)
     }
