@@ -36,8 +36,8 @@
  *   kc_model_generate        the greedy loop of Engine::generate with
  *                            SamplerConfig::greedy (crates/kestrel-engine/src/
  *                            lib.rs:116-145, sampler.rs:25-27, 104-112)
- *   kc_model_sample          the same loop with the sampler's settings (Sampler::sample,
- *                            sampler.rs:48), uniform numbers from the caller
+ *   kc_model_sample          the same loop with drawn tokens, in the place of
+ *                            Sampler::sample (sampler.rs:48), by kc_sample_dev's rules
  *   kc_model_truncate        Transformer::truncate (transformer.rs:276-278)
  *   kc_model_set_sequences / _prefill_seq / _decode_seqs / _generate_batch
  *                            n independent Engine::generate greedy loops

@@ -341,6 +341,10 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
   constexpr float kMost = kF16 ? 32768.f : 1.1e9f;
   constexpr int W_TMA = 4 * NS, W_MMA = W_TMA + 1, W_AUX = W_TMA + 2;  // W_AUX: and the next
   constexpr bool kShared = S::kShared;
+  // (SHARED: many rows see a prefix whole, where a prompt's last ones do; f32, four
+  // groups of 9 at 50587, 32 and 4 heads of 128: 3.8e-6 off in 145 us with 12 tiles,
+  // 2.3e-6 in 163 with 6, 1.7e-6 in 171 with 4.)
+  constexpr int KEEP = SHARED && kSplit ? S::KEEP / 2 : S::KEEP;
   constexpr int AHEAD = NS;  // K tiles loaded before the first V
   if (threadIdx.x < 3) prefetch_map(threadIdx.x == 0 ? &maps.k : threadIdx.x == 1 ? &maps.v : &q_map);
   pdl_enter();
@@ -587,7 +591,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
               const int w = (i - 1) & 1, t = TWO ? (i - 1) >> 1 : i - 1, k = TWO ? t : t >> 1;
               const uint32_t v = stage(v_at(t));
               if (k == 0) results_read(w);
-              values(w, kp[w] + k, v, k % S::KEEP != 0);
+              values(w, kp[w] + k, v, k % KEEP != 0);
               if (!ok) break;
               if (!TWO || w == 1) tc_commit(&kv_empty[v_at(t) % ST]);
             }
@@ -609,7 +613,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           for (int t = 0; t < nt && ok; ++t) {
             const int w = t % NS;
             const uint32_t v = stage(v_at(t));
-            values(w, kp[w] + t / NS, v, t / NS % S::KEEP != 0);
+            values(w, kp[w] + t / NS, v, t / NS % KEEP != 0);
             if (!ok) break;
             tc_commit(&kv_empty[v_at(t) % ST]);
             if (t + NS < nt) step_scores(t + NS);
@@ -940,7 +944,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
           break;
         }
         tc_fence_after();
-        if (rarely(k > 0 && k % S::KEEP == 0)) {
+        if (rarely(k > 0 && k % KEEP == 0)) {
           // The products so far are complete (with the scores, or are waited for),
           // and the next ones do not add to them.
           if constexpr (kShared) {
@@ -951,7 +955,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             }
             tc_fence_after();
           }
-          keep_sums(o_t, hd16, kept, m, k == S::KEEP ? KEEP_FIRST : KEEP_ADD);
+          keep_sums(o_t, hd16, kept, m, k == KEEP ? KEEP_FIRST : KEEP_ADD);
         }
         if constexpr (kSplit)
           if (k == 0) cq = __fdiv_rn(unit, factor_sh[used & 1][my_tile][r]);
@@ -1103,7 +1107,7 @@ __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO>::THREADS, 1)
             done[v] += TWO ? nt : (nt - v + NS - 1) / NS;
             wait(&pv_done[v], done[v] - 1);
           }
-        if (rarely(mine > S::KEEP)) {
+        if (rarely(mine > KEEP)) {
           // What was kept goes back to the accumulator.
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
