@@ -16,11 +16,11 @@
 // took 145 us.)
 //
 // Measured (B200, us a call; what has to be read at 6559 GB/s; each sequence by
-// itself): 32 samples of a prompt of 4001, 32 and 4 heads of 128, f16: 40, 5.6, 47;
-// 4 groups of 32 at 6000, bf16: 143, 98, 407; 64 at 32768, 8 and 1 heads of 128, f16:
-// 76, 21, 485. The first and last are the steps of a chain: planning 9, the prefix's
-// way to its first scores 9, its products, the join 7; the second is bound by the own
-// parts' reads, 5.0 TB/s beside the prefixes.
+// itself), heads of 128: 32 samples of a prompt of 4001, 32 and 4 heads, f32 queries:
+// 40, 5.6, 47; 4 groups of 32 at 6000, 32 and 8, bf16: 143, 98, 407; 64 at 32768, 32
+// and 4, f16: 76, 21, 485. The first and last are the steps of a chain: the plan 9, the
+// prefixes' way to their first scores 9, their products, the join 7; the second is
+// bound by what the own parts read, 5.0 TB/s beside the prefixes.
 #include <algorithm>
 
 #include "common.cuh"
