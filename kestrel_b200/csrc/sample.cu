@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     const double left = first == INT_MAX ? INFINITY : want - Quad::of(first, [&](int e) { return q.upto(e) - q.v[e]; });
     if (lane < blocks) {
       SampleShared& to = *cluster.map_shared_rank(&s, lane);
-      to.owner = first == INT_MAX ? last : first;
+      to.owner = first == INT_MAX ? max(last, 0) : first;
       to.left = left;
       to.total = total;
       to.cut = cut;
