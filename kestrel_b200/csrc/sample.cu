@@ -191,7 +191,8 @@ struct Quad {
   }
 };
 
-template <typename T>
+// ONE: a row is one block's, and no cluster is launched.
+template <typename T, bool ONE>
 struct SampleRow {
   SampleShared& s;
   T* logits;              // the block's stretch in shared memory, `chunk` of them
@@ -203,6 +204,16 @@ struct SampleRow {
   double c;               // log2(e) / T
   float c32;
 
+  // A barrier of all blocks of the row; a place in block r's shared memory.
+  __device__ __forceinline__ void sync() {
+    if constexpr (ONE) __syncthreads();
+    else cluster.sync();
+  }
+  template <class P>
+  __device__ __forceinline__ P* in_block(P* p, int r) {
+    if constexpr (ONE) return p;
+    else return cluster.map_shared_rank(p, r);
+  }
   // fn(l, index) of four values a lane at a time, over the warp's stretch (whole
   // warps). The next ones are asked for before the last are at work.
   template <class Fn>
@@ -257,7 +268,7 @@ struct SampleRow {
 #pragma unroll
     for (int y = 0; y < N; ++y) {
       v[y] = warp_sum(v[y]);
-      if (lane < blocks) *cluster.map_shared_rank(&part[y][rank * SMP_WARPS + warp], lane) = v[y];
+      if (lane < blocks) *in_block(&part[y][rank * SMP_WARPS + warp], lane) = v[y];
     }
   }
   template <int N>
@@ -306,8 +317,8 @@ struct SampleRow {
     });
     __syncthreads();
     for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
-      cluster.map_shared_rank(&s.bins[turn & 1][rank][0], y / SMP_FINE)[y % SMP_FINE] = (uint16_t)fine[y % SMP_FINE];
-    cluster.sync();
+      in_block(&s.bins[turn & 1][rank][0], y / SMP_FINE)[y % SMP_FINE] = (uint16_t)fine[y % SMP_FINE];
+    sync();
     gather_bins(turn++, n);
   }
   // Adds a token to rank 0's list (whole warps; nothing past its end).
@@ -316,11 +327,11 @@ struct SampleRow {
     if (!who) return;
     const int lead = __ffs(who) - 1;
     int base = 0;
-    if (lane == lead) base = atomicAdd(cluster.map_shared_rank(&s.listed[which], 0), __popc(who));
+    if (lane == lead) base = atomicAdd(in_block(&s.listed[which], 0), __popc(who));
     base = __shfl_sync(0xffffffffu, base, lead) + __popc(who & ((1u << lane) - 1));
     if (mine && base < SMP_LIST) {
-      *cluster.map_shared_rank(&s.comp[base], 0) = comp;
-      *cluster.map_shared_rank(&s.weight[base], 0) = (uint64_t)llrint(w * SMP_UNIT);
+      *in_block(&s.comp[base], 0) = comp;
+      *in_block(&s.weight[base], 0) = (uint64_t)llrint(w * SMP_UNIT);
     }
   }
   // For each listed token i (in rank 0), by threads that share them where the list
@@ -339,8 +350,8 @@ struct SampleRow {
   // The blocks' s.fine, summed, after a barrier: four a lane.
   __device__ __forceinline__ void gather_fine(uint64_t (&in)[4]) {
     for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
-      cluster.map_shared_rank(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
-    cluster.sync();
+      in_block(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
+    sync();
 #pragma unroll
     for (int e = 0; e < 4; ++e) in[e] = 0;
     for (int b = 0; b < blocks; ++b)
@@ -393,11 +404,11 @@ struct SampleRow {
     }
     __syncthreads();
     if (tid < blocks) {
-      uint64_t* to = cluster.map_shared_rank(&s.span[rank][0], tid);
+      uint64_t* to = in_block(&s.span[rank][0], tid);
       to[0] = s.least;
       to[1] = s.best;
     }
-    cluster.sync();
+    sync();
     for (int b = 0; b < blocks; ++b) {
       lo = min(lo, s.span[b][0]);
       hi = max(hi, s.span[b][1]);
@@ -422,21 +433,21 @@ struct SampleRow {
       want -= all - Quad::of(part, [&](int e) { return f.upto(e); });
       lo += (uint64_t)part << shift;
       hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
-      cluster.sync();  // (all have read the sums)
+      sync();  // (all have read the sums)
     }
     return lo;
   }
 };
 
-template <typename T>
+template <typename T, bool ONE>
 __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs a, int chunk, bool wide) {
   extern __shared__ __align__(16) uint8_t smp_raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(smp_raw);
   pdl_enter();
   cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int blocks = ONE ? 1 : (int)cluster.num_blocks(), rank = ONE ? 0 : (int)cluster.block_rank();
   const int row = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  SampleRow<T> x{s, reinterpret_cast<T*>(smp_raw + sizeof(SampleShared)), chunk, rank * chunk, cluster, rank, blocks,
+  SampleRow<T, ONE> x{s, reinterpret_cast<T*>(smp_raw + sizeof(SampleShared)), chunk, rank * chunk, cluster, rank, blocks,
                  tid, warp, lane, 0};
 
   // ---- the row into shared memory, its maximum and least value -------------------------
@@ -502,10 +513,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     low = fminf(low, red_f[2 * w + 1]);
   }
   if (tid < blocks) {
-    *cluster.map_shared_rank(&s.top[rank], tid) = top;
-    *cluster.map_shared_rank(&s.low[rank], tid) = low;
+    *x.in_block(&s.top[rank], tid) = top;
+    *x.in_block(&s.low[rank], tid) = low;
   }
-  cluster.sync();  // (every block's shared memory is ready for its peers)
+  x.sync();  // (every block's shared memory is ready for its peers)
   for (int b = 0; b < blocks; ++b) {
     top = fmaxf(top, s.top[b]);
     low = fminf(low, s.low[b]);
@@ -539,8 +550,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (lane == 0) red[warp] = first;
     __syncthreads();
     for (int w = 0; w < SMP_WARPS; ++w) first = min(first, red[w]);
-    if (tid == 0) *cluster.map_shared_rank(&s.first[rank], 0) = first;
-    cluster.sync();
+    if (tid == 0) *x.in_block(&s.first[rank], 0) = first;
+    x.sync();
     if (rank == 0 && tid == 0) {
       for (int b = 0; b < blocks; ++b) first = min(first, s.first[b]);
       a.tokens[row] = first;
@@ -568,7 +579,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     n += __shfl_xor_sync(0xffffffffu, n, 1);
     n += __shfl_xor_sync(0xffffffffu, n, 2);
     for (int b = tid & 3; b < blocks; b += 4) put(b, bin, n);
-    cluster.sync();
+    x.sync();
   };
 
   // ---- top-k ------------------------------------------------------------------------------------
@@ -592,8 +603,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         }
       });
       mine = __reduce_add_sync(0xffffffffu, mine);
-      if (lane < blocks) *cluster.map_shared_rank(&s.listed_by[rank * SMP_WARPS + warp], lane) = mine;
-      cluster.sync();
+      if (lane < blocks) *x.in_block(&s.listed_by[rank * SMP_WARPS + warp], lane) = mine;
+      x.sync();
       int all = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -639,7 +650,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       // histogram of a value a thread instead of all: 256 rows of 151936 by top-k 40
       // took 123 us with that of all.)
       atomicAdd(&s.coarse[x.whole(x.depth(thread_top)) / SMP_FINE][lane], 1u);
-      tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.bins[0][rank][0], b)[bin] = (uint16_t)n; });
+      tell_columns([&](int b, int bin, uint32_t n) { x.in_block(&s.bins[0][rank][0], b)[bin] = (uint16_t)n; });
       x.gather_bins(x.turn++, count);
 #pragma unroll
       for (int e = 0; e < 4; ++e) q.v[e] = count[e];
@@ -664,7 +675,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     });
     const int counts = x.turn;
     tell_columns([&](int b, int bin, uint32_t n) {
-      cluster.map_shared_rank(&s.bins[counts & 1][rank][0], b)[bin] = (uint16_t)n;
+      x.in_block(&s.bins[counts & 1][rank][0], b)[bin] = (uint16_t)n;
     });
     x.gather_bins(x.turn++, count);
     // (Whole numbers, exact in 64 bits.)
@@ -700,17 +711,17 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         for (int e = 0; e < 4; ++e) x.list(here[e], 2, order_of(v[e], i + e), 0.0);
       }
     });
-    cluster.sync();
-    const int members = *cluster.map_shared_rank(&s.listed[2], 0);
+    x.sync();
+    const int members = *x.in_block(&s.listed[2], 0);
     if (members <= SMP_LIST) {
       if (rank == 0)
         x.pairs(
             members, [&](int i, int j) { return (uint64_t)(s.comp[j] >= s.comp[i]); },
             [&](int i, uint64_t sum) {
               if (sum == (uint64_t)rest)
-                for (int b = 0; b < blocks; ++b) *cluster.map_shared_rank(&s.cut, b) = s.comp[i];
+                for (int b = 0; b < blocks; ++b) *x.in_block(&s.cut, b) = s.comp[i];
             });
-      cluster.sync();
+      x.sync();
       cut = s.cut;
     } else {
       cut = x.narrow(bin, 0, rest, false, [](float) { return 1ull; });
@@ -743,7 +754,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       for (int e = 0; e < 8; ++e)
         if (v[e] >= floor) atomicAdd(&s.coarse[b[e]][lane], w[e]);  // (not of NAN)
     });
-    tell_columns([&](int b, int bin, uint32_t n) { cluster.map_shared_rank(&s.mass[rank][0], b)[bin] = n; });
+    tell_columns([&](int b, int bin, uint32_t n) { x.in_block(&s.mass[rank][0], b)[bin] = n; });
     Quad q;
 #pragma unroll
     for (int e = 0; e < 4; ++e) q.v[e] = 0;
@@ -866,7 +877,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         if (next < 0) next = Quad::first(lane, open);
       }
       coarse = next;
-      cluster.sync();  // (all have read the weights)
+      x.sync();  // (all have read the weights)
     }
     // The bin in which the sum reaches the target, and what it lacks at its beginning.
     int fine = Quad::first(lane, [&](int e) { return f.v[e] > 0 && f.upto(e) >= rest; });
@@ -906,10 +917,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       __syncthreads();
       const double mine = warp_sum(sums[2]) + (double)s.add[warp] / SMP_UNIT;
       stretch = x.turn++;
-      if (lane == 0) *cluster.map_shared_rank(&s.part[stretch & 1][2][rank * SMP_WARPS + warp], 0) = mine;
-      cluster.sync();
+      if (lane == 0) *x.in_block(&s.part[stretch & 1][2][rank * SMP_WARPS + warp], 0) = mine;
+      x.sync();
     }
-    const int members = *cluster.map_shared_rank(&s.listed[1], 0);
+    const int members = *x.in_block(&s.listed[1], 0);
     if (members <= SMP_LIST) {
       if (rank == 0) {
         // In whole units: the order of the list does not matter.
@@ -950,7 +961,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       });
       stretch = x.turn;
       x.tell(all_kept);
-      cluster.sync();
+      x.sync();
     }
   } else {
     x.each4([&](const float (&v)[4], int i) {
@@ -964,7 +975,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     });
     stretch = x.turn;
     x.tell(sums);
-    cluster.sync();
+    x.sync();
   }
 
   // ---- the stretch that holds the token, then the token ------------------------------------------------
@@ -980,14 +991,14 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     const int last = Quad::last(lane, [&](int e) { return q.v[e] > 0; });
     const double left = first == INT_MAX ? INFINITY : want - Quad::of(first, [&](int e) { return q.upto(e) - q.v[e]; });
     if (lane < blocks) {
-      SampleShared& to = *cluster.map_shared_rank(&s, lane);
+      SampleShared& to = *x.in_block(&s, lane);
       to.owner = first == INT_MAX ? max(last, 0) : first;
       to.left = left;
       to.total = total;
       to.cut = cut;
     }
   }
-  cluster.sync();
+  x.sync();
   const int owner = s.owner;
   if (owner / SMP_WARPS != rank) return;
   // The block's threads have a few tokens of the stretch each, in their order. (One
@@ -1033,36 +1044,48 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (a.probs) a.probs[number] = (float)(w_last / s.total);
 }
 
+constexpr int SMP_FIXED = (sizeof(SampleShared) + 15) / 16 * 16;
+static_assert(SMP_FIXED == sizeof(SampleShared), "the logits behind it are aligned");
+
+template <typename T, bool ONE>
+static int run_blocks(const SampleArgs& a, int blocks, int chunk, cudaStream_t st) {
+  const int bytes = SMP_FIXED + chunk * (int)sizeof(T);
+  static PerDeviceOnce attr;
+  if (smem_attr_once(attr, sample_kernel<T, ONE>, 226 * 1024) != cudaSuccess || bytes > 226 * 1024) return KC_ERR_CUDA;
+  const bool wide = !((uintptr_t)a.logits & 15) && a.stride * sizeof(T) % 16 == 0;
+  if constexpr (ONE) {
+    launch_k(sample_kernel<T, ONE>, a.n, SMP_THREADS, bytes, st, a, chunk, wide);
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (unsigned)(a.n * blocks);
+    cfg.blockDim = SMP_THREADS;
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = blocks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, sample_kernel<T, ONE>, a, chunk, wide);
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  }
+  return KC_OK;
+}
+
 template <typename T>
 static int run_sample(const SampleArgs& a, cudaStream_t st) {
-  constexpr int FIXED = (sizeof(SampleShared) + 15) / 16 * 16;
-  static_assert(FIXED == sizeof(SampleShared), "the logits behind it are aligned");
   const auto chunk_of = [&](int blocks) { return ((a.n_vocab + blocks - 1) / blocks + SMP_THREADS * 4 - 1) / (SMP_THREADS * 4) * (SMP_THREADS * 4); };
   // As few blocks as let two share an SM; more where rows leave SMs idle.
   int blocks = 1;
-  while (blocks < SMP_CLUSTER && (FIXED + chunk_of(blocks) * (int)sizeof(T) > 112 * 1024 ||
+  while (blocks < SMP_CLUSTER && (SMP_FIXED + chunk_of(blocks) * (int)sizeof(T) > 112 * 1024 ||
                                   (a.n * blocks * 2 <= num_sms() && chunk_of(blocks) > SMP_THREADS * 8)))
     blocks *= 2;
-  const int chunk = chunk_of(blocks), bytes = FIXED + chunk * (int)sizeof(T);
-  static PerDeviceOnce attr;
-  if (smem_attr_once(attr, sample_kernel<T>, 226 * 1024) != cudaSuccess || bytes > 226 * 1024) return KC_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = (unsigned)(a.n * blocks);
-  cfg.blockDim = SMP_THREADS;
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = blocks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  const bool wide = !((uintptr_t)a.logits & 15) && a.stride * sizeof(T) % 16 == 0;
-  cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, chunk, wide);
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-  return KC_OK;
+  // (A block alone has barriers of its own and plain addresses: a row of 4096 takes 8.2
+  // us so, 9.8 as a cluster of one, 16 of mixed settings 15.3 and 20.7.)
+  return blocks == 1 ? run_blocks<T, true>(a, 1, chunk_of(1), st) : run_blocks<T, false>(a, blocks, chunk_of(blocks), st);
 }
 
 int launch_sample(const SampleArgs& a, int t, cudaStream_t st) {

@@ -530,11 +530,14 @@ class Context:
     def rope_dev(self, rope: int, x, positions, out=None):
         """Rows x [rows, heads, head_dim] turned by positions [rows] (int32 CUDA
         tensor), to out (None: in place)."""
-        out = x if out is None else out
-        xs, os_ = _dev_rows("x", x), _dev_rows("out", out)
+        xs = os_ = _dev_rows("x", x)
         rows, nh, hd = x.shape
-        if out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError("out must have x's shape and type")
+        if out is None:
+            out = x
+        elif out is not x:
+            os_ = _dev_rows("out", out)
+            if out.shape != x.shape or out.dtype != x.dtype:
+                raise ValueError("out must have x's shape and type")
         self._check(lib().kc_rope_dev(self.h, rope, _dev_ints("positions", positions, rows), rows, nh, hd,
                                       _float_type("x", x), x.data_ptr(), xs, out.data_ptr(), os_))
 
