@@ -1078,10 +1078,13 @@ static int run_blocks(const SampleArgs& a, int blocks, int chunk, cudaStream_t s
 template <typename T>
 static int run_sample(const SampleArgs& a, cudaStream_t st) {
   const auto chunk_of = [&](int blocks) { return ((a.n_vocab + blocks - 1) / blocks + SMP_THREADS * 4 - 1) / (SMP_THREADS * 4) * (SMP_THREADS * 4); };
-  // As few blocks as let two share an SM; more where rows leave SMs idle.
+  // As few blocks as let two share an SM; where rows leave SMs idle more, of 4096
+  // tokens at least, but one for up to 8192 (us, one block and two: a row of 8192 bf16
+  // under top-p 14.2 and 15.4, 32 of 8192 of mixed settings 21.4 and 22.6; of 16000
+  // 25.6 and, in four, 25.2, one under top-p 18.6 and 16.4).
   int blocks = 1;
   while (blocks < SMP_CLUSTER && (SMP_FIXED + chunk_of(blocks) * (int)sizeof(T) > 112 * 1024 ||
-                                  (a.n * blocks * 2 <= num_sms() && chunk_of(blocks) > SMP_THREADS * 8)))
+                                  (a.n * blocks * 2 <= num_sms() && chunk_of(blocks) > SMP_THREADS * (blocks > 1 ? 8 : 16))))
     blocks *= 2;
   // (A block alone has barriers of its own and plain addresses: a row of 4096 takes 8.2
   // us so, 9.8 as a cluster of one, 16 of mixed settings 15.3 and 20.7.)
