@@ -21,9 +21,9 @@
 // cut among them, pair by pair. Each warp has a stretch of indices, so that the
 // stretches' sums lead to the one that holds the token, and only it is read again.
 //
-// Measured (B200): 256 rows of 151936 f32 logits 304 us under top-p (156 MB: 23.7 us
-// at 6559 GB/s), 112 under top-k, 146 without a cut; 32 rows of mixed settings 49; one
-// row of 4096 9. Bound by the steps of a row, not by memory (DRAM 6% busy, the 64-bit
+// Measured (B200): 256 rows of 151936 f32 logits 306 us under top-p (156 MB: 23.7 us
+// at 6559 GB/s), 112 under top-k, 146 without a cut; 32 rows of mixed settings 47; one
+// row of 4096 8.2. Bound by the steps of a row, not by memory (DRAM 6% busy, the 64-bit
 // pipe 16%): 33 rows of this size are under way, each a chain of a dozen steps with a
 // barrier of the cluster behind it.
 #include <cooperative_groups.h>
@@ -788,6 +788,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         x.each4([&](const float (&v)[4], int i) {
           double w[4], over[4];
           bool here[4];
+          // (Beyond the k first there is nothing: 32 rows of mixed settings take 47 us
+          // so, 50 with the weights of all.)
+          if (decltype(bounded)::value &&
+              !__any_sync(0xffffffffu, v[0] >= floor || v[1] >= floor || v[2] >= floor || v[3] >= floor))
+            return;
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = x.weight(v[e]);
 #pragma unroll
