@@ -445,6 +445,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   SampleShared& s = *reinterpret_cast<SampleShared*>(smp_raw);
   pdl_enter();
   cg::cluster_group cluster = cg::this_cluster();
+  // A block's shared memory may be written by its peers once it runs: all say so here,
+  // and the first to write waits for it, behind its loads.
+  if constexpr (!ONE) cluster.barrier_arrive();
   const int blocks = ONE ? 1 : (int)cluster.num_blocks(), rank = ONE ? 0 : (int)cluster.block_rank();
   const int row = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   SampleRow<T, ONE> x{s, reinterpret_cast<T*>(smp_raw + sizeof(SampleShared)), chunk, rank * chunk, cluster, rank, blocks,
@@ -512,11 +515,12 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     top = fmaxf(top, red_f[2 * w]);
     low = fminf(low, red_f[2 * w + 1]);
   }
+  if constexpr (!ONE) cluster.barrier_wait();
   if (tid < blocks) {
     *x.in_block(&s.top[rank], tid) = top;
     *x.in_block(&s.low[rank], tid) = low;
   }
-  x.sync();  // (every block's shared memory is ready for its peers)
+  x.sync();  // (and what the blocks have set up of their own is ready for their peers)
   for (int b = 0; b < blocks; ++b) {
     top = fmaxf(top, s.top[b]);
     low = fminf(low, s.low[b]);
