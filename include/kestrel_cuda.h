@@ -594,8 +594,9 @@ KC_API int kc_attn_shared_dev(kc_ctx* ctx, int cache, int layer, const int32_t* 
    sum reaches top_p times all of theirs (one at least); of these those with w_j >=
    min_p (min_p above 1: 1). tokens[i] is the first in the order of the indices at
    which the running sum of what is kept exceeds u times their sum; probs[i] (NULL:
-   not wanted) its share of that sum. Weights and sums are good to 2e-13, so rows
-   whose border lies further off get the token that exact arithmetic gives.
+   not wanted) its share of that sum. Weights are good to 2e-13 and sums to 4e-13, so
+   rows whose borders lie further off than 1e-12 get the token that exact arithmetic
+   gives.
    A logit that is not a number counts as minus infinity; of infinite ones each
    weighs 1 and the others nothing; a row with nothing else than minus infinity gets
    token -1 and share 0. u below 0 or not a number counts as 0, 1 and above as the

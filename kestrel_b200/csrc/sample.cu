@@ -11,7 +11,10 @@
 //
 // Sums decide between neighbours that differ by a millionth of the row, so weights
 // are computed in 64 bits (good to 2e-13) and every sum is either of whole numbers
-// or in an order that does not depend on timing.
+// or in an order that does not depend on timing. The whole numbers are units of 2^-60
+// of the largest weight, in two words, where any number of tokens may meet, and of
+// 2^-54 in lists of 512: off by 2e-13 of it at most, for any number. (In one word, by units of
+// 2^-44, 400 thousand equal light tokens are off by 1e-8, and top-p ends elsewhere.)
 //
 // A cluster of up to eight blocks holds a row in its shared memory: the logits are
 // read once. On the way into it the maximum; then a histogram over (m - l) finds
@@ -52,7 +55,8 @@ constexpr int SMP_SHORT = 256;    // tokens that top-k leaves to one block
 constexpr int SMP_FEW = 128;      // the largest k for which the threads' maxima are looked at first
 constexpr int SMP_NEAR = 1024;    // tokens of a coarse bin that a block keeps in mind
 constexpr float SMP_SPAN = 24.f;  // the histogram reaches so far below the maximum
-constexpr double SMP_UNIT = 17592186044416.0;  // 2^44: sums of a list in whole numbers
+constexpr double SMP_UNIT = 0x1p54;  // a list's weights in whole numbers, whose sum fits 64 bits
+constexpr int SMP_LOW = 16;          // sums over more: units of 2^-60, these bits apart
 
 // What the blocks of a row share: in every block, written by its peers. What they
 // tell each other again goes to one of two places by turns: there is a barrier of
@@ -61,12 +65,15 @@ struct alignas(16) SampleShared {
   union {
     uint32_t coarse[SMP_COARSE][32];  // a column a lane: no two of a warp meet in a bank
     struct {                          // once that histogram is through:
-      uint64_t weights[SMP_CLUSTER][SMP_FINE];  // the blocks' weights by bins of a coarse bin
+      double weights[SMP_CLUSTER][SMP_FINE];  // the blocks' weights by bins of a coarse bin
       uint64_t comp[SMP_LIST];                  // listed tokens (rank 0)
       uint64_t weight[SMP_LIST];
     };
   };
+  // Sums of a block's weights, by bins of a coarse bin, then by stretches (add_weight):
+  // fewer than 2^16 tokens, so either word holds.
   uint64_t fine[SMP_FINE];
+  uint32_t fine_low[SMP_FINE];
   union {
     uint16_t bins[2][SMP_CLUSTER][SMP_COARSE];  // the blocks' counts (a block holds fewer than 2^16)
     uint32_t mass[SMP_CLUSTER][SMP_COARSE];     // or weights
@@ -85,7 +92,6 @@ struct alignas(16) SampleShared {
   int owner;
   // The block's own.
   double table[16];
-  uint64_t add[SMP_ALL];
   uint64_t best, least;
   float red[2 * SMP_WARPS];
 };
@@ -295,6 +301,22 @@ struct SampleRow {
       n[3] += y.y >> 16;
     }
   }
+  // s.fine: cleared (a barrier is the caller's), one weight more, what it holds.
+  __device__ __forceinline__ void clear_weights() {
+    if (tid < SMP_FINE) {
+      s.fine[tid] = 0;
+      s.fine_low[tid] = 0;
+    }
+  }
+  __device__ __forceinline__ void add_weight(int bin, double w) {
+    const uint64_t units = (uint64_t)llrint(w * 0x1p60);
+    const uint32_t low = (uint32_t)units & ((1u << SMP_LOW) - 1);
+    atomicAdd((unsigned long long*)&s.fine[bin], (unsigned long long)(units >> SMP_LOW));
+    if (low) atomicAdd(&s.fine_low[bin], low);
+  }
+  __device__ __forceinline__ double weights_of(int bin) const {
+    return (double)s.fine[bin] * 0x1p-44 + (double)s.fine_low[bin] * 0x1p-60;
+  }
   // Tokens by bins of one coarse bin, of all blocks.
   __device__ __forceinline__ void fine_bins(int coarse, uint32_t (&n)[4]) {
     const float begins = coarse * SMP_FINE, ends = begins + SMP_FINE;
@@ -335,22 +357,31 @@ struct SampleRow {
     }
   }
   // For each listed token i (in rank 0), by threads that share them where the list
-  // is short: sum over the list's j of get(i, j), then done(i, sum).
-  template <class Get, class Done>
-  __device__ __forceinline__ void pairs(int members, Get get, Done done) {
+  // is short: the sum of of[j] over the list's j with is(i, j), and how many there are,
+  // then done(i, sum, count).
+  template <class Is, class Done>
+  __device__ __forceinline__ void pairs(int members, const uint64_t* of, Is is, Done done) {
     const int share = members <= SMP_THREADS / 8 ? 8 : members <= SMP_THREADS / 4 ? 4 : members <= SMP_THREADS / 2 ? 2 : 1;
     for (int i0 = 0; i0 < members; i0 += SMP_THREADS / share) {
       const int i = i0 + tid / share, mine = min(i, members - 1);
       uint64_t sum = 0;
-      for (int j = tid % share; j < members; j += share) sum += get(mine, j);
-      for (int w = 1; w < share; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, (unsigned long long)sum, w);
-      if (i < members && tid % share == 0) done(i, sum);
+      int count = 0;
+      for (int j = tid % share; j < members; j += share) {
+        const bool one = is(mine, j);
+        sum += one ? of[j] : 0;
+        count += one;
+      }
+      for (int w = 1; w < share; w <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, (unsigned long long)sum, w);
+        count += __shfl_xor_sync(0xffffffffu, count, w);
+      }
+      if (i < members && tid % share == 0) done(i, sum, count);
     }
   }
   // The blocks' s.fine, summed, after a barrier: four a lane.
-  __device__ __forceinline__ void gather_fine(uint64_t (&in)[4]) {
+  __device__ __forceinline__ void gather_fine(double (&in)[4]) {
     for (int y = tid; y < SMP_FINE * blocks; y += SMP_THREADS)
-      in_block(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = s.fine[y % SMP_FINE];
+      in_block(&s.weights[rank][0], y / SMP_FINE)[y % SMP_FINE] = weights_of(y % SMP_FINE);
     sync();
 #pragma unroll
     for (int e = 0; e < 4; ++e) in[e] = 0;
@@ -359,7 +390,7 @@ struct SampleRow {
       for (int e = 0; e < 4; ++e) in[e] += s.weights[b][4 * lane + e];
   }
   // The highest place among those of `bin` (and at or past `from`) from which on
-  // `measure` of them (whole numbers) reaches `want`, for bins of more tokens than a
+  // `measure` of them (up to 1 each) reaches `want`, for bins of more tokens than a
   // list holds, as where many are equal: the range of places is cut into 128, again
   // and again. (The lowest, if rounding says that all of them do not reach it.) The
   // blocks take the same steps.
@@ -415,17 +446,14 @@ struct SampleRow {
     }
     while (lo < hi) {
       const int shift = max(0, 57 - __clzll((long long)(hi - lo)));  // (hi - lo) >> shift < 128
-      if (tid < SMP_FINE) s.fine[tid] = 0;
+      clear_weights();
       __syncthreads();
       each([&](float l, uint64_t o) {
-        if (o >= lo && o <= hi) atomicAdd((unsigned long long*)&s.fine[(o - lo) >> shift], (unsigned long long)measure(l));
+        if (o >= lo && o <= hi) add_weight((int)((o - lo) >> shift), measure(l));
       });
       __syncthreads();
-      uint64_t in[4];
-      gather_fine(in);
       Quad f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[e] = (double)in[e];
+      gather_fine(f.v);
       f.scan(lane);
       const double all = Quad::of(SMP_FINE - 1, [&](int e) { return f.upto(e); });
       int part = Quad::last(lane, [&](int e) { return f.v[e] > 0 && all - (f.upto(e) - f.v[e]) >= want; });
@@ -617,29 +645,32 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     };
     // Few enough: rank 0 does the rest with them, pair by pair.
     const auto finish = [&](int members) {
-      uint64_t *placed = s.comp + SMP_SHORT, *kept = s.weight + SMP_SHORT;
-      if (tid == 0) s.add[0] = 0;
-      // The weights of those at a token's place and above, and in the low bits its
-      // rank (256 weights of 2^44 leave room). The k-th's are all of theirs.
+      uint64_t *placed = s.comp + SMP_SHORT, *kept = s.weight + SMP_SHORT, *all = s.fine;
+      uint16_t* ranks = s.near;
+      if (tid == 0) *all = 0;
+      // The weights of those at a token's place and above, and its rank. The k-th's
+      // are all of theirs.
       x.pairs(
-          members, [&](int i, int j) { return s.comp[j] >= s.comp[i] ? (s.weight[j] << 10) + 1 : 0ull; },
-          [&](int i, uint64_t sum) {
+          members, s.weight, [&](int i, int j) { return s.comp[j] >= s.comp[i]; },
+          [&](int i, uint64_t sum, int count) {
             placed[i] = sum;
-            if ((sum & 1023) == (uint64_t)k) s.best = sum >> 10;
+            ranks[i] = (uint16_t)count;
+            if (count == k) s.best = sum;
           });
       __syncthreads();
       const double target = by_p ? p * (double)s.best : INFINITY;
       if (tid < members) {
-        const uint64_t w = s.weight[tid], rest = (placed[tid] >> 10) - w, rank_of = placed[tid] & 1023;
-        const bool keep = rank_of <= (uint64_t)k && (rank_of == 1 || (double)rest < target) && (double)w >= least * SMP_UNIT;
+        const uint64_t w = s.weight[tid], rest = placed[tid] - w;
+        const int rank_of = ranks[tid];
+        const bool keep = rank_of <= k && (rank_of == 1 || (double)rest < target) && (double)w >= least * SMP_UNIT;
         kept[tid] = keep ? w : 0;
-        if (keep) atomicAdd((unsigned long long*)&s.add[0], (unsigned long long)w);
+        if (keep) atomicAdd((unsigned long long*)all, (unsigned long long)w);
       }
       __syncthreads();
-      const double total = (double)s.add[0], want = draw * total;
+      const double total = (double)*all, want = draw * total;
       x.pairs(
-          members, [&](int i, int j) { return ~(uint32_t)s.comp[j] <= ~(uint32_t)s.comp[i] ? kept[j] : 0ull; },
-          [&](int i, uint64_t sum) {
+          members, kept, [&](int i, int j) { return ~(uint32_t)s.comp[j] <= ~(uint32_t)s.comp[i]; },
+          [&](int i, uint64_t sum, int) {
             if ((double)sum > want && (double)(sum - kept[i]) <= want && kept[i]) {
               a.tokens[row] = (int)~(uint32_t)s.comp[i];
               if (a.probs) a.probs[number] = (float)((double)kept[i] / total);
@@ -720,15 +751,15 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (members <= SMP_LIST) {
       if (rank == 0)
         x.pairs(
-            members, [&](int i, int j) { return (uint64_t)(s.comp[j] >= s.comp[i]); },
-            [&](int i, uint64_t sum) {
-              if (sum == (uint64_t)rest)
+            members, s.weight, [&](int i, int j) { return s.comp[j] >= s.comp[i]; },
+            [&](int i, uint64_t, int count) {
+              if (count == rest)
                 for (int b = 0; b < blocks; ++b) *x.in_block(&s.cut, b) = s.comp[i];
             });
       x.sync();
       cut = s.cut;
     } else {
-      cut = x.narrow(bin, 0, rest, false, [](float) { return 1ull; });
+      cut = x.narrow(bin, 0, rest, false, [](float) { return 1.0; });
     }
     floor = order_value((uint32_t)(cut >> 32));
   }
@@ -782,7 +813,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     coarse = max(coarse, 0);  // (the first token's bin, if its weight is lost in 2^-16)
     Quad f;
     for (int tries = 0;; ++tries) {
-      if (tid < SMP_FINE) s.fine[tid] = 0;
+      x.clear_weights();
       if (tid == 0) s.n_near = 0;
       __syncthreads();
 #pragma unroll
@@ -845,9 +876,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       __syncthreads();
       // The weights of the bins of the coarse one.
       const auto weigh = [&](float l, int i) {
-        if (order_of(l, i) >= cut)
-          atomicAdd((unsigned long long*)&s.fine[x.whole(x.depth(l)) & (SMP_FINE - 1)],
-                    (unsigned long long)llrint(x.weight(l) * SMP_UNIT));
+        if (order_of(l, i) >= cut) x.add_weight(x.whole(x.depth(l)) & (SMP_FINE - 1), x.weight(l));
       };
       if (s.n_near <= SMP_NEAR) {
         for (int j = tid; j < s.n_near; j += SMP_THREADS) weigh((float)x.logits[s.near[j]], x.at + s.near[j]);
@@ -863,11 +892,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       // (One barrier for both.)
       double total[2] = {sums[0], sums[1]};
       x.tell(total);
-      uint64_t in[4];
-      x.gather_fine(in);
+      x.gather_fine(f.v);
       x.gather(total);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[e] = (double)in[e] / SMP_UNIT;
       f.scan(lane);
       target = p * total[0];
       rest = target - total[1];  // of the coarse bin's
@@ -896,14 +922,13 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     {
       // Its tokens to rank 0's list, those above it to what their stretches keep.
       const float begins = coarse * SMP_FINE, at_bin = bin, ends = bin + 1;
-      if (tid < SMP_ALL) s.add[tid] = 0;
+      x.clear_weights();
       __syncthreads();
       const auto place = [&](float l, int i, bool real) {
         const float r = x.depth(l);
         const bool keep = real && order_of(l, i) >= cut, here = keep && r >= at_bin && r < ends;
         const double w = x.weight(l);
-        if (keep && r >= begins && r < at_bin && w >= least)
-          atomicAdd((unsigned long long*)&s.add[(i - x.at) / seg], (unsigned long long)llrint(w * SMP_UNIT));
+        if (keep && r >= begins && r < at_bin && w >= least) x.add_weight((i - x.at) / seg, w);
         x.list(here, 1, order_of(l, i), w);
       };
       if (s.n_near <= SMP_NEAR) {
@@ -924,7 +949,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         });
       }
       __syncthreads();
-      const double mine = warp_sum(sums[2]) + (double)s.add[warp] / SMP_UNIT;
+      const double mine = warp_sum(sums[2]) + x.weights_of(warp);
       stretch = x.turn++;
       if (lane == 0) *x.in_block(&s.part[stretch & 1][2][rank * SMP_WARPS + warp], 0) = mine;
       x.sync();
@@ -937,12 +962,12 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
           s.best = 0;
           s.least = ~0ull;
         }
-        if (tid < SMP_ALL) s.add[tid] = 0;
+        x.clear_weights();
         __syncthreads();
         const double need = rest * SMP_UNIT;
         x.pairs(
-            members, [&](int i, int j) { return s.comp[j] >= s.comp[i] ? s.weight[j] : 0ull; },
-            [&](int i, uint64_t sum) {
+            members, s.weight, [&](int i, int j) { return s.comp[j] >= s.comp[i]; },
+            [&](int i, uint64_t sum, int) {
               atomicMin((unsigned long long*)&s.least, (unsigned long long)s.comp[i]);
               if ((double)sum >= need) atomicMax((unsigned long long*)&s.best, (unsigned long long)s.comp[i]);
             });
@@ -953,13 +978,13 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         // What is kept of the list, to the stretches.
         for (int i = tid; i < members; i += SMP_THREADS)
           if (s.comp[i] >= cut && (double)s.weight[i] >= least * SMP_UNIT)
-            atomicAdd((unsigned long long*)&s.add[(int)~(uint32_t)s.comp[i] / seg], (unsigned long long)s.weight[i]);
+            x.add_weight((int)~(uint32_t)s.comp[i] / seg, (double)s.weight[i] / SMP_UNIT);
         __syncthreads();
-        if (tid < blocks * SMP_WARPS) s.part[stretch & 1][2][tid] += (double)s.add[tid] / SMP_UNIT;
+        if (tid < blocks * SMP_WARPS) s.part[stretch & 1][2][tid] += x.weights_of(tid);
         __syncthreads();
       }
     } else {
-      cut = max(cut, x.narrow(bin, cut, rest * SMP_UNIT, true, [&](float l) { return llrint(x.weight(l) * SMP_UNIT); }));
+      cut = max(cut, x.narrow(bin, cut, rest, true, [&](float l) { return x.weight(l); }));
       double all_kept[3] = {0, 0, 0};
       x.each4([&](const float (&v)[4], int i) {
         for (int e = 0; e < 4; ++e)
