@@ -343,6 +343,9 @@ struct SampleRow {
     sync();
     gather_bins(turn++, n);
   }
+  // The weight of a listed token, as it was before it became a whole number: min-p goes
+  // by it everywhere.
+  __device__ __forceinline__ double weight_at(uint64_t comp) const { return weight(order_value((uint32_t)(comp >> 32))); }
   // Adds a token to rank 0's list (whole warps; nothing past its end).
   __device__ __forceinline__ void list(bool mine, int which, uint64_t comp, double w) {
     const unsigned who = __ballot_sync(0xffffffffu, mine);
@@ -662,7 +665,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       if (tid < members) {
         const uint64_t w = s.weight[tid], rest = placed[tid] - w;
         const int rank_of = ranks[tid];
-        const bool keep = rank_of <= k && (rank_of == 1 || (double)rest < target) && (double)w >= least * SMP_UNIT;
+        const bool keep = rank_of <= k && (rank_of == 1 || (double)rest < target) && x.weight_at(s.comp[tid]) >= least;
         kept[tid] = keep ? w : 0;
         if (keep) atomicAdd((unsigned long long*)all, (unsigned long long)w);
       }
@@ -976,9 +979,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         const uint64_t end = s.best ? s.best : s.least;
         if (members) cut = max(cut, end);
         // What is kept of the list, to the stretches.
-        for (int i = tid; i < members; i += SMP_THREADS)
-          if (s.comp[i] >= cut && (double)s.weight[i] >= least * SMP_UNIT)
-            x.add_weight((int)~(uint32_t)s.comp[i] / seg, (double)s.weight[i] / SMP_UNIT);
+        for (int i = tid; i < members; i += SMP_THREADS) {
+          const double w = x.weight_at(s.comp[i]);
+          if (s.comp[i] >= cut && w >= least) x.add_weight((int)~(uint32_t)s.comp[i] / seg, w);
+        }
         __syncthreads();
         if (tid < blocks * SMP_WARPS) s.part[stretch & 1][2][tid] += x.weights_of(tid);
         __syncthreads();
