@@ -463,7 +463,7 @@ struct SampleRow {
       if (part < 0) part = max(0, Quad::first(lane, [&](int e) { return f.v[e] > 0; }) & (SMP_FINE - 1));
       want -= all - Quad::of(part, [&](int e) { return f.upto(e); });
       lo += (uint64_t)part << shift;
-      hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+      hi = lo + min(hi - lo, ((uint64_t)1 << shift) - 1);  // (the part's end may lie past 64 bits)
       sync();  // (all have read the sums)
     }
     return lo;
