@@ -208,7 +208,7 @@ struct SampleRow {
   int turn;               // of what the blocks tell each other
   float m, scale;         // the maximum; bins per unit of m - l
   double c;               // log2(e) / T
-  float c32;
+  float c32, least_l;     // in f32; the least logit that has a weight
 
   // A barrier of all blocks of the row; a place in block r's shared memory.
   __device__ __forceinline__ void sync() {
@@ -259,11 +259,12 @@ struct SampleRow {
   static __device__ __forceinline__ int whole(float depth) {
     return __float_as_int(__fadd_rd(depth, 8388608.f)) & (SMP_BINS - 1);  // (a conversion takes eight times as long)
   }
-  // Below 2^-100: zero. (Not a number: minus infinity at T = inf.) Without a branch,
-  // so that several are under way.
+  // Below 2^-100: zero, as minus infinity has at every T. (By the least logit that has
+  // a weight: (m - l) / T in f32 is not finite where m - l or 1 / T is not, though the
+  // quotient may be small.) Without a branch, so that several are under way.
   __device__ __forceinline__ double weight(float l) const {
     const double w = weight_of((double)l - (double)m, c, s.table);
-    const bool some = (m - l) * c32 < 100.f;
+    const bool some = l >= least_l;
     return __hiloint2double(some ? __double2hiint(w) : 0, some ? __double2loint(w) : 0);
   }
   // Sums of the lanes' v[y] over all blocks: told before a barrier, in every lane
@@ -596,6 +597,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   }
   x.c = 1.4426950408889634 / temperature;
   x.c32 = (float)fmin(x.c, 3e38);
+  x.least_l = fmaxf(__double2float_ru((double)top - 100.0 / x.c), -3.4028235e38f);
   x.scale = (SMP_BINS - 1) / fmaxf(fminf(SMP_SPAN, top - low), 1e-30f);
   const float u = a.u[number];
   const double draw = fminf(u > 0.f ? u : 0.f, 0x1.fffffep-1f);
@@ -782,7 +784,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       uint32_t w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float t = (x.m - v[e]) * x.scale, begins = __fadd_rd(fminf(t, SMP_BINS - 1) * (1.f / SMP_FINE), 8388608.f);
+        // (However far apart two finite logits are, their step is finite.)
+        const float t = fminf(x.m - v[e], 1e35f) * x.scale, begins = __fadd_rd(fminf(t, SMP_BINS - 1) * (1.f / SMP_FINE), 8388608.f);
         b[e] = __float_as_int(begins) & (SMP_COARSE - 1);
         const float part = exp2_fast(((begins - 8388608.f) * SMP_FINE - t) * unit);
         // (None is lost that has a weight; the last bin's many without any count nothing.)
