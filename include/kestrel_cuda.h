@@ -384,8 +384,8 @@ KC_API int kc_model_forward(kc_ctx* ctx, const uint32_t* tokens, int n, float* l
 KC_API int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, uint32_t* out_tokens);
 /* The same loop with every token drawn from its logits by kc_sample_dev's rules:
    one setting of each kind for all, u [n_gen] uniform numbers and (optional) probs
-   [n_gen] the tokens' shares, host buffers. temperature 0: kc_model_generate's
-   tokens. */
+   [n_gen] the tokens' shares, host buffers. temperature not above 0:
+   kc_model_generate's tokens, shares 1. */
 KC_API int kc_model_sample(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, float temperature, int top_k,
                            float top_p, float min_p, const float* u, uint32_t* out_tokens, float* probs);
 /* Several independent sequences on one context, each with its own KV cache
@@ -600,7 +600,8 @@ KC_API int kc_attn_shared_dev(kc_ctx* ctx, int cache, int layer, const int32_t* 
    A logit that is not a number counts as minus infinity; of infinite ones each
    weighs 1 and the others nothing; a row with nothing else than minus infinity gets
    token -1 and share 0. u below 0 or not a number counts as 0, 1 and above as the
-   largest below 1. (The greedy calls kc_model_* take the same first maximum.) */
+   largest below 1. (The greedy calls kc_model_* take the same first maximum of rows
+   of numbers; a first logit that is not one they take, as the reference's scan does.) */
 KC_API int kc_sample_dev(kc_ctx* ctx, int t, const void* logits, int64_t stride, int n, int n_vocab, const float* u,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          int32_t* tokens, float* probs);

@@ -2782,6 +2782,11 @@ int kc_model_sample(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen
   if (n_gen > 0 && !u) return fail(ctx, KC_ERR_ARG, "kc_model_sample: no uniform numbers");
   if (ctx->model && ctx->model->n_vocab > SAMPLE_MAX_VOCAB)
     return fail(ctx, KC_ERR_SHAPE, "kc_model_sample: vocabulary of %d (up to %d)", ctx->model->n_vocab, SAMPLE_MAX_VOCAB);
+  if (!(temperature > 0.f)) {  // kc_model_generate's tokens, of logits that are not numbers too
+    RC(model_tokens(ctx, "kc_model_sample", prompt, n_prompt, n_gen, nullptr, out_tokens));
+    if (probs) std::fill(probs, probs + n_gen, 1.f);
+    return KC_OK;
+  }
   const SampleSpec spec{temperature, top_k, top_p, min_p, u, probs};
   return model_tokens(ctx, "kc_model_sample", prompt, n_prompt, n_gen, &spec, out_tokens);
 }
