@@ -385,7 +385,9 @@ KC_API int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, 
 /* The same loop with every token drawn from its logits by kc_sample_dev's rules:
    one setting of each kind for all, u [n_gen] uniform numbers and (optional) probs
    [n_gen] the tokens' shares, host buffers. temperature not above 0:
-   kc_model_generate's tokens, shares 1. */
+   kc_model_generate's tokens, shares 1. A step whose logits are all minus infinity
+   or not numbers has no token: KC_ERR_STATE, with out_tokens UINT32_MAX and probs 0
+   from there on, and the tokens before it cached. */
 KC_API int kc_model_sample(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, float temperature, int top_k,
                            float top_p, float min_p, const float* u, uint32_t* out_tokens, float* probs);
 /* Several independent sequences on one context, each with its own KV cache

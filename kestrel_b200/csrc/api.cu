@@ -2678,6 +2678,7 @@ static int model_tokens(kc_ctx* ctx, const char* what, const uint32_t* prompt, i
   cudaSetDevice(ctx->device);
   Model& m = *ctx->model;
   if (!m.seq_pos.empty()) m.seq_pos[0] = -1;  // sequence 0 loses its pending token
+  const int start = m.cached;
   if (m.cached + n_prompt + std::max(0, n_gen - 1) > m.n_ctx)
     return fail(ctx, KC_ERR_ARG, "%s: context full (n_ctx = %d)", what, m.n_ctx);
   RC(model_forward(ctx, prompt, false, n_prompt));
@@ -2766,7 +2767,17 @@ static int model_tokens(kc_ctx* ctx, const char* what, const uint32_t* prompt, i
   if (graph) cudaGraphDestroy(graph);
   cudaFree(hist);
   if (rc != KC_OK) return rc;
-  return check_status(ctx);
+  rc = check_status(ctx);
+  for (int i = 0; sample && i < n_gen; ++i) {
+    if (out_tokens[i] != UINT32_MAX) continue;
+    // Nothing to draw: this is no token, and the steps after it had none to go on from
+    // (which the embedding reports).
+    std::fill(out_tokens + i, out_tokens + n_gen, UINT32_MAX);
+    if (sample->probs) std::fill(sample->probs + i, sample->probs + n_gen, 0.f);
+    m.cached = start + n_prompt + i;
+    return fail(ctx, KC_ERR_STATE, "%s: no logit of token %d is above minus infinity", what, i);
+  }
+  return rc;
 }
 
 int kc_model_generate(kc_ctx* ctx, const uint32_t* prompt, int n_prompt, int n_gen, uint32_t* out_tokens) {
