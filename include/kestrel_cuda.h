@@ -460,8 +460,8 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
                      (high - low) within 0 .. 1 (usual: low 1, high 4)
    No w_i may be above 4. gain 0 is the scaling's own: 1 + 0.1 ln(factor) under
    KC_ROPE_YARN, else 1.
-   Angles are exact to 2^-33 of a turn at every int32 position, negative ones
-   included; products are f32, each result rounded once.
+   Angles are exact to 2^-31 of a turn at every int32 position, negative ones
+   included (2^-30 where w_i is above 1); products are f32, each result rounded once.
 
    kc_rope_dev: rows of n_head heads of head_dim (even; heads contiguous, strides
    in elements; KC_F32, KC_F16 or KC_BF16) at positions[row] (device), to rows of

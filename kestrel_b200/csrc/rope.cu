@@ -4,8 +4,8 @@
 //   (a, b) -> gain (a cos - b sin, a sin + b cos).
 // The frequencies come as 64-bit fractions of a turn, w_i / 2 pi = turn / 2^64,
 // so that the phase is one integer product that drops whole turns by itself: at
-// position 2^31 it is still good to 2^-34 of a turn, without 64-bit floating
-// point. The quadrant is its top two bits; what is left, within an eighth of a
+// position 2^31 it is still good to 2^-31 of a turn (rope_turns.h), without 64-bit
+// floating point. The quadrant is its top two bits; what is left, within an eighth of a
 // turn either way, goes to sincospif, good to its last bits.
 //
 // Both calls are bound by the memory rate (3 operations a value). A block takes a
@@ -20,8 +20,6 @@
 // an f16 cache, 239 MB in 44.8 us (5.3). Angles by each thread for up to eight
 // heads of its own took 43.6 and 66.8 us, places by division instead of steps 46.4
 // and 47.7, pairs turned one by one instead of two at a time 37.3 and 47.0.
-#include <math.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -32,46 +30,11 @@
 #include "kv_dev.cuh"
 #include "rope.h"
 
-#pragma nv_diag_suppress 20208  // (long double: on the host only)
-
 namespace kc {
 
 constexpr int ROPE_THREADS = 128;
 constexpr int ROPE_ROWS = 8;                 // rows of a block, at most
 constexpr int ROPE_PAIRS = ROPE_ROWS * 64;   // and their angles
-
-bool make_rope(RopeParams& r, int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
-               float high, float gain, const float* freq_factors) {
-  const long double two_pi = 2 * acosl(-1.0L), s = factor, len = original;
-  r = RopeParams{};
-  r.dim = dim;
-  r.interleaved = interleaved;
-  r.gain = gain != 0.f ? gain : scaling == ROPE_YARN ? (float)(1 + 0.1L * logl(s)) : 1.f;
-  long double from = 0, to = 0;
-  if (scaling == ROPE_YARN) {
-    const auto pair_of = [&](long double turns) { return dim * logl(len / (two_pi * turns)) / (2 * logl(base)); };
-    from = std::max(0.0L, floorl(pair_of(high)));
-    to = std::min((long double)dim - 1, ceill(pair_of(low)));
-  }
-  for (int i = 0; i < dim / 2; ++i) {
-    long double w = powl(base, -2.0L * i / dim);
-    if (freq_factors) w /= freq_factors[i];
-    if (scaling == ROPE_LINEAR) {
-      w /= s;
-    } else if (scaling == ROPE_YARN) {
-      const long double part = std::min(1.0L, std::max(0.0L, (i - from) / std::max(0.001L, to - from)));
-      w *= part / s + 1 - part;
-    } else if (scaling == ROPE_BANDS) {
-      const long double z = std::min(1.0L, std::max(0.0L, (len * w / two_pi - low) / ((long double)high - low)));
-      w *= z + (1 - z) / s;
-    }
-    if (!(w <= ROPE_MAX_FREQUENCY)) return false;
-    long double turn = w / two_pi;
-    turn -= floorl(turn);  // whole turns a position change nothing
-    r.turn[i] = (uint64_t)(int64_t)llrintl(ldexpl(turn - (turn >= 0.5L ? 1 : 0), 64));
-  }
-  return true;
-}
 
 // gain * (cos, sin) of a phase in 64-bit fractions of a turn.
 __device__ __forceinline__ float2 cos_sin(uint64_t phase, float gain) {

@@ -1,33 +1,13 @@
-// Rotary positions (rope.cu): the rotation of a rope id as the kernels take it,
-// and the host-side launchers.
+// Rotary positions (rope.cu): the host-side launchers.
 #pragma once
 
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "kv.h"
+#include "rope_turns.h"
 
 namespace kc {
-
-constexpr int ROPE_MAX_DIM = 256;
-
-// The pairs' frequencies as 64-bit fractions of a turn per position: the phase
-// position * turn[i], modulo 2^64, is exact however far the position. Passed to
-// the kernels by value (1 KB), so a rope id holds no device memory.
-struct RopeParams {
-  int dim;           // values of a head that turn, the first ones
-  int interleaved;   // pairs (2i, 2i + 1); otherwise (i, i + dim / 2)
-  float gain;        // cos and sin are multiplied by it
-  uint64_t turn[ROPE_MAX_DIM / 2];
-};
-
-enum : int { ROPE_NONE = 0, ROPE_LINEAR = 1, ROPE_YARN = 2, ROPE_BANDS = 3 };
-
-// The formulas of kc_rope, in the host's widest type. False: a frequency above
-// ROPE_MAX_FREQUENCY, past which the far positions' phases would not be exact.
-constexpr double ROPE_MAX_FREQUENCY = 4.0;
-bool make_rope(RopeParams& r, int dim, bool interleaved, float base, int scaling, float factor, int original, float low,
-               float high, float gain, const float* freq_factors);
 
 // Rows of n_head heads of hd, strides in elements; out may be x.
 void launch_rope(const RopeParams& r, const int32_t* positions, int n_rows, int n_head, int hd, int t, const void* x,
