@@ -459,7 +459,7 @@ KC_API int kc_gguf_inspect(const char* path, char* out, int64_t cap);
      KC_ROPE_BANDS   w_i (z + (1 - z) / factor), z = (original w_i / (2 pi) - low) /
                      (high - low) within 0 .. 1 (usual: low 1, high 4)
    No w_i may be above 4. gain 0 is the scaling's own: 1 + 0.1 ln(factor) under
-   KC_ROPE_YARN, else 1.
+   KC_ROPE_YARN with a factor above 1, else 1.
    Angles are exact to 2^-31 of a turn at every int32 position, negative ones
    included (2^-30 where w_i is above 1); products are f32, each result rounded once.
 

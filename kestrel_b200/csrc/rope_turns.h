@@ -38,7 +38,7 @@ inline bool make_rope(RopeParams& r, int dim, bool interleaved, float base, int 
   r = RopeParams{};
   r.dim = dim;
   r.interleaved = interleaved;
-  r.gain = gain != 0.f ? gain : scaling == ROPE_YARN ? (float)(1 + 0.1L * logl(s)) : 1.f;
+  r.gain = gain != 0.f ? gain : scaling == ROPE_YARN && s > 1 ? (float)(1 + 0.1L * logl(s)) : 1.f;
   long double from = 0, to = 0;
   if (scaling == ROPE_YARN) {
     const auto pair_of = [&](long double turns) { return dim * logl(len / (two_pi * turns)) / (2 * logl(base)); };
