@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArg
   float top = ml.y == 0.f ? -INFINITY : ml.x;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // (Never quite nothing, so that an infinite result stays what the formula gives.)
-  float share = ml.y == 0.f ? 0.f : fmaxf(exp2f(ml.x - (top == -INFINITY ? 0.f : top)), 1e-37f) * ml.y, sum = share;
+  float share = ml.y == 0.f ? 0.f : exp2f(ml.x - (top == -INFINITY ? 0.f : top)) * ml.y, sum = share;
+  const unsigned some = __ballot_sync(0xffffffffu, ml.y != 0.f);  // parts that saw a position
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   share = sum == 0.f ? 0.f : __fdiv_rn(share, sum);
@@ -257,11 +257,13 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArg
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float w = __shfl_sync(0xffffffffu, share, min(p0 + k, 31));
-        if (p0 + k <= splits && mine_y && w != 0.f) {
-          v.x = __fmaf_rn(w, u[k].x, v.x);
-          v.y = __fmaf_rn(w, u[k].y, v.y);
-          v.z = __fmaf_rn(w, u[k].z, v.z);
-          v.w = __fmaf_rn(w, u[k].w, v.w);
+        // (What is infinite stays so, however little its part weighs.)
+        const auto of = [w](float x) { return fabsf(x) < INFINITY ? w : 1.f; };
+        if (p0 + k <= splits && mine_y && (some >> (p0 + k) & 1)) {
+          v.x = __fmaf_rn(of(u[k].x), u[k].x, v.x);
+          v.y = __fmaf_rn(of(u[k].y), u[k].y, v.y);
+          v.z = __fmaf_rn(of(u[k].z), u[k].z, v.z);
+          v.w = __fmaf_rn(of(u[k].w), u[k].w, v.w);
         }
       }
     }
