@@ -46,21 +46,23 @@ constexpr float BESIDE_BYTES = 2.8e4f, SM_BYTES = 4.2e4f, ALL_BYTES = 5.8e6f, SE
 
 // The plan, by one warp: a lane per number of SMs that the prefixes get, the last
 // one for all SMs to both in turn. False: not shared it takes no longer.
+// (Whole numbers: the same plan whichever warp adds its sums first.)
+typedef unsigned long long plan_sum;
 struct PlanSums {
-  int units;    // row tiles of the prefixes, over the heads
-  int longest;  // tiles of the longest prefix
-  float steps;  // tiles of all units
-  float prefix, own, all;  // positions: of the prefixes, the own parts, and not shared
+  int units;       // row tiles of the prefixes, over the heads
+  int longest;     // tiles of the longest prefix
+  plan_sum steps;  // tiles of all units
+  plan_sum prefix, own, all;  // positions: of the prefixes, the own parts, and not shared
 };
 __device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, bool f32, int sms, int most, int32_t* plan) {
   const int lane = threadIdx.x & 31;
-  const float bytes = 4.f * c.hd * c.nkv;
+  const float bytes = 4.f * c.hd * c.nkv, of_prefix = t.prefix, of_own = t.own;
   const bool turns = lane == 31;
   const int g = turns ? sms : max(1, (lane + 1) * sms / 32), rest = turns ? sms : sms - g;
   // A step alone, or with its part of the memory rate, which row tiles that read the
   // same positions share.
   float step = f32 ? PREFIX_STEP_F32 : PREFIX_STEP;
-  if (!turns) step = fmaxf(step, __fdividef(t.prefix * bytes, t.steps * BESIDE_BYTES));
+  if (!turns) step = fmaxf(step, __fdividef(of_prefix * bytes, (float)t.steps * BESIDE_BYTES));
   // Items (units by parts) go over the g SMs in rounds.
   int splits = 1;
   float prefix = INFINITY;
@@ -72,9 +74,9 @@ __device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, 
       splits = p;
     }
   }
-  prefix = fmaxf(prefix, PREFIX_FIXED + t.prefix * bytes / ALL_BYTES);
+  prefix = fmaxf(prefix, PREFIX_FIXED + of_prefix * bytes / ALL_BYTES);
   // (Side by side they share the memory rate.)
-  const float own = OWN_FIXED + fmaxf(t.own * bytes / (rest * SM_BYTES), (t.own + (turns ? 0 : t.prefix)) * bytes / ALL_BYTES);
+  const float own = OWN_FIXED + fmaxf(of_own * bytes / (rest * SM_BYTES), (of_own + (turns ? 0.f : of_prefix)) * bytes / ALL_BYTES);
   const float both = PREP_AND_JOIN + (turns ? prefix + own : fmaxf(prefix, own));
   const unsigned best = __reduce_min_sync(0xffffffffu, __float_as_uint(both));
   const unsigned who = __ballot_sync(0xffffffffu, __float_as_uint(both) == best);
@@ -83,7 +85,7 @@ __device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, 
     plan[PLAN_PREFIX] = g;
     plan[PLAN_OWN] = rest;
   }
-  return __uint_as_float(best) < DECODE_FIXED + t.all * bytes / SEEN_BYTES;
+  return __uint_as_float(best) < DECODE_FIXED + (float)t.all * bytes / SEEN_BYTES;
 }
 
 // A block per entry: the pages that its table has in common with that of the first
@@ -177,14 +179,14 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
         const int units = (int)(((int64_t)(hi - lo) * group + 127) / 128) * c.nkv, nt = (both + shared_tile(c.hd) - 1) / shared_tile(c.hd);
         atomicAdd(&sums.units, units);
         atomicMax(&sums.longest, nt);
-        atomicAdd(&sums.steps, (float)units * nt);  // (in any order: a plan, and its sums are whole)
-        atomicAdd(&sums.prefix, (float)both);
+        atomicAdd(&sums.steps, (plan_sum)units * nt);
+        atomicAdd(&sums.prefix, (plan_sum)both);
       }
     }
   }
   if (!whole) return;
   __syncthreads();
-  float own = 0.f, all = 0.f;
+  plan_sum own = 0, all = 0;
   for (int e = tid; e < n; e += PREP_THREADS) {
     const int len = holds(seq(e));
     own += len - __ldcg(of_entry + e);

@@ -1,0 +1,45 @@
+"""When attn_shared_dev shares, and that the choice is the same every time (run with
+-m gpu). Whether it did shows in the bits: shared, 16-bit results carry the rounding of
+16-bit weights, so that many of them round to a neighbour of the decode call's; not
+shared, both are f32 sums in different orders (2^-20 apart at most), and a result of 11
+bits falls on another side once in a few hundred times."""
+import numpy as np
+import pytest
+
+from test_gpu_paged import F16, ints
+from test_gpu_shared import branches, ctx, run  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def wide_tables(ctx, n, length, nkv, hd, page=64):  # noqa: F811
+    """n sequences of `length` positions whose tables name the same pages but for the last."""
+    pages = -(-length // page)
+    k, v = (torch.randn((1, pages + n, nkv, page, hd), device="cuda").half() for _ in range(2))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32)[None].repeat(n, 1)
+    table[:, -1] = pages + torch.arange(n, device="cuda", dtype=torch.int32)
+    length = torch.full((n,), length, device="cuda", dtype=torch.int32)
+    refs = torch.ones(pages + n, device="cuda", dtype=torch.int32)
+    ctx.kv_cache(900, k, v, table, length, refs)
+    return k, v, table, length, refs
+
+
+def test_sums_past_24_bits(ctx):  # noqa: F811
+    """Plans are made of sums over all entries: 77 million positions here, from whole
+    numbers, so that no order of adding changes a plan, and the bits stay the same."""
+    from kestrel_b200.cuda import OPT_SHARE_ALWAYS
+    ctx.set_option(OPT_SHARE_ALWAYS, 0)
+    try:
+        held = wide_tables(ctx, 96, 800001, 1, 64)
+        q, start = torch.randn((96, 4, 64), device="cuda").half(), ints(list(range(0, 97, 8)))
+        outs = []
+        for _ in range(4):
+            outs.append(torch.empty_like(q))
+            ctx.attn_shared_dev(900, 0, q, start, outs[-1])
+        ctx.sync()
+        assert all(torch.equal(outs[0], x) for x in outs[1:])
+        assert torch.isfinite(outs[0]).all()
+        del held
+    finally:
+        ctx.set_option(OPT_SHARE_ALWAYS, 1)
