@@ -41,7 +41,7 @@ int attn_shared_counts() { return 1; }
 // products and after their last, for a step of 128 (64) positions of a row tile, and
 // by the bytes that an SM, and all of them, take in.
 constexpr float PREFIX_FIXED = 9.f, ITEM_FIXED = 6.f, PREFIX_STEP = 1.15f, PREFIX_STEP_F32 = 1.8f;
-constexpr float OWN_FIXED = 16.f, DECODE_FIXED = 9.f, PREP_AND_JOIN = 12.f;
+constexpr float OWN_FIXED = 16.f, DECODE_FIXED = 9.f, PREP_AND_JOIN = 12.f, NEXT_JOIN = 6.f;
 constexpr float BESIDE_BYTES = 2.8e4f, SM_BYTES = 4.2e4f, ALL_BYTES = 5.8e6f, SEEN_BYTES = 8.5e6f;  // (of pages that L2 has seen before)
 
 // The plan, by one warp: a lane per number of SMs that the prefixes get, the last
@@ -54,7 +54,10 @@ struct PlanSums {
   plan_sum steps;  // tiles of all units
   plan_sum prefix, own, all;  // positions: of the prefixes, the own parts, and not shared
 };
-__device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, bool f32, int sms, int most, int32_t* plan) {
+// `launches` that the entries take (as many at a time as the workspace has
+// room for), each with its own start, join and rounds.
+__device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, bool f32, int sms, int most, int launches,
+                                            int32_t* plan) {
   const int lane = threadIdx.x & 31;
   const float bytes = 4.f * c.hd * c.nkv, of_prefix = t.prefix, of_own = t.own;
   const bool turns = lane == 31;
@@ -66,18 +69,18 @@ __device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, 
   // Items (units by parts) go over the g SMs in rounds.
   int splits = 1;
   float prefix = INFINITY;
-  const float units = t.units, longest = t.longest, per = __fdividef(1.f, (float)g);
+  const float times = launches, units = t.units, longest = t.longest, per = __fdividef(1.f, g * times);
   for (int p = 1; p <= min(most, max(1, t.longest / 2)); ++p) {
-    const float took = PREFIX_FIXED + ceilf(units * p * per - 1e-3f) * (ITEM_FIXED + step * ceilf(__fdividef(longest, (float)p)));
+    const float took = times * (PREFIX_FIXED + ceilf(units * p * per - 1e-3f) * (ITEM_FIXED + step * ceilf(__fdividef(longest, (float)p))));
     if (took < prefix) {
       prefix = took;
       splits = p;
     }
   }
-  prefix = fmaxf(prefix, PREFIX_FIXED + of_prefix * bytes / ALL_BYTES);
+  prefix = fmaxf(prefix, times * PREFIX_FIXED + of_prefix * bytes / ALL_BYTES);
   // (Side by side they share the memory rate.)
-  const float own = OWN_FIXED + fmaxf(of_own * bytes / (rest * SM_BYTES), (of_own + (turns ? 0.f : of_prefix)) * bytes / ALL_BYTES);
-  const float both = PREP_AND_JOIN + (turns ? prefix + own : fmaxf(prefix, own));
+  const float own = times * OWN_FIXED + fmaxf(of_own * bytes / (rest * SM_BYTES), (of_own + (turns ? 0.f : of_prefix)) * bytes / ALL_BYTES);
+  const float both = PREP_AND_JOIN + (times - 1) * NEXT_JOIN + (turns ? prefix + own : fmaxf(prefix, own));
   const unsigned best = __reduce_min_sync(0xffffffffu, __float_as_uint(both));
   const unsigned who = __ballot_sync(0xffffffffu, __float_as_uint(both) == best);
   if (lane == __ffs(who) - 1) {
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
                                                                    const int32_t* __restrict__ group_start,
                                                                    int n_groups, int32_t* of_entry, int32_t* of_group,
                                                                    int32_t* lead, int* done, int group, bool f32,
-                                                                   int sms, int most, bool whole, bool always, int32_t* plan) {
+                                                                   int sms, int most, int launches, bool always, int32_t* plan) {
   pdl_enter();
   __shared__ int differ, last, wrong, shares;
   __shared__ PlanSums sums;
@@ -184,7 +187,6 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
       }
     }
   }
-  if (!whole) return;
   __syncthreads();
   plan_sum own = 0, all = 0;
   for (int e = tid; e < n; e += PREP_THREADS) {
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
   }
   __syncthreads();
   if (warp == 0) {
-    const bool yes = sums.units > 0 && shared_plan(sums, c, f32, sms, most, plan);
+    const bool yes = sums.units > 0 && shared_plan(sums, c, f32, sms, most, launches, plan);
     if (lane == 0) shares = yes || always;
   }
   __syncthreads();
@@ -296,7 +298,7 @@ int launch_attn_shared(const AttnArgs& a, SharedArgs sh, const KvMaps& rows16, c
   // As many entries at a time as the workspace has room for.
   const int step = (int)std::min<int64_t>(a.n, room / (sh.splits + 1));
   launch_k(shared_prep_kernel, a.n, PREP_THREADS, 0, st, c, a.seqs, a.n, sh.group_start, sh.n_groups, sh.of_entry,
-           sh.of_group, sh.lead, done, (int)group, a.t_q == T_F32, num_sms(), sh.splits, step == a.n, sh.always, sh.plan);
+           sh.of_group, sh.lead, done, (int)group, a.t_q == T_F32, num_sms(), sh.splits, (a.n + step - 1) / step, sh.always, sh.plan);
   const int64_t el = a.t_q == T_F32 ? 4 : 2;
   for (sh.e0 = 0; sh.e0 < a.n; sh.e0 += step) {
     sh.e1 = std::min(a.n, sh.e0 + step);

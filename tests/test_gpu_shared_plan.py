@@ -1,8 +1,9 @@
 """When attn_shared_dev shares, and that the choice is the same every time (run with
 -m gpu). Whether it did shows in the bits: shared, 16-bit results carry the rounding of
 16-bit weights, so that many of them round to a neighbour of the decode call's; not
-shared, both are f32 sums in different orders (2^-20 apart at most), and a result of 11
-bits falls on another side once in a few hundred times."""
+shared, both are f32 sums in different orders (2^-20 apart at most; up to 8 heads to a
+key's, whose weights keep their rests), and a result of 11 bits falls on another side
+once in a few hundred times."""
 import numpy as np
 import pytest
 
@@ -43,3 +44,26 @@ def test_sums_past_24_bits(ctx):  # noqa: F811
         del held
     finally:
         ctx.set_option(OPT_SHARE_ALWAYS, 1)
+
+
+@pytest.mark.parametrize("n", [60, 900])
+def test_little_in_common(ctx, n):  # noqa: F811
+    """A page in common by twos, as many entries as the workspace takes at a time and
+    more: not worth it, and not shared unless the option says so. Groups of fifty with
+    almost everything in common are."""
+    from kestrel_b200.cuda import OPT_SHARE_ALWAYS
+    for groups, shared in (([(1, [150, 131])] * (n // 2), False), ([(40, [650 + i % 9 for i in range(n // 4)])] * 4, n > 100)):
+        c, start = branches(ctx, groups, 16, 2, 256, F16, seed=n, poison=False)
+        q = torch.randn((start[-1], 16, 256), device="cuda").half()
+        alone = torch.empty_like(q)
+        ctx.attn_decode_dev(c.id, 1, q, alone)
+        always = run(ctx, c, q, start)
+        ctx.set_option(OPT_SHARE_ALWAYS, 0)
+        try:
+            out = run(ctx, c, q, start)
+        finally:
+            ctx.set_option(OPT_SHARE_ALWAYS, 1)
+        off = lambda x: float((x != alone).float().mean())
+        assert off(always) > 0.03
+        assert off(out) > 0.03 if shared else off(out) < 0.005
+        assert (out.double() - alone.double()).norm() <= 2.0 ** -10 * alone.double().norm()
