@@ -31,6 +31,7 @@
 namespace kc {
 
 constexpr int PREP_THREADS = 128;
+constexpr int FEW = 8;  // entries of a group that one lane looks through
 constexpr int SHARED_SPLITS = 31;  // (a lane each in the join, and one for the own part)
 constexpr size_t SHARED_PART_BYTES = (size_t)24 << 20;
 
@@ -99,13 +100,13 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
                                                                    int32_t* lead, int* done, int group, bool f32,
                                                                    int sms, int most, int launches, bool always, int32_t* plan) {
   pdl_enter();
-  __shared__ int differ, last, wrong, shares;
+  __shared__ int differ, last, wrong, shares, large;
   __shared__ PlanSums sums;
   const int i = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const auto seq = [&](int e) { return seqs ? seqs[e] : e; };
   const auto holds = [&](int s) { return s >= 0 && s < c.n_seq ? kv_len(c, s) : 0; };
   if (tid == 0) {
-    wrong = 0;
+    wrong = large = 0;
     sums = PlanSums{};
   }
   {
@@ -160,13 +161,27 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
     for (int g = tid; g < n_groups; g += PREP_THREADS) of_group[g] = 0;
     return;
   }
-  for (int g = warp; g < n_groups; g += PREP_THREADS / 32) {
-    const int lo = group_start[g], hi = group_start[g + 1];
+  // What group g's entries lo .. hi - 1 have in common, of those that hold anything
+  // (`held` of them, the first `first`).
+  const auto settle = [&](int g, int lo, int hi, int least, int first, int held) {
+    const int both = held > 1 ? least : 0;
+    of_group[g] = both;
+    lead[g] = held ? seq(first) : 0;
+    if (both) {
+      const int units = (int)(((int64_t)(hi - lo) * group + 127) / 128) * c.nkv, nt = (both + shared_tile(c.hd) - 1) / shared_tile(c.hd);
+      atomicAdd(&sums.units, units);
+      atomicMax(&sums.longest, nt);
+      atomicAdd(&sums.steps, (plan_sum)units * nt);
+      atomicAdd(&sums.prefix, (plan_sum)both);
+    }
+    return both;
+  };
+  const auto by_warp = [&](int g, int lo, int hi) {
     int least = INT_MAX, first = INT_MAX, held = 0;
     for (int e = lo + lane; e < hi; e += 32) {
-      const int both = __ldcg(of_entry + e);
-      if (both < 0) continue;
-      least = min(least, both);
+      const int of = __ldcg(of_entry + e);
+      if (of < 0) continue;
+      least = min(least, of);
       first = min(first, e);
       ++held;
     }
@@ -175,20 +190,47 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
     held = __reduce_add_sync(0xffffffffu, held);
     const int both = held > 1 ? least : 0;
     for (int e = lo + lane; e < hi; e += 32) of_entry[e] = __ldcg(of_entry + e) < 0 ? 0 : both;
-    if (lane == 0) {
-      of_group[g] = both;
-      lead[g] = held ? seq(first) : 0;
-      if (both) {
-        const int units = (int)(((int64_t)(hi - lo) * group + 127) / 128) * c.nkv, nt = (both + shared_tile(c.hd) - 1) / shared_tile(c.hd);
-        atomicAdd(&sums.units, units);
-        atomicMax(&sums.longest, nt);
-        atomicAdd(&sums.steps, (plan_sum)units * nt);
-        atomicAdd(&sums.prefix, (plan_sum)both);
+    if (lane == 0) settle(g, lo, hi, least, first, held);
+  };
+  if (n_groups <= 32) {
+    for (int g = warp; g < n_groups; g += PREP_THREADS / 32) by_warp(g, group_start[g], group_start[g + 1]);
+  } else {
+    // Many groups: the small ones a lane each, since a warp's look-ups wait for each
+    // other; the others a warp each. (2000 entries in groups of their own: a call of
+    // 516 us so, of 915 with a warp for each.)
+    for (int g = tid; g < n_groups; g += PREP_THREADS) {
+      const int lo = group_start[g], hi = group_start[g + 1];
+      if (hi - lo > FEW) {
+        large = 1;
+        continue;
+      }
+      int of[FEW], least = INT_MAX, first = INT_MAX, held = 0;
+#pragma unroll
+      for (int k = 0; k < FEW; ++k) of[k] = lo + k < hi ? __ldcg(of_entry + lo + k) : -1;
+#pragma unroll
+      for (int k = 0; k < FEW; ++k)
+        if (of[k] >= 0) {
+          least = min(least, of[k]);
+          first = min(first, lo + k);
+          ++held;
+        }
+      const int both = settle(g, lo, hi, least, first, held);
+#pragma unroll
+      for (int k = 0; k < FEW; ++k)
+        if (lo + k < hi) of_entry[lo + k] = of[k] < 0 ? 0 : both;
+    }
+    __syncthreads();
+    for (int g0 = 0, ones = 0; large && g0 < n_groups; g0 += 32) {
+      const int g = g0 + lane, lo = g < n_groups ? group_start[g] : 0, hi = g < n_groups ? group_start[g + 1] : 0;
+      for (unsigned left = __ballot_sync(0xffffffffu, hi - lo > FEW); left; left &= left - 1) {
+        const int who = __ffs(left) - 1, its_lo = __shfl_sync(0xffffffffu, lo, who), its_hi = __shfl_sync(0xffffffffu, hi, who);
+        if (ones++ % (PREP_THREADS / 32) == warp) by_warp(g0 + who, its_lo, its_hi);
       }
     }
   }
   __syncthreads();
   plan_sum own = 0, all = 0;
+#pragma unroll 4
   for (int e = tid; e < n; e += PREP_THREADS) {
     const int len = holds(seq(e));
     own += len - __ldcg(of_entry + e);
