@@ -89,7 +89,9 @@ __device__ __forceinline__ bool shared_plan(const PlanSums& t, const KvView& c, 
     plan[PLAN_PREFIX] = g;
     plan[PLAN_OWN] = rest;
   }
-  return __uint_as_float(best) < DECODE_FIXED + (float)t.all * bytes / SEEN_BYTES;
+  // (Not shared, a position is read once from memory, and again from L2.)
+  const float once = of_own + of_prefix, again = (float)t.all - once;
+  return __uint_as_float(best) < DECODE_FIXED + once * bytes / ALL_BYTES + again * bytes / SEEN_BYTES;
 }
 
 // A block per entry: the pages that its table has in common with that of the first
