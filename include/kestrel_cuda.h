@@ -568,8 +568,8 @@ KC_API int kc_kv_copy_pages_dev(kc_ctx* ctx, int cache, const int32_t* src, cons
    ascending within 0 .. n. The leading pages that the tables of all of a group's
    sequences that hold positions name alike, and behind which each holds another
    position, are read once for the group; the device looks them up, so the results
-   are kc_attn_decode_dev's (within the roundings above, weights of 16-bit queries
-   rounded as in kc_attn_prompt_dev) whatever the groups are. An entry in no group
+   are kc_attn_decode_dev's (within the roundings above; the weights of what is read
+   once are good to 22 bits, or 16 of KC_BF16) whatever the groups are. An entry in no group
    is by itself; a list that does not ascend is reported, and nothing is shared. */
 KC_API int kc_attn_decode_dev(kc_ctx* ctx, int cache, int layer, const int32_t* seqs, int n, int n_head, int t,
                               const void* q, int64_t q_stride, float scale, int window, int sinks, void* out,

@@ -41,7 +41,7 @@ int attn_shared_counts() { return 1; }
 // What the two kernels take, in us, as measured on a B200: until their first
 // products and after their last, for a step of 128 (64) positions of a row tile, and
 // by the bytes that an SM, and all of them, take in.
-constexpr float PREFIX_FIXED = 9.f, ITEM_FIXED = 6.f, PREFIX_STEP = 1.15f, PREFIX_STEP_F32 = 1.8f;
+constexpr float PREFIX_FIXED = 9.f, ITEM_FIXED = 6.f, PREFIX_STEP = 1.6f, PREFIX_STEP_F32 = 1.8f;
 constexpr float OWN_FIXED = 16.f, DECODE_FIXED = 9.f, PREP_AND_JOIN = 12.f, NEXT_JOIN = 6.f;
 constexpr float BESIDE_BYTES = 2.8e4f, SM_BYTES = 4.2e4f, ALL_BYTES = 5.8e6f, SEEN_BYTES = 8.5e6f;  // (of pages that L2 has seen before)
 
