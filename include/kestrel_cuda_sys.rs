@@ -209,11 +209,12 @@ unsafe extern "C" {
     pub fn kc_load_gguf(ctx: *mut kc_ctx, path: *const c_char, n_ctx: c_int, info_json: *mut c_char,
         cap: i64) -> c_int;
     pub fn kc_gguf_inspect(path: *const c_char, out: *mut c_char, cap: i64) -> c_int;
-    // paged key-value cache and its attention (device buffers)
+    // rotary positions
     pub fn kc_rope(ctx: *mut kc_ctx, rope: c_int, dim: c_int, layout: c_int, base: f32, scaling: c_int, factor: f32,
         original: c_int, low: f32, high: f32, gain: f32, freq_factors: *const f32) -> c_int;
     pub fn kc_rope_dev(ctx: *mut kc_ctx, rope: c_int, positions: *const i32, n_rows: c_int, n_head: c_int,
         head_dim: c_int, t: c_int, x: *const c_void, x_stride: i64, out: *mut c_void, out_stride: i64) -> c_int;
+    // paged key-value cache and its attention (device buffers)
     pub fn kc_kv_cache(ctx: *mut kc_ctx, cache: c_int, t: c_int, n_layer: c_int, n_pages: c_int, page: c_int,
         n_head_kv: c_int, head_dim: c_int, n_seq: c_int, max_pages: c_int, k: *mut c_void, v: *mut c_void,
         table: *mut i32, len: *mut i32, refs: *mut i32) -> c_int;
@@ -240,10 +241,11 @@ unsafe extern "C" {
     pub fn kc_attn_prompt_dev(ctx: *mut kc_ctx, cache: c_int, layer: c_int, seqs: *const i32,
         row_start: *const i32, n: c_int, n_rows: c_int, n_head: c_int, t: c_int, q: *const c_void, q_stride: i64,
         scale: f32, window: c_int, sinks: c_int, out: *mut c_void, out_stride: i64) -> c_int;
-    // expert parallelism (one process per GPU)
+    // sampling (device buffers)
     pub fn kc_sample_dev(ctx: *mut kc_ctx, t: c_int, logits: *const c_void, stride: i64, n: c_int, n_vocab: c_int,
         u: *const f32, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32,
         tokens: *mut i32, probs: *mut f32) -> c_int;
+    // expert parallelism (one process per GPU)
     pub fn kc_ep_unique_id(out: *mut c_char) -> c_int; // out: 128 bytes
     pub fn kc_ep_init(ctx: *mut kc_ctx, rank: c_int, world: c_int, uid: *const c_char) -> c_int; // uid: 128 bytes
     pub fn kc_ep_reserve(ctx: *mut kc_ctx, max_tokens: c_int) -> c_int;

@@ -330,7 +330,7 @@ struct PromptArgs {
 
 // SHARED: an entry is a group of sequences, its rows one query of each; every row
 // sees all positions that the group has in common, and what comes of them is left
-// for the join (attn_decode.cu).
+// for the join (attn_shared.cu).
 template <typename TQ, typename TKV, int NB, bool TWO, bool SHARED>
 __global__ void __launch_bounds__(PromptShape<TQ, NB, TWO, SHARED>::THREADS, 1)
     attn_prompt_kernel(const PromptArgs d, const __grid_constant__ KvMaps maps, const __grid_constant__ KvMap q_map) {

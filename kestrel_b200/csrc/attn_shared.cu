@@ -17,8 +17,8 @@
 //
 // Measured (B200, us a call; what has to be read at 6559 GB/s; each sequence by
 // itself), heads of 128: 32 samples of a prompt of 4001, 32 and 4 heads, f32 queries:
-// 40, 5.6, 47; 4 groups of 32 at 6000, 32 and 8, bf16: 143, 98, 407; 64 at 32768, 32
-// and 4, f16: 76, 21, 485. The first and last are the steps of a chain: the plan 9, the
+// 41, 5.6, 47; 4 groups of 32 at 6000, 32 and 8, bf16: 142, 98, 407; 64 at 32768, 32
+// and 4, f16: 93, 21, 485. The first and last are the steps of a chain: the plan 9, the
 // prefixes' way to their first scores 9, their products, the join 7; the second is
 // bound by what the own parts read, 5.0 TB/s beside the prefixes.
 #include <algorithm>
@@ -263,7 +263,9 @@ __global__ void __launch_bounds__(PREP_THREADS) shared_prep_kernel(KvView c, con
 }
 
 // A warp per (entry, head): the parts' maxima and sums a lane each, then their
-// values, 16 bytes a lane, eight parts under way.
+// values, 16 bytes a lane, eight parts under way. (What it waits for is the decode
+// kernel alone, the launch before it; that the prefixes' kernel is through too rests on
+// every block of the decode kernel waiting for it before it leaves.)
 template <typename T>
 __global__ void __launch_bounds__(PREP_THREADS) shared_join_kernel(const AttnArgs a, const SharedArgs sh) {
   pdl_enter();

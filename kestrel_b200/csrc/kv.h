@@ -90,7 +90,8 @@ struct AttnArgs {
 };
 // Decode attention of groups of entries whose sequences begin with the same pages:
 // their prefix is computed once for a group (attn_prompt.cu's kernel, its rows the
-// group's queries), the rest entry by entry (attn_decode.cu's), which joins both.
+// group's queries), the rest entry by entry (attn_decode.cu's), and both are joined
+// by a kernel of their own (attn_shared.cu).
 struct SharedArgs {
   const int32_t* group_start;  // [n_groups + 1]
   int n_groups;

@@ -24,9 +24,9 @@
 // cut among them, pair by pair. Each warp has a stretch of indices, so that the
 // stretches' sums lead to the one that holds the token, and only it is read again.
 //
-// Measured (B200): 256 rows of 151936 f32 logits 306 us under top-p (156 MB: 23.7 us
-// at 6559 GB/s), 112 under top-k, 146 without a cut; 32 rows of mixed settings 47; one
-// row of 4096 8.2. Bound by the steps of a row, not by memory (DRAM 6% busy, the 64-bit
+// Measured (B200): 256 rows of 151936 f32 logits 310 us under top-p (156 MB: 23.7 us
+// at 6559 GB/s), 116 under top-k of 40, 144 without a cut; 32 rows of mixed settings 45;
+// one row of 4096 8.1. Bound by the steps of a row, not by memory (DRAM 6% busy, the 64-bit
 // pipe 16%): 33 rows of this size are under way, each a chain of a dozen steps with a
 // barrier of the cluster behind it.
 #include <cooperative_groups.h>
