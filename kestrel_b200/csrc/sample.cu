@@ -13,8 +13,9 @@
 // are computed in 64 bits (good to 2e-13) and every sum is either of whole numbers
 // or in an order that does not depend on timing. The whole numbers are units of 2^-60
 // of the largest weight, in two words, where any number of tokens may meet, and of
-// 2^-54 in lists of 512: off by 2e-13 of it at most, for any number. (In one word, by units of
-// 2^-44, 400 thousand equal light tokens are off by 1e-8, and top-p ends elsewhere.)
+// 2^-54 in lists of 512: off by 2e-13 of it at most, however many there are. (By units
+// of 2^-44, in one word, 400 thousand equal light tokens are off by 1e-8, and top-p ends
+// elsewhere.)
 //
 // A cluster of up to eight blocks holds a row in its shared memory: the logits are
 // read once. On the way into it the maximum; then a histogram over (m - l) finds
@@ -26,9 +27,9 @@
 //
 // Measured (B200): 256 rows of 151936 f32 logits 310 us under top-p (156 MB: 23.7 us
 // at 6559 GB/s), 116 under top-k of 40, 144 without a cut; 32 rows of mixed settings 45;
-// one row of 4096 8.1. Bound by the steps of a row, not by memory (DRAM 6% busy, the 64-bit
-// pipe 16%): 33 rows of this size are under way, each a chain of a dozen steps with a
-// barrier of the cluster behind it.
+// one row of 4096 8.1. Bound by the steps of a row, not by memory (DRAM 6% busy, the
+// 64-bit pipe 16%): 33 rows of this size are under way, each a chain of a dozen steps
+// with a barrier of the cluster behind it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -66,7 +67,7 @@ struct alignas(16) SampleShared {
     uint32_t coarse[SMP_COARSE][32];  // a column a lane: no two of a warp meet in a bank
     struct {                          // once that histogram is through:
       double weights[SMP_CLUSTER][SMP_FINE];  // the blocks' weights by bins of a coarse bin
-      uint64_t comp[SMP_LIST];                  // listed tokens (rank 0)
+      uint64_t comp[SMP_LIST];                // listed tokens (rank 0)
       uint64_t weight[SMP_LIST];
     };
   };
